@@ -332,6 +332,72 @@ int64_t tsfast_hip_mat_adjoint_workspace_bytes(int64_t B, int64_t L, int64_t n, 
 int tsfast_hip_mat_adjoint_bounds(int64_t B, int64_t L, int64_t n, int64_t CL, const float* jt, const float* gout,
                                   float* bnd, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Gated linear recurrence with a matrix state per head:
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = S_t^T q_t
+ * and its gradients. No counterpart in the reference (its selective scan's state is a vector a channel).
+ * Layout: q, k [B, L, Hk, K], v, grad_o [B, L, H, V], g [B, L, H], float32 or bfloat16 alike, read through
+ * strides; o, grad_v [B, L, H, V], grad_q, grad_k [B, L, Hk, K], grad_g [B, L, H] contiguous of that type;
+ * states [B, H, K, V] float32 contiguous. Hk divides H; head h reads query and key head h / (H / Hk).
+ * K, V <= 128. g may be any value up to 0 and -inf (the state is forgotten); the other inputs are finite:
+ * a value that is not may reach every step of its 64-step chunk.
+ * `strides` is host memory, in elements: batch row, step and head of q, k, v, g (and grad_o: 15 in all);
+ * the last dimension of q, k, v and grad_o is dense. No alignment is needed.
+ * state and grad_last may be NULL (zero); grad_state is required iff state is given. L = 0 copies the state.
+ */
+int64_t tsfast_hip_gated_fwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype);
+int tsfast_hip_gated_fwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,
+                         const void* k, const void* v, const void* g, const int64_t* strides, const float* state,
+                         void* o, float* state_last, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t tsfast_hip_gated_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype);
+int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,
+                         const void* k, const void* v, const void* g, const void* grad_o, const int64_t* strides,
+                         const float* state, const float* grad_last, void* grad_q, void* grad_k, void* grad_v,
+                         void* grad_g, float* grad_state, void* workspace, int64_t workspace_bytes, void* stream);
+/* One step with the state updated in place: q, k [B, Hk, K], v [B, H, V], g [B, H] through strides (batch row and
+ * head of q, k, v, g: 8 in all), state [B, H, K, V] float32 contiguous, o [B, H, V] contiguous. K <= 1024. */
+int tsfast_hip_gated_step(int64_t B, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,
+                          const void* k, const void* v, const void* g, const int64_t* strides, float* state, void* o,
+                          void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Norms before and after a block. rms(x) = x / sqrt(mean(x^2) + eps); silu(x) = x / (1 + exp(-x)).
+ *
+ * gated_norm: per row and group of `width` columns  y = rms(x) * weight * silu(gate), or with gate_first
+ *   y = rms(x * silu(gate)) * weight. x, gate, y, grad_y and their gradients are [rows, groups * width] of one
+ *   type (float32 or bfloat16); gate and weight (float32 [groups * width]) may be NULL (one).
+ * residual_norm: new = residual + scale * (post_weight ? rms(x) * post_weight : x),  y = rms(new) * weight
+ *   (of `new` before its rounding to the residual's type). x, y [rows, width] of dtype, residual and new of
+ *   res_dtype; weight, post_weight, scale float32 [width], any of them NULL (weight and scale: one; post_weight: no
+ *   norm of x).
+ * The *_stride arguments are row strides in elements of an input; outputs and gradients are contiguous. No alignment
+ * is needed. The backward's parameter gradients are sums in a fixed order, through the workspace; a parameter's
+ * gradient is required iff the parameter is given. grad_new or grad_y may be NULL (zero).
+ * Widths: groups * width up to 2^31 - 1, width up to tsfast_hip_norm_max_width(). No counterpart in the reference.
+ */
+int64_t tsfast_hip_norm_max_width(void);
+int64_t tsfast_hip_gated_norm_workspace_bytes(int64_t rows, int64_t groups, int64_t width);
+int tsfast_hip_gated_norm_fwd(int64_t rows, int64_t groups, int64_t width, int dtype, int gate_first, float eps,
+                              const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                              const float* weight, void* y, void* stream);
+int tsfast_hip_gated_norm_bwd(int64_t rows, int64_t groups, int64_t width, int dtype, int gate_first, float eps,
+                              const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                              const float* weight, const void* grad_y, int64_t grad_y_stride, void* grad_x,
+                              void* grad_gate, float* grad_weight, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+int64_t tsfast_hip_residual_norm_workspace_bytes(int64_t rows, int64_t width);
+int tsfast_hip_residual_norm_fwd(int64_t rows, int64_t width, int dtype, int res_dtype, float eps, const void* x,
+                                 int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const float* post_weight, const float* scale, const float* weight, void* new_residual,
+                                 void* y, void* stream);
+int tsfast_hip_residual_norm_bwd(int64_t rows, int64_t width, int dtype, int res_dtype, float eps, const void* x,
+                                 int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const float* post_weight, const float* scale, const float* weight,
+                                 const void* grad_new, int64_t grad_new_stride, const void* grad_y,
+                                 int64_t grad_y_stride, void* grad_x, void* grad_residual, float* grad_post_weight,
+                                 float* grad_scale, float* grad_weight, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

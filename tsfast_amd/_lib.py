@@ -22,6 +22,7 @@ _lock = threading.Lock()
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_f32 = ctypes.c_float
 _ptr = ctypes.c_void_p
 
 # Entry points and their argument types (mirrors include/tsfast_hip.h).
@@ -76,6 +77,24 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "tsfast_hip_projscan_bwd": ([_i64] * 5 + [_ptr] * 17 + [_i64, _ptr], _int),
     "tsfast_hip_wide_pack": ([_i64] * 4 + [_ptr] * 9, _int),
     "tsfast_hip_wide_unpack": ([_i64] * 6 + [_ptr] * 9, _int),
+    "tsfast_hip_gated_fwd_workspace_bytes": ([_i64] * 6 + [_int], _i64),
+    "tsfast_hip_gated_fwd": ([_i64] * 6 + [_int] + [_ptr] * 9 + [_i64, _ptr], _int),
+    "tsfast_hip_gated_bwd_workspace_bytes": ([_i64] * 6 + [_int], _i64),
+    "tsfast_hip_gated_bwd": ([_i64] * 6 + [_int] + [_ptr] * 14 + [_i64, _ptr], _int),
+    "tsfast_hip_gated_step": ([_i64] * 5 + [_int] + [_ptr] * 8, _int),
+    "tsfast_hip_norm_max_width": ([], _i64),
+    "tsfast_hip_gated_norm_workspace_bytes": ([_i64] * 3, _i64),
+    "tsfast_hip_gated_norm_fwd": ([_i64] * 3 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] * 3, _int),
+    "tsfast_hip_gated_norm_bwd": (
+        [_i64] * 3 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] + [_ptr, _i64] + [_ptr] * 4 + [_i64, _ptr],
+        _int,
+    ),
+    "tsfast_hip_residual_norm_workspace_bytes": ([_i64] * 2, _i64),
+    "tsfast_hip_residual_norm_fwd": ([_i64] * 2 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] * 6, _int),
+    "tsfast_hip_residual_norm_bwd": (
+        [_i64] * 2 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] * 3 + [_ptr, _i64] * 2 + [_ptr] * 6 + [_i64, _ptr],
+        _int,
+    ),
     "tsfast_hip_mat_adjoint_workspace_bytes": ([_i64] * 4, _i64),
     "tsfast_hip_mat_adjoint_bounds": ([_i64] * 4 + [_ptr] * 4 + [_i64, _ptr], _int),
 }

@@ -1,0 +1,228 @@
+"""HIP backend of the gated linear recurrence (``csrc/gated.hip``).
+
+``supports(q, k, v, g, state)`` / ``run(...) -> (o, last)``, differentiable in all inputs through the
+``tsfast_hip::gated_recurrence`` / ``gated_recurrence_bwd`` custom ops, and ``supports_step`` / ``step`` for
+one token with the state updated in place (``tsfast_hip::gated_recurrence_step``). Only the inputs are saved
+for the backward.
+
+q, k, v, g and their gradients are float32 or bfloat16, all alike, at any strides with a dense last
+dimension (others are copied); states are float32. The kernels sum in float32 and keep the state in it. With
+bfloat16 they multiply on the bfloat16 matrix cores: what is not bfloat16 already (the decayed scores, the state,
+the decayed keys) goes in as a sum of two or three bfloat16 numbers, so outputs are rounded once.
+"""
+
+from __future__ import annotations
+
+__all__ = ["supports", "run", "supports_step", "step"]
+
+import ctypes
+
+import torch
+
+from .. import _lib
+from ..ops import custom_op
+
+_IO_DTYPES = {torch.float32: _lib.TSF_DTYPE_F32, torch.bfloat16: _lib.TSF_DTYPE_BF16}
+_MAX_WIDTH = 128
+_STEP_MAX_K = 1024
+_MAX_GRID = (1 << 24) - 1
+
+
+def _tensor_reason(q, k, v, g, state) -> str | None:
+    dev = v.device
+    if dev.type != "cuda":
+        return f"v on {dev.type}, hip backend is GPU-only"
+    if v.dtype not in _IO_DTYPES:
+        return f"v dtype {v.dtype} not float32/bfloat16"
+    for name, t in (("q", q), ("k", k), ("g", g)):
+        if t.dtype != v.dtype:
+            return f"{name} dtype {t.dtype} != v dtype {v.dtype}"
+        if t.device != dev:
+            return f"{name} on {t.device}, v on {dev}"
+    if state is not None:
+        if state.dtype != torch.float32:
+            return f"needs float32 state, got {state.dtype}"
+        if state.device != dev:
+            return f"state on {state.device}, v on {dev}"
+    return None
+
+
+def _size_reason(B: int, L: int, H: int, K: int, V: int) -> str | None:
+    """The kernels' limits (gated.hip args_status), repeated here so that supports() makes no library call."""
+    if not (1 <= K <= _MAX_WIDTH and 1 <= V <= _MAX_WIDTH):
+        return f"head widths K={K}, V={V} outside [1, {_MAX_WIDTH}]"
+    rows = max(B, 1)
+    too_many = H > 1 << 16 or L > 1 << 30 or rows > _MAX_GRID // H or rows * H > _MAX_GRID // 64
+    if too_many or rows * H * (-(-L // 64) + 8) > _MAX_GRID:
+        return f"B={B}, L={L}, H={H} needs more workgroups than one launch has"
+    return None
+
+
+def supports(q, k, v, g, state) -> str | None:
+    """Reason the fused recurrence cannot handle these tensors, or None if it can."""
+    reason = _tensor_reason(q, k, v, g, state)
+    if reason is not None:
+        return reason
+    B, L, H, V = v.shape
+    return _size_reason(B, L, H, q.shape[-1], V)
+
+
+def supports_step(q, k, v, g, state) -> str | None:
+    """Reason the fused step cannot handle these tensors, or None if it can."""
+    reason = _tensor_reason(q, k, v, g, state)
+    if reason is not None:
+        return reason
+    if not state.is_contiguous():
+        return "the state, updated in place, must be contiguous"
+    B, H, V = v.shape
+    K = q.shape[-1]
+    if not (1 <= K <= _STEP_MAX_K and V >= 1):
+        return f"head widths K={K}, V={V}: K must be in [1, {_STEP_MAX_K}]"
+    if V > 1 << 20 or H > 1 << 20 or B * H > _MAX_GRID // -(-V // 16):
+        return f"B={B}, H={H}, V={V} needs more workgroups than one launch has"
+    return None
+
+
+def _dense(t):
+    """``t`` with a dense last dimension, the only one the kernels read without a stride."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(*ts):
+    """The leading strides of q, k, v .. [.., width] and of g (three each; two in a step), as a C array."""
+    s = [n for t, dims in ts for n in t.stride()[:dims]]
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def _workspace(nbytes: int, t):
+    return None if nbytes == 0 else _lib.workspace(nbytes, t.device)
+
+
+def _screen(v, *others):
+    if v.device.type != "cuda" or v.dtype not in _IO_DTYPES:
+        raise TypeError(f"v: {v.dtype} on {v.device}, expected float32 or bfloat16 on a GPU")
+    for name, t in others:
+        if t.dtype != v.dtype or t.device != v.device:
+            raise TypeError(f"{name}: {t.dtype} on {t.device}, expected {v.dtype} on {v.device}")
+
+
+@custom_op("tsfast_hip::gated_recurrence")
+def _recurrence_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor | None
+) -> tuple[torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    _screen(v, ("q", q), ("k", k), ("g", g))
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    state = None if state is None else state.contiguous()
+    _lib.require(state, "state", (torch.float32,), v.device)
+    B, L, H, V = v.shape
+    Hk, K = q.shape[2:]
+    o = torch.empty(B, L, H, V, device=v.device, dtype=v.dtype)
+    last = torch.empty(B, H, K, V, device=v.device, dtype=torch.float32)
+    io = _IO_DTYPES[v.dtype]
+    nbytes = lib.tsfast_hip_gated_fwd_workspace_bytes(B, L, H, Hk, K, V, io)
+    ws = _workspace(nbytes, v)
+    _lib.check(
+        lib.tsfast_hip_gated_fwd(
+            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g)), _strides((q, 3), (k, 3), (v, 3), (g, 3)),
+            *map(_lib.ptr, (state, o, last, ws)), nbytes, _lib.stream_of(v),
+        ),
+        "tsfast_hip_gated_fwd",
+    )
+    return o, last
+
+
+@_recurrence_op.register_fake
+def _(q, k, v, g, state):
+    B, L, H, V = v.shape
+    return v.new_empty(B, L, H, V), v.new_empty(B, H, q.shape[-1], V, dtype=torch.float32)
+
+
+@custom_op("tsfast_hip::gated_recurrence_bwd")
+def _recurrence_bwd_op(
+    go: torch.Tensor,
+    glast: torch.Tensor | None,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    state: torch.Tensor | None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    _screen(v, ("q", q), ("k", k), ("g", g), ("go", go))
+    q, k, v, go = _dense(q), _dense(k), _dense(v), _dense(go)
+    state, glast = (None if t is None else t.contiguous() for t in (state, glast))
+    _lib.require(state, "state", (torch.float32,), v.device)
+    _lib.require(glast, "glast", (torch.float32,), v.device)
+    B, L, H, V = v.shape
+    Hk, K = q.shape[2:]
+    gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    gg = torch.empty(B, L, H, device=v.device, dtype=v.dtype)
+    gstate = None if state is None else torch.empty_like(state)
+    io = _IO_DTYPES[v.dtype]
+    nbytes = lib.tsfast_hip_gated_bwd_workspace_bytes(B, L, H, Hk, K, V, io)
+    ws = _workspace(nbytes, v)
+    _lib.check(
+        lib.tsfast_hip_gated_bwd(
+            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g, go)), _strides((q, 3), (k, 3), (v, 3), (g, 3), (go, 3)),
+            *map(_lib.ptr, (state, glast, gq, gk, gv, gg, gstate, ws)), nbytes, _lib.stream_of(v),
+        ),
+        "tsfast_hip_gated_bwd",
+    )
+    return gq, gk, gv, gg, (gstate if gstate is not None else v.new_empty(0, dtype=torch.float32))
+
+
+@_recurrence_bwd_op.register_fake
+def _(go, glast, q, k, v, g, state):
+    outs = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, g))
+    return (*outs, torch.empty(0 if state is None else state.shape, device=v.device, dtype=torch.float32))
+
+
+def _setup(ctx, inputs, output):
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(*inputs)
+
+
+def _backward(ctx, go, glast):
+    q, k, v, g, state = ctx.saved_tensors
+    if go is None:
+        go = torch.zeros_like(v)
+    gq, gk, gv, gg, gstate = _recurrence_bwd_op(go, glast, q, k, v, g, state)
+    return gq, gk, gv, gg, (gstate if state is not None else None)
+
+
+_recurrence_op.register_autograd(_backward, setup_context=_setup)
+
+
+def run(q, k, v, g, state):
+    """The fused recurrence: ``(o [B, L, H, V], last state [B, H, K, V] float32)``."""
+    return _recurrence_op(q, k, v, g, state)
+
+
+@custom_op("tsfast_hip::gated_recurrence_step", mutates_args=("state",))
+def _step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+    lib = _lib.load()
+    _screen(v, ("q", q), ("k", k), ("g", g))
+    _lib.require(state, "state", (torch.float32,), v.device)
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    B, H, V = v.shape
+    Hk, K = q.shape[1:]
+    o = torch.empty(B, H, V, device=v.device, dtype=v.dtype)
+    _lib.check(
+        lib.tsfast_hip_gated_step(
+            B, H, Hk, K, V, _IO_DTYPES[v.dtype], *map(_lib.ptr, (q, k, v, g)), _strides((q, 2), (k, 2), (v, 2), (g, 2)),
+            _lib.ptr(state), _lib.ptr(o), _lib.stream_of(v),
+        ),
+        "tsfast_hip_gated_step",
+    )
+    return o
+
+
+@_step_op.register_fake
+def _(q, k, v, g, state):
+    return v.new_empty(v.shape)
+
+
+def step(q, k, v, g, state):
+    """One fused step; ``state`` is updated in place. Returns ``o [B, H, V]``."""
+    return _step_op(q, k, v, g, state)

@@ -15,8 +15,11 @@ from __future__ import annotations
 
 __all__ = ["custom_op"]
 
+import inspect
+
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 # bound once: every call asks all of these (the lookups were 0.5 us of a call of four tensors)
 _dispatch_keys = torch._C._dispatch_keys
@@ -29,6 +32,8 @@ _registered = torch.library._impls  # what Python code has registered on any op,
 # dispatch keys of a plain dense GPU tensor (made in and outside inference mode); any other key
 # (conjugate or negative views, subclasses, functional, sparse, nested, batched ..) needs the dispatcher
 _plain_keys: set[int] = set()
+_NUMBER_TYPES = (int, float, bool)
+_NUMBERS = (*_NUMBER_TYPES, "int", "float", "bool")  # as annotations, evaluated or not
 
 
 def _keys_of_plain(device: torch.device) -> set[int]:
@@ -64,9 +69,13 @@ def _unobserved() -> bool:
 class _Op:
     """A registered custom op and its direct form; see ``custom_op``."""
 
-    def __init__(self, name: str, fn):
+    def __init__(self, name: str, fn, mutates_args=()):
         self._fn = fn
-        self._def = torch.library.custom_op(name, fn, mutates_args=())
+        self._def = torch.library.custom_op(name, fn, mutates_args=mutates_args)
+        names = inspect.signature(fn).parameters
+        # positions of plain numbers and of tensors written in place
+        self._numbers = frozenset(i for i, p in enumerate(names.values()) if p.annotation in _NUMBERS)
+        self._written = tuple(i for i, n in enumerate(names) if n in mutates_args)
         ns, op = name.split("::")
         self._op = getattr(getattr(torch.ops, ns), op).default
         self._function = self._backward = None
@@ -107,8 +116,8 @@ class _Op:
         if kwargs or torch.compiler.is_compiling() or not _unobserved() or self._overridden():
             return self._op(*args, **kwargs)
         wants_grad = False
-        for t in args:
-            if t is None:
+        for i, t in enumerate(args):
+            if t is None or (i in self._numbers and type(t) in _NUMBER_TYPES):
                 continue
             if not _plain(t):  # also what is no tensor: the dispatcher takes or refuses it (a proxy of a trace ..)
                 return self._op(*args)
@@ -116,10 +125,15 @@ class _Op:
         if wants_grad and torch.is_grad_enabled():
             # an op without rules (a backward's) says so itself when it is differentiated
             return self._op(*args) if self._function is None else self._function.apply(*args)
-        return self._fn(*args)
+        out = self._fn(*args)
+        for i in self._written:  # what the dispatcher does: a graph that saved the tensor finds out
+            if args[i] is not None and not args[i].is_inference():
+                increment_version(args[i])
+        return out
 
 
-def custom_op(name: str):
-    """Decorator: register ``fn`` as the custom op ``name`` (no argument mutated) and return it in
-    the form described above, with ``register_fake`` and ``register_autograd``."""
-    return lambda fn: _Op(name, fn)
+def custom_op(name: str, mutates_args=()):
+    """Decorator: register ``fn`` as the custom op ``name`` (which writes the named arguments in place,
+    none by default) and return it in the form described above, with ``register_fake`` and
+    ``register_autograd``. Besides tensors, ``fn`` may take numbers annotated ``int``, ``float`` or ``bool``."""
+    return lambda fn: _Op(name, fn, mutates_args)
