@@ -12,8 +12,8 @@
 //   out_i = sum_j D x_i . y_j z_j     forward in time (j <= i):   o (q, k, v),  dq (do, v, k)
 //                                     backward in time (j >= i):  dv (k, q, do), dk (v, do, q)
 //
-// so one kernel, walk_kernel, computes all four. A workgroup owns one head of one row, a tile of FT of z's
-// columns and a run of 64-step chunks; the state tile stays in fp32 accumulator registers from the first
+// so one kernel, walk_kernel, computes all four. A workgroup owns one head of one row and a run of 64-step chunks; the
+// state stays in fp32 accumulator registers from the first
 // chunk to the last and is never written in between. Per chunk the decayed scores of x and y within
 // it (64 x 64, the causal half only) times z, x times the state before it, and the state's update are MFMA
 // products; the decays come from exact differences of a float64 running sum, so any g <= 0 down to -inf
@@ -32,8 +32,7 @@ using namespace tsf;
 namespace {
 
 constexpr int kC = 64;          // steps of a chunk
-constexpr int kThreads = 256;   // four waves; wave w owns the chunk's steps 16 w .. 16 w + 15
-constexpr int kFT = 64;         // columns of z a workgroup owns
+constexpr int kThreads = 256;   // of the small kernels
 constexpr int kMaxWidth = 128;  // of K and V
 constexpr int kStepMaxK = 1024;  // of K in a single step
 constexpr int kMaxGrid = (1 << 24) - 1;
@@ -43,8 +42,10 @@ constexpr double kNoDecayLeft = -300.0;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), may_alias));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2), may_alias));
 
 // An operand of a 16 x 16 product: 8 values of one row along the contraction, which lane group
 // lane >> 4 holds; the row is lane & 15. Both operands have the same layout, so any order of the
@@ -95,27 +96,31 @@ TSF_DEV void split(const float* x, Frag<T>* out) {
   }
 }
 
-// Eight consecutive values of a row of global memory at any alignment; `n` of them exist.
-TSF_DEV void load8(Frag<bf16>& f, const bf16* p, int n) {
-  if (n >= 8) {
-    __builtin_memcpy(&f.v, p, 16);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f.v[e] = (__bf16)0.0f;
-      if (e < n) f.v[e] = __builtin_bit_cast(__bf16, p[e].bits);
-    }
-  }
+// Eight consecutive values of a row of global memory at any alignment.
+TSF_DEV void load8(Frag<bf16>& f, const bf16* p) { __builtin_memcpy(&f.v, p, 16); }
+TSF_DEV void load8(Frag<float>& f, const float* p) {
+  __builtin_memcpy(&f.lo, p, 16);
+  __builtin_memcpy(&f.hi, p + 4, 16);
 }
-TSF_DEV void load8(Frag<float>& f, const float* p, int n) {
-  if (n >= 8) {
-    __builtin_memcpy(&f.lo, p, 16);
-    __builtin_memcpy(&f.hi, p + 4, 16);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) put(f, e, e < n ? p[e] : 0.0f);
-  }
+// The first n of a row's last values (any n: none, or all eight), zeros after, where there are eight values in a row: f was
+// read so that it ends with the row.
+TSF_DEV void fit(Frag<bf16>& f, int n) {
+  const int s = n >= 8 ? 0 : n <= 0 ? 8 : 8 - n;  // places to move by
+  u32x4 v = __builtin_bit_cast(u32x4, f.v);
+  if (s & 1) v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+  if (s & 2) v = u32x4{v[1], v[2], v[3], 0};
+  if (s & 4) v = u32x4{v[2], v[3], 0, 0};
+  if (s & 8) v = u32x4{0, 0, 0, 0};
+  f.v = __builtin_bit_cast(bf16x8, v);
 }
+TSF_DEV void fit(Frag<float>& f, int n) {
+  const int s = n >= 8 ? 0 : n <= 0 ? 8 : 8 - n;
+  if (s & 1) f.lo = f32x4{f.lo[1], f.lo[2], f.lo[3], f.hi[0]}, f.hi = f32x4{f.hi[1], f.hi[2], f.hi[3], 0.0f};
+  if (s & 2) f.lo = f32x4{f.lo[2], f.lo[3], f.hi[0], f.hi[1]}, f.hi = f32x4{f.hi[2], f.hi[3], 0.0f, 0.0f};
+  if (s & 4) f.lo = f.hi, f.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (s & 8) f.lo = f.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
 // Four consecutive values of a row of global memory at any alignment; `n` of them exist.
 TSF_DEV void store4(float* p, f32x4 v, int n) {
   if (n >= 4) {
@@ -138,30 +143,34 @@ TSF_DEV void store4(bf16* p, f32x4 v, int n) {
       if (e < n) p[e] = h[e];
   }
 }
-TSF_DEV f32x4 load4(const float* p, int n) {
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+// Four consecutive values of a row of global memory, as they are; `n` of them exist, the others are some value of the row.
+template <typename T>
+struct Four {
+  T v[4];
+};
+template <typename T>
+TSF_DEV void load4(Four<T>& f, const T* p, int n) {
   if (n >= 4) {
-    __builtin_memcpy(&v, p, 16);
+    __builtin_memcpy(&f, p, sizeof(f));
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) v[e] = p[e];
+    for (int e = 0; e < 4; ++e) f.v[e] = p[e < n ? e : 0];
   }
+}
+template <typename T>
+TSF_DEV f32x4 load4(const T* p, int n) {
+  Four<T> h;
+  load4(h, p, n);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(h.v[e]) : 0.0f;
   return v;
 }
-TSF_DEV f32x4 load4(const bf16* p, int n) {
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  bf16 h[4];
-  if (n >= 4) {
-    __builtin_memcpy(h, p, 8);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = to_f32(h[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) v[e] = to_f32(p[e]);
-  }
-  return v;
+
+// An element by a 32-bit index from an address that all lanes share.
+template <typename T>
+TSF_DEV T* at32(T* base, uint32_t idx) {
+  return (T*)((char*)base + idx * (uint32_t)sizeof(T));
 }
 
 // A sequence tensor: strides in elements of the batch row, the step and the head; `share` heads of the
@@ -171,7 +180,7 @@ struct Seq {
   T* p;
   int64_t sb, sl, sh;
   int share;
-  TSF_DEV T* row(int64_t b, int64_t t, int h) const { return p + b * sb + t * sl + (int64_t)(h / share) * sh; }
+  TSF_DEV T* head(int64_t b, int h) const { return p + b * sb + (int64_t)(h / share) * sh; }
 };
 
 template <typename T, typename OT>
@@ -180,47 +189,152 @@ struct WalkArgs {
   Seq<OT> out;
   int H, E, F;       // heads, columns of x and y, columns of z
   int64_t L, units;  // steps; rows x heads x segments
-  int nft, nseg, seg_chunks;
-  int se, sf;                // strides of a state's element (e, f)
-  const float* init;         // state entering each unit [row x head (x segment)][K V]; null: zero
-  int init_per_seg;          // whether init holds one for each segment
-  float* last;               // state leaving: of the row, [row x head][K V], or of the segment (state_only)
-  double* seg_decay;         // state_only: log2 of the segment's decay
-  Seq<const T> dot;          // out_i . dot_i is summed over this tile's columns ..
-  float* dots;               // .. into [tile][row x head][L]
-  float* anchors;            // states before every anchor chunk [row x head][anchor][K V]: written forward, read backward
-  float* anchor_dots;        // backward: <state, anchor> over this tile [tile][row x head][anchor]
+  int nseg, seg_chunks;
+  int se, sf;             // strides of a caller's state's element (e, f)
+  const float* init;      // state entering the row [row x head][K V], or null: zero
+  const f32x4* seg_init;  // state entering each unit, where rows are cut
+  float* last;            // state leaving the row
+  f32x4* seg_last;        // STATE_ONLY: state leaving each unit
+  double* seg_decay;      // STATE_ONLY: log2 of the unit's decay
+  Seq<const T> dot;       // out_i . dot_i is summed over columns ..
+  float* dots;            // .. into [row x head][L]
+  f32x4* anchors;         // states before every anchor chunk [row x head][anchor]: written forward, read backward
+  float* anchor_dots;     // backward: <state, anchor> over a wave's columns [wave][row x head][anchor]
   int anchor_chunks, nanchor;
 };
 
-template <typename T, int E>
-struct Lds {
+// 16 and 8 bytes of LDS as one access
+template <int N>
+TSF_DEV void lds_get(void* to, const char* p) {
+  if constexpr (N == 16) {
+    const u32x4 v = *(const u32x4*)p;
+    __builtin_memcpy(to, &v, 16);
+  } else {
+    const u32x2 v = *(const u32x2*)p;
+    __builtin_memcpy(to, &v, 8);
+  }
+}
+template <int N>
+TSF_DEV void lds_put(char* p, const void* from) {
+  if constexpr (N == 16) {
+    u32x4 v;
+    __builtin_memcpy(&v, from, 16);
+    *(u32x4*)p = v;
+  } else {
+    u32x2 v;
+    __builtin_memcpy(&v, from, 8);
+    *(u32x2*)p = v;
+  }
+}
+
+// LDS arrays are rows of 16-byte units; unit u of row r stands at u ^ turn(r), so that 16 rows' same unit, and
+// 16 columns of four rows, fall on different banks. x, y and the scores are operands over their columns: a
+// unit pair (fp32) or a unit (bf16) holds one operand's 8 values, columns 32 s + 16 h + 4 lg + q in the order (h, q)
+// for lane group lg, the order accumulators have them in. Rows are 128 bytes or more and a turn is below 16, so what
+// selects s or t below is an exclusive or with a constant on a lane's own offset.
+template <typename T, int COLS>
+struct Rows {
   static constexpr bool kBf = sizeof(T) == 2;
-  static constexpr int kRow = E + (kBf ? 8 : 4);  // pitch of Y and S rows: 16 bytes of padding against bank conflicts
-  static constexpr int kCol = kC + 8;             // pitch of the transposed rows (bf16)
-  static constexpr int kZRow = kFT + 4;           // pitch of z's rows (fp32)
-  static constexpr int kSplit = kBf ? 2 : 1;      // operands the state is split into
-  T y[kC * kRow];
-  T yt[kBf ? E * kCol : 1];
-  T z[kBf ? kFT * kCol : kC * kZRow];
-  T s[kSplit][kFT * kRow];
-  float hi[2][kC], lo[2][kC], w[2][kC], in[2][kC];  // running log2 decay, weights into the state and out of it
+  static constexpr int kBytes = COLS * (int)sizeof(T), kUnits = kBytes / 16, kHalf = 4 * (int)sizeof(T);
+  alignas(16) char at[kC * kBytes];
+  TSF_DEV static uint32_t turn(uint32_t r) {
+    const uint32_t a = (r >> 2) & 3;
+    if constexpr (!kBf) return r & 15;
+    return (kUnits >= 16 ? (r & 3) << 2 : (r & 2) << 1) | ((a ^ (a << 1)) & 3);
+  }
+  // columns 8 m .. of row r (below 16), split into the two halves of operands; the offset of the first
+  TSF_DEV static uint32_t piece(uint32_t r, uint32_t m) {
+    if constexpr (kBf) return r * kBytes + ((((m >> 2) * 4 + (m & 1) * 2) ^ turn(r)) << 4) + ((m >> 1) & 1) * 8;
+    return r * kBytes + (((2 * m) ^ turn(r)) << 4);
+  }
+  TSF_DEV void put_piece(uint32_t off, int row16, const Frag<T>& f) {
+    char* p = at + row16 * 16 * kBytes;
+    lds_put<kHalf>(p + off, &f);
+    lds_put<kHalf>(p + (off ^ 16), (const char*)&f + kHalf);
+  }
+  // columns 8 m .. of row r (below 16) in their own order (z)
+  TSF_DEV static uint32_t plain(uint32_t r, uint32_t m) { return kBf ? r * kBytes + ((m ^ turn(r)) << 4) : piece(r, m); }
+  TSF_DEV void put_plain(uint32_t off, int row16, const Frag<T>& f) {
+    if constexpr (kBf)
+      lds_put<16>(at + row16 * 16 * kBytes + off, &f);
+    else
+      put_piece(off, row16, f);
+  }
+  // operands whose row is row 16 t + li, over columns 32 s ..: the lane's offset, and the operand
+  TSF_DEV static uint32_t row_lane(uint32_t li, uint32_t lg) { return li * kBytes + ((lg ^ turn(li)) << 4); }
+  TSF_DEV Frag<T> row(uint32_t lane_off, int t, int s) const {
+    Frag<T> f;
+    const char* p = at + t * 16 * kBytes;
+    if constexpr (kBf) {
+      lds_get<16>(&f, p + (lane_off ^ (s << 6)));
+    } else {
+      lds_get<16>(&f.lo, p + (lane_off ^ (s << 7)));
+      lds_get<16>(&f.hi, p + (lane_off ^ (s << 7 | 64)));
+    }
+    return f;
+  }
+  // four columns 16 jt + 4 lg .. of row 16 t + li, as accumulators have them
+  TSF_DEV void put_four(uint32_t lane_off, int t, int jt, const Frag<T>& f) {
+    char* p = at + t * 16 * kBytes;
+    if constexpr (kBf)
+      lds_put<8>(p + (lane_off ^ ((jt >> 1) << 6)) + 8 * (jt & 1), &f);
+    else
+      lds_put<16>(p + (lane_off ^ (jt << 6)), &f);
+  }
+  // operands whose row is column 16 t + li and whose contraction runs over rows (steps) 32 half ..; OPERAND: columns are in
+  // operand order. bf16: the transposing read, in which lane li of a group of 16 points at 4 columns of row li / 4 and
+  // receives its own column of the 4 rows.
+  template <bool OPERAND>
+  TSF_DEV static uint32_t col_lane(uint32_t li, uint32_t lg) {
+    const uint32_t r = 4 * lg + (li >> 2), m = li & 3;
+    if constexpr (kBf) return r * kBytes + (((OPERAND ? m : m >> 1) ^ turn(r)) << 4) + (OPERAND ? 0 : 8 * (m & 1));
+    return 0;
+  }
+  template <bool OPERAND>
+  TSF_DEV Frag<T> col(uint32_t lane_off, int t, int half, uint32_t li, uint32_t lg) const {
+    Frag<T> f;
+    if constexpr (kBf) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const char* p = at + (32 * half + 16 * h) * kBytes + (OPERAND ? (lane_off ^ ((t >> 1) << 6)) + 8 * (t & 1) : (lane_off ^ (t << 5)));
+        const auto w = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
+                                                     __attribute__((address_space(3))) char*)const_cast<char*>(p)));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f.v[4 * h + q] = w[q];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t r = 4 * lg + (e & 3);
+        put(f, e, *(const float*)(at + (32 * half + 16 * (e >> 2)) * kBytes + r * kBytes + (((4 * t + (li >> 2)) ^ turn(r)) << 4) + 4 * (li & 3)));
+      }
+    }
+    return f;
+  }
 };
 
-// Where step j of a chunk stands in a transposed row: an operand's 8 values (lane group lg, 32-step half s)
-// are steps 32 s + 16 h + 4 lg + q in the order (h, q), the order the score tiles leave them in registers.
-TSF_HOST_DEV int place(int j) { return (j & 32) + ((j >> 2) & 3) * 8 + ((j >> 4) & 1) * 4 + (j & 3); }
+template <typename T, int E, int NW>
+struct Lds {
+  static constexpr int kSplit = sizeof(T) == 2 ? 2 : 1;  // operands the state and the scores are split into
+  Rows<T, E> x, y;
+  Rows<T, 16 * NW> z;
+  Rows<T, kC> p[kSplit];                                        // decayed scores, row i
+  alignas(16) float hi[2][kC], lo[2][kC], w[2][kC], in[2][kC];  // running log2 decay, weights into the state and out of it
+  float dot[NW][kC];
+};
+
+// Waves a SIMD holds of a walk: what LDS and a 512-register file allow.
+template <typename T>
+constexpr int walk_waves(int E, int NW) {
+  return sizeof(T) == 2 ? (NW == 8 ? 4 : 2) : E == 64 && NW == 4 ? 2 : NW / 4;
+}
 
 // One wave: the chunk's running log2 decay as float pairs (differences are exact to float64 rounding), the
 // weight of each step in the state leaving the chunk, and of the state entering it at each step.
-template <typename T, int E, bool FWD, typename A>
-TSF_DEV void gates(Lds<T, E>& s, int buf, const A& a, int64_t b, int h, int64_t t0, int lane) {
-  double G = 0.0;
-  const int64_t t = t0 + lane;
-  if (t < a.L) {
-    const double x = (double)to_f32(*a.g.row(b, t, h)) * 1.4426950408889634;
-    G = x < kNoDecayLeft ? kNoDecayLeft : x;  // NaN stays
-  }
+template <bool FWD, typename S>
+TSF_DEV void gates(S& s, int buf, float g, int lane) {
+  const double x = (double)g * 1.4426950408889634;
+  double G = x < kNoDecayLeft ? kNoDecayLeft : x;  // NaN stays
 #pragma unroll
   for (int d = 1; d < kC; d <<= 1) {
     const double up = __shfl_up(G, d, kWave);
@@ -235,47 +349,11 @@ TSF_DEV void gates(Lds<T, E>& s, int buf, const A& a, int64_t b, int h, int64_t 
   s.w[buf][lane] = FWD ? to : from;
 }
 
-// Operand (row, k): 8 values at k of a row-major LDS array.
-template <typename T>
-TSF_DEV Frag<T> lds_row(const T* p) {
-  Frag<T> f;
-  __builtin_memcpy(&f, __builtin_assume_aligned(p, 16), sizeof(f));
-  return f;
+// Hides from the compiler that a value is the one of the last iteration.
+template <typename V>
+TSF_DEV void again(V& v) {
+  asm volatile("" : "+v"(v));
 }
-// Operand whose row is a column of y or z and whose contraction runs over steps (half s, lane group lg).
-TSF_DEV Frag<bf16> lds_col(const bf16* t, int pitch, int col, int s, int lg) { return lds_row(t + col * pitch + 32 * s + 8 * lg); }
-TSF_DEV Frag<float> lds_col(const float* t, int pitch, int col, int s, int lg) {
-  Frag<float> f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) put(f, e, t[(32 * s + 16 * (e >> 2) + 4 * lg + (e & 3)) * pitch + col]);
-  return f;
-}
-
-// A 4-step by 8-column piece of y or z on its way from global memory to LDS.
-template <typename T>
-struct Piece {
-  Frag<T> r[4];
-};
-template <typename T>
-TSF_DEV void fetch(Piece<T>& p, const Seq<const T>& q, int64_t b, int64_t t, int64_t L, int h, int col, int width) {
-#pragma unroll
-  for (int r = 0; r < 4; ++r) load8(p.r[r], q.row(b, t + r < L ? t + r : 0, h) + col, t + r < L ? width - col : 0);
-}
-template <typename T>
-TSF_DEV void lds_rows(T* dst, int pitch, int j, int col, const Piece<T>& p) {
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    __builtin_memcpy(__builtin_assume_aligned(dst + (j + r) * pitch + col, 16), &p.r[r], sizeof(Frag<T>));
-}
-TSF_DEV void lds_cols(bf16* dst, int pitch, int j, int col, const Piece<bf16>& p) {
-  const int at = place(j);
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    __bf16 v[4] = {p.r[0].v[c], p.r[1].v[c], p.r[2].v[c], p.r[3].v[c]};
-    __builtin_memcpy(__builtin_assume_aligned(dst + (col + c) * pitch + at, 8), v, 8);
-  }
-}
-TSF_DEV void lds_cols(float*, int, int, int, const Piece<float>&) {}
 
 TSF_DEV float wave_sum(float x) {
 #pragma unroll
@@ -283,269 +361,333 @@ TSF_DEV float wave_sum(float x) {
   return x;
 }
 
-// E: columns of x and y, padded; FWD: the direction in time; STATE_ONLY: only the state leaving the unit;
-// NU: operands the weighted y is split into in the state's update (bf16).
-template <typename T, typename OT, int E, bool FWD, bool STATE_ONLY, int NU>
-__global__ __launch_bounds__(kThreads, 2) void walk_kernel(WalkArgs<T, OT> a) {
-  using M = Lds<T, E>;
-  __shared__ M s;
-  constexpr int KS = E / 32, ET = E / 64, FN = kFT / 16, NS = M::kSplit;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
-  // tiles of one unit share x and y: they follow each other on one XCD (workgroups go round the 8 in turn)
-  const int slot = blockIdx.x >> 3;
-  const int64_t unit = (int64_t)(slot / a.nft) * 8 + (blockIdx.x & 7);
-  if (unit >= a.units) return;
-  const int f0 = (slot % a.nft) * kFT, ft_id = slot % a.nft;
+TSF_DEV f32x4 four(const float* p) {
+  f32x4 v;
+  lds_get<16>(&v, (const char*)p);
+  return v;
+}
+
+// E: columns of x and y, padded; NW: waves of a workgroup; FWD: the direction in time; STATE_ONLY: only the state leaving
+// the unit; NU: operands the weighted z is split into in the state's update.
+//
+// Wave w owns the state's columns 16 w + li, all E rows of them: accumulators S[et] hold rows 16 et + 4 lg + r, which
+// two by two are operands as they stand. Per chunk: (1) x, y, z to LDS; (2) the ten live 16 x 16 score tiles, shared
+// among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update.
+template <typename T, typename OT, int E, int NW, bool FWD, bool STATE_ONLY, int NU>
+__global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(WalkArgs<T, OT> a) {
+  constexpr int kThr = 64 * NW, FT = 16 * NW, KS = E / 32, ET = E / 16, NS = Lds<T, E, NW>::kSplit;
+  __shared__ Lds<T, E, NW> s;
+  int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes, as the compiler now knows
+  const int64_t unit = blockIdx.x;
   const int seg = (int)(unit % a.nseg);
   const int64_t bh = unit / a.nseg, b = bh / a.H, nbh = a.units / a.nseg;
   const int h = (int)(bh % a.H);
   const int nchunk = (int)((a.L + kC - 1) / kC);
-  const int c_lo = seg * a.seg_chunks, c_hi = min(nchunk, c_lo + a.seg_chunks);
-  const int64_t kv = (int64_t)a.E * a.F;
+  const int c_lo = seg * a.seg_chunks, chunks = min(nchunk, c_lo + a.seg_chunks) - c_lo;
+  const T *xh = a.x.head(b, h), *yh = a.y.head(b, h), *zh = a.z.head(b, h), *gh = a.g.head(b, h);
+  OT* const oh = STATE_ONLY ? nullptr : a.out.head(b, h);
+  const T* const dh = a.dots ? a.dot.head(b, h) : nullptr;
+  // the lane's places in the LDS arrays
+  uint32_t row_off = Rows<T, E>::row_lane(li, lg), p_off = Rows<T, kC>::row_lane(li, lg);
+  uint32_t ycol_off = Rows<T, E>::template col_lane<true>(li, lg), zcol_off = Rows<T, FT>::template col_lane<false>(li, lg);
 
-  // the state tile: wave w owns rows e = 16 (w ET + et) + 4 lg + r of columns f0 + 16 ft + li
-  f32x4 S[ET][FN];
-  const float* init = a.init ? a.init + (a.init_per_seg ? unit : bh) * kv : nullptr;
+  // The state. In the workspace (segments, anchors) a state is f32x4 [et][thread], padding included; the caller's
+  // are K V floats, (e, f) at e se + f sf.
+  f32x4 S[ET];
+  const int64_t kv = (int64_t)a.E * a.F;
+  auto each_state = [&](auto f) {  // value = f(index in a caller's state, value)
 #pragma unroll
-  for (int et = 0; et < ET; ++et)
-#pragma unroll
-    for (int ft = 0; ft < FN; ++ft)
+    for (int et = 0; et < ET; ++et)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int e = 16 * (wave * ET + et) + 4 * lg + r, f = f0 + 16 * ft + li;
-        S[et][ft][r] = init && e < a.E && f < a.F ? init[(int64_t)e * a.se + (int64_t)f * a.sf] : 0.0f;
-      }
-
-  auto state_to_lds = [&]() {
-#pragma unroll
-    for (int et = 0; et < ET; ++et)
-#pragma unroll
-      for (int ft = 0; ft < FN; ++ft) {
-        T* row = s.s[0] + (16 * ft + li) * M::kRow + 16 * (wave * ET + et) + 4 * lg;
-        f32x4 rest = S[et][ft];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          T v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            v[r] = from_f32<T>(rest[r]);
-            rest[r] -= to_f32(v[r]);
-          }
-          __builtin_memcpy(__builtin_assume_aligned(row + n * kFT * M::kRow, 4 * sizeof(T)), v, sizeof(v));
-        }
+        const int e = 16 * et + 4 * lg + r, col = 16 * wave + li;
+        if (e < a.E && col < a.F) S[et][r] = f((int64_t)e * a.se + (int64_t)col * a.sf, S[et][r]);
       }
   };
+#pragma unroll
+  for (int et = 0; et < ET; ++et) S[et] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (a.seg_init) {
+#pragma unroll
+    for (int et = 0; et < ET; ++et) S[et] = a.seg_init[(unit * ET + et) * kThr + threadIdx.x];
+  } else if (a.init) {
+    const float* init = a.init + bh * kv;
+    each_state([&](int64_t at, float) { return init[at]; });
+  }
 
-  // this thread's 4 x 8 pieces of y (E / 128 or half of one) and z
-  constexpr int YC = E / 8, YN = (kC / 4) * YC, ZC = kFT / 8, ZN = (kC / 4) * ZC;
-  constexpr int YP = (YN + kThreads - 1) / kThreads;
-  Piece<T> py[YP], pz;
+  // this thread's 8-column pieces of x, y and z on their way to LDS: one of every kRowsX (kRowsZ) rows
+  constexpr int XC = E / 8, kRowsX = kThr / XC, XP = kC / kRowsX, ZC = FT / 8, kRowsZ = kThr / ZC, ZP = kC / kRowsZ;
+  Frag<T> px[STATE_ONLY ? 1 : XP], py[XP], pz[ZP];
+  int xrow = threadIdx.x / XC, xcol = threadIdx.x % XC * 8, zrow = threadIdx.x / ZC, zcol = threadIdx.x % ZC * 8;
+  uint32_t x_lds = Rows<T, E>::piece(xrow & 15, xcol / 8) + (xrow >> 4) * 16 * Rows<T, E>::kBytes;
+  uint32_t z_lds = Rows<T, FT>::plain(zrow & 15, zcol / 8) + (zrow >> 4) * 16 * Rows<T, FT>::kBytes;
+  // A piece that ends beyond its row is read so that it ends with it, a row beyond the last step is read as the last one; what does
+  // not belong goes on the way to LDS. Rows of fewer than eight columns are read by elements then.
+  const bool exact = a.E == E && a.F == FT, narrow_x = a.E < 8, narrow_z = a.F < 8;
+  const uint32_t x_most = a.E - 8, z_most = a.F - 8;
   auto fetch_chunk = [&](int c) {
     const int64_t t0 = (int64_t)c * kC;
+    const int last = (int)min((int64_t)kC, a.L - t0) - 1;
+    const T *xb = xh + t0 * a.x.sl, *yb = yh + t0 * a.y.sl, *zb = zh + t0 * a.z.sl;  // the same for all lanes
+    if (!narrow_x) {
+      const uint32_t col = min((uint32_t)xcol, x_most);
 #pragma unroll
-    for (int p = 0; p < YP; ++p) {
-      const int id = p * kThreads + threadIdx.x;
-      if (id < YN) fetch(py[p], a.y, b, t0 + id / YC * 4, a.L, h, id % YC * 8, a.E);
+      for (int p = 0; p < XP; ++p) {
+        const uint32_t row = min(p * kRowsX + xrow, last);
+        load8(py[p], at32(yb, row * (uint32_t)a.y.sl + col));
+        if constexpr (!STATE_ONLY) load8(px[p], at32(xb, row * (uint32_t)a.x.sl + col));
+      }
     }
-    if (threadIdx.x < ZN) fetch(pz, a.z, b, t0 + threadIdx.x / ZC * 4, a.L, h, f0 + threadIdx.x % ZC * 8, a.F);
-  };
-  Frag<T> x[KS];
-  auto fetch_x = [&](int c) {
-    const int64_t t = (int64_t)c * kC + 16 * wave + li;
-    const T* p = a.x.row(b, t < a.L ? t : 0, h);
+    if (!narrow_z) {
+      const uint32_t col = min((uint32_t)zcol, z_most);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) load8(x[ks], p + 32 * ks + 8 * lg, t < a.L ? a.E - 32 * ks - 8 * lg : 0);
+      for (int p = 0; p < ZP; ++p) load8(pz[p], at32(zb, (uint32_t)min(p * kRowsZ + zrow, last) * (uint32_t)a.z.sl + col));
+    }
   };
-  constexpr int kGateWave = FWD ? 0 : 3;  // the wave with the fewest score tiles
+  auto fit_chunk = [&](int64_t t0) {
+    const int steps = (int)min((int64_t)kC, a.L - t0);
+    auto by_elements = [&](Frag<T>& f, const T* row, int col, int n) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) put(f, e, e < n ? to_f32(row[col + e]) : 0.0f);
+    };
+#pragma unroll
+    for (int p = 0; p < XP; ++p) {
+      const int row = p * kRowsX + xrow, n = row < steps ? a.E - xcol : 0;
+      if (narrow_x) {
+        by_elements(py[p], yh + (t0 + row) * a.y.sl, xcol, n);
+        if constexpr (!STATE_ONLY) by_elements(px[p], xh + (t0 + row) * a.x.sl, xcol, n);
+      } else {
+        fit(py[p], n);
+        if constexpr (!STATE_ONLY) fit(px[p], n);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < ZP; ++p) {
+      const int row = p * kRowsZ + zrow, n = row < steps ? a.F - zcol : 0;
+      if (narrow_z)
+        by_elements(pz[p], zh + (t0 + row) * a.z.sl, zcol, n);
+      else
+        fit(pz[p], n);
+    }
+  };
+  constexpr int kGateWave = NW - 1;  // one of those with the fewest score tiles
+  constexpr int kStep = FWD ? 1 : -1;
+  int c = FWD ? c_lo : c_lo + chunks - 1;
+  auto fetch_gate = [&](int n) {  // of the n-th chunk walked; a step that does not exist reads another
+    const int64_t t = (int64_t)(FWD ? c_lo + n : c_lo + chunks - 1 - n) * kC + lane;
+    return gh[(n < chunks && t < a.L ? t : 0) * a.g.sl];
+  };
+  auto gate_of = [&](int n, T g) { return (int64_t)(FWD ? c_lo + n : c_lo + chunks - 1 - n) * kC + lane < a.L ? to_f32(g) : 0.0f; };
 
   double log_decay = 0.0;
-  int c = FWD ? c_lo : c_hi - 1;
-  if (c_lo < c_hi) {
+  T g_next = from_f32<T>(0.0f);
+  if (chunks > 0) {
     fetch_chunk(c);
-    if (wave == kGateWave) gates<T, E, FWD>(s, 0, a, b, h, (int64_t)c * kC, lane);
+    if (wave == kGateWave) {
+      gates<FWD>(s, 0, gate_of(0, fetch_gate(0)), lane);
+      g_next = fetch_gate(1);
+    }
   }
-  if constexpr (!STATE_ONLY) state_to_lds();
+  if constexpr (!STATE_ONLY) {  // score tiles that no step reaches stay zero
+#pragma unroll
+    for (int m = 0; m < NS; ++m)
+      for (int i = threadIdx.x * 16; i < (int)sizeof(s.p[m].at); i += kThr * 16) *(u32x4*)(s.p[m].at + i) = u32x4{0, 0, 0, 0};
+  }
 
-  for (int n = 0; n < c_hi - c_lo; ++n, c += FWD ? 1 : -1) {
+  for (int n = 0; n < chunks; ++n, c += kStep) {
+    // what follows from these is formed again in each chunk: kept over the loop it would not fit the registers beside the state
+    again(lane), again(li), again(lg), again(row_off), again(p_off), again(ycol_off), again(zcol_off), again(x_lds), again(z_lds);
+    again(xrow), again(xcol), again(zrow), again(zcol);
     const int buf = n & 1;
-    if (FWD && !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0) {
-      float* to = a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * kv;
+    const int64_t t0 = (int64_t)c * kC;
+    const bool anchor = !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0;
+    f32x4* const anchor_at = anchor ? a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * ET * kThr + threadIdx.x : nullptr;
+    if (FWD && anchor)
 #pragma unroll
-      for (int et = 0; et < ET; ++et)
+      for (int et = 0; et < ET; ++et) anchor_at[et * kThr] = S[et];
+    if (!exact || t0 + kC > a.L) fit_chunk(t0);
 #pragma unroll
-        for (int ft = 0; ft < FN; ++ft)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 16 * (wave * ET + et) + 4 * lg + r, f = f0 + 16 * ft + li;
-            if (e < a.E && f < a.F) to[(int64_t)e * a.se + (int64_t)f * a.sf] = S[et][ft][r];
-          }
+    for (int p = 0; p < XP; ++p) {
+      s.y.put_piece(x_lds, p * kRowsX / 16, py[p]);
+      if constexpr (!STATE_ONLY) s.x.put_piece(x_lds, p * kRowsX / 16, px[p]);
     }
 #pragma unroll
-    for (int p = 0; p < YP; ++p) {
-      const int id = p * kThreads + threadIdx.x;
-      if (id < YN) {
-        if (!STATE_ONLY || !M::kBf) lds_rows(s.y, M::kRow, id / YC * 4, id % YC * 8, py[p]);
-        lds_cols(s.yt, M::kCol, id / YC * 4, id % YC * 8, py[p]);
-      }
-    }
-    if (threadIdx.x < ZN) {
-      if constexpr (M::kBf)
-        lds_cols(s.z, M::kCol, threadIdx.x / ZC * 4, threadIdx.x % ZC * 8, pz);
-      else
-        lds_rows(s.z, M::kZRow, threadIdx.x / ZC * 4, threadIdx.x % ZC * 8, pz);
-    }
-    if constexpr (!STATE_ONLY) fetch_x(c);
+    for (int p = 0; p < ZP; ++p) s.z.put_plain(z_lds, p * kRowsZ / 16, pz[p]);
     __syncthreads();
-    if (n + 1 < c_hi - c_lo) {
-      fetch_chunk(c + (FWD ? 1 : -1));
-      if (wave == kGateWave) gates<T, E, FWD>(s, buf ^ 1, a, b, h, (int64_t)(c + (FWD ? 1 : -1)) * kC, lane);
-    }
-    const float tot = FWD ? s.in[buf][kC - 1] : s.w[buf][kC - 1];  // the whole chunk's decay
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
+    f32x4 acc[4];  // outputs, transposed: columns f of z by steps i = 16 it + li
+    const int f = 16 * wave + 4 * lg;
     if constexpr (!STATE_ONLY) {
-      // scores, transposed: rows j = 16 jt + 4 lg + r, column i = 16 wave + li; P as operands over steps
-      const int i = 16 * wave + li;
-      const int64_t t = (int64_t)c * kC + i;
-      const float gi_hi = s.hi[buf][i], gi_lo = s.lo[buf][i], in = s.in[buf][i];
-      Frag<T> P[2][NS];
+      // decayed scores, transposed in registers: rows j = 16 jt + 4 lg + r, column i = 16 it + li
+#pragma unroll
+      for (int k = 0; k < (10 + NW - 1) / NW; ++k) {
+        const int id = wave + NW * k;
+        if (id < 10) {
+          const int big = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, small = id - big * (big + 1) / 2;
+          const int it = FWD ? big : 3 - big, jt = FWD ? small : 3 - small;
+          f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) sc = mma(s.y.row(row_off, jt, ks), s.x.row(row_off, it, ks), sc);
+          const f32x4 j_hi = four(s.hi[buf] + 16 * jt + 4 * lg), j_lo = four(s.lo[buf] + 16 * jt + 4 * lg);
+          const float i_hi = s.hi[buf][16 * it + li], i_lo = s.lo[buf][16 * it + li];
+          float part[8];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float d = (i_hi - j_hi[r]) + (i_lo - j_lo[r]);
+            const int j = 4 * lg + r;
+            const bool live = it != jt || (FWD ? j <= li : j >= li);
+            part[r] = live ? sc[r] * fast_exp2(FWD ? d : -d) : 0.0f;
+            part[r + 4] = 0.0f;
+          }
+          Frag<T> f4[NS];
+          split<T, NS>(part, f4);
+#pragma unroll
+          for (int m = 0; m < NS; ++m) s.p[m].put_four(p_off, it, jt, f4[m]);
+        }
+      }
+      // x times the state entering
+#pragma unroll
+      for (int it = 0; it < 4; ++it) acc[it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        Frag<T> sf[NS];
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = S[2 * ks + (e >> 2)][e & 3];
+        split<T, NS>(v, sf);
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const Frag<T> xf = s.x.row(row_off, it, ks);
+#pragma unroll
+          for (int m = 0; m < NS; ++m) acc[it] = mma(sf[m], xf, acc[it]);
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) acc[it] *= s.in[buf][16 * it + li];
+    }
+    if (wave == kGateWave && n + 1 < chunks) {
+      gates<FWD>(s, buf ^ 1, gate_of(n + 1, g_next), lane);
+      g_next = fetch_gate(n + 2);
+    }
+    if constexpr (!STATE_ONLY) __syncthreads();
+
+    if constexpr (!STATE_ONLY) {
+      // the scores times z, and the outputs
+      Four<T> u[4];
+      if (a.dots)
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const uint32_t row = min(16 * it + li, (int)min((int64_t)kC, a.L - t0) - 1);
+          const T* from = at32(dh + t0 * a.dot.sl, row * (uint32_t)a.dot.sl);
+          load4(u[it], f < a.F ? from + f : from, a.F - f);
+        }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float p[8];
+        const Frag<T> zf = s.z.template col<false>(zcol_off, wave, half, li, lg);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int jt = 2 * half + q;
-          f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (FWD ? jt <= wave : jt >= wave) {
+        for (int it = 0; it < 4; ++it)
+          if (FWD ? 2 * half <= it : 2 * half + 1 >= it)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) acc = mma(lds_row(s.y + (16 * jt + li) * M::kRow + 32 * ks + 8 * lg), x[ks], acc);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * jt + 4 * lg + r;
-            const float d = (gi_hi - s.hi[buf][j]) + (gi_lo - s.lo[buf][j]);
-            const bool live = FWD ? j <= i : j >= i;
-            p[4 * q + r] = live ? acc[r] * fast_exp2(FWD ? d : -d) : 0.0f;
-          }
-        }
-        split<T, NS>(p, P[half]);
+            for (int m = 0; m < NS; ++m) acc[it] = mma(zf, s.p[m].row(p_off, it, half), acc[it]);
       }
-      float dot = 0.0f;
 #pragma unroll
-      for (int ft = 0; ft < FN; ++ft) {
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int it = 0; it < 4; ++it) {
+        const int64_t ti = t0 + 16 * it;
+        const bool live = ti + li < a.L && f < a.F;
+        if (live) store4(at32(oh + ti * a.out.sl, li * (uint32_t)a.out.sl + f), acc[it], a.F - f);
+        if (a.dots) {
+          float dot = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int m = 0; m < NS; ++m) acc = mma(lds_row(s.s[m] + (16 * ft + li) * M::kRow + 32 * ks + 8 * lg), x[ks], acc);
-        acc *= in;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          if (FWD ? 2 * half <= wave : 2 * half + 1 >= wave) {
-            const Frag<T> zf = lds_col(s.z, M::kBf ? M::kCol : M::kZRow, 16 * ft + li, half, lg);
-#pragma unroll
-            for (int m = 0; m < NS; ++m) acc = mma(zf, P[half][m], acc);
-          }
-        const int f = f0 + 16 * ft + 4 * lg;
-        if (t < a.L && f < a.F) {
-          store4(a.out.row(b, t, h) + f, acc, a.F - f);
-          if (a.dots) {
-            const f32x4 u = load4(a.dot.row(b, t, h) + f, a.F - f);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) dot = fmaf(acc[r], u[r], dot);
-          }
+          for (int r = 0; r < 4; ++r) dot = fmaf(acc[it][r], live && f + r < a.F ? to_f32(u[it].v[r]) : 0.0f, dot);
+          dot += __shfl_xor(dot, 16, kWave);
+          dot += __shfl_xor(dot, 32, kWave);
+          if (lg == 0) s.dot[wave][16 * it + li] = dot;
         }
-      }
-      if (a.dots) {
-        dot += __shfl_xor(dot, 16, kWave);
-        dot += __shfl_xor(dot, 32, kWave);
-        if (lg == 0 && t < a.L) a.dots[((int64_t)ft_id * nbh + bh) * a.L + t] = dot;
       }
     }
+    if (n + 1 < chunks) fetch_chunk(c + kStep);
 
-    // the state: S = tot S + sum_j (w_j y_j) z_j^T
-    {
-      Frag<T> zf[FN][2];
+    // the state: S = tot S + sum_j y_j (w_j z_j)^T
+    const float tot = FWD ? s.in[buf][kC - 1] : s.w[buf][kC - 1];  // the whole chunk's decay
 #pragma unroll
-      for (int ft = 0; ft < FN; ++ft)
+    for (int half = 0; half < 2; ++half) {
+      const Frag<T> zf = s.z.template col<false>(zcol_off, wave, half, li, lg);
+      const f32x4 w0 = four(s.w[buf] + 32 * half + 4 * lg), w1 = four(s.w[buf] + 32 * half + 16 + 4 * lg);
+      Frag<T> zw[NU];
+      float v[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) zf[ft][half] = lds_col(s.z, M::kBf ? M::kCol : M::kZRow, 16 * ft + li, half, lg);
+      for (int e = 0; e < 8; ++e) v[e] = get(zf, e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
+      split<T, NU>(v, zw);
 #pragma unroll
       for (int et = 0; et < ET; ++et) {
+        const Frag<T> yf = s.y.template col<true>(ycol_off, et, half, li, lg);
+        if (half == 0) S[et] *= tot;
 #pragma unroll
-        for (int ft = 0; ft < FN; ++ft) S[et][ft] *= tot;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const Frag<T> yf = lds_col(M::kBf ? s.yt : s.y, M::kBf ? M::kCol : M::kRow, 16 * (wave * ET + et) + li, half, lg);
-          float wy[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) wy[e] = get(yf, e) * s.w[buf][32 * half + 16 * (e >> 2) + 4 * lg + (e & 3)];
-          Frag<T> yw[M::kBf ? NU : 1];
-          split<T, M::kBf ? NU : 1>(wy, yw);
-#pragma unroll
-          for (int ft = 0; ft < FN; ++ft)
-#pragma unroll
-            for (int m = 0; m < (M::kBf ? NU : 1); ++m) S[et][ft] = mma(yw[m], zf[ft][half], S[et][ft]);
-        }
+        for (int m = 0; m < NU; ++m) S[et] = mma(yf, zw[m], S[et]);
       }
     }
-    if (!FWD && !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0) {
-      const float* from = a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * kv;
+    if (!FWD && anchor) {
       float d = 0.0f;
 #pragma unroll
-      for (int et = 0; et < ET; ++et)
+      for (int et = 0; et < ET; ++et) {
+        const f32x4 from = anchor_at[et * kThr];
 #pragma unroll
-        for (int ft = 0; ft < FN; ++ft)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 16 * (wave * ET + et) + 4 * lg + r, f = f0 + 16 * ft + li;
-            if (e < a.E && f < a.F) d = fmaf(from[(int64_t)e * a.se + (int64_t)f * a.sf], S[et][ft][r], d);
-          }
+        for (int r = 0; r < 4; ++r) d = fmaf(from[r], S[et][r], d);
+      }
       d = wave_sum(d);
-      if (lane == 0) s.in[buf][16 * wave] = d;  // no other wave reads this step's weight
+      if (lane == 0) a.anchor_dots[((int64_t)wave * nbh + bh) * a.nanchor + c / a.anchor_chunks] = d;
     }
     __syncthreads();
-    if (!FWD && !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0 && threadIdx.x == 0)
-      a.anchor_dots[((int64_t)ft_id * nbh + bh) * a.nanchor + c / a.anchor_chunks] = (s.in[buf][0] + s.in[buf][16]) + (s.in[buf][32] + s.in[buf][48]);
-    if constexpr (!STATE_ONLY) state_to_lds();
+    if constexpr (!STATE_ONLY)
+      if (a.dots && wave == 0 && t0 + lane < a.L) {  // written again only after two more barriers
+        float dot = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) dot += s.dot[w][lane];
+        a.dots[bh * a.L + t0 + lane] = dot;
+      }
   }
 
-  const bool end = STATE_ONLY || seg == (FWD ? a.nseg - 1 : 0);
-  if (a.last && end) {
-    float* to = a.last + (STATE_ONLY ? unit : bh) * kv;
+  if constexpr (STATE_ONLY) {
 #pragma unroll
-    for (int et = 0; et < ET; ++et)
-#pragma unroll
-      for (int ft = 0; ft < FN; ++ft)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int e = 16 * (wave * ET + et) + 4 * lg + r, f = f0 + 16 * ft + li;
-          if (e < a.E && f < a.F) to[(int64_t)e * a.se + (int64_t)f * a.sf] = S[et][ft][r];
-        }
+    for (int et = 0; et < ET; ++et) a.seg_last[(unit * ET + et) * kThr + threadIdx.x] = S[et];
+    if (threadIdx.x == 0) a.seg_decay[unit] = log_decay;
+  } else if (a.last && seg == (FWD ? a.nseg - 1 : 0)) {
+    float* to = a.last + bh * kv;
+    each_state([&](int64_t at, float v) { return to[at] = v; });
   }
-  if constexpr (STATE_ONLY)
-    if (threadIdx.x == 0 && ft_id == 0) a.seg_decay[unit] = log_decay;
 }
 
-// Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards).
-__global__ __launch_bounds__(kThreads) void join_kernel(float* seg, const double* decay, const float* init, int nseg, int64_t kv, int64_t total,
-                                                        int backward) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+// Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards). `threads`
+// and `et` are the walk's; a thread owns one f32x4 of a state.
+__global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int E, int F, int se,
+                                                   int sf, int64_t total, int backward) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;
-  const int64_t bh = at / kv, e = at % kv;
-  float s = init ? init[at] : 0.0f;
+  const int per = threads * et;
+  const int64_t bh = at / per;
+  const int in = (int)(at % per), lane = in % threads & 63;
+  const int e = in / threads * 16 + (lane >> 4) * 4, col = in % threads / 64 * 16 + (lane & 15);
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (init && col < F)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (e + r < E) s[r] = init[bh * E * F + (int64_t)(e + r) * se + (int64_t)col * sf];
+  f32x4* p = seg + (bh * nseg + (backward ? nseg - 1 : 0)) * per + in;
+  const double* d = decay + bh * nseg + (backward ? nseg - 1 : 0);
+  const int64_t step = backward ? -(int64_t)per : per;
+#pragma unroll 4
   for (int n = 0; n < nseg; ++n) {
-    const int64_t unit = bh * nseg + (backward ? nseg - 1 - n : n);
-    const float own = seg[unit * kv + e];
-    seg[unit * kv + e] = s;
-    s = fmaf(fast_exp2((float)decay[unit]), s, own);
+    const f32x4 own = p[n * step];
+    p[n * step] = s;
+    s = fast_exp2((float)d[backward ? -n : n]) * s + own;
   }
 }
 
 // dg over one anchor's steps: the anchor's value, then the running sum of c - r before each step.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dgate_kernel(const float* r, const float* c, const float* anchor_dots, Seq<const T> g, Seq<T> dg, int H,
-                                                         int64_t L, int64_t nbh, int nft, int anchor_steps, int nanchor) {
+                                                         int64_t L, int64_t nbh, int parts, int anchor_steps, int nanchor) {
   __shared__ float part[4];
   const int64_t bh = blockIdx.x / nanchor;
   const int anchor = (int)(blockIdx.x % nanchor);
@@ -553,16 +695,12 @@ __global__ __launch_bounds__(kThreads) void dgate_kernel(const float* r, const f
   const int h = (int)(bh % H);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float base = 0.0f;
-  for (int f = 0; f < nft; ++f) base += anchor_dots[((int64_t)f * nbh + bh) * nanchor + anchor];
+  for (int f = 0; f < parts; ++f) base += anchor_dots[((int64_t)f * nbh + bh) * nanchor + anchor];
   for (int o = 0; o < anchor_steps; o += kThreads) {
     const int64_t t = (int64_t)anchor * anchor_steps + o + threadIdx.x;
     const bool in = o + (int)threadIdx.x < anchor_steps && t < L;
     float v = 0.0f;
-    if (in)
-      for (int f = 0; f < nft; ++f) {
-        const int64_t at = ((int64_t)f * nbh + bh) * L + t;
-        v += c[at] - r[at];
-      }
+    if (in) v = c[bh * L + t] - r[bh * L + t];
     float sum = v;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
@@ -575,8 +713,8 @@ __global__ __launch_bounds__(kThreads) void dgate_kernel(const float* r, const f
     for (int w = 0; w < wave; ++w) before += part[w];
     if (in) {
       // where exp(g) is zero in fp32 the gradient is, whatever the sums' rounding left
-      const bool none = to_f32(*g.row(b, t, h)) < -104.0f;
-      *dg.row(b, t, h) = from_f32<T>(none ? 0.0f : before + (sum - v));
+      const bool none = to_f32(g.head(b, h)[t * g.sl]) < -104.0f;
+      dg.head(b, h)[t * dg.sl] = from_f32<T>(none ? 0.0f : before + (sum - v));
     }
     for (int w = 0; w < 4; ++w) base += part[w];
     __syncthreads();
@@ -667,17 +805,21 @@ int args_status(const Sizes& s, int dtype) {
   return TSF_OK;
 }
 
-int tiles(int64_t width) { return (int)((width + kFT - 1) / kFT); }
+// Waves of a walk over F columns: a workgroup takes all of them, so that nothing of x and y is done twice.
+int waves(int64_t F) { return F <= 64 ? 4 : 8; }
 
-// Segments a row is cut into: enough workgroups for two on each CU, segments of four chunks at least.
-int segments(const Sizes& s, int nft) {
-  const int64_t chunks = (s.L + kC - 1) / kC, wgs = s.B * s.H * nft;
-  int64_t n = wgs > 0 ? (2 * (int64_t)device_cus() + wgs - 1) / wgs : 1;
+// Segments a row is cut into. A cut row is walked twice (its segments' states first), so rows are cut only to give
+// every CU its two workgroups, into no more than fit at once and into four chunks at least.
+int segments(const Sizes& s) {
+  const int64_t chunks = (s.L + kC - 1) / kC, rows = s.B * s.H;
+  int64_t n = rows > 0 ? 2 * (int64_t)device_cus() / rows : 1;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   const int64_t per = (chunks + n - 1) / n;
   return per > 0 ? (int)((chunks + per - 1) / per) : 1;
 }
+
+int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
 
 // Chunks between dg's anchors: an anchor's states cost 8 bytes a state element, the running sum's errors
 // grow with the root of the distance; fp32 gates want the smaller error.
@@ -692,24 +834,22 @@ struct Space {
 Space space(const Sizes& s, int dtype, bool backward) {
   Space w = {};
   int64_t at = 0;
-  const int64_t bh = s.B * s.H, kv = s.K * s.V;
-  int nseg = segments(s, tiles(s.V));
-  if (backward && segments(s, tiles(s.K)) > nseg) nseg = segments(s, tiles(s.K));
+  const int64_t bh = s.B * s.H, state = padded_state(s.K, s.V) * 4, nseg = segments(s);
   auto take = [&](int64_t n) {
     const int64_t p = at;
     at += align_up(n);
     return p;
   };
   if (nseg > 1) {
-    w.seg = take(bh * nseg * kv * 4);
+    w.seg = take(bh * nseg * state);
     w.decay = take(bh * nseg * 8);
   }
   if (backward) {
-    const int64_t chunks = (s.L + kC - 1) / kC, ac = anchor_chunks(dtype), na = (chunks + ac - 1) / ac, nk = tiles(s.K);
-    w.r = take(nk * bh * s.L * 4);
-    w.c = take(nk * bh * s.L * 4);
-    w.anchors = take(bh * na * kv * 4);
-    w.anchor_dots = take(nk * bh * na * 4);
+    const int64_t chunks = (s.L + kC - 1) / kC, ac = anchor_chunks(dtype), na = (chunks + ac - 1) / ac;
+    w.r = take(bh * s.L * 4);
+    w.c = take(bh * s.L * 4);
+    w.anchors = take(bh * na * state);
+    w.anchor_dots = take(waves(s.K) * bh * na * 4);
     if (s.H != s.Hk) {
       w.dq = take(s.B * s.L * s.H * s.K * 4);
       w.dk = take(s.B * s.L * s.H * s.K * 4);
@@ -719,44 +859,39 @@ Space space(const Sizes& s, int dtype, bool backward) {
   return w;
 }
 
-template <typename T, typename OT, int E, bool FWD, int NU>
+template <typename T, typename OT, int E, int NW, bool FWD, int NU>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   const int64_t bh = a.units;
-  const int64_t kv = (int64_t)a.E * a.F;
   a.units = bh * a.nseg;
-  const unsigned grid = (unsigned)((a.units + 7) / 8 * 8 * a.nft);
   if (a.nseg > 1) {
     WalkArgs<T, OT> p = a;
-    float* seg = (float*)(ws + sp.seg);
-    double* decay = (double*)(ws + sp.decay);
-    p.init = nullptr;
-    p.last = seg;
-    p.seg_decay = decay;
-    walk_kernel<T, OT, E, FWD, true, NU><<<grid, kThreads, 0, stream>>>(p);
-    const int64_t total = bh * kv;
-    join_kernel<<<(unsigned)((total + kThreads - 1) / kThreads), kThreads, 0, stream>>>(seg, decay, init, a.nseg, kv, total, !FWD);
-    a.init = seg;
-    a.init_per_seg = 1;
+    f32x4* seg = (f32x4*)(ws + sp.seg);
+    p.seg_last = seg;
+    p.seg_decay = (double*)(ws + sp.decay);
+    walk_kernel<T, OT, E, NW, FWD, true, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
+    const int64_t total = bh * E / 16 * 64 * NW;
+    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, a.E, a.F, a.se, a.sf, total, !FWD);
+    a.seg_init = seg;
   } else {
     a.init = init;
-    a.init_per_seg = 0;
   }
   a.last = last;
-  walk_kernel<T, OT, E, FWD, false, NU><<<grid, kThreads, 0, stream>>>(a);
+  walk_kernel<T, OT, E, NW, FWD, false, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
   return tsf_launch_status();
 }
 
-// One walk. `init` and `last` are the row's states [row x head][K V]; a.units comes in as rows x heads.
+// One walk. `init` and `last` are the row's states [row x head][K V].
 template <typename T, typename OT, bool FWD, int NU>
 int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   a.H = (int)s.H;
   a.L = s.L;
   a.units = s.B * s.H;
-  a.nft = tiles(a.F);
-  a.nseg = segments(s, a.nft);
+  a.nseg = segments(s);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
   constexpr int N = sizeof(T) == 2 ? NU : 1;
-  return a.E <= 64 ? walk_e<T, OT, 64, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, FWD, N>(a, ws, sp, init, last, stream);
+  if (waves(a.F) == 4)
+    return a.E <= 64 ? walk_e<T, OT, 64, 4, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, FWD, N>(a, ws, sp, init, last, stream);
+  return a.E <= 64 ? walk_e<T, OT, 64, 8, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 8, FWD, N>(a, ws, sp, init, last, stream);
 }
 
 template <typename T>
@@ -797,7 +932,7 @@ int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<c
   a.sf = (int)s.V;
   a.dot = dot;
   a.dots = dots;
-  a.anchors = (float*)(ws + sp.anchors);
+  a.anchors = (f32x4*)(ws + sp.anchors);
   a.anchor_dots = (float*)(ws + sp.anchor_dots);
   a.anchor_chunks = anchor_chunks(dtype);
   a.nanchor = (int)(((s.L + kC - 1) / kC + a.anchor_chunks - 1) / a.anchor_chunks);
@@ -849,7 +984,7 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
   const int ac = anchor_chunks(dtype);
   const int na = (int)(((s.L + kC - 1) / kC + ac - 1) / ac);
   dgate_kernel<T><<<(unsigned)(s.B * s.H * na), kThreads, 0, stream>>>(r, c, (const float*)(ws + sp.anchor_dots), G, Seq<T>{(T*)dg, s.L * s.H, s.H, 1, 1},
-                                                                       (int)s.H, s.L, s.B * s.H, tiles(s.K), ac * kC, na);
+                                                                       (int)s.H, s.L, s.B * s.H, waves(s.K), ac * kC, na);
   return tsf_launch_status();
 }
 
