@@ -22,6 +22,8 @@
 // dg needs no product of its own: r_t = q_t . dq_t and c_t = k_t . dk_t, summed while dq and dk are still in
 // registers, give dg_{t+1} = dg_t - r_t + c_t. The rounding errors of that running sum are cut off at
 // anchors every kAnchor chunks, where dg_t = <S_{t-1}, dL/dS_{t-1}> is formed from the two states.
+#include <math.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -72,8 +74,6 @@ TSF_DEV f32x4 mma(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
   return c;
 }
 
-TSF_DEV float get(const Frag<bf16>& f, int e) { return (float)f.v[e]; }
-TSF_DEV float get(const Frag<float>& f, int e) { return e < 4 ? f.lo[e & 3] : f.hi[e & 3]; }
 TSF_DEV void put(Frag<bf16>& f, int e, float x) { f.v[e] = (__bf16)x; }
 TSF_DEV void put(Frag<float>& f, int e, float x) {
   if (e < 4)
@@ -82,18 +82,55 @@ TSF_DEV void put(Frag<float>& f, int e, float x) {
     f.hi[e & 3] = x;
 }
 
-// Eight values as the sum of N operands: bf16 carries 8 bits of each value's mantissa an operand, fp32 all.
-template <typename T, int N>
-TSF_DEV void split(const float* x, Frag<T>* out) {
+// Two floats to bf16 pairs, rounded to nearest even (one instruction), and the pair back (two).
+TSF_DEV uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+TSF_DEV float low(uint32_t p) { return __uint_as_float(p << 16); }
+TSF_DEV float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// 2 M values as the sum of N operands' words: bf16 carries 8 bits of each value's mantissa an operand.
+template <int M, int N>
+TSF_DEV void split_words(const float* x, uint32_t (&w)[N][M]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float rest = x[e];
+  for (int k = 0; k < M; ++k) {
+    float a = x[2 * k], b = x[2 * k + 1];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      put(out[n], e, rest);
-      if (n + 1 < N) rest -= get(out[n], e);
+      w[n][k] = pack2(a, b);
+      if (n + 1 < N) a -= low(w[n][k]), b -= high(w[n][k]);
     }
   }
+}
+// Eight values as the sum of N operands (fp32: as they are).
+template <int N>
+TSF_DEV void split(const float* x, Frag<bf16>* out) {
+  uint32_t w[N][4];
+  split_words<4, N>(x, w);
+#pragma unroll
+  for (int n = 0; n < N; ++n) __builtin_memcpy(&out[n].v, w[n], 16);
+}
+template <int N>
+TSF_DEV void split(const float* x, Frag<float>* out) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out->lo[e] = x[e], out->hi[e] = x[4 + e];
+}
+// The eight values of an operand, weighted.
+TSF_DEV void weigh(const Frag<bf16>& f, f32x4 w0, f32x4 w1, float* v) {
+  uint32_t p[4];
+  __builtin_memcpy(p, &f.v, 16);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f32x4& w = k < 2 ? w0 : w1;
+    v[2 * k] = low(p[k]) * w[2 * (k & 1)];
+    v[2 * k + 1] = high(p[k]) * w[2 * (k & 1) + 1];
+  }
+}
+TSF_DEV void weigh(const Frag<float>& f, f32x4 w0, f32x4 w1, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = f.lo[e] * w0[e], v[4 + e] = f.hi[e] * w1[e];
 }
 
 // Eight consecutive values of a row of global memory at any alignment.
@@ -274,12 +311,12 @@ struct Rows {
     return f;
   }
   // four columns 16 jt + 4 lg .. of row 16 t + li, as accumulators have them
-  TSF_DEV void put_four(uint32_t lane_off, int t, int jt, const Frag<T>& f) {
+  TSF_DEV void put_four(uint32_t lane_off, int t, int jt, const void* f) {
     char* p = at + t * 16 * kBytes;
     if constexpr (kBf)
-      lds_put<8>(p + (lane_off ^ ((jt >> 1) << 6)) + 8 * (jt & 1), &f);
+      lds_put<8>(p + (lane_off ^ ((jt >> 1) << 6)) + 8 * (jt & 1), f);
     else
-      lds_put<16>(p + (lane_off ^ (jt << 6)), &f);
+      lds_put<16>(p + (lane_off ^ (jt << 6)), f);
   }
   // operands whose row is column 16 t + li and whose contraction runs over rows (steps) 32 half ..; OPERAND: columns are in
   // operand order. bf16: the transposing read, in which lane li of a group of 16 points at 4 columns of row li / 4 and
@@ -313,11 +350,11 @@ struct Rows {
   }
 };
 
-template <typename T, int E, int NW>
+template <typename T, int E, int FT, int NW>
 struct Lds {
   static constexpr int kSplit = sizeof(T) == 2 ? 2 : 1;  // operands the state and the scores are split into
   Rows<T, E> x, y;
-  Rows<T, 16 * NW> z;
+  Rows<T, FT> z;
   Rows<T, kC> p[kSplit];                                        // decayed scores, row i
   alignas(16) float hi[2][kC], lo[2][kC], w[2][kC], in[2][kC];  // running log2 decay, weights into the state and out of it
   float dot[NW][kC];
@@ -325,8 +362,8 @@ struct Lds {
 
 // Waves a SIMD holds of a walk: what LDS and a 512-register file allow.
 template <typename T>
-constexpr int walk_waves(int E, int NW) {
-  return sizeof(T) == 2 ? (NW == 8 ? 4 : 2) : E == 64 && NW == 4 ? 2 : NW / 4;
+constexpr int walk_waves(int E, int NW, int FW) {
+  return sizeof(T) == 2 ? (NW == 8 ? 4 : 2) : E == 64 && FW == 1 && NW == 4 ? 2 : NW / 4;
 }
 
 // One wave: the chunk's running log2 decay as float pairs (differences are exact to float64 rounding), the
@@ -367,16 +404,16 @@ TSF_DEV f32x4 four(const float* p) {
   return v;
 }
 
-// E: columns of x and y, padded; NW: waves of a workgroup; FWD: the direction in time; STATE_ONLY: only the state leaving
+// E: columns of x and y, padded; NW: waves of a workgroup; FW: 16-column tiles of z a wave owns; FWD: the direction in time; STATE_ONLY: only the state leaving
 // the unit; NU: operands the weighted z is split into in the state's update.
 //
-// Wave w owns the state's columns 16 w + li, all E rows of them: accumulators S[et] hold rows 16 et + 4 lg + r, which
+// Wave w owns the state's columns 16 (w FW + fw) + li, all E rows of them: accumulators S[fw][et] hold rows 16 et + 4 lg + r, which
 // two by two are operands as they stand. Per chunk: (1) x, y, z to LDS; (2) the ten live 16 x 16 score tiles, shared
 // among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update.
-template <typename T, typename OT, int E, int NW, bool FWD, bool STATE_ONLY, int NU>
-__global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(WalkArgs<T, OT> a) {
-  constexpr int kThr = 64 * NW, FT = 16 * NW, KS = E / 32, ET = E / 16, NS = Lds<T, E, NW>::kSplit;
-  __shared__ Lds<T, E, NW> s;
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, int NU>
+__global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel(WalkArgs<T, OT> a) {
+  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT, NW>::kSplit;
+  __shared__ Lds<T, E, FT, NW> s;
   int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes, as the compiler now knows
   const int64_t unit = blockIdx.x;
@@ -394,22 +431,30 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
 
   // The state. In the workspace (segments, anchors) a state is f32x4 [et][thread], padding included; the caller's
   // are K V floats, (e, f) at e se + f sf.
-  f32x4 S[ET];
+  f32x4 S[FW][ET];
   const int64_t kv = (int64_t)a.E * a.F;
   auto each_state = [&](auto f) {  // value = f(index in a caller's state, value)
 #pragma unroll
-    for (int et = 0; et < ET; ++et)
+    for (int fw = 0; fw < FW; ++fw)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int e = 16 * et + 4 * lg + r, col = 16 * wave + li;
-        if (e < a.E && col < a.F) S[et][r] = f((int64_t)e * a.se + (int64_t)col * a.sf, S[et][r]);
-      }
+      for (int et = 0; et < ET; ++et)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int e = 16 * et + 4 * lg + r, col = 16 * (wave * FW + fw) + li;
+          if (e < a.E && col < a.F) S[fw][et][r] = f((int64_t)e * a.se + (int64_t)col * a.sf, S[fw][et][r]);
+        }
   };
+  auto each_tile = [&](auto f) {  // f(index of a thread's f32x4 in a workspace state, S's)
 #pragma unroll
-  for (int et = 0; et < ET; ++et) S[et] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int fw = 0; fw < FW; ++fw)
+#pragma unroll
+      for (int et = 0; et < ET; ++et) f((fw * ET + et) * kThr + threadIdx.x, S[fw][et]);
+  };
+  constexpr int kTiles = FW * ET * kThr;
+  each_tile([](int, f32x4& v) { v = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
   if (a.seg_init) {
-#pragma unroll
-    for (int et = 0; et < ET; ++et) S[et] = a.seg_init[(unit * ET + et) * kThr + threadIdx.x];
+    const f32x4* from = a.seg_init + unit * kTiles;
+    each_tile([&](int at, f32x4& v) { v = from[at]; });
   } else if (a.init) {
     const float* init = a.init + bh * kv;
     each_state([&](int64_t at, float) { return init[at]; });
@@ -423,6 +468,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
   uint32_t z_lds = Rows<T, FT>::plain(zrow & 15, zcol / 8) + (zrow >> 4) * 16 * Rows<T, FT>::kBytes;
   // A piece that ends beyond its row is read so that it ends with it, a row beyond the last step is read as the last one; what does
   // not belong goes on the way to LDS. Rows of fewer than eight columns are read by elements then.
+  const bool fours = a.F % 4 == 0;  // the same for all lanes
   const bool exact = a.E == E && a.F == FT, narrow_x = a.E < 8, narrow_z = a.F < 8;
   const uint32_t x_most = a.E - 8, z_most = a.F - 8;
   auto fetch_chunk = [&](int c) {
@@ -501,10 +547,8 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
     const int buf = n & 1;
     const int64_t t0 = (int64_t)c * kC;
     const bool anchor = !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0;
-    f32x4* const anchor_at = anchor ? a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * ET * kThr + threadIdx.x : nullptr;
-    if (FWD && anchor)
-#pragma unroll
-      for (int et = 0; et < ET; ++et) anchor_at[et * kThr] = S[et];
+    f32x4* const anchor_at = anchor ? a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * kTiles : nullptr;
+    if (FWD && anchor) each_tile([&](int at, f32x4& v) { anchor_at[at] = v; });
     if (!exact || t0 + kC > a.L) fit_chunk(t0);
 #pragma unroll
     for (int p = 0; p < XP; ++p) {
@@ -516,8 +560,8 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
     __syncthreads();
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
-    f32x4 acc[4];  // outputs, transposed: columns f of z by steps i = 16 it + li
-    const int f = 16 * wave + 4 * lg;
+    f32x4 acc[FW][4];  // outputs, transposed: columns f + 16 fw of z by steps i = 16 it + li
+    const int f0 = 16 * wave * FW + 4 * lg;
     if constexpr (!STATE_ONLY) {
       // decayed scores, transposed in registers: rows j = 16 jt + 4 lg + r, column i = 16 it + li
 #pragma unroll
@@ -531,40 +575,54 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
           for (int ks = 0; ks < KS; ++ks) sc = mma(s.y.row(row_off, jt, ks), s.x.row(row_off, it, ks), sc);
           const f32x4 j_hi = four(s.hi[buf] + 16 * jt + 4 * lg), j_lo = four(s.lo[buf] + 16 * jt + 4 * lg);
           const float i_hi = s.hi[buf][16 * it + li], i_lo = s.lo[buf][16 * it + li];
-          float part[8];
+          float part[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float d = (i_hi - j_hi[r]) + (i_lo - j_lo[r]);
             const int j = 4 * lg + r;
             const bool live = it != jt || (FWD ? j <= li : j >= li);
-            part[r] = live ? sc[r] * fast_exp2(FWD ? d : -d) : 0.0f;
-            part[r + 4] = 0.0f;
+            part[r] = sc[r] * fast_exp2(live ? (FWD ? d : -d) : -INFINITY);
           }
-          Frag<T> f4[NS];
-          split<T, NS>(part, f4);
+          if constexpr (NS == 1) {
+            s.p[0].put_four(p_off, it, jt, part);
+          } else {
+            uint32_t words[NS][2];
+            split_words<2, NS>(part, words);
 #pragma unroll
-          for (int m = 0; m < NS; ++m) s.p[m].put_four(p_off, it, jt, f4[m]);
+            for (int m = 0; m < NS; ++m) s.p[m].put_four(p_off, it, jt, words[m]);
+          }
         }
       }
       // x times the state entering
 #pragma unroll
-      for (int it = 0; it < 4; ++it) acc[it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int fw = 0; fw < FW; ++fw)
+#pragma unroll
+        for (int it = 0; it < 4; ++it) acc[fw][it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        Frag<T> sf[NS];
-        float v[8];
+        Frag<T> sf[FW][NS];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = S[2 * ks + (e >> 2)][e & 3];
-        split<T, NS>(v, sf);
+        for (int fw = 0; fw < FW; ++fw) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = S[fw][2 * ks + (e >> 2)][e & 3];
+          split<NS>(v, sf[fw]);
+        }
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const Frag<T> xf = s.x.row(row_off, it, ks);
 #pragma unroll
-          for (int m = 0; m < NS; ++m) acc[it] = mma(sf[m], xf, acc[it]);
+          for (int m = 0; m < NS; ++m)
+#pragma unroll
+            for (int fw = 0; fw < FW; ++fw) acc[fw][it] = mma(sf[fw][m], xf, acc[fw][it]);
         }
       }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) acc[it] *= s.in[buf][16 * it + li];
+      for (int it = 0; it < 4; ++it) {
+        const float in = s.in[buf][16 * it + li];
+#pragma unroll
+        for (int fw = 0; fw < FW; ++fw) acc[fw][it] *= in;
+      }
     }
     if (wave == kGateWave && n + 1 < chunks) {
       gates<FWD>(s, buf ^ 1, gate_of(n + 1, g_next), lane);
@@ -573,68 +631,89 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
     if constexpr (!STATE_ONLY) __syncthreads();
 
     if constexpr (!STATE_ONLY) {
+      if (n + 1 < chunks) fetch_chunk(c + kStep);  // before the outputs' stores, which the loads would wait behind
       // the scores times z, and the outputs
-      Four<T> u[4];
+      Four<T> u[FW][4];
       if (a.dots)
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const uint32_t row = min(16 * it + li, (int)min((int64_t)kC, a.L - t0) - 1);
           const T* from = at32(dh + t0 * a.dot.sl, row * (uint32_t)a.dot.sl);
-          load4(u[it], f < a.F ? from + f : from, a.F - f);
+#pragma unroll
+          for (int fw = 0; fw < FW; ++fw) {
+            const int f = f0 + 16 * fw;
+            load4(u[fw][it], f < a.F ? from + f : from, fours ? 4 : a.F - f);
+          }
         }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const Frag<T> zf = s.z.template col<false>(zcol_off, wave, half, li, lg);
+        Frag<T> zf[FW];
+#pragma unroll
+        for (int fw = 0; fw < FW; ++fw) zf[fw] = s.z.template col<false>(zcol_off, wave * FW + fw, half, li, lg);
 #pragma unroll
         for (int it = 0; it < 4; ++it)
           if (FWD ? 2 * half <= it : 2 * half + 1 >= it)
 #pragma unroll
-            for (int m = 0; m < NS; ++m) acc[it] = mma(zf, s.p[m].row(p_off, it, half), acc[it]);
+            for (int m = 0; m < NS; ++m) {
+              const Frag<T> pf = s.p[m].row(p_off, it, half);
+#pragma unroll
+              for (int fw = 0; fw < FW; ++fw) acc[fw][it] = mma(zf[fw], pf, acc[fw][it]);
+            }
       }
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int64_t ti = t0 + 16 * it;
-        const bool live = ti + li < a.L && f < a.F;
-        if (live) store4(at32(oh + ti * a.out.sl, li * (uint32_t)a.out.sl + f), acc[it], a.F - f);
-        if (a.dots) {
-          float dot = 0.0f;
+        float dot = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) dot = fmaf(acc[it][r], live && f + r < a.F ? to_f32(u[it].v[r]) : 0.0f, dot);
+        for (int fw = 0; fw < FW; ++fw) {
+          const int f = f0 + 16 * fw;
+          const bool live = ti + li < a.L && f < a.F;
+          if (live) store4(at32(oh + ti * a.out.sl, li * (uint32_t)a.out.sl + f), acc[fw][it], fours ? 4 : a.F - f);
+          if (a.dots)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dot = fmaf(acc[fw][it][r], live && f + r < a.F ? to_f32(u[fw][it].v[r]) : 0.0f, dot);
+        }
+        if (a.dots) {
           dot += __shfl_xor(dot, 16, kWave);
           dot += __shfl_xor(dot, 32, kWave);
           if (lg == 0) s.dot[wave][16 * it + li] = dot;
         }
       }
     }
-    if (n + 1 < chunks) fetch_chunk(c + kStep);
+    if constexpr (STATE_ONLY)
+      if (n + 1 < chunks) fetch_chunk(c + kStep);
 
     // the state: S = tot S + sum_j y_j (w_j z_j)^T
     const float tot = FWD ? s.in[buf][kC - 1] : s.w[buf][kC - 1];  // the whole chunk's decay
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const Frag<T> zf = s.z.template col<false>(zcol_off, wave, half, li, lg);
       const f32x4 w0 = four(s.w[buf] + 32 * half + 4 * lg), w1 = four(s.w[buf] + 32 * half + 16 + 4 * lg);
-      Frag<T> zw[NU];
-      float v[8];
+      Frag<T> zw[FW][NU];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = get(zf, e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
-      split<T, NU>(v, zw);
+      for (int fw = 0; fw < FW; ++fw) {
+        float v[8];
+        weigh(s.z.template col<false>(zcol_off, wave * FW + fw, half, li, lg), w0, w1, v);
+        split<NU>(v, zw[fw]);
+      }
 #pragma unroll
       for (int et = 0; et < ET; ++et) {
         const Frag<T> yf = s.y.template col<true>(ycol_off, et, half, li, lg);
-        if (half == 0) S[et] *= tot;
 #pragma unroll
-        for (int m = 0; m < NU; ++m) S[et] = mma(yf, zw[m], S[et]);
+        for (int fw = 0; fw < FW; ++fw)
+          if (half == 0) S[fw][et] *= tot;
+#pragma unroll
+        for (int m = 0; m < NU; ++m)
+#pragma unroll
+          for (int fw = 0; fw < FW; ++fw) S[fw][et] = mma(yf, zw[fw][m], S[fw][et]);
       }
     }
     if (!FWD && anchor) {
       float d = 0.0f;
+      each_tile([&](int at, f32x4& v) {
+        const f32x4 from = anchor_at[at];
 #pragma unroll
-      for (int et = 0; et < ET; ++et) {
-        const f32x4 from = anchor_at[et * kThr];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d = fmaf(from[r], S[et][r], d);
-      }
+        for (int r = 0; r < 4; ++r) d = fmaf(from[r], v[r], d);
+      });
       d = wave_sum(d);
       if (lane == 0) a.anchor_dots[((int64_t)wave * nbh + bh) * a.nanchor + c / a.anchor_chunks] = d;
     }
@@ -649,8 +728,8 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
   }
 
   if constexpr (STATE_ONLY) {
-#pragma unroll
-    for (int et = 0; et < ET; ++et) a.seg_last[(unit * ET + et) * kThr + threadIdx.x] = S[et];
+    f32x4* to = a.seg_last + unit * kTiles;
+    each_tile([&](int at, f32x4& v) { to[at] = v; });
     if (threadIdx.x == 0) a.seg_decay[unit] = log_decay;
   } else if (a.last && seg == (FWD ? a.nseg - 1 : 0)) {
     float* to = a.last + bh * kv;
@@ -658,16 +737,16 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW)) void walk_kernel(Wal
   }
 }
 
-// Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards). `threads`
-// and `et` are the walk's; a thread owns one f32x4 of a state.
-__global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int E, int F, int se,
+// Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards). `threads`,
+// `et` and `fw` are the walk's; a thread owns one f32x4 of a state.
+__global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int fw, int E, int F, int se,
                                                    int sf, int64_t total, int backward) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;
-  const int per = threads * et;
+  const int per = threads * et * fw;
   const int64_t bh = at / per;
   const int in = (int)(at % per), lane = in % threads & 63;
-  const int e = in / threads * 16 + (lane >> 4) * 4, col = in % threads / 64 * 16 + (lane & 15);
+  const int e = in / threads % et * 16 + (lane >> 4) * 4, col = (in % threads / 64 * fw + in / threads / et) * 16 + (lane & 15);
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
   if (init && col < F)
 #pragma unroll
@@ -806,7 +885,7 @@ int args_status(const Sizes& s, int dtype) {
 }
 
 // Waves of a walk over F columns: a workgroup takes all of them, so that nothing of x and y is done twice.
-int waves(int64_t F) { return F <= 64 ? 4 : 8; }
+int waves(int64_t) { return 4; }
 
 // Segments a row is cut into. A cut row is walked twice (its segments' states first), so rows are cut only to give
 // every CU its two workgroups, into no more than fit at once and into four chunks at least.
@@ -859,7 +938,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
   return w;
 }
 
-template <typename T, typename OT, int E, int NW, bool FWD, int NU>
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, int NU>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   const int64_t bh = a.units;
   a.units = bh * a.nseg;
@@ -868,15 +947,15 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
     p.seg_decay = (double*)(ws + sp.decay);
-    walk_kernel<T, OT, E, NW, FWD, true, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
-    const int64_t total = bh * E / 16 * 64 * NW;
-    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, a.E, a.F, a.se, a.sf, total, !FWD);
+    walk_kernel<T, OT, E, NW, FW, FWD, true, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
+    const int64_t total = bh * E / 16 * 64 * NW * FW;
+    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD);
     a.seg_init = seg;
   } else {
     a.init = init;
   }
   a.last = last;
-  walk_kernel<T, OT, E, NW, FWD, false, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
+  walk_kernel<T, OT, E, NW, FW, FWD, false, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
   return tsf_launch_status();
 }
 
@@ -889,9 +968,9 @@ int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const flo
   a.nseg = segments(s);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
   constexpr int N = sizeof(T) == 2 ? NU : 1;
-  if (waves(a.F) == 4)
-    return a.E <= 64 ? walk_e<T, OT, 64, 4, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, FWD, N>(a, ws, sp, init, last, stream);
-  return a.E <= 64 ? walk_e<T, OT, 64, 8, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 8, FWD, N>(a, ws, sp, init, last, stream);
+  if (a.F <= 64)
+    return a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 1, FWD, N>(a, ws, sp, init, last, stream);
+  return a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 2, FWD, N>(a, ws, sp, init, last, stream);
 }
 
 template <typename T>
