@@ -180,28 +180,56 @@ TSF_DEV void store4(bf16* p, f32x4 v, int n) {
       if (e < n) p[e] = h[e];
   }
 }
-// Four consecutive values of a row of global memory, as they are; `n` of them exist, the others are some value of the row.
-template <typename T>
-struct Four {
-  T v[4];
-};
-template <typename T>
-TSF_DEV void load4(Four<T>& f, const T* p, int n) {
-  if (n >= 4) {
-    __builtin_memcpy(&f, p, sizeof(f));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f.v[e] = p[e < n ? e : 0];
-  }
-}
+// Four consecutive values of a row of global memory at any alignment, zeros where there are fewer than n.
 template <typename T>
 TSF_DEV f32x4 load4(const T* p, int n) {
-  Four<T> h;
-  load4(h, p, n);
-  f32x4 v;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (n >= 4) {
+    T h[4];
+    __builtin_memcpy(h, p, sizeof(h));
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = e < n ? to_f32(h.v[e]) : 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = to_f32(h[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) v[e] = to_f32(p[e]);
+  }
   return v;
+}
+
+// The first n of eight outputs to a row of global memory at any alignment; `rest` is what their rounding left.
+TSF_DEV float value(const Frag<bf16>& o, int e) { return (float)o.v[e]; }
+TSF_DEV float value(const Frag<float>& o, int e) { return e < 4 ? o.lo[e & 3] : o.hi[e & 3]; }
+template <typename F>
+TSF_DEV void store8(float* p, const F& o, const F& rest, int n) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = value(o, e) + value(rest, e);
+  if (n >= 8) {
+    __builtin_memcpy(p, v, 32);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = v[e];
+  }
+}
+TSF_DEV void store8(bf16* p, const Frag<bf16>& o, const Frag<bf16>&, int n) {
+  if (n >= 8) {
+    __builtin_memcpy(p, &o.v, 16);
+  } else {
+    bf16 v[8];
+    __builtin_memcpy(v, &o.v, 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = v[e];
+  }
+}
+template <typename F>
+TSF_DEV float dot8(const F& o, const F& rest, const F& u) {
+  float d = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d = fmaf(value(o, e) + value(rest, e), value(u, e), d);
+  return d;
 }
 
 // An element by a 32-bit index from an address that all lanes share.
@@ -297,6 +325,20 @@ struct Rows {
     else
       put_piece(off, row16, f);
   }
+  TSF_DEV Frag<T> get_plain(uint32_t off, int row16) const {
+    Frag<T> f;
+    const char* p = at + row16 * 16 * kBytes;
+    lds_get<16>(&f, p + off);
+    if constexpr (!kBf) lds_get<16>(&f.hi, p + (off ^ 16));
+    return f;
+  }
+  // four columns 16 tile + 4 lg .. of row 16 t + li, as accumulators have them, to plain places: the lane's offset, and the move
+  TSF_DEV static uint32_t four_lane(uint32_t li, uint32_t lg) {
+    return kBf ? li * kBytes + (((lg >> 1) ^ turn(li)) << 4) + 8 * (lg & 1) : li * kBytes + ((lg ^ turn(li)) << 4);
+  }
+  TSF_DEV void put_plain_four(uint32_t lane_off, int t, int tile, const void* f) {
+    lds_put<kHalf>(at + t * 16 * kBytes + (lane_off ^ (tile << (kBf ? 5 : 6))), f);
+  }
   // operands whose row is row 16 t + li, over columns 32 s ..: the lane's offset, and the operand
   TSF_DEV static uint32_t row_lane(uint32_t li, uint32_t lg) { return li * kBytes + ((lg ^ turn(li)) << 4); }
   TSF_DEV Frag<T> row(uint32_t lane_off, int t, int s) const {
@@ -350,14 +392,20 @@ struct Rows {
   }
 };
 
-template <typename T, int E, int FT, int NW>
+template <typename T, int E, int FT>
 struct Lds {
   static constexpr int kSplit = sizeof(T) == 2 ? 2 : 1;  // operands the state and the scores are split into
-  Rows<T, E> x, y;
+  union {
+    Rows<T, E> x;
+    Rows<T, FT> o;  // the outputs on their way to memory, once x has been used
+  };
+  Rows<T, E> y;
   Rows<T, FT> z;
-  Rows<T, kC> p[kSplit];                                        // decayed scores, row i
+  union {
+    Rows<T, kC> p[kSplit];  // decayed scores, row i
+    Rows<T, FT> o_rest;     // what the outputs' rounding left (bf16), once the scores have been used
+  };
   alignas(16) float hi[2][kC], lo[2][kC], w[2][kC], in[2][kC];  // running log2 decay, weights into the state and out of it
-  float dot[NW][kC];
 };
 
 // Waves a SIMD holds of a walk: what LDS and a 512-register file allow.
@@ -404,16 +452,20 @@ TSF_DEV f32x4 four(const float* p) {
   return v;
 }
 
-// E: columns of x and y, padded; NW: waves of a workgroup; FW: 16-column tiles of z a wave owns; FWD: the direction in time; STATE_ONLY: only the state leaving
-// the unit; NU: operands the weighted z is split into in the state's update.
+// E: columns of x and y, padded; NW: waves of a workgroup; FW: 16-column tiles of z a wave owns; FWD: the direction in time;
+// STATE_ONLY: only the state leaving the unit; DOTS: out_i . dot_i too, and the anchors.
+//
+// The weighted z of the state's update is split into three bf16 operands where the caller gets the state (2^-24), two where
+// only bf16 outputs and their products follow (2^-16).
 //
 // Wave w owns the state's columns 16 (w FW + fw) + li, all E rows of them: accumulators S[fw][et] hold rows 16 et + 4 lg + r, which
 // two by two are operands as they stand. Per chunk: (1) x, y, z to LDS; (2) the ten live 16 x 16 score tiles, shared
 // among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update.
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, int NU>
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, bool DOTS>
 __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel(WalkArgs<T, OT> a) {
-  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT, NW>::kSplit;
-  __shared__ Lds<T, E, FT, NW> s;
+  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT>::kSplit, NU = sizeof(T) == 4 ? 1 : DOTS ? 2 : 3;
+  constexpr bool kRest = DOTS && sizeof(T) == 2;  // outputs go to LDS in two parts: the sums of products want more than bf16
+  __shared__ Lds<T, E, FT> s;
   int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes, as the compiler now knows
   const int64_t unit = blockIdx.x;
@@ -424,10 +476,10 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
   const int c_lo = seg * a.seg_chunks, chunks = min(nchunk, c_lo + a.seg_chunks) - c_lo;
   const T *xh = a.x.head(b, h), *yh = a.y.head(b, h), *zh = a.z.head(b, h), *gh = a.g.head(b, h);
   OT* const oh = STATE_ONLY ? nullptr : a.out.head(b, h);
-  const T* const dh = a.dots ? a.dot.head(b, h) : nullptr;
+  const T* const dh = DOTS && !STATE_ONLY ? a.dot.head(b, h) : nullptr;
   // the lane's places in the LDS arrays
   uint32_t row_off = Rows<T, E>::row_lane(li, lg), p_off = Rows<T, kC>::row_lane(li, lg);
-  uint32_t ycol_off = Rows<T, E>::template col_lane<true>(li, lg), zcol_off = Rows<T, FT>::template col_lane<false>(li, lg);
+  uint32_t ycol_off = Rows<T, E>::template col_lane<true>(li, lg), zcol_off = Rows<T, FT>::template col_lane<false>(li, lg), o_off = Rows<T, FT>::four_lane(li, lg);
 
   // The state. In the workspace (segments, anchors) a state is f32x4 [et][thread], padding included; the caller's
   // are K V floats, (e, f) at e se + f sf.
@@ -462,13 +514,12 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 
   // this thread's 8-column pieces of x, y and z on their way to LDS: one of every kRowsX (kRowsZ) rows
   constexpr int XC = E / 8, kRowsX = kThr / XC, XP = kC / kRowsX, ZC = FT / 8, kRowsZ = kThr / ZC, ZP = kC / kRowsZ;
-  Frag<T> px[STATE_ONLY ? 1 : XP], py[XP], pz[ZP];
+  Frag<T> px[STATE_ONLY ? 1 : XP], py[XP], pz[ZP], pu[DOTS && !STATE_ONLY ? ZP : 1];
   int xrow = threadIdx.x / XC, xcol = threadIdx.x % XC * 8, zrow = threadIdx.x / ZC, zcol = threadIdx.x % ZC * 8;
   uint32_t x_lds = Rows<T, E>::piece(xrow & 15, xcol / 8) + (xrow >> 4) * 16 * Rows<T, E>::kBytes;
   uint32_t z_lds = Rows<T, FT>::plain(zrow & 15, zcol / 8) + (zrow >> 4) * 16 * Rows<T, FT>::kBytes;
   // A piece that ends beyond its row is read so that it ends with it, a row beyond the last step is read as the last one; what does
   // not belong goes on the way to LDS. Rows of fewer than eight columns are read by elements then.
-  const bool fours = a.F % 4 == 0;  // the same for all lanes
   const bool exact = a.E == E && a.F == FT, narrow_x = a.E < 8, narrow_z = a.F < 8;
   const uint32_t x_most = a.E - 8, z_most = a.F - 8;
   auto fetch_chunk = [&](int c) {
@@ -490,12 +541,12 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
       for (int p = 0; p < ZP; ++p) load8(pz[p], at32(zb, (uint32_t)min(p * kRowsZ + zrow, last) * (uint32_t)a.z.sl + col));
     }
   };
+  auto by_elements = [&](Frag<T>& f, const T* row, int col, int n) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) put(f, e, e < n ? to_f32(row[col + e]) : 0.0f);
+  };
   auto fit_chunk = [&](int64_t t0) {
     const int steps = (int)min((int64_t)kC, a.L - t0);
-    auto by_elements = [&](Frag<T>& f, const T* row, int col, int n) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) put(f, e, e < n ? to_f32(row[col + e]) : 0.0f);
-    };
 #pragma unroll
     for (int p = 0; p < XP; ++p) {
       const int row = p * kRowsX + xrow, n = row < steps ? a.E - xcol : 0;
@@ -534,19 +585,13 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
       g_next = fetch_gate(1);
     }
   }
-  if constexpr (!STATE_ONLY) {  // score tiles that no step reaches stay zero
-#pragma unroll
-    for (int m = 0; m < NS; ++m)
-      for (int i = threadIdx.x * 16; i < (int)sizeof(s.p[m].at); i += kThr * 16) *(u32x4*)(s.p[m].at + i) = u32x4{0, 0, 0, 0};
-  }
-
   for (int n = 0; n < chunks; ++n, c += kStep) {
     // what follows from these is formed again in each chunk: kept over the loop it would not fit the registers beside the state
-    again(lane), again(li), again(lg), again(row_off), again(p_off), again(ycol_off), again(zcol_off), again(x_lds), again(z_lds);
+    again(lane), again(li), again(lg), again(row_off), again(p_off), again(ycol_off), again(zcol_off), again(o_off), again(x_lds), again(z_lds);
     again(xrow), again(xcol), again(zrow), again(zcol);
     const int buf = n & 1;
     const int64_t t0 = (int64_t)c * kC;
-    const bool anchor = !STATE_ONLY && a.anchors && c % a.anchor_chunks == 0;
+    const bool anchor = !STATE_ONLY && DOTS && c % a.anchor_chunks == 0;
     f32x4* const anchor_at = anchor ? a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * kTiles : nullptr;
     if (FWD && anchor) each_tile([&](int at, f32x4& v) { anchor_at[at] = v; });
     if (!exact || t0 + kC > a.L) fit_chunk(t0);
@@ -561,13 +606,17 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
     f32x4 acc[FW][4];  // outputs, transposed: columns f + 16 fw of z by steps i = 16 it + li
-    const int f0 = 16 * wave * FW + 4 * lg;
     if constexpr (!STATE_ONLY) {
       // decayed scores, transposed in registers: rows j = 16 jt + 4 lg + r, column i = 16 it + li
 #pragma unroll
-      for (int k = 0; k < (10 + NW - 1) / NW; ++k) {
+      for (int k = 0; k < 12 / NW; ++k) {
         const int id = wave + NW * k;
-        if (id < 10) {
+        if (id >= 10) {  // the two beside the diagonal that operands reach into
+          const int it = FWD ? 2 * (id - 10) : 3 - 2 * (id - 10), jt = FWD ? it + 1 : it - 1;
+          const float none[4] = {};
+#pragma unroll
+          for (int m = 0; m < NS; ++m) s.p[m].put_four(p_off, it, jt, none);
+        } else {
           const int big = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, small = id - big * (big + 1) / 2;
           const int it = FWD ? big : 3 - big, jt = FWD ? small : 3 - small;
           f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -632,19 +681,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 
     if constexpr (!STATE_ONLY) {
       if (n + 1 < chunks) fetch_chunk(c + kStep);  // before the outputs' stores, which the loads would wait behind
-      // the scores times z, and the outputs
-      Four<T> u[FW][4];
-      if (a.dots)
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const uint32_t row = min(16 * it + li, (int)min((int64_t)kC, a.L - t0) - 1);
-          const T* from = at32(dh + t0 * a.dot.sl, row * (uint32_t)a.dot.sl);
-#pragma unroll
-          for (int fw = 0; fw < FW; ++fw) {
-            const int f = f0 + 16 * fw;
-            load4(u[fw][it], f < a.F ? from + f : from, fours ? 4 : a.F - f);
-          }
-        }
+      // the scores times z
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         Frag<T> zf[FW];
@@ -660,25 +697,22 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
               for (int fw = 0; fw < FW; ++fw) acc[fw][it] = mma(zf[fw], pf, acc[fw][it]);
             }
       }
+      if constexpr (kRest) __syncthreads();  // the scores have been used
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int64_t ti = t0 + 16 * it;
-        float dot = 0.0f;
+      for (int it = 0; it < 4; ++it)
 #pragma unroll
         for (int fw = 0; fw < FW; ++fw) {
-          const int f = f0 + 16 * fw;
-          const bool live = ti + li < a.L && f < a.F;
-          if (live) store4(at32(oh + ti * a.out.sl, li * (uint32_t)a.out.sl + f), acc[fw][it], fours ? 4 : a.F - f);
-          if (a.dots)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) dot = fmaf(acc[fw][it][r], live && f + r < a.F ? to_f32(u[fw][it].v[r]) : 0.0f, dot);
+          if constexpr (sizeof(T) == 4) {
+            s.o.put_plain_four(o_off, it, wave * FW + fw, &acc[fw][it]);
+          } else {
+            float v[4];
+            __builtin_memcpy(v, &acc[fw][it], 16);
+            uint32_t words[kRest ? 2 : 1][2];
+            split_words<2, kRest ? 2 : 1>(v, words);
+            s.o.put_plain_four(o_off, it, wave * FW + fw, words[0]);
+            if constexpr (kRest) s.o_rest.put_plain_four(o_off, it, wave * FW + fw, words[1]);
+          }
         }
-        if (a.dots) {
-          dot += __shfl_xor(dot, 16, kWave);
-          dot += __shfl_xor(dot, 32, kWave);
-          if (lg == 0) s.dot[wave][16 * it + li] = dot;
-        }
-      }
     }
     if constexpr (STATE_ONLY)
       if (n + 1 < chunks) fetch_chunk(c + kStep);
@@ -707,6 +741,20 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
           for (int fw = 0; fw < FW; ++fw) S[fw][et] = mma(yf, zw[fw][m], S[fw][et]);
       }
     }
+    if constexpr (DOTS && !STATE_ONLY) {  // what the outputs are multiplied with
+      const int steps = (int)min((int64_t)kC, a.L - t0);
+      const T* from = dh + t0 * a.dot.sl;
+#pragma unroll
+      for (int p = 0; p < ZP; ++p) {
+        const int row = p * kRowsZ + zrow, n = row < steps ? a.F - zcol : 0;
+        if (narrow_z) {
+          by_elements(pu[p], dh + (t0 + row) * a.dot.sl, zcol, n);
+        } else {
+          load8(pu[p], at32(from, (uint32_t)min(row, steps - 1) * (uint32_t)a.dot.sl + min((uint32_t)zcol, z_most)));
+          if (!exact || steps < kC) fit(pu[p], n);
+        }
+      }
+    }
     if (!FWD && anchor) {
       float d = 0.0f;
       each_tile([&](int at, f32x4& v) {
@@ -718,13 +766,25 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
       if (lane == 0) a.anchor_dots[((int64_t)wave * nbh + bh) * a.nanchor + c / a.anchor_chunks] = d;
     }
     __syncthreads();
-    if constexpr (!STATE_ONLY)
-      if (a.dots && wave == 0 && t0 + lane < a.L) {  // written again only after two more barriers
-        float dot = 0.0f;
+    if constexpr (!STATE_ONLY) {
+      // the outputs leave in whole rows
+      const int steps = (int)min((int64_t)kC, a.L - t0);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) dot += s.dot[w][lane];
-        a.dots[bh * a.L + t0 + lane] = dot;
+      for (int p = 0; p < ZP; ++p) {
+        const int row = p * kRowsZ + zrow, n = row < steps ? a.F - zcol : 0;
+        const Frag<T> o = s.o.get_plain(z_lds, p * kRowsZ / 16);
+        Frag<T> rest = {};
+        if constexpr (kRest) rest = s.o_rest.get_plain(z_lds, p * kRowsZ / 16);
+        if (n > 0) store8(at32(oh + t0 * a.out.sl, row * (uint32_t)a.out.sl + zcol), o, rest, n);
+        if constexpr (DOTS) {
+          float d = dot8(o, rest, pu[p]);
+#pragma unroll
+          for (int m = ZC / 2; m >= 1; m >>= 1) d += __shfl_xor(d, m, kWave);
+          if (zcol == 0 && row < steps) a.dots[bh * a.L + t0 + row] = d;
+        }
       }
+      __syncthreads();  // x's place is free again
+    }
   }
 
   if constexpr (STATE_ONLY) {
@@ -938,7 +998,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
   return w;
 }
 
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, int NU>
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool DOTS>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   const int64_t bh = a.units;
   a.units = bh * a.nseg;
@@ -947,7 +1007,7 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
     p.seg_decay = (double*)(ws + sp.decay);
-    walk_kernel<T, OT, E, NW, FW, FWD, true, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
+    walk_kernel<T, OT, E, NW, FW, FWD, true, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
     const int64_t total = bh * E / 16 * 64 * NW * FW;
     join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD);
     a.seg_init = seg;
@@ -955,22 +1015,21 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     a.init = init;
   }
   a.last = last;
-  walk_kernel<T, OT, E, NW, FW, FWD, false, NU><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
+  walk_kernel<T, OT, E, NW, FW, FWD, false, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
   return tsf_launch_status();
 }
 
 // One walk. `init` and `last` are the row's states [row x head][K V].
-template <typename T, typename OT, bool FWD, int NU>
+template <typename T, typename OT, bool FWD, bool DOTS>
 int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   a.H = (int)s.H;
   a.L = s.L;
   a.units = s.B * s.H;
   a.nseg = segments(s);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
-  constexpr int N = sizeof(T) == 2 ? NU : 1;
   if (a.F <= 64)
-    return a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 1, FWD, N>(a, ws, sp, init, last, stream);
-  return a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, N>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 2, FWD, N>(a, ws, sp, init, last, stream);
+    return a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream);
+  return a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, DOTS>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 2, FWD, DOTS>(a, ws, sp, init, last, stream);
 }
 
 template <typename T>
@@ -992,7 +1051,7 @@ int forward(const Sizes& s, const void* q, const void* k, const void* v, const v
   a.F = (int)s.V;
   a.se = (int)s.V;
   a.sf = 1;
-  return walk<T, T, true, 3>(a, s, ws, sp, state, last, stream);
+  return walk<T, T, true, false>(a, s, ws, sp, state, last, stream);
 }
 
 // dq or dk: a walk over K's columns with V contracted, the dots of the gate's gradient beside it.
@@ -1015,7 +1074,7 @@ int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<c
   a.anchor_dots = (float*)(ws + sp.anchor_dots);
   a.anchor_chunks = anchor_chunks(dtype);
   a.nanchor = (int)(((s.L + kC - 1) / kC + a.anchor_chunks - 1) / a.anchor_chunks);
-  return walk<T, OT, FWD, 2>(a, s, ws, sp, init, nullptr, stream);
+  return walk<T, OT, FWD, true>(a, s, ws, sp, init, nullptr, stream);
 }
 
 template <typename T>
@@ -1036,7 +1095,7 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
     a.F = (int)s.V;
     a.se = (int)s.V;
     a.sf = 1;
-    const int rc = walk<T, T, false, 3>(a, s, ws, sp, dlast, dstate, stream);
+    const int rc = walk<T, T, false, false>(a, s, ws, sp, dlast, dstate, stream);
     if (rc != TSF_OK) return rc;
   }
   if (s.L == 0) return TSF_OK;
