@@ -37,6 +37,7 @@ constexpr int kC = 64;          // steps of a chunk
 constexpr int kThreads = 256;   // of the small kernels
 constexpr int kMaxWidth = 128;  // of K and V
 constexpr int kStepMaxK = 1024;  // of K in a single step
+constexpr int64_t kMaxStep = 1 << 23;  // elements between the steps of a row
 constexpr int kMaxGrid = (1 << 24) - 1;
 // log2 decay that stands for all smaller ones, -inf among them: 2^-300 is zero in fp32, and sums of
 // 64 such gates keep 1e-11 in their float64 sums
@@ -932,6 +933,13 @@ struct Sizes {
   int64_t B, L, H, Hk, K, V;
 };
 
+// Steps of a chunk are reached by 32-bit byte offsets from its first.
+bool steps_fit(const int64_t* strides, int tensors) {
+  for (int i = 0; i < tensors; ++i)
+    if (strides[3 * i + 1] < 0 || strides[3 * i + 1] > kMaxStep) return false;
+  return true;
+}
+
 int args_status(const Sizes& s, int dtype) {
   if (s.B < 0 || s.L < 0 || s.H < 1 || s.Hk < 1 || s.K < 1 || s.V < 1 || s.H % s.Hk != 0) return TSF_ERR_ARG;
   if (dtype != TSF_DTYPE_F32 && dtype != TSF_DTYPE_BF16) return TSF_ERR_ARG;
@@ -1148,6 +1156,7 @@ int tsfast_hip_gated_fwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K,
   if (rc != TSF_OK) return rc;
   if (B == 0) return TSF_OK;
   if (!strides || !state_last || (L > 0 && (!q || !k || !v || !g || !o))) return TSF_ERR_ARG;
+  if (!steps_fit(strides, 3)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, false);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
   return dtype == TSF_DTYPE_BF16 ? forward<bf16>(s, q, k, v, g, strides, state, o, state_last, (char*)workspace, sp, (hipStream_t)stream)
@@ -1163,6 +1172,7 @@ int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K,
   if (B == 0) return TSF_OK;
   if (!strides || (state && !grad_state)) return TSF_ERR_ARG;
   if (L > 0 && (!q || !k || !v || !g || !grad_o || !grad_q || !grad_k || !grad_v || !grad_g)) return TSF_ERR_ARG;
+  if (!steps_fit(strides, 3) || !steps_fit(strides + 12, 1)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, true);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
   return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state,

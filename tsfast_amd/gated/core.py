@@ -35,24 +35,21 @@ _AUTO_ORDER = {"cuda": ("hip",)}
 _CHUNK = 64  # steps whose products the torch path forms at once
 
 
-def _check_heads(q, k, v, g, lead: str):
-    """Shapes of a call; ``lead`` names the leading dimensions."""
-    n = len(lead.split(", "))
-    if v.dim() != n + 2:
-        raise ValueError(f"v must be [{lead}, H, V], got {tuple(v.shape)}")
-    if q.dim() != n + 2 or q.shape[:n] != v.shape[:n] or q.shape != k.shape:
-        raise ValueError(f"q and k must be alike, [{lead}, Hk, K] for v {tuple(v.shape)}; got {tuple(q.shape)} and {tuple(k.shape)}")
-    H, Hk = v.shape[-2], q.shape[-2]
-    if Hk < 1 or H % Hk != 0:
+def _check_shapes(q, k, v, g, state, lead: str):
+    """Shapes of a call whose leading dimensions (one or two) are ``lead``."""
+    qs, vs = q.shape, v.shape
+    n = 2 if lead == "B, L" else 1
+    if len(vs) != n + 2:
+        raise ValueError(f"v must be [{lead}, H, V], got {tuple(vs)}")
+    if len(qs) != n + 2 or qs[:n] != vs[:n] or qs != k.shape:
+        raise ValueError(f"q and k must be alike, [{lead}, Hk, K] for v {tuple(vs)}; got {tuple(qs)} and {tuple(k.shape)}")
+    H, Hk = vs[n], qs[n]
+    if Hk < 1 or H < 1 or H % Hk != 0:
         raise ValueError(f"{H} heads of v do not share {Hk} heads of q and k evenly")
-    if g.shape != v.shape[:-1]:
-        raise ValueError(f"g must be [{lead}, H] = {tuple(v.shape[:-1])}, got {tuple(g.shape)}")
-
-
-def _check_state(q, v, state):
-    want = (v.shape[0], v.shape[-2], q.shape[-1], v.shape[-1])
-    if tuple(state.shape) != want:
-        raise ValueError(f"state must be [B, H, K, V] = {want}, got {tuple(state.shape)}")
+    if g.shape != vs[:-1]:
+        raise ValueError(f"g must be [{lead}, H] = {tuple(vs[:-1])}, got {tuple(g.shape)}")
+    if state is not None and state.shape != (vs[0], H, qs[-1], vs[-1]):
+        raise ValueError(f"state must be [B, H, K, V] = {(vs[0], H, qs[-1], vs[-1])}, got {tuple(state.shape)}")
 
 
 def _wide(t):
@@ -102,9 +99,7 @@ def gated_recurrence(q, k, v, g, state=None):
     All of q, k, v must be finite: the fused kernel works in chunks of 64 steps, and a value that is not may
     reach every step of its chunk.
     """
-    _check_heads(q, k, v, g, "B, L")
-    if state is not None:
-        _check_state(q, v, state)
+    _check_shapes(q, k, v, g, state, "B, L")
     mod = resolve("gated.recurrence", _RECURRENCE_BACKENDS, _AUTO_ORDER.get(v.device.type, ()), (q, k, v, g, state))
     if mod is not None:
         return mod.run(q, k, v, g, state)
@@ -130,10 +125,9 @@ def gated_recurrence_step(q, k, v, g, state):
     Returns:
         ``o [B, H, V]``. For prediction: the step has no gradient, and asking for one is an error.
     """
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no gradient: call it under torch.no_grad(), or use gated_recurrence")
-    _check_heads(q, k, v, g, "B")
-    _check_state(q, v, state)
+    _check_shapes(q, k, v, g, state, "B")
     mod = resolve("gated.recurrence_step", _STEP_BACKENDS, _AUTO_ORDER.get(v.device.type, ()), (q, k, v, g, state))
     if mod is not None:
         return mod.run(q, k, v, g, state)

@@ -44,29 +44,44 @@ def supports(x, other, params, width: int) -> str | None:
 
 
 def _rows(t, D: int):
-    """``t`` as ``[rows, D]`` with dense columns, and its row stride."""
+    """``t`` as rows of ``D`` dense columns: a tensor that keeps them alive, their address and row stride."""
     if t is None:
-        return None, 0
+        return None, None, 0
+    if t.is_contiguous():
+        return t, t.data_ptr(), D
     t = t.reshape(-1, D)
     if t.stride(1) != 1 and D > 1:
         t = t.contiguous()
-    return t, t.stride(0)
+    return t, t.data_ptr(), t.stride(0)
 
 
 def _param(t):
     return None if t is None else t.float().contiguous()
 
 
-def _screen(x, *others):
-    if x.device.type != "cuda" or x.dtype not in _IO_DTYPES:
-        raise TypeError(f"x: {x.dtype} on {x.device}, expected float32 or bfloat16 on a GPU")
-    for name, t, dtypes in others:
-        if t is not None and (t.dtype not in dtypes or t.device != x.device):
-            raise TypeError(f"{name}: {t.dtype} on {t.device}, expected {dtypes} on {x.device}")
+def _screen(x, likes, params, residual=None):
+    """What a raw-pointer kernel relies on: x's type and device, ``likes`` of both, float32 dense ``params``."""
+    dtype, dev = x.dtype, x.get_device()
+    if dev < 0 or dtype not in _IO_DTYPES:
+        raise TypeError(f"x: {dtype} on {x.device}, expected float32 or bfloat16 on a GPU")
+    for t in likes:
+        if t is not None and (t.dtype != dtype or t.get_device() != dev):
+            raise TypeError(f"{t.dtype} on {t.device}, expected {dtype} on {x.device}")
+    if residual is not None and (residual.dtype not in (dtype, torch.float32) or residual.get_device() != dev):
+        raise TypeError(f"residual: {residual.dtype} on {residual.device}, expected {dtype} or float32 on {x.device}")
+    for t in params:
+        if t is not None and (t.dtype != torch.float32 or t.get_device() != dev or not t.is_contiguous()):
+            raise TypeError(f"a parameter is {t.dtype} on {t.device}, expected dense float32 on {x.device}")
 
 
 def _empty(t):
+    if t.is_contiguous():
+        return torch.empty_like(t)  # the cheaper call
     return torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 @custom_op("tsfast_hip::gated_norm")
@@ -74,15 +89,14 @@ def _gated_op(
     x: torch.Tensor, gate: torch.Tensor | None, weight: torch.Tensor | None, groups: int, eps: float, gate_first: bool
 ) -> torch.Tensor:
     lib = _lib.load()
-    _screen(x, ("gate", gate, (x.dtype,)))
-    _lib.require(weight, "weight", (torch.float32,), x.device)
+    _screen(x, (gate,), (weight,))
     D = x.shape[-1]
     y = _empty(x)
-    (x2, sx), (g2, sg) = _rows(x, D), _rows(gate, D)
+    (_x, px, sx), (_g, pg, sg) = _rows(x, D), _rows(gate, D)
     _lib.check(
         lib.tsfast_hip_gated_norm_fwd(
-            x2.shape[0], groups, D // groups, _IO_DTYPES[x.dtype], gate_first, eps, _lib.ptr(x2), sx, _lib.ptr(g2), sg,
-            _lib.ptr(weight), _lib.ptr(y), _lib.stream_of(x),
+            x.numel() // D, groups, D // groups, _IO_DTYPES[x.dtype], gate_first, eps, px, sx, pg, sg, _ptr(weight), y.data_ptr(),
+            _lib.stream_of(x),
         ),
         "tsfast_hip_gated_norm_fwd",
     )
@@ -99,19 +113,19 @@ def _gated_bwd_op(
     gy: torch.Tensor, x: torch.Tensor, gate: torch.Tensor | None, weight: torch.Tensor | None, groups: int, eps: float, gate_first: bool
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     lib = _lib.load()
-    _screen(x, ("gate", gate, (x.dtype,)), ("gy", gy, (x.dtype,)))
-    _lib.require(weight, "weight", (torch.float32,), x.device)
+    _screen(x, (gate, gy), (weight,))
     D = x.shape[-1]
+    rows = x.numel() // D
     gx = _empty(x)
     ggate = None if gate is None else _empty(gate)
-    gw = None if weight is None else _empty(weight)
-    (x2, sx), (g2, sg), (d2, sd) = _rows(x, D), _rows(gate, D), _rows(gy, D)
-    nbytes = lib.tsfast_hip_gated_norm_workspace_bytes(x2.shape[0], groups, D // groups) if weight is not None else 0
+    gw = None if weight is None else torch.empty_like(weight)
+    (_x, px, sx), (_g, pg, sg), (_d, pd, sd) = _rows(x, D), _rows(gate, D), _rows(gy, D)
+    nbytes = lib.tsfast_hip_gated_norm_workspace_bytes(rows, groups, D // groups) if weight is not None else 0
     ws = _lib.workspace(nbytes, x.device) if nbytes > 0 else None
     _lib.check(
         lib.tsfast_hip_gated_norm_bwd(
-            x2.shape[0], groups, D // groups, _IO_DTYPES[x.dtype], gate_first, eps, _lib.ptr(x2), sx, _lib.ptr(g2), sg,
-            _lib.ptr(weight), _lib.ptr(d2), sd, *map(_lib.ptr, (gx, ggate, gw, ws)), nbytes, _lib.stream_of(x),
+            rows, groups, D // groups, _IO_DTYPES[x.dtype], gate_first, eps, px, sx, pg, sg, _ptr(weight), pd, sd, gx.data_ptr(),
+            _ptr(ggate), _ptr(gw), _ptr(ws), nbytes, _lib.stream_of(x),
         ),
         "tsfast_hip_gated_norm_bwd",
     )
@@ -156,16 +170,14 @@ def _residual_op(
     eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     lib = _lib.load()
-    _screen(x, ("residual", residual, (x.dtype, torch.float32)))
-    for name, t in (("weight", weight), ("post_weight", post_weight), ("scale", scale)):
-        _lib.require(t, name, (torch.float32,), x.device)
+    _screen(x, (), (weight, post_weight, scale), residual)
     D = x.shape[-1]
     new, y = _empty(residual), _empty(x)
-    (x2, sx), (r2, sr) = _rows(x, D), _rows(residual, D)
+    (_x, px, sx), (_r, pr, sr) = _rows(x, D), _rows(residual, D)
     _lib.check(
         lib.tsfast_hip_residual_norm_fwd(
-            x2.shape[0], D, _IO_DTYPES[x.dtype], _IO_DTYPES[residual.dtype], eps, _lib.ptr(x2), sx, _lib.ptr(r2), sr,
-            *map(_lib.ptr, (post_weight, scale, weight, new, y)), _lib.stream_of(x),
+            x.numel() // D, D, _IO_DTYPES[x.dtype], _IO_DTYPES[residual.dtype], eps, px, sx, pr, sr, _ptr(post_weight), _ptr(scale),
+            _ptr(weight), new.data_ptr(), y.data_ptr(), _lib.stream_of(x),
         ),
         "tsfast_hip_residual_norm_fwd",
     )
@@ -189,21 +201,21 @@ def _residual_bwd_op(
     eps: float,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     lib = _lib.load()
-    _screen(x, ("residual", residual, (x.dtype, torch.float32)), ("gnew", gnew, (residual.dtype,)), ("gy", gy, (x.dtype,)))
-    for name, t in (("weight", weight), ("post_weight", post_weight), ("scale", scale)):
-        _lib.require(t, name, (torch.float32,), x.device)
+    _screen(x, (gy,), (weight, post_weight, scale), residual)
+    if gnew is not None and (gnew.dtype != residual.dtype or gnew.device != x.device):
+        raise TypeError(f"gnew: {gnew.dtype} on {gnew.device}, expected {residual.dtype} on {x.device}")
     D = x.shape[-1]
+    rows = x.numel() // D
     gx, gres = _empty(x), _empty(residual)
     params = (post_weight, scale, weight)
-    gparams = [None if t is None else _empty(t) for t in params]
-    (x2, sx), (r2, sr), (n2, sn), (d2, sd) = _rows(x, D), _rows(residual, D), _rows(gnew, D), _rows(gy, D)
-    nbytes = lib.tsfast_hip_residual_norm_workspace_bytes(x2.shape[0], D)
+    gparams = [None if t is None else torch.empty_like(t) for t in params]
+    (_x, px, sx), (_r, pr, sr), (_n, pn, sn), (_d, pd, sd) = _rows(x, D), _rows(residual, D), _rows(gnew, D), _rows(gy, D)
+    nbytes = lib.tsfast_hip_residual_norm_workspace_bytes(rows, D)
     ws = _lib.workspace(nbytes, x.device)
     _lib.check(
         lib.tsfast_hip_residual_norm_bwd(
-            x2.shape[0], D, _IO_DTYPES[x.dtype], _IO_DTYPES[residual.dtype], eps, _lib.ptr(x2), sx, _lib.ptr(r2), sr,
-            *map(_lib.ptr, params), _lib.ptr(n2), sn, _lib.ptr(d2), sd, *map(_lib.ptr, (gx, gres, *gparams, ws)), nbytes,
-            _lib.stream_of(x),
+            rows, D, _IO_DTYPES[x.dtype], _IO_DTYPES[residual.dtype], eps, px, sx, pr, sr, *map(_ptr, params), pn, sn, pd, sd,
+            gx.data_ptr(), gres.data_ptr(), *map(_ptr, gparams), _ptr(ws), nbytes, _lib.stream_of(x),
         ),
         "tsfast_hip_residual_norm_bwd",
     )

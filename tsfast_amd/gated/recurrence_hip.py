@@ -26,19 +26,19 @@ _IO_DTYPES = {torch.float32: _lib.TSF_DTYPE_F32, torch.bfloat16: _lib.TSF_DTYPE_
 _MAX_WIDTH = 128
 _STEP_MAX_K = 1024
 _MAX_GRID = (1 << 24) - 1
+_MAX_STEP = 1 << 23  # elements between the steps of a row
 
 
 def _tensor_reason(q, k, v, g, state) -> str | None:
-    dev = v.device
+    dtype, dev = v.dtype, v.device
     if dev.type != "cuda":
         return f"v on {dev.type}, hip backend is GPU-only"
-    if v.dtype not in _IO_DTYPES:
-        return f"v dtype {v.dtype} not float32/bfloat16"
-    for name, t in (("q", q), ("k", k), ("g", g)):
-        if t.dtype != v.dtype:
-            return f"{name} dtype {t.dtype} != v dtype {v.dtype}"
-        if t.device != dev:
-            return f"{name} on {t.device}, v on {dev}"
+    if dtype not in _IO_DTYPES:
+        return f"v dtype {dtype} not float32/bfloat16"
+    if q.dtype != dtype or k.dtype != dtype or g.dtype != dtype:
+        return f"q dtype {q.dtype}, k dtype {k.dtype} or g dtype {g.dtype} != v dtype {dtype}"
+    if q.device != dev or k.device != dev or g.device != dev:
+        return f"q on {q.device}, k on {k.device} or g on {g.device}, v on {dev}"
     if state is not None:
         if state.dtype != torch.float32:
             return f"needs float32 state, got {state.dtype}"
@@ -84,14 +84,15 @@ def supports_step(q, k, v, g, state) -> str | None:
 
 
 def _dense(t):
-    """``t`` with a dense last dimension, the only one the kernels read without a stride."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """``t`` with a dense last dimension, the only one the kernels read without a stride, and steps that 64-step chunks
+    reach with 32-bit offsets."""
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) <= _MAX_STEP):
+        return t
+    return t.contiguous()
 
 
-def _strides(*ts):
-    """The leading strides of q, k, v .. [.., width] and of g (three each; two in a step), as a C array."""
-    s = [n for t, dims in ts for n in t.stride()[:dims]]
-    return (ctypes.c_int64 * len(s))(*s)
+# the leading strides of q, k, v, g (and go): batch row, step and head; batch row and head in a step
+_Strides8, _Strides12, _Strides15 = (ctypes.c_int64 * n for n in (8, 12, 15))
 
 
 def _workspace(nbytes: int, t):
@@ -99,11 +100,12 @@ def _workspace(nbytes: int, t):
 
 
 def _screen(v, *others):
-    if v.device.type != "cuda" or v.dtype not in _IO_DTYPES:
-        raise TypeError(f"v: {v.dtype} on {v.device}, expected float32 or bfloat16 on a GPU")
-    for name, t in others:
-        if t.dtype != v.dtype or t.device != v.device:
-            raise TypeError(f"{name}: {t.dtype} on {t.device}, expected {v.dtype} on {v.device}")
+    dtype, dev = v.dtype, v.get_device()
+    if dev < 0 or dtype not in _IO_DTYPES:
+        raise TypeError(f"v: {dtype} on {v.device}, expected float32 or bfloat16 on a GPU")
+    for t in others:
+        if t.dtype != dtype or t.get_device() != dev:
+            raise TypeError(f"{t.dtype} on {t.device}, expected {dtype} on {v.device}")
 
 
 @custom_op("tsfast_hip::gated_recurrence")
@@ -111,7 +113,7 @@ def _recurrence_op(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor | None
 ) -> tuple[torch.Tensor, torch.Tensor]:
     lib = _lib.load()
-    _screen(v, ("q", q), ("k", k), ("g", g))
+    _screen(v, q, k, g)
     q, k, v = _dense(q), _dense(k), _dense(v)
     state = None if state is None else state.contiguous()
     _lib.require(state, "state", (torch.float32,), v.device)
@@ -124,7 +126,7 @@ def _recurrence_op(
     ws = _workspace(nbytes, v)
     _lib.check(
         lib.tsfast_hip_gated_fwd(
-            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g)), _strides((q, 3), (k, 3), (v, 3), (g, 3)),
+            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g)), _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()),
             *map(_lib.ptr, (state, o, last, ws)), nbytes, _lib.stream_of(v),
         ),
         "tsfast_hip_gated_fwd",
@@ -149,7 +151,7 @@ def _recurrence_bwd_op(
     state: torch.Tensor | None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     lib = _lib.load()
-    _screen(v, ("q", q), ("k", k), ("g", g), ("go", go))
+    _screen(v, q, k, g, go)
     q, k, v, go = _dense(q), _dense(k), _dense(v), _dense(go)
     state, glast = (None if t is None else t.contiguous() for t in (state, glast))
     _lib.require(state, "state", (torch.float32,), v.device)
@@ -164,7 +166,8 @@ def _recurrence_bwd_op(
     ws = _workspace(nbytes, v)
     _lib.check(
         lib.tsfast_hip_gated_bwd(
-            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g, go)), _strides((q, 3), (k, 3), (v, 3), (g, 3), (go, 3)),
+            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g, go)), 
+            _Strides15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *go.stride()[:3]),
             *map(_lib.ptr, (state, glast, gq, gk, gv, gg, gstate, ws)), nbytes, _lib.stream_of(v),
         ),
         "tsfast_hip_gated_bwd",
@@ -202,16 +205,17 @@ def run(q, k, v, g, state):
 @custom_op("tsfast_hip::gated_recurrence_step", mutates_args=("state",))
 def _step_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     lib = _lib.load()
-    _screen(v, ("q", q), ("k", k), ("g", g))
-    _lib.require(state, "state", (torch.float32,), v.device)
+    _screen(v, q, k, g)
+    if state.dtype != torch.float32 or state.get_device() != v.get_device() or not state.is_contiguous():
+        raise TypeError(f"state: {state.dtype} on {state.device}, expected dense float32 on {v.device}")
     q, k, v = _dense(q), _dense(k), _dense(v)
     B, H, V = v.shape
-    Hk, K = q.shape[1:]
+    _, Hk, K = q.shape
     o = torch.empty(B, H, V, device=v.device, dtype=v.dtype)
     _lib.check(
         lib.tsfast_hip_gated_step(
-            B, H, Hk, K, V, _IO_DTYPES[v.dtype], *map(_lib.ptr, (q, k, v, g)), _strides((q, 2), (k, 2), (v, 2), (g, 2)),
-            _lib.ptr(state), _lib.ptr(o), _lib.stream_of(v),
+            B, H, Hk, K, V, _IO_DTYPES[v.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+            _Strides8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *g.stride()), state.data_ptr(), o.data_ptr(), _lib.stream_of(v),
         ),
         "tsfast_hip_gated_step",
     )
