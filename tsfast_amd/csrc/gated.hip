@@ -799,9 +799,10 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 }
 
 // Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards). `threads`,
-// `et` and `fw` are the walk's; a thread owns one f32x4 of a state.
+// `et` and `fw` are the walk's; a thread owns one f32x4 of a state. `turned`, if any, gets the same states as the walk over the other
+// columns holds them (rows and columns exchanged; `et_turned` and `fw_turned` are that walk's).
 __global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int fw, int E, int F, int se,
-                                                   int sf, int64_t total, int backward) {
+                                                   int sf, int64_t total, int backward, float* turned, int et_turned, int fw_turned) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;
   const int per = threads * et * fw;
@@ -816,10 +817,18 @@ __global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* dec
   f32x4* p = seg + (bh * nseg + (backward ? nseg - 1 : 0)) * per + in;
   const double* d = decay + bh * nseg + (backward ? nseg - 1 : 0);
   const int64_t step = backward ? -(int64_t)per : per;
+  // the place of (e, col), (e + 1, col) .. in a turned state: columns e .., row col
+  const int tile = e / 16;
+  float* t = turned ? turned + ((bh * nseg + (backward ? nseg - 1 : 0)) * per +
+                                (tile % fw_turned * et_turned + col / 16) * threads + tile / fw_turned * 64 + (col % 16 / 4) * 16 + e % 16) * 4 + col % 4
+                    : nullptr;
 #pragma unroll 4
   for (int n = 0; n < nseg; ++n) {
     const f32x4 own = p[n * step];
     p[n * step] = s;
+    if (t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[n * step * 4 + r * 4] = s[r];
     s = fast_exp2((float)d[backward ? -n : n]) * s + own;
   }
 }
@@ -956,10 +965,13 @@ int args_status(const Sizes& s, int dtype) {
 int waves(int64_t) { return 4; }
 
 // Segments a row is cut into. A cut row is walked twice (its segments' states first), so rows are cut only to give
-// every CU its two workgroups, into no more than fit at once and into four chunks at least.
-int segments(const Sizes& s) {
+// every CU the workgroups it holds, into no more than fit at once (86 instead of 85 segments of 6 rows took twice the time) and
+// into four chunks at least. Measured, forward and backward: 32 rows of 4096 steps, 128 x 128, bf16: 1 segment 330 + 1180 us, 5:
+// 180 + 590; 384 rows of 1024 steps, 64 x 64: 1 segment 64 + 229, 4: 87 + 283.
+int segments(const Sizes& s, int dtype) {
   const int64_t chunks = (s.L + kC - 1) / kC, rows = s.B * s.H;
-  int64_t n = rows > 0 ? 2 * (int64_t)device_cus() / rows : 1;
+  const int per_cu = dtype == TSF_DTYPE_BF16 && s.K <= 64 && s.V <= 64 ? 3 : 2;
+  int64_t n = rows > 0 ? per_cu * (int64_t)device_cus() / rows : 1;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   const int64_t per = (chunks + n - 1) / n;
@@ -974,14 +986,14 @@ int anchor_chunks(int dtype) { return dtype == TSF_DTYPE_BF16 ? 16 : 4; }
 
 int64_t align_up(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
-// Workspace: [segment states][segment decays] of the widest walk; backward also [r][c][anchors][anchor dots][dq, dk per head].
+// Workspace: [segment states][segment decays]; backward also [segment states, turned][r][c][anchors][anchor dots][dq, dk per head].
 struct Space {
-  int64_t seg, decay, r, c, anchors, anchor_dots, dq, dk, bytes;
+  int64_t seg, decay, turned, r, c, anchors, anchor_dots, dq, dk, bytes;
 };
 Space space(const Sizes& s, int dtype, bool backward) {
   Space w = {};
   int64_t at = 0;
-  const int64_t bh = s.B * s.H, state = padded_state(s.K, s.V) * 4, nseg = segments(s);
+  const int64_t bh = s.B * s.H, state = padded_state(s.K, s.V) * 4, nseg = segments(s, dtype);
   auto take = [&](int64_t n) {
     const int64_t p = at;
     at += align_up(n);
@@ -990,6 +1002,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
   if (nseg > 1) {
     w.seg = take(bh * nseg * state);
     w.decay = take(bh * nseg * 8);
+    if (backward) w.turned = take(bh * nseg * state);
   }
   if (backward) {
     const int64_t chunks = (s.L + kC - 1) / kC, ac = anchor_chunks(dtype), na = (chunks + ac - 1) / ac;
@@ -1006,21 +1019,26 @@ Space space(const Sizes& s, int dtype, bool backward) {
   return w;
 }
 
+// One walk, cut rows' segment states first. dv's and dk's walks, backwards both, have the same states between segments with
+// rows and columns exchanged: dv's, the first to run, leaves them for dk's.
 template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool DOTS>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
   const int64_t bh = a.units;
   a.units = bh * a.nseg;
-  if (a.nseg > 1) {
+  if (a.nseg == 1) {
+    a.init = init;
+  } else if constexpr (!FWD && DOTS) {  // dk's, after dv's
+    a.seg_init = (const f32x4*)(ws + sp.turned);
+  } else {
     WalkArgs<T, OT> p = a;
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
     p.seg_decay = (double*)(ws + sp.decay);
     walk_kernel<T, OT, E, NW, FW, FWD, true, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
     const int64_t total = bh * E / 16 * 64 * NW * FW;
-    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD);
+    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
+                                                                  FWD ? nullptr : (float*)(ws + sp.turned), FW * NW, E / 16 / NW);
     a.seg_init = seg;
-  } else {
-    a.init = init;
   }
   a.last = last;
   walk_kernel<T, OT, E, NW, FW, FWD, false, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
@@ -1033,7 +1051,7 @@ int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const flo
   a.H = (int)s.H;
   a.L = s.L;
   a.units = s.B * s.H;
-  a.nseg = segments(s);
+  a.nseg = segments(s, sizeof(T) == 2 ? TSF_DTYPE_BF16 : TSF_DTYPE_F32);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
   if (a.F <= 64)
     return a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream);
