@@ -101,6 +101,15 @@ def test_residual_norm_torch_path(post, scale):
         assert _rel(got, ref) < 1e-11
 
 
+@pytest.mark.parametrize("first", [False, True])
+def test_norm_gradients_agree_with_differences(first):
+    r = torch.Generator().manual_seed(7)
+    x, z = (torch.randn(3, 8, generator=r, dtype=torch.float64, requires_grad=True) for _ in range(2))
+    w, p, s = (torch.rand(8, generator=r, dtype=torch.float64).add(0.5).requires_grad_() for _ in range(3))
+    assert torch.autograd.gradcheck(lambda x, z, w: gated.gated_norm(x, z, w, groups=2, gate_first=first), (x, z, w))
+    assert torch.autograd.gradcheck(lambda x, z, w, p, s: gated.residual_norm(x, z, w, post_weight=p, scale=s), (x, z, w, p, s))
+
+
 def test_refusals():
     q, k, v, g, state, *_ = _inputs(2, 5, 4, 2, 3, 6)
     ok = gated.gated_recurrence

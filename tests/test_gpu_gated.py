@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from oracle import gated_oracle as G
-from tsfast_amd import dispatch, gated
+from tsfast_amd import _lib, dispatch, gated
 from tsfast_amd.gated import core, recurrence_hip
 
 pytestmark = pytest.mark.gpu
@@ -65,7 +65,7 @@ def _check(q, k, v, g, state, go, gl):
         (1, 1, 1, 1, 1, 1), (2, 2, 3, 1, 3, 5), (1, 16, 2, 2, 16, 16), (3, 63, 1, 1, 33, 17), (1, 64, 2, 2, 64, 64),
         (2, 65, 4, 2, 48, 80), (1, 128, 1, 1, 128, 128), (2, 129, 6, 3, 65, 127), (5, 200, 2, 1, 100, 24), (1, 300, 12, 4, 20, 128),
         (1, 1000, 1, 1, 128, 100), (1, 2050, 2, 1, 40, 72), (1, 511, 2, 2, 7, 128), (1, 512, 1, 1, 72, 8), (1, 513, 1, 1, 127, 65),
-        (300, 70, 2, 2, 16, 16),
+        (300, 70, 2, 2, 16, 16), (1, 1300, 2, 1, 33, 64), (2, 900, 1, 1, 64, 20), (1, 4000, 1, 1, 64, 100), (1, 700, 3, 3, 4, 6),
     ],
 )
 def test_matches_the_oracle(gpu, B, L, H, Hk, K, V, dtype):
@@ -190,6 +190,51 @@ def test_offsets_beyond_32_bits(gpu):
         at += 4096 + 8 * w
     a, b = _run(*views, s, go, gl), _run(q, k, v, g, s, go, gl)
     assert torch.equal(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[2], b[2]))
+
+
+def test_steps_far_apart_are_copied(gpu):
+    """Steps beyond the 32-bit offsets of a chunk: the Python side copies, the library refuses."""
+    q, k, v, g, s, go, gl = _inputs(1, 3, 1, 1, 16, 16, torch.bfloat16)
+    far = recurrence_hip._MAX_STEP + 8
+    big = torch.zeros(4 * far, device="cuda", dtype=torch.bfloat16)
+    view = big.as_strided(v.shape, (3 * far, far, 16, 1))
+    view.copy_(v)
+    a, b = _run(q, k, view, g, s, go, gl), _run(q, k, v, g, s, go, gl)
+    assert torch.equal(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[2], b[2]))
+    strides = recurrence_hip._Strides12(*q.stride()[:3], *k.stride()[:3], *view.stride()[:3], *g.stride())
+    o, last = torch.empty_like(v), torch.empty_like(s)
+    ptrs = [t.data_ptr() for t in (q, k, view, g)]
+    status = _lib.load().tsfast_hip_gated_fwd(1, 3, 1, 1, 16, 16, 1, *ptrs, strides, None, o.data_ptr(), last.data_ptr(), None, 0, _lib.stream_of(v))
+    assert status == -3
+
+
+@pytest.mark.parametrize("dtype", _DTYPES)
+def test_gradients_against_differences(gpu, dtype):
+    """Central differences of the kernel's own forward over a random direction of each input, the loss summed in float64.
+    A step of 1/8 along directions of the inputs' size: the loss is a polynomial of q, k, v and the state (exact for one
+    input at a time up to second order), and exp's third order adds below 1e-2 for g's; bfloat16 outputs, rounded at 2^-9,
+    leave noise of sqrt(outputs) 2^-9 on sums of as many terms."""
+    q, k, v, g, s, go, gl = _inputs(2, 150, 2, 1, 24, 32, dtype)
+    g = g - 0.1  # no decay near 0, where a step would cross it
+    _, _, grads = _run(q, k, v, g, s, go, gl)
+
+    def loss(*a):
+        o, last = gated.gated_recurrence(*a)
+        return float((o.double() * go.double()).sum() + (last.double() * gl.double()).sum())
+
+    r = torch.Generator().manual_seed(11)
+    for n, t in enumerate((q, k, v, g, s)):
+        d = torch.randn(t.shape, generator=r).to(t) * (0.5 if n < 3 else 0.02 if n == 3 else 0.5)
+        ends = []
+        for sign in (1, -1):
+            moved = [q, k, v, g, s]
+            moved[n] = (t.double() + sign * 0.125 * d.double()).to(t.dtype)
+            ends.append((moved[n].double(), loss(*moved)))
+        step = ends[0][0] - ends[1][0]  # what rounding made of it
+        want, got = ends[0][1] - ends[1][1], float((grads[n].double() * step).sum())
+        scale = float((grads[n].double() * step).norm())  # of a sum of such terms with random signs
+        noise = 0.0 if dtype == torch.float32 else 2**-8 * float(go.double().norm()) * float(v.double().abs().mean()) * 2
+        assert abs(got - want) < 0.05 * scale + 0.01 * abs(want) + noise, n
 
 
 @pytest.mark.parametrize("dtype", _DTYPES)

@@ -13,18 +13,28 @@
 //                                     backward in time (j >= i):  dv (k, q, do), dk (v, do, q)
 //
 // so one kernel, walk_kernel, computes all four. A workgroup owns one head of one row and a run of 64-step chunks; the
-// state stays in fp32 accumulator registers from the first
-// chunk to the last and is never written in between. Per chunk the decayed scores of x and y within
-// it (64 x 64, the causal half only) times z, x times the state before it, and the state's update are MFMA
-// products; the decays come from exact differences of a float64 running sum, so any g <= 0 down to -inf
-// keeps its accuracy.
+// state stays in fp32 accumulator registers from the first chunk to the last and is never written in between. Per chunk
+// the decayed scores of x and y within it (64 x 64, the causal half only) times z, x times the state before it, and the
+// state's update are MFMA products; the decays come from exact differences of a float64 running sum, so any g <= 0 down
+// to -inf keeps its accuracy. Few rows are cut into segments: a walk of the state alone, a join of the segments' states, the
+// walk proper.
 //
-// dg needs no product of its own: r_t = q_t . dq_t and c_t = k_t . dk_t, summed while dq and dk are still in
-// registers, give dg_{t+1} = dg_t - r_t + c_t. The rounding errors of that running sum are cut off at
-// anchors every kAnchor chunks, where dg_t = <S_{t-1}, dL/dS_{t-1}> is formed from the two states.
+// dg needs no product of its own: r_t = q_t . dq_t and c_t = k_t . dk_t, summed from dq and dk before they are rounded, give
+// dg_{t+1} = dg_t - r_t + c_t. The rounding errors of that running sum are cut off at anchors every few chunks, where
+// dg_t = <S_{t-1}, dL/dS_{t-1}> is formed from the two states.
+//
+// bf16 inputs are multiplied on the bf16 matrix cores. Products of inputs are exact there; what is fp32 (the decayed
+// scores, the state, the decayed z of an update) goes in as a sum of two or three bf16 operands, because one alone (2^-9)
+// would cost the outputs 1.4 times their own rounding, the fp32 state its type, and dg, a difference of near sums, far more.
+// fp32 inputs use the fp32 matrix cores.
+//
+// Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 290 us for o's walk and 125 us for the segment
+// states before it, 290 for dv's, 330 and 340 for dq's and dk's. No one unit bounds a chunk (3.4 us a workgroup at two on a CU):
+// of it matrix products take 1.4 us, LDS 1.1 us and vector instructions about as much, waits for memory the rest. Kept
+// out, for they measured slower: the state in LDS as well (2 times), transposed copies of y and z in LDS instead of
+// transposing reads (2 times, for their bank conflicts), eight waves of one column tile each (1.3 times),
+// outputs stored from accumulators, 8 bytes a lane (1.35 times).
 #include <math.h>
-
-#include <type_traits>
 
 #include "common.h"
 #include "tsfast_hip.h"
@@ -33,10 +43,10 @@ using namespace tsf;
 
 namespace {
 
-constexpr int kC = 64;          // steps of a chunk
-constexpr int kThreads = 256;   // of the small kernels
-constexpr int kMaxWidth = 128;  // of K and V
-constexpr int kStepMaxK = 1024;  // of K in a single step
+constexpr int kC = 64;                 // steps of a chunk
+constexpr int kThreads = 256;          // of the small kernels
+constexpr int kMaxWidth = 128;         // of K and V
+constexpr int kStepMaxK = 1024;        // of K in a single step
 constexpr int64_t kMaxStep = 1 << 23;  // elements between the steps of a row
 constexpr int kMaxGrid = (1 << 24) - 1;
 // log2 decay that stands for all smaller ones, -inf among them: 2^-300 is zero in fp32, and sums of
@@ -604,6 +614,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 #pragma unroll
     for (int p = 0; p < ZP; ++p) s.z.put_plain(z_lds, p * kRowsZ / 16, pz[p]);
     __syncthreads();
+    if (n + 1 < chunks) fetch_chunk(c + kStep);  // before the outputs' stores, which the loads would wait behind
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
     f32x4 acc[FW][4];  // outputs, transposed: columns f + 16 fw of z by steps i = 16 it + li
@@ -681,7 +692,6 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     if constexpr (!STATE_ONLY) __syncthreads();
 
     if constexpr (!STATE_ONLY) {
-      if (n + 1 < chunks) fetch_chunk(c + kStep);  // before the outputs' stores, which the loads would wait behind
       // the scores times z
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -715,9 +725,6 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
           }
         }
     }
-    if constexpr (STATE_ONLY)
-      if (n + 1 < chunks) fetch_chunk(c + kStep);
-
     // the state: S = tot S + sum_j y_j (w_j z_j)^T
     const float tot = FWD ? s.in[buf][kC - 1] : s.w[buf][kC - 1];  // the whole chunk's decay
 #pragma unroll
@@ -891,13 +898,15 @@ struct StepArgs {
   int H, share, K, V, ntile;
 };
 
-// One step: a workgroup owns LANES 4-column pieces of one head's state; its threads split the K rows and
-// each reads and writes its elements of the state once.
-template <typename T, int LANES>
+// One step: a workgroup owns 64 columns of one head's state, 16 threads a row of them and 16 rows at a time; each
+// thread reads and writes its elements of the state once, in 16-byte pieces at any alignment, and HBM bounds it. For 256
+// rows of 12 heads of 128 x 128: 60 us, 403 MB. Tiles of 16 and 128 columns took 108 and 60 us there, 11.5 and 7.4 against
+// 6.6 us for 16 rows, 4.0 and 4.0 against 3.4 us for one row of 4 heads of 64 x 64.
+constexpr int kStepLanes = 16, kStepRows = kThreads / kStepLanes;
+template <typename T>
 __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
-  constexpr int kRows = kThreads / LANES;
   __shared__ float qs[kStepMaxK], ks[kStepMaxK];
-  __shared__ f32x4 part[kRows][LANES];
+  __shared__ f32x4 part[kStepRows][kStepLanes];
   const int tile = blockIdx.x % a.ntile;
   const int64_t bh = blockIdx.x / a.ntile, b = bh / a.H;
   const int h = (int)(bh % a.H), hk = h / a.share;
@@ -907,8 +916,8 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
     qs[i] = to_f32(q[i]);
     ks[i] = to_f32(k[i]);
   }
-  const int lane = threadIdx.x % LANES, row = threadIdx.x / LANES;
-  const int col = (tile * LANES + lane) * 4, n = a.V - col;
+  const int lane = threadIdx.x % kStepLanes, row = threadIdx.x / kStepLanes;
+  const int col = (tile * kStepLanes + lane) * 4, n = a.V - col;
   const f32x4 v = n > 0 ? load4((const T*)a.v + b * a.vb + h * a.vh + col, n) : f32x4{0, 0, 0, 0};
   const float decay = fast_exp2(to_f32(((const T*)a.g)[b * a.gb + h * a.gh]) * kLog2e);
   __syncthreads();
@@ -916,7 +925,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
   if (n > 0) {
     float* st = a.state + bh * a.K * a.V + col;
 #pragma unroll 8
-    for (int i = row; i < a.K; i += kRows) {
+    for (int i = row; i < a.K; i += kStepRows) {
       f32x4 s = load4(st + (int64_t)i * a.V, n);
       const float kk = ks[i], qq = qs[i];
 #pragma unroll
@@ -931,7 +940,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(StepArgs a) {
   __syncthreads();
   if (row == 0 && n > 0) {
 #pragma unroll
-    for (int r = 1; r < kRows; ++r) sum += part[r][lane];
+    for (int r = 1; r < kStepRows; ++r) sum += part[r][lane];
     store4((T*)a.o + bh * a.V + col, sum, n);
   }
 }
@@ -961,8 +970,8 @@ int args_status(const Sizes& s, int dtype) {
   return TSF_OK;
 }
 
-// Waves of a walk over F columns: a workgroup takes all of them, so that nothing of x and y is done twice.
-int waves(int64_t) { return 4; }
+// Waves of a walk: a workgroup takes all of its columns, so that nothing of x and y is done twice.
+constexpr int kWaves = 4;
 
 // Segments a row is cut into. A cut row is walked twice (its segments' states first), so rows are cut only to give
 // every CU the workgroups it holds, into no more than fit at once (86 instead of 85 segments of 6 rows took twice the time) and
@@ -980,8 +989,8 @@ int segments(const Sizes& s, int dtype) {
 
 int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
 
-// Chunks between dg's anchors: an anchor's states cost 8 bytes a state element, the running sum's errors
-// grow with the root of the distance; fp32 gates want the smaller error.
+// Chunks between dg's anchors: an anchor's states cost 8 bytes a state element, the running sum's errors grow with the root
+// of the distance, and what is rounded to bf16 can bear 16 chunks of them (4 e-4 of its size at worst here), fp32 four.
 int anchor_chunks(int dtype) { return dtype == TSF_DTYPE_BF16 ? 16 : 4; }
 
 int64_t align_up(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -1009,7 +1018,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
     w.r = take(bh * s.L * 4);
     w.c = take(bh * s.L * 4);
     w.anchors = take(bh * na * state);
-    w.anchor_dots = take(waves(s.K) * bh * na * 4);
+    w.anchor_dots = take(kWaves * bh * na * 4);
     if (s.H != s.Hk) {
       w.dq = take(s.B * s.L * s.H * s.K * 4);
       w.dk = take(s.B * s.L * s.H * s.K * 4);
@@ -1148,7 +1157,7 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
   const int ac = anchor_chunks(dtype);
   const int na = (int)(((s.L + kC - 1) / kC + ac - 1) / ac);
   dgate_kernel<T><<<(unsigned)(s.B * s.H * na), kThreads, 0, stream>>>(r, c, (const float*)(ws + sp.anchor_dots), G, Seq<T>{(T*)dg, s.L * s.H, s.H, 1, 1},
-                                                                       (int)s.H, s.L, s.B * s.H, waves(s.K), ac * kC, na);
+                                                                       (int)s.H, s.L, s.B * s.H, kWaves, ac * kC, na);
   return tsf_launch_status();
 }
 
@@ -1207,26 +1216,14 @@ int tsfast_hip_gated_step(int64_t B, int64_t H, int64_t Hk, int64_t K, int64_t V
   if (!q || !k || !v || !g || !strides || !state || !o) return TSF_ERR_ARG;
   StepArgs a{q, k, v, g, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], state, o,
              (int)H, (int)(H / Hk), (int)K, (int)V, 0};
-  // wide pieces read whole rows of the state; narrow ones make more workgroups of a few heads
   const int64_t heads = B * H;
-  const int lanes = V > 64 && heads >= 2 * (int64_t)device_cus() ? 32 : V > 16 && heads * ((V + 63) / 64) >= device_cus() ? 16 : 4;
-  a.ntile = (int)((V + 4 * lanes - 1) / (4 * lanes));
+  a.ntile = (int)((V + 4 * kStepLanes - 1) / (4 * kStepLanes));
   if (heads > kMaxGrid / a.ntile) return TSF_ERR_UNSUPPORTED;
   const unsigned grid = (unsigned)(heads * a.ntile);
-  const hipStream_t st = (hipStream_t)stream;
-  auto go = [&](auto lanes_c) {
-    constexpr int N = decltype(lanes_c)::value;
-    if (dtype == TSF_DTYPE_BF16)
-      step_kernel<bf16, N><<<grid, kThreads, 0, st>>>(a);
-    else
-      step_kernel<float, N><<<grid, kThreads, 0, st>>>(a);
-  };
-  if (lanes == 32)
-    go(std::integral_constant<int, 32>{});
-  else if (lanes == 16)
-    go(std::integral_constant<int, 16>{});
+  if (dtype == TSF_DTYPE_BF16)
+    step_kernel<bf16><<<grid, kThreads, 0, (hipStream_t)stream>>>(a);
   else
-    go(std::integral_constant<int, 4>{});
+    step_kernel<float><<<grid, kThreads, 0, (hipStream_t)stream>>>(a);
   return tsf_launch_status();
 }
 

@@ -78,7 +78,7 @@ def supports_step(q, k, v, g, state) -> str | None:
     K = q.shape[-1]
     if not (1 <= K <= _STEP_MAX_K and V >= 1):
         return f"head widths K={K}, V={V}: K must be in [1, {_STEP_MAX_K}]"
-    if V > 1 << 20 or H > 1 << 20 or B * H > _MAX_GRID // -(-V // 16):
+    if V > 1 << 20 or H > 1 << 20 or B * H > _MAX_GRID // -(-V // 64):
         return f"B={B}, H={H}, V={V} needs more workgroups than one launch has"
     return None
 

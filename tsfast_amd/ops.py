@@ -117,10 +117,12 @@ class _Op:
             return self._op(*args, **kwargs)
         wants_grad = False
         for i, t in enumerate(args):
-            if t is None or (i in self._numbers and type(t) in _NUMBER_TYPES):
+            if t is None:
                 continue
-            if not _plain(t):  # also what is no tensor: the dispatcher takes or refuses it (a proxy of a trace ..)
-                return self._op(*args)
+            if not _plain(t):
+                if i in self._numbers and type(t) in _NUMBER_TYPES:
+                    continue
+                return self._op(*args)  # also what is no tensor: the dispatcher takes or refuses it (a proxy of a trace ..)
             wants_grad = wants_grad or t.requires_grad
         if wants_grad and torch.is_grad_enabled():
             # an op without rules (a backward's) says so itself when it is differentiated
