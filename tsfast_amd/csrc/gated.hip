@@ -808,9 +808,11 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 // Segment states to entering states, in place: seg[n] becomes the state before segment n (after it, backwards). `threads`,
 // `et` and `fw` are the walk's; a thread owns one f32x4 of a state. `turned`, if any, gets the same states as the walk over the other
 // columns holds them (rows and columns exchanged; `et_turned` and `fw_turned` are that walk's).
-__global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int fw, int E, int F, int se,
+constexpr int kJoinThreads = 64;  // few states make few workgroups
+template <int N>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(f32x4* seg, const double* decay, const float* init, int nseg, int threads, int et, int fw, int E, int F, int se,
                                                    int sf, int64_t total, int backward, float* turned, int et_turned, int fw_turned) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
   if (at >= total) return;
   const int per = threads * et * fw;
   const int64_t bh = at / per;
@@ -829,14 +831,25 @@ __global__ __launch_bounds__(256) void join_kernel(f32x4* seg, const double* dec
   float* t = turned ? turned + ((bh * nseg + (backward ? nseg - 1 : 0)) * per +
                                 (tile % fw_turned * et_turned + col / 16) * threads + tile / fw_turned * 64 + (col % 16 / 4) * 16 + e % 16) * 4 + col % 4
                     : nullptr;
-#pragma unroll 4
-  for (int n = 0; n < nseg; ++n) {
-    const f32x4 own = p[n * step];
-    p[n * step] = s;
-    if (t)
+  // several segments' loads at a time, as each would otherwise wait for the last one's store (128 segments: 40 us, so 15)
+  for (int n0 = 0; n0 < nseg; n0 += N) {
+    f32x4 own[N];
+    float keep[N];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[n * step * 4 + r * 4] = s[r];
-    s = fast_exp2((float)d[backward ? -n : n]) * s + own;
+    for (int k = 0; k < N; ++k) {
+      const int n = min(n0 + k, nseg - 1);
+      own[k] = p[n * step];
+      keep[k] = (float)d[backward ? -n : n];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (n0 + k < nseg) {
+        p[(n0 + k) * step] = s;
+        if (t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) t[(n0 + k) * step * 4 + r * 4] = s[r];
+        s = fast_exp2(keep[k]) * s + own[k];
+      }
   }
 }
 
@@ -1045,7 +1058,8 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     p.seg_decay = (double*)(ws + sp.decay);
     walk_kernel<T, OT, E, NW, FW, FWD, true, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
     const int64_t total = bh * E / 16 * 64 * NW * FW;
-    join_kernel<<<(unsigned)((total + 255) / 256), 256, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
+    const auto join = a.nseg <= 4 ? join_kernel<4> : join_kernel<16>;
+    join<<<(unsigned)((total + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
                                                                   FWD ? nullptr : (float*)(ws + sp.turned), FW * NW, E / 16 / NW);
     a.seg_init = seg;
   }
