@@ -354,6 +354,19 @@ int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K,
                          const void* k, const void* v, const void* g, const void* grad_o, const int64_t* strides,
                          const float* state, const float* grad_last, void* grad_q, void* grad_k, void* grad_v,
                          void* grad_g, float* grad_state, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same pair for a training step: where few rows are cut into segments, `kept` (device memory of kept_bytes, 0 where rows are
+ * whole; contents are the library's) takes the forward's states between segments, and the backward of the same inputs takes
+ * them from it instead of walking the rows for them again. NULL: as above. */
+int64_t tsfast_hip_gated_kept_bytes(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype);
+int tsfast_hip_gated_fwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,
+                               const void* k, const void* v, const void* g, const int64_t* strides, const float* state,
+                               void* o, float* state_last, void* kept, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+int tsfast_hip_gated_bwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,
+                               const void* k, const void* v, const void* g, const void* grad_o, const int64_t* strides,
+                               const float* state, const float* grad_last, void* grad_q, void* grad_k, void* grad_v,
+                               void* grad_g, float* grad_state, const void* kept, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 /* One step with the state updated in place: q, k [B, Hk, K], v [B, H, V], g [B, H] through strides (batch row and
  * head of q, k, v, g: 8 in all), state [B, H, K, V] float32 contiguous, o [B, H, V] contiguous. K <= 1024. */
 int tsfast_hip_gated_step(int64_t B, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q,

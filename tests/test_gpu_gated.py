@@ -263,6 +263,29 @@ def test_pieces_of_a_row_carry_the_state(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", _DTYPES)
+@pytest.mark.parametrize("L,H,Hk,K,V", [(1500, 4, 2, 24, 100), (700, 2, 2, 100, 24), (70, 2, 1, 16, 16)])
+def test_states_kept_for_the_backward(gpu, L, H, Hk, K, V, dtype):
+    """The backward with the forward's states between segments (none where rows are whole) and without, and again."""
+    q, k, v, g, state, go, gl = _inputs(2, L, H, Hk, K, V, dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, state)]
+    o, last = recurrence_hip.run(*leaves)
+    first = torch.autograd.grad([o, last], leaves, [go, gl], retain_graph=True)
+    again = torch.autograd.grad([o, last], leaves, [go, gl])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with torch.no_grad():
+        _, _, kept = recurrence_hip._recurrence_train_op(q, k, v, g, state)
+        assert (kept.numel() > 0) == (L > 256)
+        without = recurrence_hip._recurrence_bwd_op(go, gl, q, k, v, g, state)
+        assert all(torch.equal(a, b) for a, b in zip(first, recurrence_hip._recurrence_bwd_op(go, gl, q, k, v, g, state, kept)))
+        with pytest.raises(TypeError, match="kept"):
+            recurrence_hip._recurrence_bwd_op(go, gl, q, k, v, g, state, kept.new_empty(kept.numel() + 16))
+    bf = dtype == torch.bfloat16
+    bars = (2**-8, 2**-8, 2**-8, 1e-2, 2e-5) if bf else (1e-5, 1e-5, 1e-5, 3e-5, 1e-5)
+    for got, want, bar in zip(without, G.recurrence_grads(go, gl, q, k, v, g, state), bars):
+        assert _rel(got, want) < bar
+
+
+@pytest.mark.parametrize("dtype", _DTYPES)
 @pytest.mark.parametrize("B,H,Hk,K,V", [(1, 1, 1, 1, 1), (1, 4, 2, 64, 64), (3, 6, 2, 33, 17), (2, 5, 5, 200, 130), (600, 2, 1, 128, 128),
                                         (300, 2, 2, 7, 65), (1, 2, 1, 1024, 3)])
 def test_step_matches_the_oracle(gpu, B, H, Hk, K, V, dtype):

@@ -81,6 +81,9 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "tsfast_hip_gated_fwd": ([_i64] * 6 + [_int] + [_ptr] * 9 + [_i64, _ptr], _int),
     "tsfast_hip_gated_bwd_workspace_bytes": ([_i64] * 6 + [_int], _i64),
     "tsfast_hip_gated_bwd": ([_i64] * 6 + [_int] + [_ptr] * 14 + [_i64, _ptr], _int),
+    "tsfast_hip_gated_kept_bytes": ([_i64] * 6 + [_int], _i64),
+    "tsfast_hip_gated_fwd_train": ([_i64] * 6 + [_int] + [_ptr] * 10 + [_i64, _ptr], _int),
+    "tsfast_hip_gated_bwd_train": ([_i64] * 6 + [_int] + [_ptr] * 15 + [_i64, _ptr], _int),
     "tsfast_hip_gated_step": ([_i64] * 5 + [_int] + [_ptr] * 8, _int),
     "tsfast_hip_norm_max_width": ([], _i64),
     "tsfast_hip_gated_norm_workspace_bytes": ([_i64] * 3, _i64),

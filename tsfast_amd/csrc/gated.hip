@@ -17,7 +17,7 @@
 // the decayed scores of x and y within it (64 x 64, the causal half only) times z, x times the state before it, and the
 // state's update are MFMA products; the decays come from exact differences of a float64 running sum, so any g <= 0 down
 // to -inf keeps its accuracy. Few rows are cut into segments: a walk of the state alone, a join of the segments' states, the
-// walk proper.
+// walk proper; dk's walk takes its segments' states from dv's, and a training step's dq from o's.
 //
 // dg needs no product of its own: r_t = q_t . dq_t and c_t = k_t . dk_t, summed from dq and dk before they are rounded, give
 // dg_{t+1} = dg_t - r_t + c_t. The rounding errors of that running sum are cut off at anchors every few chunks, where
@@ -1059,17 +1059,19 @@ Space space(const Sizes& s, int dtype, bool backward) {
   return w;
 }
 
-// One walk, cut rows' segment states first. dv's and dk's walks, backwards both, have the same states between segments with
-// rows and columns exchanged: dv's, the first to run, leaves them for dk's.
+// One walk, cut rows' segment states first, unless `entering` has them. o's and dq's walks, and dv's and dk's, have the same
+// states between segments with rows and columns exchanged: o's and dv's leave them in `turned` for the other (16 rows of 4096
+// steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 11 less each, for 25 MB that o's keeps).
 template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool DOTS>
-int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
+int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
+           hipStream_t stream) {
   const int64_t bh = a.units;
   a.units = bh * a.nseg;
   if (a.nseg == 1) {
     a.init = init;
-  } else if constexpr (!FWD && DOTS) {  // dk's, after dv's
-    a.seg_init = (const f32x4*)(ws + sp.turned);
-  } else {
+  } else if (entering || (!FWD && DOTS)) {  // dk's always has them
+    a.seg_init = (const f32x4*)entering;
+  } else if constexpr (FWD || !DOTS) {
     WalkArgs<T, OT> p = a;
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
@@ -1078,7 +1080,7 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     const int64_t total = bh * E / 16 * 64 * NW * FW;
     const auto join = a.nseg <= 4 ? join_kernel<4> : join_kernel<16>;
     join<<<(unsigned)((total + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
-                                                                  FWD ? nullptr : (float*)(ws + sp.turned), FW * NW, E / 16 / NW);
+                                                                  (float*)turned, FW * NW, E / 16 / NW);
     a.seg_init = seg;
   }
   a.last = last;
@@ -1088,15 +1090,16 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
 
 // One walk. `init` and `last` are the row's states [row x head][K V].
 template <typename T, typename OT, bool FWD, bool DOTS>
-int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const float* init, float* last, hipStream_t stream) {
+int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
+         hipStream_t stream) {
   a.H = (int)s.H;
   a.L = s.L;
   a.units = s.B * s.H;
   a.nseg = segments(s, sizeof(T) == 2 ? TSF_DTYPE_BF16 : TSF_DTYPE_F32);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
-  if (a.F <= 64)
-    return a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 1, FWD, DOTS>(a, ws, sp, init, last, stream);
-  return a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, DOTS>(a, ws, sp, init, last, stream) : walk_e<T, OT, 128, 4, 2, FWD, DOTS>(a, ws, sp, init, last, stream);
+  const auto run = a.F <= 64 ? (a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, DOTS> : walk_e<T, OT, 128, 4, 1, FWD, DOTS>)
+                             : (a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, DOTS> : walk_e<T, OT, 128, 4, 2, FWD, DOTS>);
+  return run(a, ws, sp, init, last, entering, turned, stream);
 }
 
 template <typename T>
@@ -1106,7 +1109,7 @@ Seq<const T> seq_in(const void* p, const int64_t* st, int share) {
 
 template <typename T>
 int forward(const Sizes& s, const void* q, const void* k, const void* v, const void* g, const int64_t* st, const float* state, void* o, float* last,
-            char* ws, const Space& sp, hipStream_t stream) {
+            void* kept, char* ws, const Space& sp, hipStream_t stream) {
   const int share = (int)(s.H / s.Hk);
   WalkArgs<T, T> a = {};
   a.x = seq_in<T>(q, st, share);
@@ -1118,13 +1121,13 @@ int forward(const Sizes& s, const void* q, const void* k, const void* v, const v
   a.F = (int)s.V;
   a.se = (int)s.V;
   a.sf = 1;
-  return walk<T, T, true, false>(a, s, ws, sp, state, last, stream);
+  return walk<T, T, true, false>(a, s, ws, sp, state, last, nullptr, kept, stream);
 }
 
 // dq or dk: a walk over K's columns with V contracted, the dots of the gate's gradient beside it.
 template <typename T, typename OT, bool FWD>
 int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<const T> g, Seq<const T> dot, Seq<OT> out, float* dots, int dtype, char* ws, const Space& sp,
-           const float* init, hipStream_t stream) {
+           const float* init, const void* entering, hipStream_t stream) {
   WalkArgs<T, OT> a = {};
   a.x = x;
   a.y = y;
@@ -1141,12 +1144,13 @@ int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<c
   a.anchor_dots = (float*)(ws + sp.anchor_dots);
   a.anchor_chunks = anchor_chunks(dtype);
   a.nanchor = (int)(((s.L + kC - 1) / kC + a.anchor_chunks - 1) / a.anchor_chunks);
-  return walk<T, OT, FWD, true>(a, s, ws, sp, init, nullptr, stream);
+  return walk<T, OT, FWD, true>(a, s, ws, sp, init, nullptr, entering, nullptr, stream);
 }
 
 template <typename T>
 int backward(const Sizes& s, int dtype, const void* q, const void* k, const void* v, const void* g, const void* d_o, const int64_t* st, const float* state,
-             const float* dlast, void* dq, void* dk, void* dv, void* dg, float* dstate, char* ws, const Space& sp, hipStream_t stream) {
+             const float* dlast, void* dq, void* dk, void* dv, void* dg, float* dstate, const void* kept, char* ws, const Space& sp,
+             hipStream_t stream) {
   const int share = (int)(s.H / s.Hk);
   const Seq<const T> Q = seq_in<T>(q, st, share), Kk = seq_in<T>(k, st + 3, share), Vv = seq_in<T>(v, st + 6, 1), G = seq_in<T>(g, st + 9, 1),
                      DO = seq_in<T>(d_o, st + 12, 1);
@@ -1162,7 +1166,7 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
     a.F = (int)s.V;
     a.se = (int)s.V;
     a.sf = 1;
-    const int rc = walk<T, T, false, false>(a, s, ws, sp, dlast, dstate, stream);
+    const int rc = walk<T, T, false, false>(a, s, ws, sp, dlast, dstate, nullptr, ws + sp.turned, stream);
     if (rc != TSF_OK) return rc;
   }
   if (s.L == 0) return TSF_OK;
@@ -1170,16 +1174,16 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
   int rc;
   if (share == 1) {
     const int64_t sl = s.H * s.K;
-    rc = walk_k<T, T, true>(s, DO, Vv, Kk, G, Q, Seq<T>{(T*)dq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, stream);
+    rc = walk_k<T, T, true>(s, DO, Vv, Kk, G, Q, Seq<T>{(T*)dq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, kept, stream);
     if (rc != TSF_OK) return rc;
-    rc = walk_k<T, T, false>(s, Vv, DO, Q, G, Kk, Seq<T>{(T*)dk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, stream);
+    rc = walk_k<T, T, false>(s, Vv, DO, Q, G, Kk, Seq<T>{(T*)dk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, ws + sp.turned, stream);
     if (rc != TSF_OK) return rc;
   } else {
     const int64_t sl = s.H * s.K, total = s.B * s.L * s.Hk * s.K;
     float *pq = (float*)(ws + sp.dq), *pk = (float*)(ws + sp.dk);
-    rc = walk_k<T, float, true>(s, DO, Vv, Kk, G, Q, Seq<float>{pq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, stream);
+    rc = walk_k<T, float, true>(s, DO, Vv, Kk, G, Q, Seq<float>{pq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, kept, stream);
     if (rc != TSF_OK) return rc;
-    rc = walk_k<T, float, false>(s, Vv, DO, Q, G, Kk, Seq<float>{pk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, stream);
+    rc = walk_k<T, float, false>(s, Vv, DO, Q, G, Kk, Seq<float>{pk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, ws + sp.turned, stream);
     if (rc != TSF_OK) return rc;
     const int64_t blocks = (total + kThreads - 1) / kThreads;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
@@ -1207,9 +1211,17 @@ int64_t tsfast_hip_gated_bwd_workspace_bytes(int64_t B, int64_t L, int64_t H, in
   return args_status(s, dtype) == TSF_OK ? space(s, dtype, true).bytes : -1;
 }
 
-int tsfast_hip_gated_fwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
-                         const void* g, const int64_t* strides, const float* state, void* o, float* state_last, void* workspace, int64_t workspace_bytes,
-                         void* stream) {
+// States between segments that the backward can take from the forward.
+int64_t tsfast_hip_gated_kept_bytes(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype) {
+  const Sizes s{B, L, H, Hk, K, V};
+  if (args_status(s, dtype) != TSF_OK) return -1;
+  const int64_t nseg = segments(s, dtype);
+  return nseg > 1 ? B * H * nseg * padded_state(K, V) * 4 : 0;
+}
+
+int tsfast_hip_gated_fwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
+                               const void* g, const int64_t* strides, const float* state, void* o, float* state_last, void* kept, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   const Sizes s{B, L, H, Hk, K, V};
   const int rc = args_status(s, dtype);
   if (rc != TSF_OK) return rc;
@@ -1218,13 +1230,19 @@ int tsfast_hip_gated_fwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K,
   if (!steps_fit(strides, 3)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, false);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
-  return dtype == TSF_DTYPE_BF16 ? forward<bf16>(s, q, k, v, g, strides, state, o, state_last, (char*)workspace, sp, (hipStream_t)stream)
-                                 : forward<float>(s, q, k, v, g, strides, state, o, state_last, (char*)workspace, sp, (hipStream_t)stream);
+  return dtype == TSF_DTYPE_BF16 ? forward<bf16>(s, q, k, v, g, strides, state, o, state_last, kept, (char*)workspace, sp, (hipStream_t)stream)
+                                 : forward<float>(s, q, k, v, g, strides, state, o, state_last, kept, (char*)workspace, sp, (hipStream_t)stream);
 }
 
-int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
+int tsfast_hip_gated_fwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
+                         const void* g, const int64_t* strides, const float* state, void* o, float* state_last, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
+  return tsfast_hip_gated_fwd_train(B, L, H, Hk, K, V, dtype, q, k, v, g, strides, state, o, state_last, nullptr, workspace, workspace_bytes, stream);
+}
+
+int tsfast_hip_gated_bwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
                          const void* g, const void* grad_o, const int64_t* strides, const float* state, const float* grad_last, void* grad_q, void* grad_k,
-                         void* grad_v, void* grad_g, float* grad_state, void* workspace, int64_t workspace_bytes, void* stream) {
+                         void* grad_v, void* grad_g, float* grad_state, const void* kept, void* workspace, int64_t workspace_bytes, void* stream) {
   const Sizes s{B, L, H, Hk, K, V};
   const int rc = args_status(s, dtype);
   if (rc != TSF_OK) return rc;
@@ -1234,10 +1252,17 @@ int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K,
   if (!steps_fit(strides, 3) || !steps_fit(strides + 12, 1)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, true);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
-  return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state,
+  return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
                                                   (char*)workspace, sp, (hipStream_t)stream)
-                                 : backward<float>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state,
+                                 : backward<float>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
                                                    (char*)workspace, sp, (hipStream_t)stream);
+}
+
+int tsfast_hip_gated_bwd(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v,
+                         const void* g, const void* grad_o, const int64_t* strides, const float* state, const float* grad_last, void* grad_q, void* grad_k,
+                         void* grad_v, void* grad_g, float* grad_state, void* workspace, int64_t workspace_bytes, void* stream) {
+  return tsfast_hip_gated_bwd_train(B, L, H, Hk, K, V, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state,
+                                    nullptr, workspace, workspace_bytes, stream);
 }
 
 int tsfast_hip_gated_step(int64_t B, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype, const void* q, const void* k, const void* v, const void* g,

@@ -2,8 +2,8 @@
 
 ``supports(q, k, v, g, state)`` / ``run(...) -> (o, last)``, differentiable in all inputs through the
 ``tsfast_hip::gated_recurrence`` / ``gated_recurrence_bwd`` custom ops, and ``supports_step`` / ``step`` for
-one token with the state updated in place (``tsfast_hip::gated_recurrence_step``). Only the inputs are saved
-for the backward.
+one token with the state updated in place (``tsfast_hip::gated_recurrence_step``). The inputs are saved for the
+backward, and the states between the segments of cut rows (``gated_recurrence_train``).
 
 q, k, v, g and their gradients are float32 or bfloat16, all alike, at any strides with a dense last
 dimension (others are copied); states are float32. The kernels sum in float32 and keep the state in it. With
@@ -23,6 +23,7 @@ from .. import _lib
 from ..ops import custom_op
 
 _IO_DTYPES = {torch.float32: _lib.TSF_DTYPE_F32, torch.bfloat16: _lib.TSF_DTYPE_BF16}
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MAX_WIDTH = 128
 _STEP_MAX_K = 1024
 _MAX_GRID = (1 << 24) - 1
@@ -108,10 +109,7 @@ def _screen(v, *others):
             raise TypeError(f"{t.dtype} on {t.device}, expected {dtype} on {v.device}")
 
 
-@custom_op("tsfast_hip::gated_recurrence")
-def _recurrence_op(
-    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor | None
-) -> tuple[torch.Tensor, torch.Tensor]:
+def _forward(q, k, v, g, state, train: bool):
     lib = _lib.load()
     _screen(v, q, k, g)
     q, k, v = _dense(q), _dense(k), _dense(v)
@@ -122,22 +120,48 @@ def _recurrence_op(
     o = torch.empty(B, L, H, V, device=v.device, dtype=v.dtype)
     last = torch.empty(B, H, K, V, device=v.device, dtype=torch.float32)
     io = _IO_DTYPES[v.dtype]
+    kept = torch.empty(lib.tsfast_hip_gated_kept_bytes(B, L, H, Hk, K, V, io), device=v.device, dtype=torch.uint8) if train else None
     nbytes = lib.tsfast_hip_gated_fwd_workspace_bytes(B, L, H, Hk, K, V, io)
     ws = _workspace(nbytes, v)
     _lib.check(
-        lib.tsfast_hip_gated_fwd(
+        lib.tsfast_hip_gated_fwd_train(
             B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g)), _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()),
-            *map(_lib.ptr, (state, o, last, ws)), nbytes, _lib.stream_of(v),
+            *map(_lib.ptr, (state, o, last)), _kept_ptr(kept), _lib.ptr(ws), nbytes, _lib.stream_of(v),
         ),
-        "tsfast_hip_gated_fwd",
+        "tsfast_hip_gated_fwd_train",
     )
-    return o, last
+    return o, last, kept
+
+
+def _kept_ptr(kept):
+    return None if kept is None or not kept.numel() else kept.data_ptr()
+
+
+@custom_op("tsfast_hip::gated_recurrence")
+def _recurrence_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor | None
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return _forward(q, k, v, g, state, train=False)[:2]
+
+
+@custom_op("tsfast_hip::gated_recurrence_train")
+def _recurrence_train_op(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor | None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _forward(q, k, v, g, state, train=True)
 
 
 @_recurrence_op.register_fake
 def _(q, k, v, g, state):
     B, L, H, V = v.shape
     return v.new_empty(B, L, H, V), v.new_empty(B, H, q.shape[-1], V, dtype=torch.float32)
+
+
+@_recurrence_train_op.register_fake
+def _(q, k, v, g, state):
+    B, L, H, V = v.shape
+    kept = v.new_empty(torch.library.get_ctx().new_dynamic_size(), dtype=torch.uint8)  # the library's rule, by the chip's size
+    return v.new_empty(B, L, H, V), v.new_empty(B, H, q.shape[-1], V, dtype=torch.float32), kept
 
 
 @custom_op("tsfast_hip::gated_recurrence_bwd")
@@ -149,6 +173,7 @@ def _recurrence_bwd_op(
     v: torch.Tensor,
     g: torch.Tensor,
     state: torch.Tensor | None,
+    kept: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     lib = _lib.load()
     _screen(v, q, k, g, go)
@@ -162,43 +187,53 @@ def _recurrence_bwd_op(
     gg = torch.empty(B, L, H, device=v.device, dtype=v.dtype)
     gstate = None if state is None else torch.empty_like(state)
     io = _IO_DTYPES[v.dtype]
+    if kept is not None:
+        need = lib.tsfast_hip_gated_kept_bytes(B, L, H, Hk, K, V, io)
+        if kept.dtype != torch.uint8 or kept.numel() != need or kept.get_device() != v.get_device() or not kept.is_contiguous():
+            raise TypeError(f"kept: {kept.numel()} of {kept.dtype} on {kept.device}, expected {need} dense bytes on {v.device}")
     nbytes = lib.tsfast_hip_gated_bwd_workspace_bytes(B, L, H, Hk, K, V, io)
     ws = _workspace(nbytes, v)
     _lib.check(
-        lib.tsfast_hip_gated_bwd(
-            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g, go)), 
+        lib.tsfast_hip_gated_bwd_train(
+            B, L, H, Hk, K, V, io, *map(_lib.ptr, (q, k, v, g, go)),
             _Strides15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *go.stride()[:3]),
-            *map(_lib.ptr, (state, glast, gq, gk, gv, gg, gstate, ws)), nbytes, _lib.stream_of(v),
+            *map(_lib.ptr, (state, glast, gq, gk, gv, gg, gstate)), _kept_ptr(kept), _lib.ptr(ws), nbytes, _lib.stream_of(v),
         ),
-        "tsfast_hip_gated_bwd",
+        "tsfast_hip_gated_bwd_train",
     )
     return gq, gk, gv, gg, (gstate if gstate is not None else v.new_empty(0, dtype=torch.float32))
 
 
 @_recurrence_bwd_op.register_fake
-def _(go, glast, q, k, v, g, state):
+def _(go, glast, q, k, v, g, state, kept=None):
     outs = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, g))
     return (*outs, torch.empty(0 if state is None else state.shape, device=v.device, dtype=torch.float32))
 
 
 def _setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(*inputs)
+    ctx.save_for_backward(*inputs, *output[2:])
 
 
-def _backward(ctx, go, glast):
-    q, k, v, g, state = ctx.saved_tensors
+def _backward(ctx, go, glast, gkept=None):
+    q, k, v, g, state, *kept = ctx.saved_tensors
     if go is None:
         go = torch.zeros_like(v)
-    gq, gk, gv, gg, gstate = _recurrence_bwd_op(go, glast, q, k, v, g, state)
+    gq, gk, gv, gg, gstate = _recurrence_bwd_op(go, glast, q, k, v, g, state, *kept)
     return gq, gk, gv, gg, (gstate if state is not None else None)
 
 
 _recurrence_op.register_autograd(_backward, setup_context=_setup)
+_recurrence_train_op.register_autograd(_backward, setup_context=_setup)
 
 
 def run(q, k, v, g, state):
-    """The fused recurrence: ``(o [B, L, H, V], last state [B, H, K, V] float32)``."""
+    """The fused recurrence: ``(o [B, L, H, V], last state [B, H, K, V] float32)``. A call that will be differentiated
+    keeps the states between a row's segments (33 MB at most) for the backward, which would walk the rows for them again."""
+    # a trace keeps the inputs alone: how many bytes more is not known to it
+    if torch.is_grad_enabled() and not torch.compiler.is_compiling() and type(v) in _PLAIN:
+        if q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or (state is not None and state.requires_grad):
+            return _recurrence_train_op(q, k, v, g, state)[:2]
     return _recurrence_op(q, k, v, g, state)
 
 
