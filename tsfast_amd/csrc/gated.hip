@@ -481,6 +481,8 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes, as the compiler now knows
   const int64_t unit = blockIdx.x;
   const int seg = (int)(unit % a.nseg);
+  if constexpr (STATE_ONLY)
+    if (seg == (FWD ? a.nseg - 1 : 0)) return;  // no segment enters with its state
   const int64_t bh = unit / a.nseg, b = bh / a.H, nbh = a.units / a.nseg;
   const int h = (int)(bh % a.H);
   const int nchunk = (int)((a.L + kC - 1) / kC);
@@ -837,7 +839,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(f32x4* seg, const do
     float keep[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int n = min(n0 + k, nseg - 1);
+      const int n = min(n0 + k, nseg - 2);  // nothing follows the last one, and its own state was not formed
       own[k] = p[n * step];
       keep[k] = (float)d[backward ? -n : n];
     }
