@@ -1005,21 +1005,32 @@ int args_status(const Sizes& s, int dtype) {
 // Waves of a walk: a workgroup takes all of its columns, so that nothing of x and y is done twice.
 constexpr int kWaves = 4;
 
-// Segments a row is cut into. A cut row is walked twice (its segments' states first), so rows are cut only to give
-// every CU the workgroups it holds, into no more than fit at once (86 instead of 85 segments of 6 rows took twice the time) and
-// into four chunks at least. Measured, forward and backward: 32 rows of 4096 steps, 128 x 128, bf16: 1 segment 330 + 1180 us, 5:
-// 180 + 590; 384 rows of 1024 steps, 64 x 64: 1 segment 64 + 229, 4: 87 + 283.
+int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
+
+// Segments a row is cut into: the number with the least time, in chunks walked one after the other, of one and those that
+// fill every CU once or twice (a workgroup more, and the whole chip waits for another round: 86 instead of 85 segments of 6 rows took
+// twice the time). A cut row's chunks are walked for the states too, at 0.45 times a chunk's time, and the states
+// go to memory and back five times. Four chunks a segment at least. Measured, training, against once alone: 192 rows of 4096 steps,
+// 128 x 128, bf16: 5 segments 1366 us, 2: 1460; 288 rows, 64 x 64: 5: 822, 2: 857; 192 rows of 2048, 64 x 64, fp32: 5: 786, 2: 856.
 int segments(const Sizes& s, int dtype) {
   const int64_t chunks = (s.L + kC - 1) / kC, rows = s.B * s.H;
-  const int per_cu = dtype == TSF_DTYPE_BF16 && s.K <= 64 && s.V <= 64 ? 3 : 2;
-  int64_t n = rows > 0 ? per_cu * (int64_t)device_cus() / rows : 1;
-  if (n > chunks / 4) n = chunks / 4;
-  if (n < 1) n = 1;
-  const int64_t per = (chunks + n - 1) / n;
-  return per > 0 ? (int)((chunks + per - 1) / per) : 1;
+  const bool narrow = s.K <= 64 && s.V <= 64;
+  const int64_t slots = (int64_t)device_cus() * (dtype == TSF_DTYPE_BF16 ? (narrow ? 3 : 2) : narrow ? 2 : 1);  // by their LDS
+  if (rows < 1 || chunks < 8) return 1;
+  double least = (double)((rows + slots - 1) / slots * chunks);
+  int64_t best = 1;
+  for (int64_t rounds = 1; rounds <= 2; ++rounds) {
+    int64_t n = rounds * slots / rows;
+    if (n > chunks / 4) n = chunks / 4;
+    if (n < 2) continue;
+    const int64_t per = (chunks + n - 1) / n;
+    n = (chunks + per - 1) / per;
+    const double time = (double)((rows * n + slots - 1) / slots * per) + 0.45 * (double)((rows * (n - 1) + slots - 1) / slots * per) +
+                        1.2e-7 * (double)(padded_state(s.K, s.V) * 4 * rows * n);
+    if (time < least) least = time, best = n;
+  }
+  return (int)best;
 }
-
-int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
 
 // Chunks between dg's anchors: an anchor's states cost 8 bytes a state element, the running sum's errors grow with the root
 // of the distance. What is rounded to bf16 can bear 16 chunks of them; fp32 heads that forget within a few steps, the worst

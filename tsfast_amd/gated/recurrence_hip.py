@@ -229,7 +229,7 @@ _recurrence_train_op.register_autograd(_backward, setup_context=_setup)
 
 def run(q, k, v, g, state):
     """The fused recurrence: ``(o [B, L, H, V], last state [B, H, K, V] float32)``. A call that will be differentiated
-    keeps the states between a row's segments (33 MB at most) for the backward, which would walk the rows for them again."""
+    keeps the states between a row's segments (67 MB at most) for the backward, which would walk the rows for them again."""
     # a trace keeps the inputs alone: how many bytes more is not known to it
     if torch.is_grad_enabled() and not torch.compiler.is_compiling() and type(v) in _PLAIN:
         if q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or (state is not None and state.requires_grad):
