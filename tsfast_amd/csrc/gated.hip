@@ -28,8 +28,8 @@
 // would cost the outputs 1.4 times their own rounding, the fp32 state its type, and dg, a difference of near sums, far more.
 // fp32 inputs use the fp32 matrix cores.
 //
-// Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 290 us for o's walk and 125 us for the segment
-// states before it, 290 for dv's, 330 and 340 for dq's and dk's. No one unit bounds a chunk (3.4 us a workgroup at two on a CU):
+// Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 255 us for o's walk, 109 us for the
+// segments' states before it and 37 for their join, 256 for dv's, 302 and 314 for dq's and dk's. No one unit bounds a chunk (5.3 us of a CU):
 // of it matrix products take 1.4 us, LDS 1.1 us and vector instructions about as much, waits for memory the rest. Kept
 // out, for they measured slower: the state in LDS as well (2 times), transposed copies of y and z in LDS instead of
 // transposing reads (2 times, for their bank conflicts), eight waves of one column tile each (1.3 times),
@@ -1074,7 +1074,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
 
 // One walk, cut rows' segment states first, unless `entering` has them. o's and dq's walks, and dv's and dk's, have the same
 // states between segments with rows and columns exchanged: o's and dv's leave them in `turned` for the other (16 rows of 4096
-// steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 11 less each, for 25 MB that o's keeps).
+// steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 37 less each, for 63 MB that o's keeps).
 template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool DOTS>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
            hipStream_t stream) {
