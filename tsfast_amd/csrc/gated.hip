@@ -19,13 +19,19 @@
 // to -inf keeps its accuracy. Few rows are cut into segments: a walk of the state alone, a join of the segments' states, the
 // walk proper; dk's walk takes its segments' states from dv's, and a training step's dq from o's.
 //
-// dg needs no product of its own: r_t = q_t . dq_t and c_t = k_t . dk_t, summed from dq and dk before they are rounded, give
-// dg_{t+1} = dg_t - r_t + c_t. The rounding errors of that running sum are cut off at anchors every few chunks, where
-// dg_t = <S_{t-1}, dL/dS_{t-1}> is formed from the two states.
+// dg is a sum of terms that each carry their own decay from j < t to i >= t, so that it keeps its relative accuracy however
+// strongly a head forgets, and a step that forgets all (g = -inf) parts the sequences of a packed row exactly. Within a chunk whose
+// entering state is S and whose adjoint from beyond is T, with in_i and w_j the decays from its start and to its end,
+//
+//   dg_t = sum_{j < t <= i} D (q_i . k_j)(do_i . v_j) + sum_{i >= t} in_i q_i . (S do_i) + sum_{j < t} w_j k_j . (T v_j) + tot <S, T>.
+//
+// dq's walk has S and gives the first two, from its decayed scores and the part of dq that S makes, and leaves every chunk's S;
+// dk's walk has T, adds the other two and writes dg. (The shorter dg_{t+1} = dg_t - q_t . dq_t + k_t . dk_t is a difference of
+// terms without exp(g_t): its rounding errors were as large as dg itself from g = -8 on.)
 //
 // bf16 inputs are multiplied on the bf16 matrix cores. Products of inputs are exact there; what is fp32 (the decayed
 // scores, the state, the decayed z of an update) goes in as a sum of two or three bf16 operands, because one alone (2^-9)
-// would cost the outputs 1.4 times their own rounding, the fp32 state its type, and dg, a difference of near sums, far more.
+// would cost the outputs 1.4 times their own rounding, the fp32 state its type.
 // fp32 inputs use the fp32 matrix cores.
 //
 // Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 255 us for o's walk, 109 us for the
@@ -45,6 +51,7 @@ namespace {
 
 constexpr int kC = 64;                 // steps of a chunk
 constexpr int kThreads = 256;          // of the small kernels
+constexpr int kWaves = 4;              // of a walk: a workgroup takes all of its columns, so that nothing of x and y is done twice
 constexpr int kMaxWidth = 128;         // of K and V
 constexpr int kStepMaxK = 1024;        // of K in a single step
 constexpr int64_t kMaxStep = 1 << 23;  // elements between the steps of a row
@@ -235,14 +242,6 @@ TSF_DEV void store8(bf16* p, const Frag<bf16>& o, const Frag<bf16>&, int n) {
       if (e < n) p[e] = v[e];
   }
 }
-template <typename F>
-TSF_DEV float dot8(const F& o, const F& rest, const F& u) {
-  float d = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) d = fmaf(value(o, e) + value(rest, e), value(u, e), d);
-  return d;
-}
-
 // An element by a 32-bit index from an address that all lanes share.
 template <typename T>
 TSF_DEV T* at32(T* base, uint32_t idx) {
@@ -272,11 +271,12 @@ struct WalkArgs {
   float* last;            // state leaving the row
   f32x4* seg_last;        // STATE_ONLY: state leaving each unit
   double* seg_decay;      // STATE_ONLY: log2 of the unit's decay
-  Seq<const T> dot;       // out_i . dot_i is summed over columns ..
-  float* dots;            // .. into [row x head][L]
-  f32x4* anchors;         // states before every anchor chunk [row x head][anchor]: written forward, read backward
-  float* anchor_dots;     // backward: <state, anchor> over a wave's columns [wave][row x head][anchor]
-  int anchor_chunks, nanchor;
+  // of the gate's gradient (GATE): q for dq's walk, k for dk's; dg's part that dq's walk gives [row x head][L]; the states
+  // entering the chunks [row x head][chunk]; both written forward, read backward
+  Seq<const T> u;
+  float* partial;
+  f32x4* states;
+  Seq<T> dg;
 };
 
 // 16 and 8 bytes of LDS as one access
@@ -350,6 +350,11 @@ struct Rows {
   TSF_DEV void put_plain_four(uint32_t lane_off, int t, int tile, const void* f) {
     lds_put<kHalf>(at + t * 16 * kBytes + (lane_off ^ (tile << (kBf ? 5 : 6))), f);
   }
+  TSF_DEV f32x4 get_plain_four(uint32_t lane_off, int t, int tile) const {
+    T v[4];
+    lds_get<kHalf>(v, at + t * 16 * kBytes + (lane_off ^ (tile << (kBf ? 5 : 6))));
+    return f32x4{to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3])};
+  }
   // operands whose row is row 16 t + li, over columns 32 s ..: the lane's offset, and the operand
   TSF_DEV static uint32_t row_lane(uint32_t li, uint32_t lg) { return li * kBytes + ((lg ^ turn(li)) << 4); }
   TSF_DEV Frag<T> row(uint32_t lane_off, int t, int s) const {
@@ -408,16 +413,111 @@ struct Lds {
   static constexpr int kSplit = sizeof(T) == 2 ? 2 : 1;  // operands the state and the scores are split into
   union {
     Rows<T, E> x;
-    Rows<T, FT> o;  // the outputs on their way to memory, once x has been used
+    Rows<T, FT> u;  // GATE: q or k, once x has been used
+    Rows<T, FT> o;  // the outputs on their way to memory, once x (and u) have been used
   };
   Rows<T, E> y;
   Rows<T, FT> z;
   union {
     Rows<T, kC> p[kSplit];  // decayed scores, row i
-    Rows<T, FT> o_rest;     // what the outputs' rounding left (bf16), once the scores have been used
+    Rows<T, FT> o_rest;     // what the outputs' rounding left (fp32 from bf16), once the scores have been used
   };
   alignas(16) float hi[2][kC], lo[2][kC], w[2][kC], in[2][kC];  // running log2 decay, weights into the state and out of it
 };
+
+// Sums of the gate's gradient on their way between waves.
+struct GateLds {
+  float dots[kWaves][kC];               // u_i . (x_i times the state) over a wave's columns
+  float rows[6][16], cols[6][16];       // of the score tiles below the diagonal, by tile_slot: sums over j of row i, over i of column j
+  float diag[kC];                       // the pairs within a diagonal tile
+  float with[kWaves];                   // <entering state, state> over a wave's columns
+};
+TSF_DEV int tile_slot(int it, int jt) { return it * (it - 1) / 2 + jt; }
+
+// Four values over the 16 lanes of a row (`li`), each summed over them: lane li has the sum of value (li >> 2) of all.
+TSF_DEV float sum_lanes16(const float (&v)[4], int li) {
+  const bool b3 = li & 8, b2 = li & 4;
+  float a0 = b3 ? v[2] : v[0], a1 = b3 ? v[3] : v[1];
+  a0 += __shfl_xor(b3 ? v[0] : v[2], 8, kWave);
+  a1 += __shfl_xor(b3 ? v[1] : v[3], 8, kWave);
+  float a = b2 ? a1 : a0;
+  a += __shfl_xor(b2 ? a0 : a1, 4, kWave);
+  a += __shfl_xor(a, 2, kWave);
+  return a + __shfl_xor(a, 1, kWave);
+}
+// Four values over the four groups of lanes (`lg`), each summed over them: group lg has the sum of value lg of all.
+TSF_DEV float sum_groups(const float (&v)[4], int lg) {
+  const bool b1 = lg & 2, b0 = lg & 1;
+  float a0 = b1 ? v[2] : v[0], a1 = b1 ? v[3] : v[1];
+  a0 += __shfl_xor(b1 ? v[0] : v[2], 32, kWave);
+  a1 += __shfl_xor(b1 ? v[1] : v[3], 32, kWave);
+  return (b0 ? a1 : a0) + __shfl_xor(b0 ? a0 : a1, 16, kWave);
+}
+// Sums over the lanes from a lane on, and up to one, of every W lanes.
+template <int W>
+TSF_DEV float suffix_sum(float x, int lane) {
+#pragma unroll
+  for (int d = 1; d < W; d <<= 1) {
+    const float v = __shfl_down(x, d, kWave);
+    if ((lane & (W - 1)) + d < W) x += v;
+  }
+  return x;
+}
+template <int W>
+TSF_DEV float prefix_before(float x, int lane) {
+#pragma unroll
+  for (int d = 1; d < W; d <<= 1) {
+    const float v = __shfl_up(x, d, kWave);
+    if ((lane & (W - 1)) >= d) x += v;
+  }
+  x = __shfl_up(x, 1, kWave);
+  return (lane & (W - 1)) ? x : 0.0f;
+}
+
+// One tile of the pairs' terms p = D (q_i . k_j)(do_i . v_j), rows i = 16 it + li, columns j = 16 jt + 4 lg + r: what the sums over
+// j < t <= i need of it.
+TSF_DEV void put_pairs(GateLds& g, const float (&p)[4], int it, int jt, int li, int lg, int lane) {
+  const int col = 4 * lg + (li >> 2);
+  if (it != jt) {
+    float row = (p[0] + p[1]) + (p[2] + p[3]);
+    row += __shfl_xor(row, 16, kWave);
+    row += __shfl_xor(row, 32, kWave);
+    const float sum = sum_lanes16(p, li);
+    const int at = tile_slot(it, jt);
+    if (lg == 0) g.rows[at][li] = row;
+    if ((li & 3) == 0) g.cols[at][col] = sum;
+  } else {
+    // row i's sum over j < t, for the t of the columns; of rows i >= t alone
+    const float s1 = p[0] + p[1], s2 = s1 + p[2];
+    float before = s2 + p[3];
+    float v = __shfl_up(before, 16, kWave);
+    if (lane >= 16) before += v;
+    v = __shfl_up(before, 32, kWave);
+    if (lane >= 32) before += v;
+    before = __shfl_up(before, 16, kWave);
+    if (lane < 16) before = 0.0f;
+    const float r[4] = {li >= 4 * lg ? before : 0.0f, li >= 4 * lg + 1 ? before + p[0] : 0.0f, li >= 4 * lg + 2 ? before + s1 : 0.0f,
+                        li >= 4 * lg + 3 ? before + s2 : 0.0f};
+    const float sum = sum_lanes16(r, li);
+    if ((li & 3) == 0) g.diag[16 * it + col] = sum;
+  }
+}
+// One wave, lane t: the pairs' sum over j < t <= i of the whole chunk.
+TSF_DEV float pair_sums(const GateLds& g, int li, int lg, int lane) {
+  float a = 0.0f, b = 0.0f, m = 0.0f;  // tiles of t's rows, of its columns, and below and left of both
+#pragma unroll
+  for (int it = 1; it < 4; ++it)
+#pragma unroll
+    for (int jt = 0; jt < it; ++jt) {
+      const float row = g.rows[tile_slot(it, jt)][li], col = g.cols[tile_slot(it, jt)][li];
+      if (lg == it) a += row;
+      if (lg == jt) b += col;
+      if (lg > jt && lg < it) m += row;
+    }
+#pragma unroll
+  for (int d = 8; d >= 1; d >>= 1) m += __shfl_xor(m, d, kWave);
+  return g.diag[lane] + suffix_sum<16>(a, lane) + prefix_before<16>(b, lane) + m;
+}
 
 // Waves a SIMD holds of a walk: what LDS and a 512-register file allow.
 template <typename T>
@@ -464,37 +564,40 @@ TSF_DEV f32x4 four(const float* p) {
 }
 
 // E: columns of x and y, padded; NW: waves of a workgroup; FW: 16-column tiles of z a wave owns; FWD: the direction in time;
-// STATE_ONLY: only the state leaving the unit; DOTS: out_i . dot_i too, and the anchors.
+// STATE_ONLY: only the state leaving the unit; GATE: the gate's gradient too (dq's and dk's walks).
 //
 // The weighted z of the state's update is split into three bf16 operands where the caller gets the state (2^-24), two where
-// only bf16 outputs and their products follow (2^-16).
+// only results follow that are rounded to bf16 (2^-16).
 //
 // Wave w owns the state's columns 16 (w FW + fw) + li, all E rows of them: accumulators S[fw][et] hold rows 16 et + 4 lg + r, which
 // two by two are operands as they stand. Per chunk: (1) x, y, z to LDS; (2) the ten live 16 x 16 score tiles, shared
-// among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update.
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, bool DOTS>
+// among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update. With
+// GATE, u takes x's place before (3), for its products with x times the state and, in dq's walk, with z = k: the pairs' second score.
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, bool GATE>
 __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel(WalkArgs<T, OT> a) {
-  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT>::kSplit, NU = sizeof(T) == 4 ? 1 : DOTS ? 2 : 3;
-  constexpr bool kRest = DOTS && sizeof(T) == 2;  // outputs go to LDS in two parts: the sums of products want more than bf16
+  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT>::kSplit, NU = sizeof(T) == 4 ? 1 : GATE ? 2 : 3;
+  constexpr bool kRest = sizeof(T) == 2 && sizeof(OT) == 4;  // heads that share q and k, summed before they are rounded: outputs go to LDS in two parts
+  constexpr bool kGate = GATE && !STATE_ONLY;
   __shared__ Lds<T, E, FT> s;
+  __shared__ GateLds gs;
   int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the same in all lanes, as the compiler now knows
   const int64_t unit = blockIdx.x;
   const int seg = (int)(unit % a.nseg);
   if constexpr (STATE_ONLY)
     if (seg == (FWD ? a.nseg - 1 : 0)) return;  // no segment enters with its state
-  const int64_t bh = unit / a.nseg, b = bh / a.H, nbh = a.units / a.nseg;
+  const int64_t bh = unit / a.nseg, b = bh / a.H;
   const int h = (int)(bh % a.H);
   const int nchunk = (int)((a.L + kC - 1) / kC);
   const int c_lo = seg * a.seg_chunks, chunks = min(nchunk, c_lo + a.seg_chunks) - c_lo;
   const T *xh = a.x.head(b, h), *yh = a.y.head(b, h), *zh = a.z.head(b, h), *gh = a.g.head(b, h);
   OT* const oh = STATE_ONLY ? nullptr : a.out.head(b, h);
-  const T* const dh = DOTS && !STATE_ONLY ? a.dot.head(b, h) : nullptr;
+  const T* const uh = kGate ? a.u.head(b, h) : nullptr;
   // the lane's places in the LDS arrays
   uint32_t row_off = Rows<T, E>::row_lane(li, lg), p_off = Rows<T, kC>::row_lane(li, lg);
   uint32_t ycol_off = Rows<T, E>::template col_lane<true>(li, lg), zcol_off = Rows<T, FT>::template col_lane<false>(li, lg), o_off = Rows<T, FT>::four_lane(li, lg);
 
-  // The state. In the workspace (segments, anchors) a state is f32x4 [et][thread], padding included; the caller's
+  // The state. In the workspace a segment's state is f32x4 [et][thread], padding included; the caller's
   // are K V floats, (e, f) at e se + f sf.
   f32x4 S[FW][ET];
   const int64_t kv = (int64_t)a.E * a.F;
@@ -527,7 +630,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 
   // this thread's 8-column pieces of x, y and z on their way to LDS: one of every kRowsX (kRowsZ) rows
   constexpr int XC = E / 8, kRowsX = kThr / XC, XP = kC / kRowsX, ZC = FT / 8, kRowsZ = kThr / ZC, ZP = kC / kRowsZ;
-  Frag<T> px[STATE_ONLY ? 1 : XP], py[XP], pz[ZP], pu[DOTS && !STATE_ONLY ? ZP : 1];
+  Frag<T> px[STATE_ONLY ? 1 : XP], py[XP], pz[ZP], pu[kGate ? ZP : 1];
   int xrow = threadIdx.x / XC, xcol = threadIdx.x % XC * 8, zrow = threadIdx.x / ZC, zcol = threadIdx.x % ZC * 8;
   uint32_t x_lds = Rows<T, E>::piece(xrow & 15, xcol / 8) + (xrow >> 4) * 16 * Rows<T, E>::kBytes;
   uint32_t z_lds = Rows<T, FT>::plain(zrow & 15, zcol / 8) + (zrow >> 4) * 16 * Rows<T, FT>::kBytes;
@@ -580,6 +683,14 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
         fit(pz[p], n);
     }
   };
+  auto fetch_u = [&](int64_t t0) {  // for which x's place is free after the scores
+    const int last = (int)min((int64_t)kC, a.L - t0) - 1;
+    const T* ub = uh + t0 * a.u.sl;
+    const uint32_t col = min((uint32_t)zcol, z_most);
+    if (!narrow_z)
+#pragma unroll
+      for (int p = 0; p < ZP; ++p) load8(pu[p], at32(ub, (uint32_t)min(p * kRowsZ + zrow, last) * (uint32_t)a.u.sl + col));
+  };
   constexpr int kGateWave = NW - 1;  // one of those with the fewest score tiles
   constexpr int kStep = FWD ? 1 : -1;
   int c = FWD ? c_lo : c_lo + chunks - 1;
@@ -588,6 +699,34 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     return gh[(n < chunks && t < a.L ? t : 0) * a.g.sl];
   };
   auto gate_of = [&](int n, T g) { return (int64_t)(FWD ? c_lo + n : c_lo + chunks - 1 - n) * kC + lane < a.L ? to_f32(g) : 0.0f; };
+
+  // The states entering the chunks: dq's walk leaves them, dk's multiplies them with its own, 32 rows at a time. Columns of padding
+  // are left out, and any others read for them: their states are zero.
+  const int ft_n = (a.F + 15) / 16;
+  auto state_at = [&](int c, int fw) { return a.states + ((bh * nchunk + c) * ft_n + min(wave * FW + fw, ft_n - 1)) * (ET * 64); };  // [et][lane]
+  auto put_state = [&](int c) {
+#pragma unroll
+    for (int fw = 0; fw < FW; ++fw)
+      if (wave * FW + fw < ft_n)
+#pragma unroll
+        for (int et = 0; et < ET; ++et) *at32(state_at(c, fw), et * 64 + lane) = S[fw][et];
+  };
+  f32x4 other[kGate && !FWD ? 2 : 1][FW][2];
+  auto fetch_state = [&](int c, int ks) {
+#pragma unroll
+    for (int fw = 0; fw < FW; ++fw)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) other[ks & 1][fw][e] = *at32(state_at(c, fw), (2 * ks + e) * 64 + lane);
+  };
+  auto use_state = [&](float& sum, int ks) {
+#pragma unroll
+    for (int fw = 0; fw < FW; ++fw)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum = fmaf(other[ks & 1][fw][e][r], S[fw][2 * ks + e][r], sum);
+    again(sum);  // formed here: beside its use it would hold the loads' registers until then
+  };
 
   double log_decay = 0.0;
   T g_next = from_f32<T>(0.0f);
@@ -604,9 +743,11 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     again(xrow), again(xcol), again(zrow), again(zcol);
     const int buf = n & 1;
     const int64_t t0 = (int64_t)c * kC;
-    const bool anchor = !STATE_ONLY && DOTS && c % a.anchor_chunks == 0;
-    f32x4* const anchor_at = anchor ? a.anchors + (bh * a.nanchor + c / a.anchor_chunks) * kTiles : nullptr;
-    if (FWD && anchor) each_tile([&](int at, f32x4& v) { anchor_at[at] = v; });
+    [[maybe_unused]] float with = 0.0f, part_dg = 0.0f;
+    if constexpr (kGate) {
+      fetch_u(t0);
+      if (!FWD && wave == 0) part_dg = a.partial[bh * a.L + min(t0 + lane, a.L - 1)];
+    }
     if (!exact || t0 + kC > a.L) fit_chunk(t0);
 #pragma unroll
     for (int p = 0; p < XP; ++p) {
@@ -616,10 +757,13 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 #pragma unroll
     for (int p = 0; p < ZP; ++p) s.z.put_plain(z_lds, p * kRowsZ / 16, pz[p]);
     __syncthreads();
-    if (n + 1 < chunks) fetch_chunk(c + kStep);  // before the outputs' stores, which the loads would wait behind
+    if constexpr (kGate && !FWD) fetch_state(c, 0), fetch_state(c, 1);
+    if (n + 1 < chunks) fetch_chunk(c + kStep);  // before any stores, which the loads would wait behind
+    if constexpr (kGate && FWD) put_state(c);
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
     f32x4 acc[FW][4];  // outputs, transposed: columns f + 16 fw of z by steps i = 16 it + li
+    [[maybe_unused]] float scores[12 / NW][4];  // decayed, of this wave's tiles
     if constexpr (!STATE_ONLY) {
       // decayed scores, transposed in registers: rows j = 16 jt + 4 lg + r, column i = 16 it + li
 #pragma unroll
@@ -645,6 +789,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
             const int j = 4 * lg + r;
             const bool live = it != jt || (FWD ? j <= li : j >= li);
             part[r] = sc[r] * fast_exp2(live ? (FWD ? d : -d) : -INFINITY);
+            if constexpr (kGate && FWD) scores[k][r] = part[r];
           }
           if constexpr (NS == 1) {
             s.p[0].put_four(p_off, it, jt, part);
@@ -663,6 +808,10 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
         for (int it = 0; it < 4; ++it) acc[fw][it] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (kGate && !FWD) {
+          use_state(with, ks);
+          if (ks + 2 < KS) fetch_state(c, ks + 2);
+        }
         Frag<T> sf[FW][NS];
 #pragma unroll
         for (int fw = 0; fw < FW; ++fw) {
@@ -693,6 +842,52 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     }
     if constexpr (!STATE_ONLY) __syncthreads();
 
+    if constexpr (kGate) {
+      if (!exact || t0 + kC > a.L)
+#pragma unroll
+        for (int p = 0; p < ZP; ++p) {
+          const int64_t t = t0 + p * kRowsZ + zrow;
+          const int n = t < a.L ? a.F - zcol : 0;
+          if (narrow_z)
+            by_elements(pu[p], uh + t * a.u.sl, zcol, n);
+          else
+            fit(pu[p], n);
+        }
+#pragma unroll
+      for (int p = 0; p < ZP; ++p) s.u.put_plain(z_lds, p * kRowsZ / 16, pu[p]);
+      __syncthreads();
+      // u_i . (x_i times the state)
+      float d[4];
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        d[it] = 0.0f;
+#pragma unroll
+        for (int fw = 0; fw < FW; ++fw) {
+          const f32x4 u = s.u.get_plain_four(o_off, it, wave * FW + fw);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d[it] = fmaf(u[r], acc[fw][it][r], d[it]);
+        }
+      }
+      gs.dots[wave][lane] = sum_groups(d, lg);
+      if constexpr (FWD) {
+        const uint32_t zrow_off = Rows<T, FT>::row_lane(li, lg);
+#pragma unroll
+        for (int k = 0; k < 12 / NW; ++k) {
+          const int id = wave + NW * k;
+          if (id < 10) {
+            const int it = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, jt = id - it * (it + 1) / 2;
+            f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < FT / 32; ++ks) sc = mma(s.z.row(zrow_off, jt, ks), s.u.row(zrow_off, it, ks), sc);
+            const float p[4] = {scores[k][0] * sc[0], scores[k][1] * sc[1], scores[k][2] * sc[2], scores[k][3] * sc[3]};
+            put_pairs(gs, p, it, jt, li, lg, lane);
+          }
+        }
+      } else {
+        with = wave_sum(with);
+        if (lane == 0) gs.with[wave] = with;
+      }
+    }
     if constexpr (!STATE_ONLY) {
       // the scores times z
 #pragma unroll
@@ -710,7 +905,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
               for (int fw = 0; fw < FW; ++fw) acc[fw][it] = mma(zf[fw], pf, acc[fw][it]);
             }
       }
-      if constexpr (kRest) __syncthreads();  // the scores have been used
+      if constexpr (kGate) __syncthreads();  // the scores and u have been used
 #pragma unroll
       for (int it = 0; it < 4; ++it)
 #pragma unroll
@@ -751,29 +946,22 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
           for (int fw = 0; fw < FW; ++fw) S[fw][et] = mma(yf, zw[fw][m], S[fw][et]);
       }
     }
-    if constexpr (DOTS && !STATE_ONLY) {  // what the outputs are multiplied with
-      const int steps = (int)min((int64_t)kC, a.L - t0);
-      const T* from = dh + t0 * a.dot.sl;
+    if constexpr (kGate) {
+      if (wave == 0) {
+        float d = 0.0f;
 #pragma unroll
-      for (int p = 0; p < ZP; ++p) {
-        const int row = p * kRowsZ + zrow, n = row < steps ? a.F - zcol : 0;
-        if (narrow_z) {
-          by_elements(pu[p], dh + (t0 + row) * a.dot.sl, zcol, n);
+        for (int w = 0; w < NW; ++w) d += gs.dots[w][lane];
+        if constexpr (FWD) {
+          d = suffix_sum<kC>(d, lane) + pair_sums(gs, li, lg, lane);
+          if (t0 + lane < a.L) a.partial[bh * a.L + t0 + lane] = d;
         } else {
-          load8(pu[p], at32(from, (uint32_t)min(row, steps - 1) * (uint32_t)a.dot.sl + min((uint32_t)zcol, z_most)));
-          if (!exact || steps < kC) fit(pu[p], n);
+          float both = 0.0f;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) both += gs.with[w];
+          d = part_dg + prefix_before<kC>(d, lane) + tot * both;
+          if (t0 + lane < a.L) a.dg.head(b, h)[(t0 + lane) * a.dg.sl] = from_f32<T>(d);
         }
       }
-    }
-    if (!FWD && anchor) {
-      float d = 0.0f;
-      each_tile([&](int at, f32x4& v) {
-        const f32x4 from = anchor_at[at];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d = fmaf(from[r], v[r], d);
-      });
-      d = wave_sum(d);
-      if (lane == 0) a.anchor_dots[((int64_t)wave * nbh + bh) * a.nanchor + c / a.anchor_chunks] = d;
     }
     __syncthreads();
     if constexpr (!STATE_ONLY) {
@@ -786,12 +974,6 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
         Frag<T> rest = {};
         if constexpr (kRest) rest = s.o_rest.get_plain(z_lds, p * kRowsZ / 16);
         if (n > 0) store8(at32(oh + t0 * a.out.sl, row * (uint32_t)a.out.sl + zcol), o, rest, n);
-        if constexpr (DOTS) {
-          float d = dot8(o, rest, pu[p]);
-#pragma unroll
-          for (int m = ZC / 2; m >= 1; m >>= 1) d += __shfl_xor(d, m, kWave);
-          if (zcol == 0 && row < steps) a.dots[bh * a.L + t0 + row] = d;
-        }
       }
       __syncthreads();  // x's place is free again
     }
@@ -852,60 +1034,6 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(f32x4* seg, const do
           for (int r = 0; r < 4; ++r) t[(n0 + k) * step * 4 + r * 4] = s[r];
         s = fast_exp2(keep[k]) * s + own[k];
       }
-  }
-}
-
-// dg over one anchor's steps: the anchor's value, then the running sum of c - r before each step. What the sum misses the next
-// anchor by (after the last step: zero, where the last state has no gradient) is what rounding left in it; taken back in
-// proportion to the steps passed, it leaves 0.6 times the error.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void dgate_kernel(const float* r, const float* c, const float* anchor_dots, Seq<const T> g, Seq<T> dg, int H,
-                                                         int64_t L, int64_t nbh, int parts, int anchor_steps, int nanchor, int ends_at_zero) {
-  __shared__ float part[4];
-  const int64_t bh = blockIdx.x / nanchor;
-  const int anchor = (int)(blockIdx.x % nanchor);
-  const int64_t b = bh / H, t0 = (int64_t)anchor * anchor_steps;
-  const int h = (int)(bh % H), steps = (int)min((int64_t)anchor_steps, L - t0);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  r += bh * L + t0;
-  c += bh * L + t0;
-  auto anchor_of = [&](int n) {
-    float v = 0.0f;
-    for (int f = 0; f < parts; ++f) v += anchor_dots[((int64_t)f * nbh + bh) * nanchor + n];
-    return v;
-  };
-  float base = anchor_of(anchor), slope = 0.0f;
-  if (anchor + 1 < nanchor || ends_at_zero) {
-    float sum = 0.0f;
-    for (int at = threadIdx.x; at < steps; at += kThreads) sum += c[at] - r[at];
-    sum = wave_sum(sum);
-    if (lane == 0) part[wave] = sum;
-    __syncthreads();
-    const float end = base + ((part[0] + part[1]) + (part[2] + part[3]));
-    slope = ((anchor + 1 < nanchor ? anchor_of(anchor + 1) : 0.0f) - end) / (float)steps;
-    if (!isfinite(slope)) slope = 0.0f;  // a NaN further on is no reason to lose the steps before it
-    __syncthreads();
-  }
-  for (int o = 0; o < steps; o += kThreads) {
-    const int at = o + (int)threadIdx.x;
-    const float v = at < steps ? c[at] - r[at] : 0.0f;
-    float sum = v;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const float up = __shfl_up(sum, d, kWave);
-      if (lane >= d) sum += up;
-    }
-    if (lane == 63) part[wave] = sum;
-    __syncthreads();
-    float before = base;
-    for (int w = 0; w < wave; ++w) before += part[w];
-    if (at < steps) {
-      // where exp(g) is zero in fp32 the gradient is, whatever the sums' rounding left
-      const bool none = to_f32(g.head(b, h)[(t0 + at) * g.sl]) < -104.0f;
-      dg.head(b, h)[(t0 + at) * dg.sl] = from_f32<T>(none ? 0.0f : fmaf(slope, (float)at, before + (sum - v)));
-    }
-    for (int w = 0; w < 4; ++w) base += part[w];
-    __syncthreads();
   }
 }
 
@@ -994,16 +1122,13 @@ int args_status(const Sizes& s, int dtype) {
   if (s.B < 0 || s.L < 0 || s.H < 1 || s.Hk < 1 || s.K < 1 || s.V < 1 || s.H % s.Hk != 0) return TSF_ERR_ARG;
   if (dtype != TSF_DTYPE_F32 && dtype != TSF_DTYPE_BF16) return TSF_ERR_ARG;
   if (s.K > kMaxWidth || s.V > kMaxWidth) return TSF_ERR_UNSUPPORTED;
-  // workgroups of the largest launches: one a segment and tile, one an anchor, one per 256 state elements
+  // workgroups of the largest launches: one a segment, one per 64 pieces of a state
   const int64_t chunks = (s.L + kC - 1) / kC, rows = s.B > 0 ? s.B : 1;
   if (s.H > (1 << 16) || s.L > ((int64_t)1 << 30) || rows > kMaxGrid / s.H) return TSF_ERR_UNSUPPORTED;
   const int64_t bh = rows * s.H;
   if (bh > kMaxGrid / 64 || bh * (chunks + 8) > kMaxGrid) return TSF_ERR_UNSUPPORTED;
   return TSF_OK;
 }
-
-// Waves of a walk: a workgroup takes all of its columns, so that nothing of x and y is done twice.
-constexpr int kWaves = 4;
 
 int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
 
@@ -1032,16 +1157,14 @@ int segments(const Sizes& s, int dtype) {
   return (int)best;
 }
 
-// Chunks between dg's anchors: an anchor's states cost 8 bytes a state element, the running sum's errors grow with the root
-// of the distance. What is rounded to bf16 can bear 16 chunks of them; fp32 heads that forget within a few steps, the worst
-// case, have 1.4e-6 of dg's size at four chunks and no correction, 7e-7 at two with it.
-int anchor_chunks(int dtype) { return dtype == TSF_DTYPE_BF16 ? 16 : 2; }
+// Bytes of a chunk's state as dq's walk leaves it for dk's.
+int64_t chunk_state(int64_t K, int64_t V) { return (K + 15) / 16 * 64 * (V <= 64 ? 64 : 128); }
 
 int64_t align_up(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
-// Workspace: [segment states][segment decays]; backward also [segment states, turned][r][c][anchors][anchor dots][dq, dk per head].
+// Workspace: [segment states][segment decays]; backward also [segment states, turned][part of dg][chunks' states][dq, dk per head].
 struct Space {
-  int64_t seg, decay, turned, r, c, anchors, anchor_dots, dq, dk, bytes;
+  int64_t seg, decay, turned, partial, states, dq, dk, bytes;
 };
 Space space(const Sizes& s, int dtype, bool backward) {
   Space w = {};
@@ -1058,11 +1181,8 @@ Space space(const Sizes& s, int dtype, bool backward) {
     if (backward) w.turned = take(bh * nseg * state);
   }
   if (backward) {
-    const int64_t chunks = (s.L + kC - 1) / kC, ac = anchor_chunks(dtype), na = (chunks + ac - 1) / ac;
-    w.r = take(bh * s.L * 4);
-    w.c = take(bh * s.L * 4);
-    w.anchors = take(bh * na * state);
-    w.anchor_dots = take(kWaves * bh * na * 4);
+    w.partial = take(bh * s.L * 4);
+    w.states = take(bh * ((s.L + kC - 1) / kC) * chunk_state(s.K, s.V));
     if (s.H != s.Hk) {
       w.dq = take(s.B * s.L * s.H * s.K * 4);
       w.dk = take(s.B * s.L * s.H * s.K * 4);
@@ -1075,21 +1195,21 @@ Space space(const Sizes& s, int dtype, bool backward) {
 // One walk, cut rows' segment states first, unless `entering` has them. o's and dq's walks, and dv's and dk's, have the same
 // states between segments with rows and columns exchanged: o's and dv's leave them in `turned` for the other (16 rows of 4096
 // steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 37 less each, for 63 MB that o's keeps).
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool DOTS>
+template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool GATE>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
            hipStream_t stream) {
   const int64_t bh = a.units;
   a.units = bh * a.nseg;
   if (a.nseg == 1) {
     a.init = init;
-  } else if (entering || (!FWD && DOTS)) {  // dk's always has them
+  } else if (entering || (!FWD && GATE)) {  // dk's always has them
     a.seg_init = (const f32x4*)entering;
-  } else if constexpr (FWD || !DOTS) {
+  } else if constexpr (FWD || !GATE) {
     WalkArgs<T, OT> p = a;
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
     p.seg_decay = (double*)(ws + sp.decay);
-    walk_kernel<T, OT, E, NW, FW, FWD, true, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
+    walk_kernel<T, OT, E, NW, FW, FWD, true, GATE><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
     const int64_t total = bh * E / 16 * 64 * NW * FW;
     const auto join = a.nseg <= 4 ? join_kernel<4> : join_kernel<16>;
     join<<<(unsigned)((total + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
@@ -1097,12 +1217,12 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     a.seg_init = seg;
   }
   a.last = last;
-  walk_kernel<T, OT, E, NW, FW, FWD, false, DOTS><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
+  walk_kernel<T, OT, E, NW, FW, FWD, false, GATE><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
   return tsf_launch_status();
 }
 
 // One walk. `init` and `last` are the row's states [row x head][K V].
-template <typename T, typename OT, bool FWD, bool DOTS>
+template <typename T, typename OT, bool FWD, bool GATE>
 int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
          hipStream_t stream) {
   a.H = (int)s.H;
@@ -1110,8 +1230,8 @@ int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const flo
   a.units = s.B * s.H;
   a.nseg = segments(s, sizeof(T) == 2 ? TSF_DTYPE_BF16 : TSF_DTYPE_F32);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
-  const auto run = a.F <= 64 ? (a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, DOTS> : walk_e<T, OT, 128, 4, 1, FWD, DOTS>)
-                             : (a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, DOTS> : walk_e<T, OT, 128, 4, 2, FWD, DOTS>);
+  const auto run = a.F <= 64 ? (a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, GATE> : walk_e<T, OT, 128, 4, 1, FWD, GATE>)
+                             : (a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, GATE> : walk_e<T, OT, 128, 4, 2, FWD, GATE>);
   return run(a, ws, sp, init, last, entering, turned, stream);
 }
 
@@ -1137,9 +1257,9 @@ int forward(const Sizes& s, const void* q, const void* k, const void* v, const v
   return walk<T, T, true, false>(a, s, ws, sp, state, last, nullptr, kept, stream);
 }
 
-// dq or dk: a walk over K's columns with V contracted, the dots of the gate's gradient beside it.
+// dq or dk: a walk over K's columns with V contracted, the gate's gradient beside it.
 template <typename T, typename OT, bool FWD>
-int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<const T> g, Seq<const T> dot, Seq<OT> out, float* dots, int dtype, char* ws, const Space& sp,
+int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<const T> g, Seq<const T> u, Seq<OT> out, void* dg, char* ws, const Space& sp,
            const float* init, const void* entering, hipStream_t stream) {
   WalkArgs<T, OT> a = {};
   a.x = x;
@@ -1151,17 +1271,15 @@ int walk_k(const Sizes& s, Seq<const T> x, Seq<const T> y, Seq<const T> z, Seq<c
   a.F = (int)s.K;
   a.se = 1;
   a.sf = (int)s.V;
-  a.dot = dot;
-  a.dots = dots;
-  a.anchors = (f32x4*)(ws + sp.anchors);
-  a.anchor_dots = (float*)(ws + sp.anchor_dots);
-  a.anchor_chunks = anchor_chunks(dtype);
-  a.nanchor = (int)(((s.L + kC - 1) / kC + a.anchor_chunks - 1) / a.anchor_chunks);
+  a.u = u;
+  a.partial = (float*)(ws + sp.partial);
+  a.states = (f32x4*)(ws + sp.states);
+  a.dg = Seq<T>{(T*)dg, s.L * s.H, s.H, 1, 1};
   return walk<T, OT, FWD, true>(a, s, ws, sp, init, nullptr, entering, nullptr, stream);
 }
 
 template <typename T>
-int backward(const Sizes& s, int dtype, const void* q, const void* k, const void* v, const void* g, const void* d_o, const int64_t* st, const float* state,
+int backward(const Sizes& s, const void* q, const void* k, const void* v, const void* g, const void* d_o, const int64_t* st, const float* state,
              const float* dlast, void* dq, void* dk, void* dv, void* dg, float* dstate, const void* kept, char* ws, const Space& sp,
              hipStream_t stream) {
   const int share = (int)(s.H / s.Hk);
@@ -1183,30 +1301,25 @@ int backward(const Sizes& s, int dtype, const void* q, const void* k, const void
     if (rc != TSF_OK) return rc;
   }
   if (s.L == 0) return TSF_OK;
-  float *r = (float*)(ws + sp.r), *c = (float*)(ws + sp.c);
   int rc;
   if (share == 1) {
     const int64_t sl = s.H * s.K;
-    rc = walk_k<T, T, true>(s, DO, Vv, Kk, G, Q, Seq<T>{(T*)dq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, kept, stream);
+    rc = walk_k<T, T, true>(s, DO, Vv, Kk, G, Q, Seq<T>{(T*)dq, s.L * sl, sl, s.K, 1}, dg, ws, sp, state, kept, stream);
     if (rc != TSF_OK) return rc;
-    rc = walk_k<T, T, false>(s, Vv, DO, Q, G, Kk, Seq<T>{(T*)dk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, ws + sp.turned, stream);
+    rc = walk_k<T, T, false>(s, Vv, DO, Q, G, Kk, Seq<T>{(T*)dk, s.L * sl, sl, s.K, 1}, dg, ws, sp, dlast, ws + sp.turned, stream);
     if (rc != TSF_OK) return rc;
   } else {
     const int64_t sl = s.H * s.K, total = s.B * s.L * s.Hk * s.K;
     float *pq = (float*)(ws + sp.dq), *pk = (float*)(ws + sp.dk);
-    rc = walk_k<T, float, true>(s, DO, Vv, Kk, G, Q, Seq<float>{pq, s.L * sl, sl, s.K, 1}, r, dtype, ws, sp, state, kept, stream);
+    rc = walk_k<T, float, true>(s, DO, Vv, Kk, G, Q, Seq<float>{pq, s.L * sl, sl, s.K, 1}, dg, ws, sp, state, kept, stream);
     if (rc != TSF_OK) return rc;
-    rc = walk_k<T, float, false>(s, Vv, DO, Q, G, Kk, Seq<float>{pk, s.L * sl, sl, s.K, 1}, c, dtype, ws, sp, dlast, ws + sp.turned, stream);
+    rc = walk_k<T, float, false>(s, Vv, DO, Q, G, Kk, Seq<float>{pk, s.L * sl, sl, s.K, 1}, dg, ws, sp, dlast, ws + sp.turned, stream);
     if (rc != TSF_OK) return rc;
     const int64_t blocks = (total + kThreads - 1) / kThreads;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
     share_kernel<T><<<grid, kThreads, 0, stream>>>(pq, (T*)dq, share, (int)s.K, total);
     share_kernel<T><<<grid, kThreads, 0, stream>>>(pk, (T*)dk, share, (int)s.K, total);
   }
-  const int ac = anchor_chunks(dtype);
-  const int na = (int)(((s.L + kC - 1) / kC + ac - 1) / ac);
-  dgate_kernel<T><<<(unsigned)(s.B * s.H * na), kThreads, 0, stream>>>(r, c, (const float*)(ws + sp.anchor_dots), G, Seq<T>{(T*)dg, s.L * s.H, s.H, 1, 1},
-                                                                       (int)s.H, s.L, s.B * s.H, kWaves, ac * kC, na, dlast == nullptr);
   return tsf_launch_status();
 }
 
@@ -1265,9 +1378,9 @@ int tsfast_hip_gated_bwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int6
   if (!steps_fit(strides, 3) || !steps_fit(strides + 12, 1)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, true);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
-  return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
+  return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
                                                   (char*)workspace, sp, (hipStream_t)stream)
-                                 : backward<float>(s, dtype, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
+                                 : backward<float>(s, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,
                                                    (char*)workspace, sp, (hipStream_t)stream);
 }
 

@@ -97,7 +97,7 @@ def gated_recurrence(q, k, v, g, state=None):
         (float64 for float64 inputs) whatever the others' type.
 
     All of q, k, v must be finite: the fused kernel works in chunks of 64 steps, and a value that is not may
-    reach every step of its chunk, and the gradient of g for up to 1024 steps after it.
+    reach every step of its chunk and, with the state, the chunks after it (in gradients before it), whatever g is.
     """
     _check_shapes(q, k, v, g, state, "B, L")
     mod = resolve("gated.recurrence", _RECURRENCE_BACKENDS, _AUTO_ORDER.get(v.device.type, ()), (q, k, v, g, state))
