@@ -342,7 +342,7 @@ int tsfast_hip_mat_adjoint_bounds(int64_t B, int64_t L, int64_t n, int64_t CL, c
  * K, V <= 128. g may be any value up to 0 and -inf (the state is forgotten); the other inputs are finite:
  * a value that is not may reach every step of its 64-step chunk.
  * `strides` is host memory, in elements: batch row, step and head of q, k, v, g (and grad_o: 15 in all);
- * the last dimension of q, k, v and grad_o is dense, their steps are at most 2^23 elements apart. No alignment is needed.
+ * the last dimension of q, k, v and grad_o is dense, their steps (of L > 1) are at most 2^23 elements apart. No alignment is needed.
  * state and grad_last may be NULL (zero); grad_state is required iff state is given. L = 0 copies the state.
  */
 int64_t tsfast_hip_gated_fwd_workspace_bytes(int64_t B, int64_t L, int64_t H, int64_t Hk, int64_t K, int64_t V, int dtype);

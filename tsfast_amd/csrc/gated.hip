@@ -1111,8 +1111,9 @@ struct Sizes {
   int64_t B, L, H, Hk, K, V;
 };
 
-// Steps of a chunk are reached by 32-bit byte offsets from its first.
-bool steps_fit(const int64_t* strides, int tensors) {
+// Steps of a chunk are reached by 32-bit byte offsets from its first; a single one may be at any distance from none.
+bool steps_fit(const int64_t* strides, int tensors, int64_t L) {
+  if (L <= 1) return true;
   for (int i = 0; i < tensors; ++i)
     if (strides[3 * i + 1] < 0 || strides[3 * i + 1] > kMaxStep) return false;
   return true;
@@ -1353,7 +1354,7 @@ int tsfast_hip_gated_fwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int6
   if (rc != TSF_OK) return rc;
   if (B == 0) return TSF_OK;
   if (!strides || !state_last || (L > 0 && (!q || !k || !v || !g || !o))) return TSF_ERR_ARG;
-  if (!steps_fit(strides, 3)) return TSF_ERR_UNSUPPORTED;
+  if (!steps_fit(strides, 3, L)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, false);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
   return dtype == TSF_DTYPE_BF16 ? forward<bf16>(s, q, k, v, g, strides, state, o, state_last, kept, (char*)workspace, sp, (hipStream_t)stream)
@@ -1375,7 +1376,7 @@ int tsfast_hip_gated_bwd_train(int64_t B, int64_t L, int64_t H, int64_t Hk, int6
   if (B == 0) return TSF_OK;
   if (!strides || (state && !grad_state)) return TSF_ERR_ARG;
   if (L > 0 && (!q || !k || !v || !g || !grad_o || !grad_q || !grad_k || !grad_v || !grad_g)) return TSF_ERR_ARG;
-  if (!steps_fit(strides, 3) || !steps_fit(strides + 12, 1)) return TSF_ERR_UNSUPPORTED;
+  if (!steps_fit(strides, 3, L) || !steps_fit(strides + 12, 1, L)) return TSF_ERR_UNSUPPORTED;
   const Space sp = space(s, dtype, true);
   if (sp.bytes > 0 && (!workspace || workspace_bytes < sp.bytes)) return TSF_ERR_WORKSPACE;
   return dtype == TSF_DTYPE_BF16 ? backward<bf16>(s, q, k, v, g, grad_o, strides, state, grad_last, grad_q, grad_k, grad_v, grad_g, grad_state, kept,

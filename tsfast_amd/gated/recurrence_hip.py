@@ -85,9 +85,9 @@ def supports_step(q, k, v, g, state) -> str | None:
 
 
 def _dense(t):
-    """``t`` with a dense last dimension, the only one the kernels read without a stride, and steps that 64-step chunks
-    reach with 32-bit offsets."""
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) <= _MAX_STEP):
+    """``t`` with a dense last dimension, the only one the kernels read without a stride, and steps (if there is more than one) that
+    64-step chunks reach with 32-bit offsets."""
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) <= _MAX_STEP or t.shape[1] <= 1):
         return t
     return t.contiguous()
 
