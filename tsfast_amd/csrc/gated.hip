@@ -521,8 +521,8 @@ TSF_DEV float pair_sums(const GateLds& g, int li, int lg, int lane) {
 
 // Waves a SIMD holds of a walk: what LDS and a 512-register file allow.
 template <typename T>
-constexpr int walk_waves(int E, int NW, int FW) {
-  return sizeof(T) == 2 ? (NW == 8 ? 4 : 2) : E == 64 && FW == 1 && NW == 4 ? 2 : NW / 4;
+constexpr int walk_waves(int E, int FW) {
+  return sizeof(T) == 2 || (E == 64 && FW == 1) ? 2 : 1;
 }
 
 // One wave: the chunk's running log2 decay as float pairs (differences are exact to float64 rounding), the
@@ -563,7 +563,7 @@ TSF_DEV f32x4 four(const float* p) {
   return v;
 }
 
-// E: columns of x and y, padded; NW: waves of a workgroup; FW: 16-column tiles of z a wave owns; FWD: the direction in time;
+// E: columns of x and y, padded; FW: 16-column tiles of z a wave owns; FWD: the direction in time;
 // STATE_ONLY: only the state leaving the unit; GATE: the gate's gradient too (dq's and dk's walks).
 //
 // The weighted z of the state's update is split into three bf16 operands where the caller gets the state (2^-24), two where
@@ -573,9 +573,9 @@ TSF_DEV f32x4 four(const float* p) {
 // two by two are operands as they stand. Per chunk: (1) x, y, z to LDS; (2) the ten live 16 x 16 score tiles, shared
 // among the waves, decayed and split into LDS, and x times the state; (3) the scores times z, the outputs, the state's update. With
 // GATE, u takes x's place before (3), for its products with x times the state and, in dq's walk, with z = k: the pairs' second score.
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool STATE_ONLY, bool GATE>
-__global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel(WalkArgs<T, OT> a) {
-  constexpr int kThr = 64 * NW, FT = 16 * NW * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT>::kSplit, NU = sizeof(T) == 4 ? 1 : GATE ? 2 : 3;
+template <typename T, typename OT, int E, int FW, bool FWD, bool STATE_ONLY, bool GATE>
+__global__ __launch_bounds__(64 * kWaves, walk_waves<T>(E, FW)) void walk_kernel(WalkArgs<T, OT> a) {
+  constexpr int kThr = 64 * kWaves, FT = 16 * kWaves * FW, KS = E / 32, ET = E / 16, NS = Lds<T, E, FT>::kSplit, NU = sizeof(T) == 4 ? 1 : GATE ? 2 : 3;
   constexpr bool kRest = sizeof(T) == 2 && sizeof(OT) == 4;  // heads that share q and k, summed before they are rounded: outputs go to LDS in two parts
   constexpr bool kGate = GATE && !STATE_ONLY;
   __shared__ Lds<T, E, FT> s;
@@ -691,7 +691,7 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
 #pragma unroll
       for (int p = 0; p < ZP; ++p) load8(pu[p], at32(ub, (uint32_t)min(p * kRowsZ + zrow, last) * (uint32_t)a.u.sl + col));
   };
-  constexpr int kGateWave = NW - 1;  // one of those with the fewest score tiles
+  constexpr int kGateWave = kWaves - 1;  // one of those with the fewest score tiles
   constexpr int kStep = FWD ? 1 : -1;
   int c = FWD ? c_lo : c_lo + chunks - 1;
   auto fetch_gate = [&](int n) {  // of the n-th chunk walked; a step that does not exist reads another
@@ -763,12 +763,12 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
     if constexpr (STATE_ONLY) log_decay += (double)s.hi[buf][kC - 1] + (double)s.lo[buf][kC - 1];
 
     f32x4 acc[FW][4];  // outputs, transposed: columns f + 16 fw of z by steps i = 16 it + li
-    [[maybe_unused]] float scores[12 / NW][4];  // decayed, of this wave's tiles
+    [[maybe_unused]] float scores[12 / kWaves][4];  // decayed, of this wave's tiles
     if constexpr (!STATE_ONLY) {
       // decayed scores, transposed in registers: rows j = 16 jt + 4 lg + r, column i = 16 it + li
 #pragma unroll
-      for (int k = 0; k < 12 / NW; ++k) {
-        const int id = wave + NW * k;
+      for (int k = 0; k < 12 / kWaves; ++k) {
+        const int id = wave + kWaves * k;
         if (id >= 10) {  // the two beside the diagonal that operands reach into
           const int it = FWD ? 2 * (id - 10) : 3 - 2 * (id - 10), jt = FWD ? it + 1 : it - 1;
           const float none[4] = {};
@@ -872,8 +872,8 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
       if constexpr (FWD) {
         const uint32_t zrow_off = Rows<T, FT>::row_lane(li, lg);
 #pragma unroll
-        for (int k = 0; k < 12 / NW; ++k) {
-          const int id = wave + NW * k;
+        for (int k = 0; k < 12 / kWaves; ++k) {
+          const int id = wave + kWaves * k;
           if (id < 10) {
             const int it = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, jt = id - it * (it + 1) / 2;
             f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -950,14 +950,14 @@ __global__ __launch_bounds__(64 * NW, walk_waves<T>(E, NW, FW)) void walk_kernel
       if (wave == 0) {
         float d = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) d += gs.dots[w][lane];
+        for (int w = 0; w < kWaves; ++w) d += gs.dots[w][lane];
         if constexpr (FWD) {
           d = suffix_sum<kC>(d, lane) + pair_sums(gs, li, lg, lane);
           if (t0 + lane < a.L) a.partial[bh * a.L + t0 + lane] = d;
         } else {
           float both = 0.0f;
 #pragma unroll
-          for (int w = 0; w < NW; ++w) both += gs.with[w];
+          for (int w = 0; w < kWaves; ++w) both += gs.with[w];
           d = part_dg + prefix_before<kC>(d, lane) + tot * both;
           if (t0 + lane < a.L) a.dg.head(b, h)[(t0 + lane) * a.dg.sl] = from_f32<T>(d);
         }
@@ -1196,7 +1196,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
 // One walk, cut rows' segment states first, unless `entering` has them. o's and dq's walks, and dv's and dk's, have the same
 // states between segments with rows and columns exchanged: o's and dv's leave them in `turned` for the other (16 rows of 4096
 // steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 37 less each, for 63 MB that o's keeps).
-template <typename T, typename OT, int E, int NW, int FW, bool FWD, bool GATE>
+template <typename T, typename OT, int E, int FW, bool FWD, bool GATE>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
            hipStream_t stream) {
   const int64_t bh = a.units;
@@ -1210,15 +1210,16 @@ int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, floa
     f32x4* seg = (f32x4*)(ws + sp.seg);
     p.seg_last = seg;
     p.seg_decay = (double*)(ws + sp.decay);
-    walk_kernel<T, OT, E, NW, FW, FWD, true, GATE><<<(unsigned)a.units, 64 * NW, 0, stream>>>(p);
-    const int64_t total = bh * E / 16 * 64 * NW * FW;
+    walk_kernel<T, OT, E, FW, FWD, true, GATE><<<(unsigned)a.units, 64 * kWaves, 0, stream>>>(p);
+    const int64_t total = bh * E / 16 * 64 * kWaves * FW;
     const auto join = a.nseg <= 4 ? join_kernel<4> : join_kernel<16>;
-    join<<<(unsigned)((total + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * NW, E / 16, FW, a.E, a.F, a.se, a.sf, total, !FWD,
-                                                                  (float*)turned, FW * NW, E / 16 / NW);
+    join<<<(unsigned)((total + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(seg, p.seg_decay, init, a.nseg, 64 * kWaves, E / 16, FW, a.E, a.F,
+                                                                                            a.se, a.sf, total, !FWD, (float*)turned, FW * kWaves,
+                                                                                            E / 16 / kWaves);
     a.seg_init = seg;
   }
   a.last = last;
-  walk_kernel<T, OT, E, NW, FW, FWD, false, GATE><<<(unsigned)a.units, 64 * NW, 0, stream>>>(a);
+  walk_kernel<T, OT, E, FW, FWD, false, GATE><<<(unsigned)a.units, 64 * kWaves, 0, stream>>>(a);
   return tsf_launch_status();
 }
 
@@ -1231,8 +1232,8 @@ int walk(WalkArgs<T, OT> a, const Sizes& s, char* ws, const Space& sp, const flo
   a.units = s.B * s.H;
   a.nseg = segments(s, sizeof(T) == 2 ? TSF_DTYPE_BF16 : TSF_DTYPE_F32);
   a.seg_chunks = (int)(((s.L + kC - 1) / kC + a.nseg - 1) / a.nseg);
-  const auto run = a.F <= 64 ? (a.E <= 64 ? walk_e<T, OT, 64, 4, 1, FWD, GATE> : walk_e<T, OT, 128, 4, 1, FWD, GATE>)
-                             : (a.E <= 64 ? walk_e<T, OT, 64, 4, 2, FWD, GATE> : walk_e<T, OT, 128, 4, 2, FWD, GATE>);
+  const auto run = a.F <= 64 ? (a.E <= 64 ? walk_e<T, OT, 64, 1, FWD, GATE> : walk_e<T, OT, 128, 1, FWD, GATE>)
+                             : (a.E <= 64 ? walk_e<T, OT, 64, 2, FWD, GATE> : walk_e<T, OT, 128, 2, FWD, GATE>);
   return run(a, ws, sp, init, last, entering, turned, stream);
 }
 
