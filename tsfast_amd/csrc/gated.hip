@@ -13,10 +13,10 @@
 //                                     backward in time (j >= i):  dv (k, q, do), dk (v, do, q)
 //
 // so one kernel, walk_kernel, computes all four. A workgroup owns one head of one row and a run of 64-step chunks; the
-// state stays in fp32 accumulator registers from the first chunk to the last and is never written in between. Per chunk
+// state stays in fp32 accumulator registers from the first chunk to the last. Per chunk
 // the decayed scores of x and y within it (64 x 64, the causal half only) times z, x times the state before it, and the
-// state's update are MFMA products; the decays come from exact differences of a float64 running sum, so any g <= 0 down
-// to -inf keeps its accuracy. Few rows are cut into segments: a walk of the state alone, a join of the segments' states, the
+// state's update are MFMA products; the decays come from exact differences of a float64 running sum, so that o, dq, dk and dv
+// keep their accuracy for any g <= 0 down to -inf. Few rows are cut into segments: a walk of the state alone, a join of the segments' states, the
 // walk proper; dk's walk takes its segments' states from dv's, and a training step's dq from o's.
 //
 // dg is a sum of terms that each carry their own decay from j < t to i >= t, so that it keeps its relative accuracy however
@@ -26,17 +26,20 @@
 //   dg_t = sum_{j < t <= i} D (q_i . k_j)(do_i . v_j) + sum_{i >= t} in_i q_i . (S do_i) + sum_{j < t} w_j k_j . (T v_j) + tot <S, T>.
 //
 // dq's walk has S and gives the first two, from its decayed scores and the part of dq that S makes, and leaves every chunk's S;
-// dk's walk has T, adds the other two and writes dg. (The shorter dg_{t+1} = dg_t - q_t . dq_t + k_t . dk_t is a difference of
-// terms without exp(g_t): its rounding errors were as large as dg itself from g = -8 on.)
+// dk's walk has T, adds the other two and writes dg. One head of 64 x 64, 1024 steps of constant g from -0.02 to -30, relative to the largest
+// dg: 1e-7 to 1.2e-6 in fp32, 0.9e-3 to 2.5e-3 in bf16, one rounding of the result. (The shorter dg_{t+1} = dg_t - q_t . dq_t + k_t . dk_t
+// is a difference of terms without exp(g_t): with it bf16 had 3e-2 at g = -8 and more than dg itself at -12, fp32 4e-2 there.) It costs
+// a state a chunk, written and read: 2 x 805 MB at the size below, 13% of the training step.
 //
 // bf16 inputs are multiplied on the bf16 matrix cores. Products of inputs are exact there; what is fp32 (the decayed
 // scores, the state, the decayed z of an update) goes in as a sum of two or three bf16 operands, because one alone (2^-9)
 // would cost the outputs 1.4 times their own rounding, the fp32 state its type.
 // fp32 inputs use the fp32 matrix cores.
 //
-// Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 255 us for o's walk, 109 us for the
-// segments' states before it and 37 for their join, 256 for dv's, 302 and 314 for dq's and dk's. No one unit bounds a chunk (5.3 us of a CU):
-// of it matrix products take 1.4 us, LDS 1.1 us and vector instructions about as much, waits for memory the rest. Kept
+// Time, 16 rows of 4096 steps, 12 heads of 128 x 128, bf16 (805 MB forward): 225 us for o's walk, 97 us for the
+// segments' states before it and 34 for their join, 222 for dv's, 390 and 423 for dq's and dk's. No one unit bounds a chunk (4.7 us of a CU
+// in o's walk): of it matrix products take 1.4 us, LDS 1.1 us and vector instructions about as much, waits for memory the rest; dq's and
+// dk's add the chunks' states (64 KB each) and dq's the second score. Kept
 // out, for they measured slower: the state in LDS as well (2 times), transposed copies of y and z in LDS instead of
 // transposing reads (2 times, for their bank conflicts), eight waves of one column tile each (1.3 times),
 // outputs stored from accumulators, 8 bytes a lane (1.35 times).
@@ -1134,10 +1137,14 @@ int args_status(const Sizes& s, int dtype) {
 int64_t padded_state(int64_t E, int64_t F) { return (E <= 64 ? 64 : 128) * (F <= 64 ? 64 : 128); }
 
 // Segments a row is cut into: the number with the least time, in chunks walked one after the other, of one and those that
-// fill every CU once or twice (a workgroup more, and the whole chip waits for another round: 86 instead of 85 segments of 6 rows took
-// twice the time). A cut row's chunks are walked for the states too, at 0.45 times a chunk's time, and the states
-// go to memory and back five times. Four chunks a segment at least. Measured, training, against once alone: 192 rows of 4096 steps,
-// 128 x 128, bf16: 5 segments 1366 us, 2: 1460; 288 rows, 64 x 64: 5: 822, 2: 857; 192 rows of 2048, 64 x 64, fp32: 5: 786, 2: 856.
+// fill every CU once or twice (a workgroup more, and the whole chip waits for another round: where two fitted a CU, 86 instead of 85
+// segments of 6 rows took twice the time). A cut row's chunks are walked for the states too, at 0.45 times a chunk's time, and the states
+// go to memory and back five times. Measured, training: 192 rows of 4096 steps, 128 x 128, bf16: whole 1999 us, 2 segments 1656, 5: 1537;
+// 288 rows, 64 x 64: 1195, 972, 912; 192 rows of 2048, 64 x 64, fp32: 1032, 902, 826.
+// Four chunks a segment at least. It is right for short bf16 rows (forward, 4 heads of 448 steps, 64 x 64: whole 23 us, in 4: 26) and for
+// windows (128 rows of 512 steps, fp32, training: in 2, as they are, 192 us; 4: 188; 8: 209), and too high for few rows of slower chunks
+// (forward, 4 heads, 512 steps of 64 x 64, fp32: in 2 43 us, 4: 27, 8: 26; 2048 of 128 x 128, bf16: in 8 44 us, 16: 32, 32: 30; training,
+// 30 rows of 3001 of 48 x 80, bf16: in 10 234 us, 16: 188, 32: 215).
 int segments(const Sizes& s, int dtype) {
   const int64_t chunks = (s.L + kC - 1) / kC, rows = s.B * s.H;
   const bool narrow = s.K <= 64 && s.V <= 64;
@@ -1195,7 +1202,7 @@ Space space(const Sizes& s, int dtype, bool backward) {
 
 // One walk, cut rows' segment states first, unless `entering` has them. o's and dq's walks, and dv's and dk's, have the same
 // states between segments with rows and columns exchanged: o's and dv's leave them in `turned` for the other (16 rows of 4096
-// steps, 12 heads of 128 x 128, bf16: a state-only walk of 107 us and a join of 37 less each, for 63 MB that o's keeps).
+// steps, 12 heads of 128 x 128, bf16: a state-only walk of 97 us and a join of 34 less each, for 63 MB that o's keeps).
 template <typename T, typename OT, int E, int FW, bool FWD, bool GATE>
 int walk_e(WalkArgs<T, OT> a, char* ws, const Space& sp, const float* init, float* last, const void* entering, void* turned,
            hipStream_t stream) {
