@@ -340,7 +340,8 @@ int tsfast_hip_mat_adjoint_bounds(int64_t B, int64_t L, int64_t n, int64_t CL, c
  * strides; o, grad_v [B, L, H, V], grad_q, grad_k [B, L, Hk, K], grad_g [B, L, H] contiguous of that type;
  * states [B, H, K, V] float32 contiguous. Hk divides H; head h reads query and key head h / (H / Hk).
  * K, V <= 128. g may be any value up to 0 and -inf (the state is forgotten); the other inputs are finite:
- * a value that is not may reach every step of its 64-step chunk.
+ * a value that is not may reach every step of its 64-step chunk and, with the state, the chunks after it.
+ * The backward's workspace holds one float32 state per 64-step chunk.
  * `strides` is host memory, in elements: batch row, step and head of q, k, v, g (and grad_o: 15 in all);
  * the last dimension of q, k, v and grad_o is dense, their steps (of L > 1) are at most 2^23 elements apart. No alignment is needed.
  * state and grad_last may be NULL (zero); grad_state is required iff state is given. L = 0 copies the state.
