@@ -412,6 +412,33 @@ int tsfast_hip_residual_norm_bwd(int64_t rows, int64_t width, int dtype, int res
                                  float* grad_scale, float* grad_weight, void* workspace, int64_t workspace_bytes,
                                  void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Gated feed-forward block:  a = x Wg^T + bg,  b = x Wu^T + bu,  y = act(a) * b  and its gradients.
+ * Layout: x [rows, D], w_gate and w_up [F, D], grad_y [rows, F] read through row strides in elements (D or F .. 2^22);
+ * b_gate, b_up [F] or NULL; y, grad_x and the weights' and biases' gradients contiguous; float32 or bfloat16, all alike. No
+ * alignment is needed; bfloat16 rows of a multiple of 8 elements, 16-byte aligned, are read in place, others are packed into
+ * the workspace first (which is why its size depends on the addresses and strides). activation: 0 silu, 1 gelu (erf), 2 sigmoid.
+ * `kept` (feed_kept_bytes; contents are the library's) takes a training forward's projections for the backward of the same
+ * inputs; NULL: inference. grad_x may be NULL (not wanted), grad_w_gate and grad_w_up both, grad_b_gate and grad_b_up each.
+ * Sums are float32 in a fixed order. float32 values must be finite. D, F up to 2^20. No counterpart in the reference.
+ */
+int64_t tsfast_hip_feed_kept_bytes(int64_t rows, int64_t D, int64_t F, int dtype);
+int64_t tsfast_hip_feed_fwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride,
+                                            const void* w_gate, int64_t w_gate_stride, const void* w_up,
+                                            int64_t w_up_stride, int train);
+int64_t tsfast_hip_feed_bwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride,
+                                            const void* w_gate, int64_t w_gate_stride, const void* w_up,
+                                            int64_t w_up_stride);
+int tsfast_hip_feed_fwd(int64_t rows, int64_t D, int64_t F, int dtype, int activation, const void* x, int64_t x_stride,
+                        const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
+                        const void* b_gate, const void* b_up, void* y, void* kept, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int tsfast_hip_feed_bwd(int64_t rows, int64_t D, int64_t F, int dtype, int activation, const void* x, int64_t x_stride,
+                        const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
+                        const void* grad_y, int64_t grad_y_stride, const void* kept, void* grad_x, void* grad_w_gate,
+                        void* grad_w_up, void* grad_b_gate, void* grad_b_up, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

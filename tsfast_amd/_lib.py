@@ -8,6 +8,7 @@ naming the path and the loader's reason.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -98,6 +99,11 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
         [_i64] * 2 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] * 3 + [_ptr, _i64] * 2 + [_ptr] * 6 + [_i64, _ptr],
         _int,
     ),
+    "tsfast_hip_feed_kept_bytes": ([_i64] * 3 + [_int], _i64),
+    "tsfast_hip_feed_fwd_workspace_bytes": ([_i64] * 3 + [_int] + [_ptr, _i64] * 3 + [_int], _i64),
+    "tsfast_hip_feed_bwd_workspace_bytes": ([_i64] * 3 + [_int] + [_ptr, _i64] * 3, _i64),
+    "tsfast_hip_feed_fwd": ([_i64] * 3 + [_int, _int] + [_ptr, _i64] * 3 + [_ptr] * 5 + [_i64, _ptr], _int),
+    "tsfast_hip_feed_bwd": ([_i64] * 3 + [_int, _int] + [_ptr, _i64] * 4 + [_ptr] * 7 + [_i64, _ptr], _int),
     "tsfast_hip_mat_adjoint_workspace_bytes": ([_i64] * 4, _i64),
     "tsfast_hip_mat_adjoint_bounds": ([_i64] * 4 + [_ptr] * 4 + [_i64, _ptr], _int),
 }
@@ -230,6 +236,14 @@ def stream_of(t: torch.Tensor) -> int:
     """The current HIP stream of the tensor's device, as an integer handle (torch's raw-stream
     query: a fraction of the cost of building a ``torch.cuda.Stream`` object on every call)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_same_device = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """A context in which the tensor's device is the current one, as launches on its streams need."""
+    return _same_device if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def require(t: torch.Tensor | None, name: str, dtypes: tuple, device: torch.device) -> None:

@@ -1,0 +1,1020 @@
+// Gated feed-forward block (gfx950): two projections, an activation and their product, with its gradients.
+//
+//   a = x Wg^T + bg,  b = x Wu^T + bu,  y = act(a) b          act: silu, gelu (erf) or sigmoid
+//   da = dy b act'(a),  db = dy act(a)
+//   dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x,  dbg = sum da,  dbu = sum db
+//
+// One kernel, product_kernel, forms the three matrix products: C[q][p] = sum_k Q[q][k] P[p][k], bf16 operands, fp32 sums.
+#include <math.h>
+
+#include "common.h"
+#include "tsfast_hip.h"
+
+using namespace tsf;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kK = 32;               // of a stage: the contraction of one matrix instruction
+constexpr int kStages = 4;           // stages in LDS: one is read, three are on their way
+constexpr int kMaxSegs = 12;         // products whose sum is formed: 2 sources x 6 pairs of planes
+constexpr int64_t kMaxLd = 1 << 22;  // elements between the rows of an operand: 256 rows stay below 2^31 bytes
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), may_alias));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2), may_alias));
+
+enum Act { kSilu = 0, kGelu = 1, kSigmoid = 2 };
+enum Form { kForward = 0, kInput = 1, kWeight = 2 };  // y; dx; dWg and dWu
+
+TSF_DEV uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+TSF_DEV float low(uint32_t p) { return __uint_as_float(p << 16); }
+TSF_DEV float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// ------------------------------------------------------------------------------------ activations
+// The upper tail of the normal distribution, erfc(s) / 2 with s = |a| / sqrt 2, as exp(-s^2) t P(t), t = 1 / (1 + s / 2): P is fitted to the
+// least relative error over s <= 12 (4e-8; beyond, the exp is zero in fp32), so gelu keeps its relative accuracy where it is small.
+template <int ACT>
+TSF_DEV void activate(float a, float& f, float& df) {
+  if constexpr (ACT == kGelu) {
+    const float s = fabsf(a) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.5f, s, 1.0f));
+    const float e = fast_exp2(-s * s * kLog2e);
+    const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.029682316f, 0.14300884f), -0.24509346f), 0.14074159f), -0.014488542f), 0.101840235f), 0.12142658f), 0.14120482f), 0.14104223f);
+    const float tail = t * poly * e;
+    const float phi = a < 0.0f ? tail : 1.0f - tail;
+    f = a * phi;
+    df = fmaf(a * 0.39894228040143268f, e, phi);
+  } else {
+    const float sig = sigmoid_fast(a);
+    f = ACT == kSilu ? a * sig : sig;
+    df = ACT == kSilu ? fmaf(a * sig, 1.0f - sig, sig) : sig * (1.0f - sig);
+  }
+}
+TSF_DEV float activate(int act, float a) {
+  float f, df;
+  if (act == kSilu)
+    activate<kSilu>(a, f, df);
+  else if (act == kGelu)
+    activate<kGelu>(a, f, df);
+  else
+    activate<kSigmoid>(a, f, df);
+  return f;
+}
+
+// ------------------------------------------------------------------------------------- operands
+// A matrix operand as planes of bf16 whose sum it is: one for bf16 values, three for fp32 ones (8 bits of the mantissa each). Rows
+// are 16-byte aligned and their length is a multiple of 8, zeros where the matrix ends before.
+struct PackJob {
+  const void* src;
+  bf16* dst;
+  int64_t ld, rows, items;  // items: of 8 columns
+  int cols, cols8;
+};
+struct PackArgs {
+  PackJob job[3];
+};
+
+TSF_DEV void split3(float x, float* part) {
+  // the first part of a finite value is finite
+  float h = (float)(__bf16)x;
+  if (!(fabsf(h) <= 3.0e38f) && fabsf(x) <= 3.4028235e38f) h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  const bool fin = fabsf(x) <= 3.4028235e38f;
+  const float r = fin ? x - h : 0.0f;
+  const float m = (float)(__bf16)r;
+  part[0] = h, part[1] = m, part[2] = r - m;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack_kernel(PackArgs a) {
+  const PackJob& j = a.job[blockIdx.y];
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= j.items) return;
+  const int per = j.cols8 / 8;
+  const int64_t row = i / per;
+  const int c = (int)(i % per) * 8;
+  const T* src = (const T*)j.src + row * j.ld + c;
+  T v[8];
+  if (c + 8 <= j.cols) {
+    __builtin_memcpy(v, src, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < j.cols ? src[e] : from_f32<T>(0.0f);
+  }
+  bf16* dst = j.dst + row * j.cols8 + c;
+  if constexpr (sizeof(T) == 2) {
+    __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, 16);
+  } else {
+    const int64_t plane = j.rows * j.cols8;
+    u32x4 w[3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float p0[3], p1[3];
+      split3(v[2 * k], p0);
+      split3(v[2 * k + 1], p1);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) w[n][k] = pack2(p0[n], p1[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) *(u32x4*)(dst + n * plane) = w[n];
+  }
+}
+
+// --------------------------------------------------------------------------------- the products
+// C[q][p] = sum over segments and k of Q[q][k] P[p][k]. An operand is read as it lies: rows over k, or (a "turned" panel) rows of k over
+// its q or p. P comes in two halves of a tile: gate and up rows (forward), or its columns' halves.
+struct ProductArgs {
+  const bf16 *q[kMaxSegs], *p0[kMaxSegs], *p1[kMaxSegs];
+  int64_t ldq, ldp, kq, kp;  // kq, kp: rows of k that each operand has in a segment, as many stages
+  int64_t nq, np;           // extent of C (forward: np of each half)
+  int64_t tiles_q, tiles_p, stages, split_stages;
+  int segs, act, train;
+  const void *bg, *bu;      // forward
+  void *y, *y1;             // y, dx; dWg and dWu
+  float* part;              // dW: sums of each split [split][nq][np], or null
+  char *save_hi, *save_lo;  // forward of a training step: a and b, see save_pre
+  int64_t save_fb;          // blocks of 16 columns
+  int64_t half_rows, valid_rows;  // dW: rows of q a half has, and those of them that exist
+};
+
+template <int BQ_, int BP_, int WQ_, int WP_>
+struct Tile {
+  static constexpr int BQ = BQ_, BP = BP_, HP = BP_ / 2, WQ = WQ_, WP = WP_, kWaves = WQ * WP, TH = 64 * kWaves;
+  static constexpr int NQ = BQ / WQ / 16, NH = HP / WP / 16;  // 16-row blocks a wave has of q, and of each half of p
+  static constexpr int kQBytes = BQ * kK * 2, kHBytes = HP * kK * 2, kStage = kQBytes + 2 * kHBytes;
+  static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave a stage
+  static constexpr int kRow = HP * 4 + 16;               // bytes of a row of outputs in LDS, at most
+  static constexpr int kLds = kStages * kStage > BQ * kRow ? kStages * kStage : BQ * kRow;
+  static_assert(kStage % (1024 * kWaves) == 0 && kQBytes % 1024 == 0 && kHBytes % 1024 == 0, "");
+};
+
+// One 1 KB piece of a panel of ROWS rows (of q or p) x 32 k, by one wave straight into LDS. As it lies: 16 rows of 64 bytes, the four
+// 16-byte chunks of a row turned so that 8 and 16 consecutive rows' same chunk fall on different banks. Turned: rows of k.
+template <int ROWS, bool TURNED>
+struct Panel {
+  static constexpr int kChunks = ROWS / 8;  // of a row of k
+  static constexpr uint32_t kNone = 0x80000000u;
+  TSF_DEV static uint32_t swz(uint32_t r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+  TSF_DEV static uint32_t turn(uint32_t kr) { return (((kr & 3) << 1) | (((kr >> 3) & 1) << 3)) & (kChunks - 1); }
+
+  uint32_t off, need;  // the lane's byte offset in a stage, and which of the stage's k it starts at
+  // `unit`: which 1 KB; rows: of the panel that exist
+  TSF_DEV void set(uint32_t unit, uint32_t lane, int64_t ld, uint32_t rows) {
+    if constexpr (!TURNED) {
+      const uint32_t r = 16 * unit + (lane >> 2), c = (lane & 3) ^ swz(r & 15);
+      off = (uint32_t)(r * ld * 2) + c * 16;
+      need = r < rows ? c * 8 : ~0u;
+    } else {
+      constexpr uint32_t per = 64 / kChunks;  // rows of k in 1 KB
+      const uint32_t kr = per * unit + lane / kChunks, c = (lane % kChunks) ^ turn(kr);
+      off = (uint32_t)(kr * ld * 2) + c * 16;
+      need = c * 8 < rows ? kr : ~0u;
+    }
+  }
+  // at: the panel's first row (as it lies: at k = 0, so: bytes from there to the stage's k; turned: the stage's first row of k);
+  // left: of the stage's k that exist. A lane whose values do not exist reads beyond the resource's end: zeros.
+  TSF_DEV void load(const bf16* at, uint32_t bytes, uint32_t so, uint32_t left, char* lds) const {
+    const uint32_t v = need < left ? off : kNone;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(at, bytes), (__attribute__((address_space(3))) void*)lds, 16, v, so, 0, 0);
+  }
+  // the bytes from `at` that the lanes which read may reach
+  TSF_DEV static uint32_t reach(uint32_t rows, uint32_t k, int64_t ld) {
+    return TURNED ? (uint32_t)((kK - 1) * ld + ROWS) * 2 : rows == 0 ? 0 : (uint32_t)((rows - 1) * ld + k) * 2;
+  }
+};
+
+// The wave's operand blocks of a panel: 16 rows, 8 of the 32 k a lane.
+template <int ROWS, bool TURNED>
+struct Reader {
+  using P = Panel<ROWS, TURNED>;
+  uint32_t lane_off;
+  uint32_t t, b;  // turned: what the chunk is turned by, and the rest of the lane's offset
+  TSF_DEV void set(uint32_t li, uint32_t lg) {
+    if constexpr (!TURNED) {
+      lane_off = li * 64 + ((lg ^ P::swz(li)) << 4);
+    } else {
+      const uint32_t r = 8 * lg + (li >> 2);
+      t = P::turn(r);
+      b = r * (ROWS * 2) + 8 * (li & 1);
+      lane_off = (li >> 1) & 1;
+    }
+  }
+  TSF_DEV bf16x8 get(const char* panel, uint32_t block) const {
+    bf16x8 v;
+    if constexpr (!TURNED) {
+      const u32x4 w = *(const u32x4*)(panel + block * 1024 + lane_off);
+      __builtin_memcpy(&v, &w, 16);
+    } else {
+      // the transposing read: lane li of a group of 16 points at 4 columns of row li / 4 and receives its own column of the 4
+      // rows. Rows 4 further on are turned alike.
+      const char* p = panel + b + (((2 * block + lane_off) ^ t) << 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const auto w = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
+                                                     __attribute__((address_space(3))) char*)const_cast<char*>(p + h * 4 * ROWS * 2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * h + e] = w[e];
+      }
+    }
+    return v;
+  }
+};
+
+// Waits for all but the last `n` loads into LDS and for this wave's own reads of it, then for the other waves.
+template <int N>
+TSF_DEV void stage_barrier() {
+  __builtin_amdgcn_sched_barrier(0);  // the products before it are issued before it
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <typename T>
+TSF_DEV void put4(char* p, f32x4 v) {
+  if constexpr (sizeof(T) == 2) {
+    *(u32x2*)p = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+  } else {
+    *(u32x4*)p = __builtin_bit_cast(u32x4, v);
+  }
+}
+
+// A half tile of outputs, from accumulators to LDS and from there to memory in whole rows. `row(q)`: the address of row q of the tile, or
+// null; n: columns that exist.
+template <typename C, typename T, typename V, typename R>
+TSF_DEV void store_half(char* lds, uint32_t wq, uint32_t wp, uint32_t li, uint32_t lg, int n, V value, R row) {
+  constexpr int kRow = C::HP * (int)sizeof(T) + 16;
+  static_assert(C::BQ * kRow <= C::kLds, "");
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < C::NQ; ++j)
+#pragma unroll
+    for (int i = 0; i < C::NH; ++i)
+      put4<T>(lds + ((wq * C::NQ + j) * 16 + li) * kRow + ((wp * C::NH + i) * 16 + 4 * lg) * sizeof(T), value(i, j));
+  __syncthreads();
+  constexpr int kPer = 16 / (int)sizeof(T), kRowPieces = C::HP / kPer;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < C::BQ * kRowPieces; e += C::TH) {
+    const int q = e / kRowPieces, c = (e % kRowPieces) * kPer;
+    T* to = row(q);
+    if (!to || c >= n) continue;
+    const char* from = lds + q * kRow + c * sizeof(T);
+    if (c + kPer <= n && ((uintptr_t)(to + c) & 15) == 0) {
+      *(u32x4*)(to + c) = *(const u32x4*)from;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (c + k < n) to[c + k] = ((const T*)from)[k];
+    }
+  }
+}
+
+// What a training step's forward leaves for its backward: a and b in blocks of 16 rows x 16 columns as accumulators have them (four columns
+// a lane). fp32 as it is, 32 bytes a lane; for bf16 24 bits of each, in 16 bytes (the upper 16 bits of a's and b's) and 8 (the next 8):
+// rounded to bf16 they would cost the gradients as much again as the rounding of da and db.
+TSF_DEV uint32_t round24(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x7fffffffu) < 0x7f800000u ? u + 0x7fu + ((u >> 8) & 1) : u;  // to nearest even; infinities and NaN as they are
+}
+template <typename T>
+TSF_DEV void save_pre(char* hi, char* lo, int64_t block, uint32_t lane, f32x4 a, f32x4 b) {
+  if constexpr (sizeof(T) == 4) {
+    char* p = hi + (block * 64 + lane) * 32;
+    *(u32x4*)p = __builtin_bit_cast(u32x4, a);
+    *(u32x4*)(p + 16) = __builtin_bit_cast(u32x4, b);
+  } else {
+    uint32_t r[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = round24(a[e]), r[4 + e] = round24(b[e]);
+    u32x4 h;
+    u32x2 l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x07060302);  // the upper halves
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t x = __builtin_amdgcn_perm(r[4 * k + 1], r[4 * k], 0x0c0c0501), y = __builtin_amdgcn_perm(r[4 * k + 3], r[4 * k + 2], 0x0c0c0501);
+      l[k] = x | y << 16;
+    }
+    *(u32x4*)(hi + (block * 64 + lane) * 16) = h;
+    *(u32x2*)(lo + (block * 64 + lane) * 8) = l;
+  }
+}
+template <typename T>
+TSF_DEV void load_pre(const char* hi, const char* lo, int64_t block, uint32_t lane, f32x4& a, f32x4& b) {
+  if constexpr (sizeof(T) == 4) {
+    const char* p = hi + (block * 64 + lane) * 32;
+    a = __builtin_bit_cast(f32x4, *(const u32x4*)p);
+    b = __builtin_bit_cast(f32x4, *(const u32x4*)(p + 16));
+  } else {
+    const u32x4 h = *(const u32x4*)(hi + (block * 64 + lane) * 16);
+    const u32x2 l = *(const u32x2*)(lo + (block * 64 + lane) * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t top = e & 1 ? h[e / 2] & 0xffff0000u : h[e / 2] << 16;
+      const float v = __uint_as_float(top | ((l[e / 4] >> (8 * (e & 3))) & 0xffu) << 8);
+      if (e < 4)
+        a[e] = v;
+      else
+        b[e - 4] = v;
+    }
+  }
+}
+
+template <typename T, typename C, int FORM>
+__global__ void __launch_bounds__(C::TH, C::kWaves == 8 ? 2 : 2) product_kernel(ProductArgs g) {
+  constexpr bool TQ = FORM == kWeight, TP = FORM != kForward;  // turned operands
+  constexpr int NQ = C::NQ, NH = C::NH;
+  __shared__ __attribute__((aligned(1024))) char lds[C::kLds];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave / C::WP, wp = wave % C::WP;
+
+  // Workgroups go to the 8 XCDs in turn: each takes a contiguous range of tiles, in groups of 8 tiles of q that share what they read of p.
+  const uint32_t total = gridDim.x;
+  uint32_t lin = blockIdx.x;
+  {
+    const uint32_t full = total / 8, rest = total % 8, x = lin % 8, at = lin / 8;
+    lin = x * full + (x < rest ? x : rest) + at;
+  }
+  const uint32_t tiles = (uint32_t)(g.tiles_q * g.tiles_p), split = lin / tiles;
+  lin %= tiles;
+  const uint32_t gq = 8, group = lin / (gq * (uint32_t)g.tiles_p), first = group * gq;
+  const uint32_t in_group = (uint32_t)g.tiles_q - first < gq ? (uint32_t)g.tiles_q - first : gq;
+  const uint32_t within = lin - group * gq * (uint32_t)g.tiles_p;
+  const int64_t q0 = (int64_t)(first + within % in_group) * C::BQ;
+  const int64_t pt = within / in_group;
+  const int64_t p0 = pt * (FORM == kForward ? C::HP : C::BP);                 // of the first half
+  const int64_t p1 = FORM == kForward ? p0 : p0 + C::HP;                      // of the second
+  const uint32_t rows_q = (uint32_t)(g.nq - q0 < C::BQ ? g.nq - q0 : C::BQ);
+  const uint32_t rows_0 = (uint32_t)(g.np - p0 < C::HP ? g.np - p0 : C::HP);
+  const uint32_t rows_1 = (uint32_t)(g.np - p1 < C::HP ? (g.np > p1 ? g.np - p1 : 0) : C::HP);
+
+  // loads: this wave's pieces of a stage, q's first, then those of p's halves
+  constexpr int kQ = C::kQBytes / 1024, kH = C::kHBytes / 1024, kQw = kQ / C::kWaves, kPw = 2 * kH / C::kWaves;
+  static_assert(kQw * C::kWaves == kQ && kPw * C::kWaves == 2 * kH, "");
+  Panel<C::BQ, TQ> lq[kQw];
+  Panel<C::HP, TP> lp[kPw];
+  // a piece of p lies in one of its halves
+  const bool second[2] = {wave >= kH, wave + C::kWaves >= kH};
+  static_assert(kPw <= 2, "");
+#pragma unroll
+  for (int i = 0; i < kQw; ++i) lq[i].set(wave + i * C::kWaves, lane, g.ldq, rows_q);
+#pragma unroll
+  for (int i = 0; i < kPw; ++i) lp[i].set((wave + i * C::kWaves) % kH, lane, g.ldp, second[i] ? rows_1 : rows_0);
+  const int kq = (int)g.kq, kp = (int)g.kp, per_seg = (kq + kK - 1) / kK;
+  const int begin = (int)(split * g.split_stages);
+  const int count = (int)(g.stages - begin < g.split_stages ? g.stages - begin : g.split_stages);
+  const int rounds = (count + 1) / 2;  // two stages a round: one past the end adds zeros
+  int to_load = count, seg = begin / per_seg, k0 = (begin % per_seg) * kK;
+  const bf16 *qb, *pb[2];
+  auto enter = [&]() __attribute__((always_inline)) {
+    qb = g.q[seg] + (TQ ? q0 + k0 * g.ldq : q0 * g.ldq);
+#pragma unroll
+    for (int i = 0; i < kPw; ++i) {
+      const int64_t at = second[i] ? p1 : p0;
+      pb[i] = (second[i] ? g.p1 : g.p0)[seg] + (TP ? at + k0 * g.ldp : at * g.ldp);
+    }
+  };
+  enter();
+  const uint32_t reach_q = Panel<C::BQ, TQ>::reach(rows_q, kq, g.ldq);
+  const uint32_t reach_0 = Panel<C::HP, TP>::reach(rows_0, kp, g.ldp), reach_1 = Panel<C::HP, TP>::reach(rows_1, kp, g.ldp);
+  auto load_stage = [&](int buf) __attribute__((always_inline)) {
+    char* to = lds + buf * C::kStage;
+    const int lq_ = to_load > 0 ? kq - k0 : 0, lp_ = to_load > 0 ? kp - k0 : 0;
+    const uint32_t left_q = lq_ > 0 ? lq_ : 0, left_p = lp_ > 0 ? lp_ : 0;
+#pragma unroll
+    for (int i = 0; i < kQw; ++i) lq[i].load(qb, reach_q, TQ ? 0 : k0 * 2, left_q, to + (wave + i * C::kWaves) * 1024);
+#pragma unroll
+    for (int i = 0; i < kPw; ++i)
+      lp[i].load(pb[i], second[i] ? reach_1 : reach_0, TP ? 0 : k0 * 2, left_p, to + C::kQBytes + (wave + i * C::kWaves) * 1024);
+    --to_load;
+    k0 += kK;
+    if (k0 >= kq && to_load > 0) {
+      k0 = 0, ++seg;
+      enter();
+    } else {
+      if (TQ) qb += kK * g.ldq;
+#pragma unroll
+      for (int i = 0; i < kPw; ++i)
+        if (TP) pb[i] += kK * g.ldp;
+    }
+  };
+
+  Reader<C::BQ, TQ> rq;
+  Reader<C::HP, TP> rp;
+  rq.set(li, lg);
+  rp.set(li, lg);
+  struct Blocks {
+    bf16x8 q[NQ], p[2 * NH];
+  };
+  auto read_stage = [&](Blocks& f, int buf) __attribute__((always_inline)) {
+    const char* from = lds + buf * C::kStage;
+#pragma unroll
+    for (int i = 0; i < 2 * NH; ++i) f.p[i] = rp.get(from + C::kQBytes + (i / NH) * C::kHBytes, wp * NH + i % NH);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) f.q[j] = rq.get(from, wq * NQ + j);
+  };
+  f32x4 acc[2 * NH][NQ];
+#pragma unroll
+  for (int i = 0; i < 2 * NH; ++i)
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const Blocks& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int i = 0; i < 2 * NH; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], f.q[j], acc[i][j], 0, 0, 0);
+  };
+
+  // Stage t's blocks are in registers when its turn comes. Its products run while stage t + 1's blocks are read from LDS and
+  // stage t + 4 is loaded into the place that stage t has left; t + 2 and t + 3 are on their way.
+  Blocks f0, f1;
+  load_stage(0);
+  load_stage(1);
+  load_stage(2);
+  load_stage(3);
+  stage_barrier<3 * C::kLoads>();
+  read_stage(f0, 0);
+  int buf = 0;
+  for (int r = 0; r < rounds; ++r) {
+    stage_barrier<2 * C::kLoads>();
+    load_stage(buf);
+    read_stage(f1, buf + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f0);
+    stage_barrier<2 * C::kLoads>();
+    load_stage(buf + 1);
+    read_stage(f0, (buf + 2) & 3);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f1);
+    buf = (buf + 2) & 3;
+  }
+  stage_barrier<0>();
+
+  if constexpr (FORM == kForward) {
+    const T *bg = (const T*)g.bg, *bu = (const T*)g.bu;
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      const int64_t f = p0 + (wp * NH + i) * 16 + 4 * lg;
+      f32x4 va = {0.0f, 0.0f, 0.0f, 0.0f}, vb = va;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (bg && f + e < g.np) va[e] = to_f32(bg[f + e]);
+        if (bu && f + e < g.np) vb[e] = to_f32(bu[f + e]);
+      }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        f32x4& a = acc[i][j];
+        f32x4& b = acc[NH + i][j];
+        a += va;
+        b += vb;
+        if (g.train) {
+          const int64_t mb = q0 / 16 + wq * NQ + j, fb = p0 / 16 + wp * NH + i;
+          if (mb * 16 < g.nq && fb < g.save_fb) save_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = activate(g.act, a[e]) * b[e];
+      }
+    }
+    T* y = (T*)g.y;
+    store_half<C, T>(lds, wq, wp, li, lg, (int)rows_0, [&](int i, int j) { return acc[i][j]; },
+                     [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + p0 : (T*)nullptr; });
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t c0 = h ? p1 : p0;
+      const int n = (int)(h ? rows_1 : rows_0);
+      auto value = [&](int i, int j) { return acc[h * NH + i][j]; };
+      if (FORM == kInput) {
+        T* y = (T*)g.y;
+        store_half<C, T>(lds, wq, wp, li, lg, n, value, [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + c0 : (T*)nullptr; });
+      } else if (g.part) {
+        float* y = g.part + (int64_t)split * g.nq * g.np;
+        store_half<C, float>(lds, wq, wp, li, lg, n, value,
+                             [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + c0 : (float*)nullptr; });
+      } else {
+        store_half<C, T>(lds, wq, wp, li, lg, n, value, [&](int q) {
+          const int64_t r = q0 + q, in = r < g.half_rows ? r : r - g.half_rows;
+          T* y = (T*)(r < g.half_rows ? g.y : g.y1);
+          return (uint32_t)q < rows_q && in < g.valid_rows ? y + in * g.np + c0 : (T*)nullptr;
+        });
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ da and db of dy
+// A workgroup has 64 columns and a run of rows; each wave takes every fourth block of 16 rows. da and db go out as the operand planes of
+// both products behind, [plane][rows][2 F8], and their column sums as one partial a workgroup.
+struct AdjointArgs {
+  const void* dy;
+  int64_t ld_dy, rows, F, F8, save_fb, blocks;  // blocks: of 16 rows a workgroup has
+  const char *save_hi, *save_lo;
+  bf16* d;
+  float* part;  // [workgroups along rows][2][F], or null
+};
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
+  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
+  const int64_t f0 = (int64_t)blockIdx.x * 64, first = (int64_t)blockIdx.y * g.blocks;
+  const int64_t all = (g.rows + 15) / 16, last = first + g.blocks < all ? first + g.blocks : all;
+  const int64_t plane = g.rows * 2 * g.F8;
+  f32x4 sa[4], sb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sa[i] = sb[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t mb = first + wave; mb < last; mb += 4) {
+    const int64_t m = mb * 16 + li;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t fb = f0 / 16 + i, f = f0 + 16 * i + 4 * lg;
+      if (fb >= g.save_fb) continue;
+      f32x4 a, b, da, db;
+      load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
+      float dy[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (m < g.rows) {
+        const T* p = (const T*)g.dy + m * g.ld_dy + f;
+        if (f + 4 <= g.F) {
+          T v[4];
+          __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dy[e] = to_f32(v[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (f + e < g.F) dy[e] = to_f32(p[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v, dv;
+        activate<ACT>(a[e], v, dv);
+        const bool in = m < g.rows && f + e < g.F;
+        da[e] = in ? dy[e] * b[e] * dv : 0.0f;
+        db[e] = in ? dy[e] * v : 0.0f;
+      }
+      sa[i] += da;
+      sb[i] += db;
+      if (m < g.rows && f < g.F8) {
+        bf16* to = g.d + m * 2 * g.F8 + f;
+        if constexpr (kPlanes == 1) {
+          *(u32x2*)to = u32x2{pack2(da[0], da[1]), pack2(da[2], da[3])};
+          *(u32x2*)(to + g.F8) = u32x2{pack2(db[0], db[1]), pack2(db[2], db[3])};
+        } else {
+          float pa[4][3], pb[4][3];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) split3(da[e], pa[e]), split3(db[e], pb[e]);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) {
+            *(u32x2*)(to + n * plane) = u32x2{pack2(pa[0][n], pa[1][n]), pack2(pa[2][n], pa[3][n])};
+            *(u32x2*)(to + n * plane + g.F8) = u32x2{pack2(pb[0][n], pb[1][n]), pack2(pb[2][n], pb[3][n])};
+          }
+        }
+      }
+    }
+  }
+  if (!g.part) return;
+  __shared__ float sums[4][2][64];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = sa[i][e], y = sb[i][e];
+#pragma unroll
+      for (int mask = 1; mask < 16; mask <<= 1) x += __shfl_xor(x, mask, kWave), y += __shfl_xor(y, mask, kWave);
+      if (li == 0) sums[wave][0][16 * i + 4 * lg + e] = x, sums[wave][1][16 * i + 4 * lg + e] = y;
+    }
+  __syncthreads();
+  if (tid < 128) {
+    const int h = tid >> 6, c = tid & 63;
+    if (f0 + c < g.F) g.part[((int64_t)blockIdx.y * 2 + h) * g.F + f0 + c] = (sums[0][h][c] + sums[1][h][c]) + (sums[2][h][c] + sums[3][h][c]);
+  }
+}
+
+// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in order
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int64_t parts, int64_t stride, int64_t n, T* out0, T* out1) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= 2 * n) return;
+  const int64_t h = i >= n, c = i - h * n;
+  T* out = h ? out1 : out0;
+  if (!out) return;
+  const float* p = part + h * stride + c;
+  float s = 0.0f;
+  for (int64_t k = 0; k < parts; ++k) s += p[k * 2 * stride];
+  out[c] = from_f32<T>(s);
+}
+
+// --------------------------------------------------------------------------------- a few rows
+// Up to 16 NT rows: the weights are read once and nothing else matters. A workgroup has 16 columns of y; its four waves share the
+// contraction, 32 k in turn, both operands straight from memory at any alignment.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<bf16> {
+  bf16x8 v;
+};
+template <>
+struct Frag<float> {
+  f32x4 lo, hi;
+};
+TSF_DEV f32x4 mma(const Frag<bf16>& a, const Frag<bf16>& b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0); }
+TSF_DEV f32x4 mma(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[e], b.lo[e], c, 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[e], b.hi[e], c, 0, 0, 0);
+  return c;
+}
+// 8 values of a row, the first n of them, zeros after; `in`: the row exists
+template <typename T>
+TSF_DEV Frag<T> load8(const T* p, int64_t n, bool in) {
+  T v[8];
+  if (in && n >= 8) {
+    __builtin_memcpy(v, p, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = in && e < n ? p[e] : from_f32<T>(0.0f);
+  }
+  Frag<T> f;
+  __builtin_memcpy(&f, v, sizeof(v));
+  return f;
+}
+
+struct FewArgs {
+  const void *x, *wg, *wu, *bg, *bu;
+  void* y;
+  int64_t rows, D, F, ldx, ldg, ldu;
+  int act;
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads) few_kernel(FewArgs g) {
+  __shared__ f32x4 sums[4][2 * NT][64];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
+  const int64_t f0 = (int64_t)blockIdx.x * 16;
+  const bool fin = f0 + li < g.F;
+  const T *wg = (const T*)g.wg + (f0 + li) * g.ldg, *wu = (const T*)g.wu + (f0 + li) * g.ldu;
+  const T* x = (const T*)g.x + li * g.ldx;
+  f32x4 acc[2][NT];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[h][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int64_t k = 32 * wave + 8 * lg; k - 8 * lg < g.D; k += 128) {
+    const Frag<T> a = load8(wg + k, g.D - k, fin), b = load8(wu + k, g.D - k, fin);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Frag<T> v = load8(x + 16 * t * g.ldx + k, g.D - k, 16 * t + li < g.rows);
+      acc[0][t] = mma(a, v, acc[0][t]);
+      acc[1][t] = mma(b, v, acc[1][t]);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sums[wave][h * NT + t][lane] = acc[h][t];
+  __syncthreads();
+  // a thread has column tid % 16 of row tid / 16 of each tile of rows: element (column 4 l + e, row li) of lane 16 l + li
+  const uint32_t c = tid & 15, r = tid >> 4;
+  const int64_t f = f0 + c;
+  if (f >= g.F) return;
+  const float ba = g.bg ? to_f32(((const T*)g.bg)[f]) : 0.0f, bb = g.bu ? to_f32(((const T*)g.bu)[f]) : 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t row = 16 * t + r;
+    if (row >= g.rows) continue;
+    float v[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = (c >> 2) * 16 + r, e = c & 3;
+      v[h] = (sums[0][h * NT + t][at][e] + sums[1][h * NT + t][at][e]) + (sums[2][h * NT + t][at][e] + sums[3][h * NT + t][at][e]);
+    }
+    ((T*)g.y)[row * g.F + f] = from_f32<T>(activate(g.act, v[0] + ba) * (v[1] + bb));
+  }
+}
+
+// ----------------------------------------------------------------------------------------- host
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t up8(int64_t a) { return up(a, 8) * 8; }
+int64_t up256(int64_t a) { return up(a, 256) * 256; }
+
+constexpr int64_t kFewRows = 32;
+
+using Large = Tile<256, 256, 4, 2>;
+using Medium = Tile<128, 128, 2, 2>;
+using Small = Tile<64, 64, 2, 2>;
+
+// How a product of nq x np outputs (np of each half where `dual`) and `stages` of k is cut.
+struct Plan {
+  int tile;  // 0: Large, 1: Medium, 2: Small
+  int64_t tiles_q, tiles_p, splits, split_stages;
+};
+Plan plan_for(int64_t nq, int64_t np, int64_t stages, bool dual, bool may_split) {
+  const int64_t cus = device_cus();
+  const struct {
+    int bq, bp, per_cu;
+    double cost;  // of a stage of one workgroup, when the CU is full of them
+  } tiles[3] = {{256, 256, 1, 1.0}, {128, 128, 2, 0.35}, {64, 64, 4, 0.16}};
+  Plan best = {};
+  double least = 0;
+  for (int t = 0; t < 3; ++t) {
+    const int64_t tq = up(nq, tiles[t].bq), tp = up(np, dual ? tiles[t].bp / 2 : tiles[t].bp);
+    for (int64_t s = 1; s <= (may_split ? 64 : 1); s *= 2) {
+      if (s > 1 && stages / s < 8) break;
+      const double rounds = (double)up(tq * tp * s, cus * tiles[t].per_cu);
+      double time = rounds * ((double)up(stages, s) + 12) * tiles[t].cost * tiles[t].per_cu;
+      if (s > 1) time += (double)(nq * np * s) / (double)(cus * 4096) + 8;
+      if (!best.splits || time < least) {
+        least = time;
+        best = Plan{t, tq, tp, s, up(stages, s)};
+      }
+    }
+  }
+  best.splits = up(stages, best.split_stages);
+  return best;
+}
+
+template <typename T, typename C, int FORM>
+void launch_product(ProductArgs& g, const Plan& p, hipStream_t st) {
+  product_kernel<T, C, FORM><<<(unsigned)(p.tiles_q * p.tiles_p * p.splits), C::TH, 0, st>>>(g);
+}
+template <typename T, int FORM>
+void product(ProductArgs& g, const Plan& p, hipStream_t st) {
+  g.tiles_q = p.tiles_q, g.tiles_p = p.tiles_p, g.split_stages = p.split_stages;
+  if (p.tile == 0)
+    launch_product<T, Large, FORM>(g, p, st);
+  else if (p.tile == 1)
+    launch_product<T, Medium, FORM>(g, p, st);
+  else
+    launch_product<T, Small, FORM>(g, p, st);
+}
+
+// An operand's planes: as the matrix lies where its rows are aligned bf16, or packed into the workspace
+struct Operand {
+  const bf16* p;
+  int64_t ld, plane;
+  int64_t bytes;  // of the workspace
+};
+bool lies_well(int dtype, const void* p, int64_t cols, int64_t ld) {
+  return dtype == TSF_DTYPE_BF16 && cols % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0;
+}
+Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t ld, bool as_it_lies) {
+  if (as_it_lies) return Operand{(const bf16*)p, ld, 0, 0};
+  const int64_t planes = dtype == TSF_DTYPE_BF16 ? 1 : 3, c8 = up8(cols);
+  return Operand{nullptr, c8, rows * c8, up256(planes * rows * c8 * 2)};
+}
+
+// pairs of planes whose products make up that of fp32 matrices to 2^-24, the least first
+constexpr int kPairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+
+int feed_status(int64_t rows, int64_t D, int64_t F, int dtype, int act) {
+  if (rows < 0 || D < 1 || F < 1 || act < 0 || act > 2) return TSF_ERR_ARG;
+  if (dtype != TSF_DTYPE_F32 && dtype != TSF_DTYPE_BF16) return TSF_ERR_ARG;
+  if (D > kMaxLd / 4 || F > kMaxLd / 4 || rows > ((int64_t)1 << 31) - 64) return TSF_ERR_UNSUPPORTED;
+  // tiles of a launch, with the smallest tile and the most splits
+  if (up(rows, 64) * up(F, 32) > (1 << 24) || up(rows, 64) * up(D, 64) > (1 << 24)) return TSF_ERR_UNSUPPORTED;
+  return TSF_OK;
+}
+bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > kMaxLd; }
+
+int64_t pre_bytes(int64_t rows, int64_t F, int dtype) { return up(rows, 16) * up(F, 16) * 64 * (dtype == TSF_DTYPE_BF16 ? 24 : 32); }
+char* pre_lo(char* pre, int64_t rows, int64_t F) { return pre + up(rows, 16) * up(F, 16) * 64 * 16; }
+
+struct Shape {
+  int64_t rows, D, F;
+  int dtype;
+  int64_t F8, stages_f, stages_x, stages_w;  // of the three products
+  int pairs;
+};
+Shape shape_of(int64_t rows, int64_t D, int64_t F, int dtype) {
+  Shape s = {rows, D, F, dtype, up8(F), 0, 0, 0, dtype == TSF_DTYPE_BF16 ? 1 : 6};
+  s.stages_f = s.pairs * up(D, kK);
+  s.stages_x = 2 * s.pairs * up(F, kK);
+  s.stages_w = s.pairs * up(rows, kK);
+  return s;
+}
+
+struct Call {
+  const void *x, *wg, *wu;
+  int64_t ldx, ldg, ldu;
+};
+// x and the weights as operands of the products; both weights' rows are equally far apart
+struct Operands {
+  Operand x, wg, wu;
+  int64_t bytes;
+};
+Operands operands_of(const Shape& s, const Call& c) {
+  const bool w = lies_well(s.dtype, c.wg, s.D, c.ldg) && lies_well(s.dtype, c.wu, s.D, c.ldu) && c.ldg == c.ldu;
+  Operands o;
+  o.x = operand(s.dtype, c.x, s.rows, s.D, c.ldx, lies_well(s.dtype, c.x, s.D, c.ldx));
+  o.wg = operand(s.dtype, c.wg, s.F, s.D, c.ldg, w);
+  o.wu = operand(s.dtype, c.wu, s.F, s.D, c.ldu, w);
+  o.bytes = o.x.bytes + o.wg.bytes + o.wu.bytes;
+  return o;
+}
+// packs what has to be, into ws
+template <typename T>
+void pack_operands(const Shape& s, const Call& c, Operands& o, char* ws, hipStream_t st) {
+  PackArgs a = {};
+  int jobs = 0;
+  int64_t most = 0;
+  auto add = [&](Operand& op, const void* src, int64_t rows, int64_t ld) {
+    if (op.p || rows == 0) return;
+    op.p = (const bf16*)ws;
+    const int64_t items = rows * (op.ld / 8);
+    a.job[jobs++] = PackJob{src, (bf16*)ws, ld, rows, items, (int)s.D, (int)op.ld};
+    most = items > most ? items : most;
+    ws += op.bytes;
+  };
+  add(o.x, c.x, s.rows, c.ldx);
+  add(o.wg, c.wg, s.F, c.ldg);
+  add(o.wu, c.wu, s.F, c.ldu);
+  if (jobs) pack_kernel<T><<<dim3((unsigned)up(most, kThreads), (unsigned)jobs), kThreads, 0, st>>>(a);
+}
+
+template <typename T>
+int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void* bu, void* y, char* pre, char* ws, int64_t ws_bytes, hipStream_t st) {
+  if (s.rows <= kFewRows && !pre) {
+    FewArgs a = {c.x, c.wg, c.wu, bg, bu, y, s.rows, s.D, s.F, c.ldx, c.ldg, c.ldu, act};
+    const unsigned grid = (unsigned)up(s.F, 16);
+    if (s.rows <= 16)
+      few_kernel<T, 1><<<grid, kThreads, 0, st>>>(a);
+    else
+      few_kernel<T, 2><<<grid, kThreads, 0, st>>>(a);
+    return tsf_launch_status();
+  }
+  Operands o = operands_of(s, c);
+  if (o.bytes && (!ws || ws_bytes < o.bytes)) return TSF_ERR_WORKSPACE;
+  pack_operands<T>(s, c, o, ws, st);
+  ProductArgs g = {};
+  for (int i = 0; i < s.pairs; ++i) {
+    const int* pr = kPairs[s.pairs == 1 ? 5 : i];
+    g.q[i] = o.x.p + pr[0] * o.x.plane;
+    g.p0[i] = o.wg.p + pr[1] * o.wg.plane;
+    g.p1[i] = o.wu.p + pr[1] * o.wu.plane;
+  }
+  g.ldq = o.x.ld, g.ldp = o.wg.ld, g.kq = g.kp = up8(s.D), g.nq = s.rows, g.np = s.F;
+  g.segs = s.pairs, g.stages = s.stages_f, g.act = act, g.train = pre != nullptr, g.bg = bg, g.bu = bu, g.y = y;
+  if (pre) g.save_hi = pre, g.save_lo = pre_lo(pre, s.rows, s.F), g.save_fb = up(s.F, 16);
+  product<T, kForward>(g, plan_for(s.rows, s.F, s.stages_f, true, false), st);
+  return tsf_launch_status();
+}
+
+// the parts of a backward's workspace behind the operands
+struct BwdSpace {
+  Plan px, pw;
+  int64_t wgs, blocks;  // of the adjoint's rows
+  int64_t d, bias, part;
+};
+BwdSpace bwd_space(const Shape& s) {
+  BwdSpace b;
+  b.px = plan_for(s.rows, s.D, s.stages_x, false, false);
+  b.pw = plan_for(2 * s.F8, s.D, s.stages_w, false, true);
+  const int64_t all = up(s.rows, 16), cols = up(s.F, 64);
+  // rows of a workgroup: four blocks a wave or more, and about 2048 workgroups
+  b.blocks = up(all * cols, 2048);
+  if (b.blocks < 16) b.blocks = 16;
+  b.wgs = up(all, b.blocks);
+  b.d = up256((s.dtype == TSF_DTYPE_BF16 ? 1 : 3) * s.rows * 2 * s.F8 * 2);
+  b.bias = up256(b.wgs * 2 * s.F * 4);
+  b.part = b.pw.splits > 1 ? up256(b.pw.splits * 2 * s.F8 * s.D * 4) : 0;
+  return b;
+}
+
+template <typename T>
+void launch_adjoint(const AdjointArgs& a, int act, dim3 grid, hipStream_t st) {
+  if (act == kSilu)
+    adjoint_kernel<T, kSilu><<<grid, kThreads, 0, st>>>(a);
+  else if (act == kGelu)
+    adjoint_kernel<T, kGelu><<<grid, kThreads, 0, st>>>(a);
+  else
+    adjoint_kernel<T, kSigmoid><<<grid, kThreads, 0, st>>>(a);
+}
+
+template <typename T>
+int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_dy, const char* pre, void* dx, void* dwg, void* dwu, void* dbg,
+             void* dbu, char* ws, int64_t ws_bytes, hipStream_t st) {
+  Operands o = operands_of(s, c);
+  const BwdSpace b = bwd_space(s);
+  if (!ws || ws_bytes < o.bytes + b.d + b.bias + b.part) return TSF_ERR_WORKSPACE;
+  pack_operands<T>(s, c, o, ws, st);
+  char* at = ws + o.bytes;
+  bf16* d = (bf16*)at;
+  float* bias = (float*)(at + b.d);
+  float* part = (float*)(at + b.d + b.bias);
+  const bool want_bias = dbg || dbu;
+
+  AdjointArgs a = {};
+  a.dy = dy, a.ld_dy = ld_dy, a.rows = s.rows, a.F = s.F, a.F8 = s.F8, a.save_fb = up(s.F, 16), a.blocks = b.blocks;
+  a.save_hi = pre, a.save_lo = pre_lo(const_cast<char*>(pre), s.rows, s.F), a.d = d, a.part = want_bias ? bias : nullptr;
+  launch_adjoint<T>(a, act, dim3((unsigned)up(s.F, 64), (unsigned)b.wgs), st);
+  if (want_bias) sum_kernel<T><<<(unsigned)up(2 * s.F, kThreads), kThreads, 0, st>>>(bias, b.wgs, s.F, s.F, (T*)dbg, (T*)dbu);
+
+  const int64_t plane = s.rows * 2 * s.F8;
+  if (dx) {
+    ProductArgs g = {};
+    for (int src = 0; src < 2; ++src)
+      for (int i = 0; i < s.pairs; ++i) {
+        const int* pr = kPairs[s.pairs == 1 ? 5 : i];
+        const Operand& w = src ? o.wu : o.wg;
+        const int n = src * s.pairs + i;
+        g.q[n] = d + pr[0] * plane + src * s.F8;
+        g.p0[n] = g.p1[n] = w.p + pr[1] * w.plane;
+      }
+    g.ldq = 2 * s.F8, g.ldp = o.wg.ld, g.kq = s.F8, g.kp = s.F, g.nq = s.rows, g.np = s.D;
+    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx;
+    product<T, kInput>(g, b.px, st);
+  }
+  if (dwg || dwu) {
+    ProductArgs g = {};
+    for (int i = 0; i < s.pairs; ++i) {
+      const int* pr = kPairs[s.pairs == 1 ? 5 : i];
+      g.q[i] = d + pr[0] * plane;
+      g.p0[i] = g.p1[i] = o.x.p + pr[1] * o.x.plane;
+    }
+    g.ldq = 2 * s.F8, g.ldp = o.x.ld, g.kq = g.kp = s.rows, g.nq = 2 * s.F8, g.np = s.D;
+    g.segs = s.pairs, g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
+    g.part = b.pw.splits > 1 ? part : nullptr;
+    product<T, kWeight>(g, b.pw, st);
+    if (g.part)
+      sum_kernel<T><<<(unsigned)up(2 * s.F * s.D, kThreads), kThreads, 0, st>>>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, (T*)dwg, (T*)dwu);
+  }
+  return tsf_launch_status();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) zero_kernel(T* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i < n) p[i] = from_f32<T>(0.0f);
+}
+template <typename T>
+void zero(void* p, int64_t n, hipStream_t st) {
+  if (p && n > 0) zero_kernel<T><<<(unsigned)up(n, kThreads), kThreads, 0, st>>>((T*)p, n);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tsfast_hip_feed_kept_bytes(int64_t rows, int64_t D, int64_t F, int dtype) {
+  if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;
+  return pre_bytes(rows, F, dtype);
+}
+
+int64_t tsfast_hip_feed_fwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride, const void* w_gate,
+                                            int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int train) {
+  if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;
+  if (rows <= kFewRows && !train) return 0;
+  return operands_of(shape_of(rows, D, F, dtype), Call{x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride}).bytes;
+}
+
+int64_t tsfast_hip_feed_bwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride, const void* w_gate,
+                                            int64_t w_gate_stride, const void* w_up, int64_t w_up_stride) {
+  if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;
+  const Shape s = shape_of(rows, D, F, dtype);
+  const BwdSpace b = bwd_space(s);
+  return operands_of(s, Call{x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride}).bytes + b.d + b.bias + b.part;
+}
+
+int tsfast_hip_feed_fwd(int64_t rows, int64_t D, int64_t F, int dtype, int activation, const void* x, int64_t x_stride, const void* w_gate,
+                        int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, const void* b_gate, const void* b_up, void* y, void* kept,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = feed_status(rows, D, F, dtype, activation);
+  if (rc != TSF_OK) return rc;
+  if (rows == 0) return TSF_OK;
+  if (!x || !w_gate || !w_up || !y) return TSF_ERR_ARG;
+  if (bad_ld(x_stride, D) || bad_ld(w_gate_stride, D) || bad_ld(w_up_stride, D)) return TSF_ERR_ARG;
+  const Shape s = shape_of(rows, D, F, dtype);
+  const Call c = {x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride};
+  auto* f = dtype == TSF_DTYPE_BF16 ? feed_fwd<bf16> : feed_fwd<float>;
+  return f(s, c, activation, b_gate, b_up, y, (char*)kept, (char*)workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int tsfast_hip_feed_bwd(int64_t rows, int64_t D, int64_t F, int dtype, int activation, const void* x, int64_t x_stride, const void* w_gate,
+                        int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, const void* grad_y, int64_t grad_y_stride,
+                        const void* kept, void* grad_x, void* grad_w_gate, void* grad_w_up, void* grad_b_gate, void* grad_b_up, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  const int rc = feed_status(rows, D, F, dtype, activation);
+  if (rc != TSF_OK) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) {
+    auto* z = dtype == TSF_DTYPE_BF16 ? zero<bf16> : zero<float>;
+    z(grad_w_gate, F * D, st), z(grad_w_up, F * D, st), z(grad_b_gate, F, st), z(grad_b_up, F, st);
+    return tsf_launch_status();
+  }
+  if (!x || !w_gate || !w_up || !grad_y || !kept || !grad_w_gate != !grad_w_up) return TSF_ERR_ARG;
+  if (bad_ld(x_stride, D) || bad_ld(w_gate_stride, D) || bad_ld(w_up_stride, D) || grad_y_stride < F) return TSF_ERR_ARG;
+  const Shape s = shape_of(rows, D, F, dtype);
+  const Call c = {x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride};
+  auto* f = dtype == TSF_DTYPE_BF16 ? feed_bwd<bf16> : feed_bwd<float>;
+  return f(s, c, activation, grad_y, grad_y_stride, (const char*)kept, grad_x, grad_w_gate, grad_w_up, grad_b_gate, grad_b_up, (char*)workspace,
+           workspace_bytes, st);
+}
+
+}  // extern "C"

@@ -6,6 +6,7 @@ residual stream that ``residual_norm`` continues into the next block::
     o, state = gated_recurrence(q, k, v, g, state)        # or gated_recurrence_step, token by token
     y = gated_norm(o.flatten(-2), gate, weight, groups=H) @ W_out
     stream, x = residual_norm(y, stream, next_weight, post_weight=.., scale=..)
+    y = gated_feed_forward(x, W_gate, W_up) @ W_down  # the feed-forward block behind a mixer
 
 The recurrence is linear with a matrix state per head and one decay per head and step,
 
@@ -19,17 +20,18 @@ serves what it declines (CPU tensors, float64, wider heads), in float32 at least
 
 from __future__ import annotations
 
-__all__ = ["gated_recurrence", "gated_recurrence_step", "gated_norm", "residual_norm"]
+__all__ = ["gated_recurrence", "gated_recurrence_step", "gated_norm", "residual_norm", "gated_feed_forward"]
 
 import torch
 import torch.nn.functional as F
 
 from ..dispatch import resolve
-from . import norm_hip, recurrence_hip
+from . import feed_hip, norm_hip, recurrence_hip
 
 # Module objects, not import paths: this dispatch may run inside a compiled forward.
 _RECURRENCE_BACKENDS = {"hip": recurrence_hip}
 _NORM_BACKENDS = {"hip": norm_hip}
+_FEED_BACKENDS = {"hip": feed_hip}
 _AUTO_ORDER = {"cuda": ("hip",)}
 
 _CHUNK = 64  # steps whose products the torch path forms at once
@@ -215,3 +217,38 @@ def residual_norm(x, residual, weight, post_weight=None, scale=None, eps: float 
     if weight is not None:
         y = y * weight
     return new.to(residual.dtype), y.to(x.dtype)
+
+
+_ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid}
+
+
+def gated_feed_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, activation: str = "silu"):
+    """The gated half of a feed-forward block: ``act(x W_gate^T + b_gate) * (x W_up^T + b_up)``.
+
+    Args:
+        x: ``[..., D]``; weight_gate, weight_up: ``[F, D]``; bias_gate, bias_up: ``[F]`` or None. All of one type.
+        activation: ``"silu"``, ``"gelu"`` (by erf) or ``"sigmoid"`` (a gated linear unit).
+
+    Returns:
+        ``[..., F]`` in x's type, differentiable in all tensors. The projection back to the stream's width is the caller's.
+
+    All values must be finite for float32: the fused kernel forms float32 products from parts of the factors, and an
+    infinite factor makes NaN of the rows or columns that it reaches.
+    """
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}, expected one of {tuple(_ACTIVATIONS)}")
+    if weight_gate.dim() != 2 or 0 in weight_gate.shape or weight_up.shape != weight_gate.shape:
+        raise ValueError(f"the weights must be [F, D] alike, got {tuple(weight_gate.shape)} and {tuple(weight_up.shape)}")
+    n, D = weight_gate.shape
+    if x.dim() < 1 or x.shape[-1] != D:
+        raise ValueError(f"x must be [..., {D}] for weights {tuple(weight_gate.shape)}, got {tuple(x.shape)}")
+    for t, name in ((bias_gate, "bias_gate"), (bias_up, "bias_up")):
+        _check_param(t, name, n)
+    for t in (weight_gate, weight_up, bias_gate, bias_up):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"weights and biases must be of x's type {x.dtype}, got {t.dtype}")
+    mod = resolve("gated.feed", _FEED_BACKENDS, _AUTO_ORDER.get(x.device.type, ()), (x, weight_gate, weight_up, bias_gate, bias_up))
+    if mod is not None:
+        return mod.run(x, weight_gate, weight_up, bias_gate, bias_up, activation)
+    a, b = (F.linear(_wide(x), _wide(w), None if t is None else _wide(t)) for w, t in ((weight_gate, bias_gate), (weight_up, bias_up)))
+    return (_ACTIVATIONS[activation](a) * b).to(x.dtype)
