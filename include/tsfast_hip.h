@@ -439,6 +439,37 @@ int tsfast_hip_feed_bwd(int64_t rows, int64_t D, int64_t F, int dtype, int activ
                         void* grad_w_up, void* grad_b_gate, void* grad_b_up, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A Mamba layer in service: its convolution and scan over sequences packed into one row of T tokens, and one token of
+ * each of B sequences. Sequence s has the tokens starts[s] .. starts[s + 1) (starts: [S + 1] int32 or int64 on the device, not
+ * decreasing, within [0, T]; where it is not, results are undefined but no access leaves the tensors). A sequence may be
+ * empty: it leaves the states it was given. Tokens without a sequence give zeros. The *_stride arguments are distances between
+ * tokens (rows) in elements; outputs and states are contiguous; no alignment is needed. No gradients.
+ *
+ * conv_packed:  u_t = silu(bias + sum_{k<K} w_k x_{t-(K-1)+k}), left of a sequence's first token its tail [S, D, K - 1] (NULL: zeros).
+ *   tails_out [S, D, K - 1]: each sequence's last K - 1 inputs. x, tails, out, tails_out of io_dtype, weight [D, K] and bias [D] (or
+ *   NULL) of weight_dtype and bias_dtype. 2 <= K <= 8.
+ * mamba_packed: the scan of tsfast_hip_mamba_fwd over each sequence, from h0 [S, D, N] (NULL: zeros) to h_last, float32. N <= 64.
+ * mamba_step:   conv, x_proj [R + 2 N, D], dt_proj [D, R] with dt_bias [D] (or NULL), softplus, scan step, D skip and gate of one token x, z
+ *   [B, D]; conv_state [B, D, K - 1] of io_dtype and ssm_state [B, D, N] float32 are overwritten. param_dtypes (host memory): the types of
+ *   conv_weight, conv_bias, x_proj, dt_proj, dt_bias. 2 <= K <= 8, N <= 64, R + 2 N <= 2048.
+ */
+int tsfast_hip_conv_packed(int64_t T, int64_t S, int64_t D, int64_t K, int io_dtype, int starts_int64, int weight_dtype,
+                           int bias_dtype, const void* x, int64_t x_stride, const void* starts, const void* tails,
+                           const void* weight, const void* bias, void* out, void* tails_out, void* stream);
+int64_t tsfast_hip_mamba_packed_workspace_bytes(int64_t T, int64_t S, int64_t D, int64_t N);
+int tsfast_hip_mamba_packed(int64_t T, int64_t S, int64_t D, int64_t N, int io_dtype, int starts_int64, const void* draw,
+                            int64_t draw_stride, const float* A, const void* Bt, int64_t b_stride, const void* Ct,
+                            int64_t c_stride, const void* u, int64_t u_stride, const void* z, int64_t z_stride,
+                            const float* Dp, const void* starts, const float* h0, void* out, float* h_last, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+int64_t tsfast_hip_mamba_step_workspace_bytes(int64_t B, int64_t D, int64_t N, int64_t R, int64_t K);
+int tsfast_hip_mamba_step(int64_t B, int64_t D, int64_t N, int64_t R, int64_t K, int io_dtype, const int* param_dtypes,
+                          const void* x, int64_t x_stride, const void* z, int64_t z_stride, void* conv_state,
+                          float* ssm_state, const void* conv_weight, const void* conv_bias, const void* x_proj,
+                          const void* dt_proj, const void* dt_bias, const float* A, const float* Dp, void* out,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,14 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "tsfast_hip_feed_bwd_workspace_bytes": ([_i64] * 3 + [_int] + [_ptr, _i64] * 3, _i64),
     "tsfast_hip_feed_fwd": ([_i64] * 3 + [_int, _int] + [_ptr, _i64] * 3 + [_ptr] * 5 + [_i64, _ptr], _int),
     "tsfast_hip_feed_bwd": ([_i64] * 3 + [_int, _int] + [_ptr, _i64] * 4 + [_ptr] * 7 + [_i64, _ptr], _int),
+    "tsfast_hip_conv_packed": ([_i64] * 4 + [_int] * 4 + [_ptr, _i64] + [_ptr] * 7, _int),
+    "tsfast_hip_mamba_packed_workspace_bytes": ([_i64] * 4, _i64),
+    "tsfast_hip_mamba_packed": (
+        [_i64] * 4 + [_int, _int, _ptr, _i64, _ptr] + [_ptr, _i64] * 4 + [_ptr] * 6 + [_i64, _ptr],
+        _int,
+    ),
+    "tsfast_hip_mamba_step_workspace_bytes": ([_i64] * 5, _i64),
+    "tsfast_hip_mamba_step": ([_i64] * 5 + [_int, _ptr] + [_ptr, _i64] * 2 + [_ptr] * 11 + [_i64, _ptr], _int),
     "tsfast_hip_mat_adjoint_workspace_bytes": ([_i64] * 4, _i64),
     "tsfast_hip_mat_adjoint_bounds": ([_i64] * 4 + [_ptr] * 4 + [_i64, _ptr], _int),
 }

@@ -1,0 +1,500 @@
+// A Mamba layer's convolution and scan over sequences packed into one row of tokens, in service (gfx950).
+//
+//   u_t   = silu(bias + sum_k w_k x_{t-(K-1)+k})            left of a sequence's first token: its carried tail
+//   h_t   = exp(delta_t A) h_{t-1} + delta_t u_t B_t,       delta = softplus(draw)
+//   out_t = (sum_n h_t C_t + Dp u_t) silu(z_t)              h before a sequence's first token: its carried state
+//
+// Sequence s has the tokens starts[s] .. starts[s + 1) of T; a sequence may be empty. The states that a sequence leaves (its
+// last K - 1 inputs; h after its last token) go out for the steps token by token behind it. Tokens without a sequence give zeros.
+// starts is read on the device: the host knows T and S only. Whatever starts holds, no access leaves the tensors and every loop ends.
+#include "common.h"
+#include "tsfast_hip.h"
+
+using namespace tsf;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxK = 8;
+
+// ---------------------------------------------------------------------------------- the sequences
+struct Starts {
+  const void* p;
+  int wide;  // int64, else int32
+  int64_t S, T;
+  // where sequence s begins (s = S: where the last one ends), within the tokens there are
+  TSF_DEV int64_t at(int64_t s) const {
+    const int64_t v = wide ? ((const int64_t*)p)[s] : (int64_t)((const int32_t*)p)[s];
+    return v < 0 ? 0 : v > T ? T : v;
+  }
+  // the sequence of token t: the last one that begins at or before it; -1: none yet, S: behind the last one
+  TSF_DEV int64_t of(int64_t t) const {
+    int64_t lo = 0, hi = S + 1;  // the first start behind t is in [lo, hi]
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (at(mid) <= t)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    return lo - 1;
+  }
+};
+
+// ------------------------------------------------------------------------------------ convolution
+// A thread has 16 bytes of channels (8 bf16, 4 fp32) and kRun tokens, with the last K - 1 inputs in registers.
+constexpr int kRun = 16;
+struct ConvArgs {
+  const void *x, *tails, *weight, *bias;
+  void *out, *tails_out;
+  int64_t D, sx, groups, runs;  // groups of channels; runs of tokens
+  Starts starts;
+  int w_bf16, b_bf16;
+};
+TSF_DEV float param(const void* p, int64_t i, int is_bf16) { return is_bf16 ? to_f32(((const bf16*)p)[i]) : ((const float*)p)[i]; }
+
+template <typename T, int VL>
+TSF_DEV void load_row(float* v, const T* p, int n) {
+  T h[VL];
+  if (n >= VL) {
+    __builtin_memcpy(h, p, sizeof(h));
+  } else {
+#pragma unroll
+    for (int e = 0; e < VL; ++e) h[e] = e < n ? p[e] : from_f32<T>(0.0f);
+  }
+#pragma unroll
+  for (int e = 0; e < VL; ++e) v[e] = to_f32(h[e]);
+}
+template <typename T, int VL>
+TSF_DEV void store_row(T* p, const float* v, int n) {
+  T h[VL];
+#pragma unroll
+  for (int e = 0; e < VL; ++e) h[e] = from_f32<T>(v[e]);
+  if (n >= VL) {
+    __builtin_memcpy(p, h, sizeof(h));
+  } else {
+#pragma unroll
+    for (int e = 0; e < VL; ++e)
+      if (e < n) p[e] = h[e];
+  }
+}
+
+template <typename T, int K>
+__global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
+  constexpr int VL = 16 / (int)sizeof(T);
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t run = i / g.groups, c0 = (i % g.groups) * VL, T_all = g.starts.T, S = g.starts.S;
+  const int n = (int)(g.D - c0 < VL ? g.D - c0 : VL);
+  const T *x = (const T*)g.x + c0, *tails = (const T*)g.tails;
+  T *out = (T*)g.out + c0, *tails_out = (T*)g.tails_out;
+  if (run >= g.runs) {  // an empty sequence leaves what it was given
+    const int64_t s = run - g.runs;
+    if (s >= S || g.starts.at(s + 1) > g.starts.at(s)) return;
+    const int64_t at = (s * g.D + c0) * (K - 1);
+    for (int e = 0; e < n * (K - 1); ++e) tails_out[at + e] = tails ? tails[at + e] : from_f32<T>(0.0f);
+    return;
+  }
+  float w[K][VL], b[VL], past[K - 1][VL];  // past[k]: the input K - 1 - k tokens ago
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    b[e] = g.bias && e < n ? param(g.bias, c0 + e, g.b_bf16) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][e] = e < n ? param(g.weight, (c0 + e) * K + k, g.w_bf16) : 0.0f;
+  }
+  const int64_t t0 = run * kRun, t1 = t0 + kRun < T_all ? t0 + kRun : T_all;
+  int64_t s = g.starts.of(t0);
+  int64_t begin = s < 0 ? 0 : g.starts.at(s), end = s < S ? g.starts.at(s + 1) : T_all;
+  if (s < 0) end = g.starts.at(0);
+  // tail value k of sequence s
+  auto carried = [&](int k, int e) __attribute__((always_inline)) {
+    return tails && e < n ? to_f32(tails[(s * g.D + c0 + e) * (K - 1) + k]) : 0.0f;
+  };
+  if (s >= 0 && s < S) {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      const int64_t t = t0 - (K - 1) + k;
+      if (t >= begin) {
+        load_row<T, VL>(past[k], x + t * g.sx, n);
+      } else {
+        const int64_t from = t - begin + (K - 1);  // in [0, K - 1): t >= t0 - (K - 1) >= begin - (K - 1)
+#pragma unroll
+        for (int e = 0; e < VL; ++e) past[k][e] = carried((int)from, e);
+      }
+    }
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    if (t >= end) {  // the next sequence that is not empty begins here, or none
+      do {
+        ++s;
+        begin = end;
+        end = s < S ? g.starts.at(s + 1) : T_all;
+      } while (s < S && end <= t);
+      if (s < S) {
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+          for (int e = 0; e < VL; ++e) past[k][e] = carried(k, e);
+      }
+    }
+    float y[VL];
+    if (s < 0 || s >= S) {
+#pragma unroll
+      for (int e = 0; e < VL; ++e) y[e] = 0.0f;
+      store_row<T, VL>(out + t * g.D, y, n);
+      continue;
+    }
+    float now[VL];
+    load_row<T, VL>(now, x + t * g.sx, n);
+#pragma unroll
+    for (int e = 0; e < VL; ++e) {
+      float a = b[e];
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) a = fmaf(w[k][e], past[k][e], a);
+      a = fmaf(w[K - 1][e], now[e], a);
+      y[e] = a * sigmoid_fast(a);
+    }
+    store_row<T, VL>(out + t * g.D, y, n);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+      for (int e = 0; e < VL; ++e) past[k][e] = k + 1 < K - 1 ? past[k + 1 < K - 1 ? k + 1 : k][e] : now[e];
+    if (t == end - 1) {
+#pragma unroll
+      for (int e = 0; e < VL; ++e)
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+          if (e < n) tails_out[(s * g.D + c0 + e) * (K - 1) + k] = from_f32<T>(past[k][e]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ scan
+// A workgroup has 64 channels and a run of tokens (a segment). Each of its four waves has a quarter of the states of all 64, a
+// channel a lane, in registers; what depends on a token and a channel (softplus, gates) is done once, by the thread that owns the pair,
+// and goes through LDS, a chunk of kTok tokens at a time.
+constexpr int kTok = 16;
+constexpr int kCh = 64;
+struct ScanArgs {
+  const void *draw, *Bt, *Ct, *u, *z;
+  const float *A, *Dp, *h0;
+  void* out;
+  float* h_last;
+  int64_t sdraw, sb, sc, su, sz;  // distances between tokens
+  int64_t D, tiles, seg_len, segs;
+  int N;
+  Starts starts;
+  float* maps;  // of segments: sums of delta [segs][D], then states [segs][N][D]
+};
+
+// The walk of one segment. MAP: only the state it hands to the next one, from the last sequence's first token in it (or its own
+// first token with no state), with the sum of delta that decays what enters; -1: nothing that enters reaches the next segment.
+template <typename T, int NPT, bool MAP>
+__global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
+  __shared__ float2 s_sc[kTok][kCh];         // delta, delta u
+  __shared__ float2 s_bc[kTok][4 * NPT];     // B, C
+  __shared__ float s_y[MAP ? 1 : kTok][4][kCh];  // each wave's sum over its states
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t tile = blockIdx.x % g.tiles, seg = blockIdx.x / g.tiles, d = tile * kCh + lane, S = g.starts.S, T_all = g.starts.T;
+  const int N = g.N, n0 = wave * NPT;
+  const bool act = d < g.D;
+  int64_t t0 = seg * g.seg_len;
+  const int64_t t1 = t0 + g.seg_len < T_all ? t0 + g.seg_len : T_all;
+
+  float A2[NPT], h[NPT];
+#pragma unroll
+  for (int j = 0; j < NPT; ++j) A2[j] = act && n0 + j < N ? g.A[d * N + n0 + j] * kLog2e : 0.0f, h[j] = 0.0f;
+  auto begin_state = [&](int64_t s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NPT; ++j) h[j] = g.h0 && act && n0 + j < N ? g.h0[(s * g.D + d) * N + n0 + j] : 0.0f;
+  };
+  auto end_state = [&](int64_t s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NPT; ++j)
+      if (act && n0 + j < N) g.h_last[(s * g.D + d) * N + n0 + j] = h[j];
+  };
+
+  int64_t s, end;  // the sequence of the present token, and its end
+  bool whole = false;
+  if (MAP) {
+    // the sequence that goes on in the next segment, if one does
+    s = g.starts.of(t1 - 1);
+    if (s < 0 || s >= S || t1 >= T_all || g.starts.at(s + 1) <= t1) return;
+    const int64_t begin = g.starts.at(s);
+    whole = begin < t0;  // the segment lies within the sequence
+    if (!whole) {
+      t0 = begin;
+      begin_state(s);
+    }
+    end = g.starts.at(s + 1);
+  } else {
+    // sequences without a token leave what they were given
+    for (int64_t e = seg; e < S; e += g.segs)
+      if (g.starts.at(e + 1) <= g.starts.at(e)) begin_state(e), end_state(e);
+    s = g.starts.of(t0);
+    end = s < 0 ? g.starts.at(0) : s < S ? g.starts.at(s + 1) : T_all;
+#pragma unroll
+    for (int j = 0; j < NPT; ++j) h[j] = 0.0f;
+    if (s >= 0 && s < S) {
+      if (g.starts.at(s) == t0) {
+        begin_state(s);
+      } else {
+        const float* from = g.maps + g.segs * g.D + (seg - 1) * N * g.D;
+#pragma unroll
+        for (int j = 0; j < NPT; ++j) h[j] = act && n0 + j < N ? from[(n0 + j) * g.D + d] : 0.0f;
+      }
+    }
+  }
+
+  constexpr int kOwn = kTok / 4;  // tokens of its channel that a thread owns in a chunk: wave + 4 k
+  constexpr int kBc = (kTok * 4 * NPT + kThreads - 1) / kThreads;
+  T r_dr[kOwn], r_u[kOwn], r_z[kOwn], r_b[kBc], r_c[kBc];
+  auto load = [&](int64_t tc) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int64_t t = tc + wave + 4 * k;
+      const bool in = act && t < t1;
+      r_dr[k] = in ? ((const T*)g.draw)[t * g.sdraw + d] : from_f32<T>(0.0f);
+      r_u[k] = in ? ((const T*)g.u)[t * g.su + d] : from_f32<T>(0.0f);
+      if (!MAP) r_z[k] = in ? ((const T*)g.z)[t * g.sz + d] : from_f32<T>(0.0f);
+    }
+#pragma unroll
+    for (int k = 0; k < kBc; ++k) {
+      const int i = tid + k * kThreads, n = i % (4 * NPT);
+      const int64_t t = tc + i / (4 * NPT);
+      const bool in = n < N && t < t1;
+      r_b[k] = in ? ((const T*)g.Bt)[t * g.sb + n] : from_f32<T>(0.0f);
+      if (!MAP) r_c[k] = in ? ((const T*)g.Ct)[t * g.sc + n] : from_f32<T>(0.0f);
+    }
+  };
+  const float dp = !MAP && act ? g.Dp[d] : 0.0f;
+  const int64_t first = g.starts.at(0), last = g.starts.at(S);  // tokens that have a sequence
+  float sum = 0.0f;
+  load(t0);
+  for (int64_t tc = t0; tc < t1; tc += kTok) {
+    const int len = (int)(t1 - tc < kTok ? t1 - tc : kTok);
+    float o_u[kOwn], o_z[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int i = wave + 4 * k;
+      o_u[k] = to_f32(r_u[k]);
+      if (!MAP) o_z[k] = to_f32(r_z[k]);
+      // tokens past the end: delta = 0 and no input, a step that changes nothing
+      const float delta = i < len ? softplus_fast(to_f32(r_dr[k])) : 0.0f;
+      if (MAP) sum += delta;
+      s_sc[i][lane] = make_float2(delta, delta * o_u[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kBc; ++k) {
+      const int i = tid + k * kThreads;
+      if (kTok * 4 * NPT % kThreads == 0 || i < kTok * 4 * NPT)
+        s_bc[i / (4 * NPT)][i % (4 * NPT)] = make_float2(to_f32(r_b[k]), MAP ? 0.0f : to_f32(r_c[k]));
+    }
+    if (tc + kTok < t1) load(tc + kTok);
+    __syncthreads();
+    auto step = [&](int i) __attribute__((always_inline)) {
+      const float2 sc = s_sc[i][lane];
+      float y = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NPT; ++j) {
+        const float2 bc = s_bc[i][n0 + j];
+        h[j] = fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x);
+        y = fmaf(h[j], bc.y, y);
+      }
+      if (!MAP) s_y[i][wave][lane] = y;
+    };
+    // no sequence ends within the chunk, but for its last token
+    if (MAP || (s >= 0 && end - tc >= len)) {
+      if (len == kTok) {
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) step(i);
+      } else {
+        for (int i = 0; i < len; ++i) step(i);
+      }
+      if (!MAP && s < S && end == tc + len) end_state(s);
+    } else {
+      for (int i = 0; i < len; ++i) {
+        const int64_t t = tc + i;
+        if (t >= end) {  // the next sequence that is not empty begins here, or none
+          do {
+            ++s;
+            end = s < S ? g.starts.at(s + 1) : T_all;
+          } while (s < S && end <= t);
+          if (s < S) begin_state(s);
+        }
+        step(i);
+        if (s >= 0 && s < S && t == end - 1) end_state(s);
+      }
+    }
+    __syncthreads();
+    if (!MAP) {
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        const int i = wave + 4 * k;
+        const int64_t t = tc + i;
+        if (i < len && act) {
+          const float y = (s_y[i][0][lane] + s_y[i][1][lane]) + (s_y[i][2][lane] + s_y[i][3][lane]);
+          const bool has = t >= first && t < last;
+          const float o = fmaf(dp, o_u[k], y) * (o_z[k] * sigmoid_fast(o_z[k]));
+          ((T*)g.out)[t * g.D + d] = from_f32<T>(has ? o : 0.0f);
+        }
+      }
+    }
+  }
+  if (MAP) {
+    float* sums = &s_sc[0][0].x;
+    __syncthreads();
+    sums[tid] = sum;
+    __syncthreads();
+    if (wave == 0 && act) g.maps[seg * g.D + d] = whole ? (sums[lane] + sums[64 + lane]) + (sums[128 + lane] + sums[192 + lane]) : -1.0f;
+    float* to = g.maps + g.segs * g.D + seg * N * g.D;
+#pragma unroll
+    for (int j = 0; j < NPT; ++j)
+      if (act && n0 + j < N) to[(n0 + j) * g.D + d] = h[j];
+  }
+}
+
+// The states that enter the segments, in order: the state that segment k - 1 leaves replaces its map's. A lane has one state of one
+// channel. Segments that no sequence leaves have no map; what stands in its place is not used.
+__global__ void __launch_bounds__(64) join_kernel(ScanArgs g) {
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (i >= g.D * g.N) return;
+  const int64_t d = i % g.D, n = i / g.D;
+  const float a = g.A[d * g.N + n] * kLog2e;
+  float* state = g.maps + g.segs * g.D + n * g.D + d;
+  float x = 0.0f;
+  constexpr int kAhead = 8;
+  for (int64_t k = 0; k + 1 < g.segs; k += kAhead) {
+    float S[kAhead], e[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int64_t kk = k + q < g.segs ? k + q : g.segs - 1;
+      S[q] = g.maps[kk * g.D + d];
+      e[q] = state[kk * g.N * g.D];
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      if (k + q + 1 >= g.segs) break;
+      // in two parts: a segment's factor may lie outside fp32 where its product with the state does not
+      const float p = a * S[q], p0 = fminf(fmaxf(p, -126.0f), 127.0f), p1 = fminf(fmaxf(p - p0, -126.0f), 127.0f);
+      x = S[q] < 0.0f ? e[q] : fmaf(fast_exp2(p0), x * fast_exp2(p1), e[q]);
+      state[(k + q) * g.N * g.D] = x;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kMaxGrid = (1 << 24) - 1;
+constexpr int kMaxN = 64;
+
+int per_wave(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+
+// Tokens of a segment: about four workgroups a CU, of 256 tokens or more
+int64_t segment_length(int64_t T, int64_t tiles) {
+  int64_t segs = up(4 * (int64_t)device_cus(), tiles);
+  if (segs > 256) segs = 256;
+  int64_t len = up(up(T, segs), kTok) * kTok;
+  return len < 256 ? 256 : len;
+}
+
+int packed_status(int64_t T, int64_t S, int64_t D, int io) {
+  if (T < 0 || S < 0 || D < 0 || (io != TSF_DTYPE_F32 && io != TSF_DTYPE_BF16)) return TSF_ERR_ARG;
+  if (T > (int64_t)1 << 40 || S > (int64_t)1 << 31 || D > (int64_t)1 << 24) return TSF_ERR_UNSUPPORTED;
+  return TSF_OK;
+}
+
+template <typename T>
+void launch_conv(const ConvArgs& a, int64_t K, unsigned grid, hipStream_t st) {
+  switch (K) {
+    case 2: conv_kernel<T, 2><<<grid, kThreads, 0, st>>>(a); break;
+    case 3: conv_kernel<T, 3><<<grid, kThreads, 0, st>>>(a); break;
+    case 4: conv_kernel<T, 4><<<grid, kThreads, 0, st>>>(a); break;
+    case 5: conv_kernel<T, 5><<<grid, kThreads, 0, st>>>(a); break;
+    case 6: conv_kernel<T, 6><<<grid, kThreads, 0, st>>>(a); break;
+    case 7: conv_kernel<T, 7><<<grid, kThreads, 0, st>>>(a); break;
+    default: conv_kernel<T, 8><<<grid, kThreads, 0, st>>>(a); break;
+  }
+}
+
+template <typename T, bool MAP>
+void launch_scan(const ScanArgs& a, unsigned grid, hipStream_t st) {
+  switch (per_wave(a.N)) {
+    case 1: scan_kernel<T, 1, MAP><<<grid, kThreads, 0, st>>>(a); break;
+    case 2: scan_kernel<T, 2, MAP><<<grid, kThreads, 0, st>>>(a); break;
+    case 4: scan_kernel<T, 4, MAP><<<grid, kThreads, 0, st>>>(a); break;
+    case 8: scan_kernel<T, 8, MAP><<<grid, kThreads, 0, st>>>(a); break;
+    default: scan_kernel<T, 16, MAP><<<grid, kThreads, 0, st>>>(a); break;
+  }
+}
+
+int64_t conv_grid(int64_t T, int64_t S, int64_t D, int io) {
+  return up((up(T, kRun) + S) * up(D, io == TSF_DTYPE_BF16 ? 8 : 4), kThreads);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tsfast_hip_conv_packed(int64_t T, int64_t S, int64_t D, int64_t K, int io_dtype, int starts_int64, int weight_dtype, int bias_dtype,
+                           const void* x, int64_t x_stride, const void* starts, const void* tails, const void* weight, const void* bias,
+                           void* out, void* tails_out, void* stream) {
+  const int rc = packed_status(T, S, D, io_dtype);
+  if (rc != TSF_OK) return rc;
+  if (K < 2) return TSF_ERR_ARG;
+  if (K > kMaxK || conv_grid(T, S, D, io_dtype) > kMaxGrid) return TSF_ERR_UNSUPPORTED;
+  if (D == 0 || (T == 0 && S == 0)) return TSF_OK;
+  if (!starts || !weight || (T > 0 && (!x || !out || x_stride < 0)) || (S > 0 && !tails_out)) return TSF_ERR_ARG;
+  ConvArgs a = {x, tails, weight, bias, out, tails_out, D, x_stride, up(D, io_dtype == TSF_DTYPE_BF16 ? 8 : 4), up(T, kRun),
+                Starts{starts, starts_int64, S, T}, weight_dtype == TSF_DTYPE_BF16, bias_dtype == TSF_DTYPE_BF16};
+  const unsigned grid = (unsigned)conv_grid(T, S, D, io_dtype);
+  if (io_dtype == TSF_DTYPE_BF16)
+    launch_conv<bf16>(a, K, grid, (hipStream_t)stream);
+  else
+    launch_conv<float>(a, K, grid, (hipStream_t)stream);
+  return tsf_launch_status();
+}
+
+int64_t tsfast_hip_mamba_packed_workspace_bytes(int64_t T, int64_t S, int64_t D, int64_t N) {
+  if (packed_status(T, S, D, TSF_DTYPE_F32) != TSF_OK || N < 1 || N > kMaxN) return -1;
+  if (D == 0 || T == 0) return 0;
+  const int64_t segs = up(T, segment_length(T, up(D, kCh)));
+  return segs > 1 ? segs * (N + 1) * D * 4 : 0;
+}
+
+int tsfast_hip_mamba_packed(int64_t T, int64_t S, int64_t D, int64_t N, int io_dtype, int starts_int64, const void* draw, int64_t draw_stride,
+                            const float* A, const void* Bt, int64_t b_stride, const void* Ct, int64_t c_stride, const void* u,
+                            int64_t u_stride, const void* z, int64_t z_stride, const float* Dp, const void* starts, const float* h0,
+                            void* out, float* h_last, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = packed_status(T, S, D, io_dtype);
+  if (rc != TSF_OK) return rc;
+  if (N < 1) return TSF_ERR_ARG;
+  if (N > kMaxN) return TSF_ERR_UNSUPPORTED;
+  if (D == 0 || (T == 0 && S == 0)) return TSF_OK;
+  if (!A || !Dp || !starts || (S > 0 && !h_last)) return TSF_ERR_ARG;
+  if (T > 0 && (!draw || !Bt || !Ct || !u || !z || !out)) return TSF_ERR_ARG;
+  if (draw_stride < 0 || b_stride < 0 || c_stride < 0 || u_stride < 0 || z_stride < 0) return TSF_ERR_ARG;
+  ScanArgs a = {draw, Bt, Ct, u, z, A, Dp, h0, out, h_last, draw_stride, b_stride, c_stride, u_stride, z_stride, D, up(D, kCh), 0, 1, (int)N,
+                Starts{starts, starts_int64, S, T}, (float*)workspace};
+  a.seg_len = segment_length(T, a.tiles);
+  a.segs = T > 0 ? up(T, a.seg_len) : 1;
+  if (a.segs * a.tiles > kMaxGrid) return TSF_ERR_UNSUPPORTED;
+  const hipStream_t st = (hipStream_t)stream;
+  if (a.segs > 1) {
+    if (!workspace || workspace_bytes < tsfast_hip_mamba_packed_workspace_bytes(T, S, D, N)) return TSF_ERR_WORKSPACE;
+    const unsigned grid = (unsigned)((a.segs - 1) * a.tiles);
+    if (io_dtype == TSF_DTYPE_BF16)
+      launch_scan<bf16, true>(a, grid, st);
+    else
+      launch_scan<float, true>(a, grid, st);
+    join_kernel<<<(unsigned)up(D * N, 64), 64, 0, st>>>(a);
+  }
+  const unsigned grid = (unsigned)(a.segs * a.tiles);
+  if (io_dtype == TSF_DTYPE_BF16)
+    launch_scan<bf16, false>(a, grid, st);
+  else
+    launch_scan<float, false>(a, grid, st);
+  return tsf_launch_status();
+}
+
+}  // extern "C"
