@@ -7,6 +7,8 @@
 // One kernel, product_kernel, forms the three matrix products: C[q][p] = sum_k Q[q][k] P[p][k], bf16 operands, fp32 sums.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "tsfast_hip.h"
 
@@ -23,6 +25,7 @@ constexpr int64_t kMaxLd = 1 << 22;  // elements between the rows of an operand:
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2), may_alias));
@@ -82,14 +85,15 @@ struct PackArgs {
   PackJob job[3];
 };
 
+// What is left of a value beside its first part, the nearest bf16; nothing of an infinity or of a value that rounds to one.
+TSF_DEV float split_rest(float x) {
+  const float h = (float)(__bf16)x;
+  return fabsf(h) <= 3.4028235e38f ? x - h : 0.0f;
+}
 TSF_DEV void split3(float x, float* part) {
-  // the first part of a finite value is finite
-  float h = (float)(__bf16)x;
-  if (!(fabsf(h) <= 3.0e38f) && fabsf(x) <= 3.4028235e38f) h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const bool fin = fabsf(x) <= 3.4028235e38f;
-  const float r = fin ? x - h : 0.0f;
-  const float m = (float)(__bf16)r;
-  part[0] = h, part[1] = m, part[2] = r - m;
+  part[0] = x;
+  part[1] = split_rest(x);
+  part[2] = split_rest(part[1]);
 }
 
 template <typename T>
@@ -147,6 +151,7 @@ struct ProductArgs {
 template <int BQ_, int BP_, int WQ_, int WP_>
 struct Tile {
   static constexpr int BQ = BQ_, BP = BP_, HP = BP_ / 2, WQ = WQ_, WP = WP_, kWaves = WQ * WP, TH = 64 * kWaves;
+  static constexpr int kPerSimd = BQ * BP >= 256 * 256 ? kWaves / 4 : 2;  // waves
   static constexpr int NQ = BQ / WQ / 16, NH = HP / WP / 16;  // 16-row blocks a wave has of q, and of each half of p
   static constexpr int kQBytes = BQ * kK * 2, kHBytes = HP * kK * 2, kStage = kQBytes + 2 * kHBytes;
   static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave a stage
@@ -161,7 +166,7 @@ template <int ROWS, bool TURNED>
 struct Panel {
   static constexpr int kChunks = ROWS / 8;  // of a row of k
   static constexpr uint32_t kNone = 0x80000000u;
-  TSF_DEV static uint32_t swz(uint32_t r) { return ((r >> 1) & 3) ^ ((r >> 3) & 1); }
+  TSF_DEV static uint32_t swz(uint32_t r) { return (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 3) & 1); }
   TSF_DEV static uint32_t turn(uint32_t kr) { return (((kr & 3) << 1) | (((kr >> 3) & 1) << 3)) & (kChunks - 1); }
 
   uint32_t off, need;  // the lane's byte offset in a stage, and which of the stage's k it starts at
@@ -180,9 +185,14 @@ struct Panel {
   }
   // at: the panel's first row (as it lies: at k = 0, so: bytes from there to the stage's k; turned: the stage's first row of k);
   // left: of the stage's k that exist. A lane whose values do not exist reads beyond the resource's end: zeros.
-  TSF_DEV void load(const bf16* at, uint32_t bytes, uint32_t so, uint32_t left, char* lds) const {
+  TSF_DEV void load(const bf16* at, uint32_t bytes, uint32_t so, uint32_t left, uint32_t to) const {
     const uint32_t v = need < left ? off : kNone;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(at, bytes), (__attribute__((address_space(3))) void*)lds, 16, v, so, 0, 0);
+    const uint64_t a = (uint64_t)at;
+    const auto uniform = [](uint32_t v) __attribute__((always_inline)) { return (int)__builtin_amdgcn_readfirstlane(v); };
+    const i32x4 rsrc = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffff), uniform(bytes), kBufWord3};
+    // Written out, for the compiler makes every later read of LDS wait for the builtin's loads to arrive (vmcnt(0)), which would
+    // leave one stage on its way instead of three. Only the waits of stage_barrier cover these loads.
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(to)), "v"(v), "s"(rsrc), "s"(uniform(so)) : "memory");
   }
   // the bytes from `at` that the lanes which read may reach
   TSF_DEV static uint32_t reach(uint32_t rows, uint32_t k, int64_t ld) {
@@ -284,8 +294,8 @@ template <typename T>
 TSF_DEV void save_pre(char* hi, char* lo, int64_t block, uint32_t lane, f32x4 a, f32x4 b) {
   if constexpr (sizeof(T) == 4) {
     char* p = hi + (block * 64 + lane) * 32;
-    *(u32x4*)p = __builtin_bit_cast(u32x4, a);
-    *(u32x4*)(p + 16) = __builtin_bit_cast(u32x4, b);
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, a), (u32x4*)p);
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, b), (u32x4*)(p + 16));
   } else {
     uint32_t r[8];
 #pragma unroll
@@ -299,8 +309,8 @@ TSF_DEV void save_pre(char* hi, char* lo, int64_t block, uint32_t lane, f32x4 a,
       const uint32_t x = __builtin_amdgcn_perm(r[4 * k + 1], r[4 * k], 0x0c0c0501), y = __builtin_amdgcn_perm(r[4 * k + 3], r[4 * k + 2], 0x0c0c0501);
       l[k] = x | y << 16;
     }
-    *(u32x4*)(hi + (block * 64 + lane) * 16) = h;
-    *(u32x2*)(lo + (block * 64 + lane) * 8) = l;
+    __builtin_nontemporal_store(h, (u32x4*)(hi + (block * 64 + lane) * 16));
+    __builtin_nontemporal_store(l, (u32x2*)(lo + (block * 64 + lane) * 8));
   }
 }
 template <typename T>
@@ -325,7 +335,7 @@ TSF_DEV void load_pre(const char* hi, const char* lo, int64_t block, uint32_t la
 }
 
 template <typename T, typename C, int FORM>
-__global__ void __launch_bounds__(C::TH, C::kWaves == 8 ? 2 : 2) product_kernel(ProductArgs g) {
+__global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs g) {
   constexpr bool TQ = FORM == kWeight, TP = FORM != kForward;  // turned operands
   constexpr int NQ = C::NQ, NH = C::NH;
   __shared__ __attribute__((aligned(1024))) char lds[C::kLds];
@@ -357,39 +367,46 @@ __global__ void __launch_bounds__(C::TH, C::kWaves == 8 ? 2 : 2) product_kernel(
   static_assert(kQw * C::kWaves == kQ && kPw * C::kWaves == 2 * kH, "");
   Panel<C::BQ, TQ> lq[kQw];
   Panel<C::HP, TP> lp[kPw];
-  // a piece of p lies in one of its halves
-  const bool second[2] = {wave >= kH, wave + C::kWaves >= kH};
-  static_assert(kPw <= 2, "");
+  // a piece of p lies in one of its halves: which one goes by the piece, or by the wave
+  constexpr bool kByPiece = kH % C::kWaves == 0;
+  static_assert(kByPiece || kPw == 1, "");
+  constexpr int kHalves = kByPiece ? 2 : 1;
+  auto half_of = [&](int i) __attribute__((always_inline)) { return kByPiece ? i / (kPw / kHalves) : (int)(wave >= kH); };
 #pragma unroll
   for (int i = 0; i < kQw; ++i) lq[i].set(wave + i * C::kWaves, lane, g.ldq, rows_q);
 #pragma unroll
-  for (int i = 0; i < kPw; ++i) lp[i].set((wave + i * C::kWaves) % kH, lane, g.ldp, second[i] ? rows_1 : rows_0);
+  for (int i = 0; i < kPw; ++i) lp[i].set((wave + i * C::kWaves) % kH, lane, g.ldp, half_of(i) ? rows_1 : rows_0);
   const int kq = (int)g.kq, kp = (int)g.kp, per_seg = (kq + kK - 1) / kK;
   const int begin = (int)(split * g.split_stages);
   const int count = (int)(g.stages - begin < g.split_stages ? g.stages - begin : g.split_stages);
   const int rounds = (count + 1) / 2;  // two stages a round: one past the end adds zeros
   int to_load = count, seg = begin / per_seg, k0 = (begin % per_seg) * kK;
-  const bf16 *qb, *pb[2];
+  const bf16 *qb, *pb[kHalves];
   auto enter = [&]() __attribute__((always_inline)) {
     qb = g.q[seg] + (TQ ? q0 + k0 * g.ldq : q0 * g.ldq);
 #pragma unroll
-    for (int i = 0; i < kPw; ++i) {
-      const int64_t at = second[i] ? p1 : p0;
-      pb[i] = (second[i] ? g.p1 : g.p0)[seg] + (TP ? at + k0 * g.ldp : at * g.ldp);
+    for (int h = 0; h < kHalves; ++h) {
+      const bool second = kByPiece ? h != 0 : wave >= kH;
+      const int64_t at = second ? p1 : p0;
+      pb[h] = (second ? g.p1 : g.p0)[seg] + (TP ? at + k0 * g.ldp : at * g.ldp);
     }
   };
   enter();
   const uint32_t reach_q = Panel<C::BQ, TQ>::reach(rows_q, kq, g.ldq);
   const uint32_t reach_0 = Panel<C::HP, TP>::reach(rows_0, kp, g.ldp), reach_1 = Panel<C::HP, TP>::reach(rows_1, kp, g.ldp);
-  auto load_stage = [&](int buf) __attribute__((always_inline)) {
-    char* to = lds + buf * C::kStage;
-    const int lq_ = to_load > 0 ? kq - k0 : 0, lp_ = to_load > 0 ? kp - k0 : 0;
-    const uint32_t left_q = lq_ > 0 ? lq_ : 0, left_p = lp_ > 0 ? lp_ : 0;
-#pragma unroll
-    for (int i = 0; i < kQw; ++i) lq[i].load(qb, reach_q, TQ ? 0 : k0 * 2, left_q, to + (wave + i * C::kWaves) * 1024);
-#pragma unroll
-    for (int i = 0; i < kPw; ++i)
-      lp[i].load(pb[i], second[i] ? reach_1 : reach_0, TP ? 0 : k0 * 2, left_p, to + C::kQBytes + (wave + i * C::kWaves) * 1024);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // piece i of the next stage, of kLoads; `advance` goes on to the stage after it
+  auto load_piece = [&](int buf, int i) __attribute__((always_inline)) {
+    const uint32_t to = lds_at + buf * C::kStage + (i < kQw ? 0 : C::kQBytes) + (wave + (i < kQw ? i : i - kQw) * C::kWaves) * 1024;
+    const int left = to_load > 0 ? (i < kQw ? kq : kp) - k0 : 0;
+    if (i < kQw) {
+      lq[i].load(qb, reach_q, TQ ? 0 : k0 * 2, left > 0 ? left : 0, to);
+    } else {
+      const int n = i - kQw;
+      lp[n].load(pb[kByPiece ? half_of(n) : 0], half_of(n) ? reach_1 : reach_0, TP ? 0 : k0 * 2, left > 0 ? left : 0, to);
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
     --to_load;
     k0 += kK;
     if (k0 >= kq && to_load > 0) {
@@ -398,8 +415,8 @@ __global__ void __launch_bounds__(C::TH, C::kWaves == 8 ? 2 : 2) product_kernel(
     } else {
       if (TQ) qb += kK * g.ldq;
 #pragma unroll
-      for (int i = 0; i < kPw; ++i)
-        if (TP) pb[i] += kK * g.ldp;
+      for (int h = 0; h < kHalves; ++h)
+        if (TP) pb[h] += kK * g.ldp;
     }
   };
 
@@ -410,75 +427,99 @@ __global__ void __launch_bounds__(C::TH, C::kWaves == 8 ? 2 : 2) product_kernel(
   struct Blocks {
     bf16x8 q[NQ], p[2 * NH];
   };
-  auto read_stage = [&](Blocks& f, int buf) __attribute__((always_inline)) {
+  // part j of a stage's blocks, of NQ: one of q and as many of p
+  constexpr int kPart = 2 * NH / NQ;
+  static_assert(kPart * NQ == 2 * NH && C::kLoads == NQ, "");
+  auto read_part = [&](Blocks& f, int buf, int j) __attribute__((always_inline)) {
     const char* from = lds + buf * C::kStage;
 #pragma unroll
-    for (int i = 0; i < 2 * NH; ++i) f.p[i] = rp.get(from + C::kQBytes + (i / NH) * C::kHBytes, wp * NH + i % NH);
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) f.q[j] = rq.get(from, wq * NQ + j);
+    for (int i = j * kPart; i < (j + 1) * kPart; ++i) f.p[i] = rp.get(from + C::kQBytes + (i / NH) * C::kHBytes, wp * NH + i % NH);
+    f.q[j] = rq.get(from, wq * NQ + j);
   };
   f32x4 acc[2 * NH][NQ];
 #pragma unroll
   for (int i = 0; i < 2 * NH; ++i)
 #pragma unroll
     for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  auto multiply = [&](const Blocks& f) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < NQ; ++j)
-#pragma unroll
-      for (int i = 0; i < 2 * NH; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.p[i], f.q[j], acc[i][j], 0, 0, 0);
-  };
 
   // Stage t's blocks are in registers when its turn comes. Its products run while stage t + 1's blocks are read from LDS and
-  // stage t + 4 is loaded into the place that stage t has left; t + 2 and t + 3 are on their way.
+  // stage t + 4 is loaded into the place that stage t has left; t + 2 and t + 3 are on their way. A wave issues in order, so loads and
+  // reads stand evenly between the products: in front of them, they would wait for the other waves' (2.1 -> 1.4 ms, see below).
+  auto stage = [&](const Blocks& now, Blocks& next, int load_to, int read_from) __attribute__((always_inline)) {
+    stage_barrier<2 * C::kLoads>();
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      load_piece(load_to, j);
+      read_part(next, read_from, j);
+#pragma unroll
+      for (int i = 0; i < 2 * NH; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(now.p[i], now.q[j], acc[i][j], 0, 0, 0);
+      constexpr int kReads = (TQ ? 2 : 1) + kPart * (TP ? 2 : 1), kEach = 2 * NH / kReads > 0 ? 2 * NH / kReads : 1;
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * NH, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    advance();
+  };
   Blocks f0, f1;
-  load_stage(0);
-  load_stage(1);
-  load_stage(2);
-  load_stage(3);
+#pragma unroll
+  for (int t = 0; t < kStages; ++t) {
+#pragma unroll
+    for (int j = 0; j < C::kLoads; ++j) load_piece(t, j);
+    advance();
+  }
   stage_barrier<3 * C::kLoads>();
-  read_stage(f0, 0);
+#pragma unroll
+  for (int j = 0; j < NQ; ++j) read_part(f0, 0, j);
   int buf = 0;
   for (int r = 0; r < rounds; ++r) {
-    stage_barrier<2 * C::kLoads>();
-    load_stage(buf);
-    read_stage(f1, buf + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(f0);
-    stage_barrier<2 * C::kLoads>();
-    load_stage(buf + 1);
-    read_stage(f0, (buf + 2) & 3);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(f1);
+    stage(f0, f1, buf, buf + 1);
+    stage(f1, f0, buf + 1, (buf + 2) & 3);
     buf = (buf + 2) & 3;
   }
   stage_barrier<0>();
 
   if constexpr (FORM == kForward) {
     const T *bg = (const T*)g.bg, *bu = (const T*)g.bu;
+    auto finish = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NH; ++i) {
-      const int64_t f = p0 + (wp * NH + i) * 16 + 4 * lg;
-      f32x4 va = {0.0f, 0.0f, 0.0f, 0.0f}, vb = va;
+      for (int i = 0; i < NH; ++i) {
+        const int64_t f = p0 + (wp * NH + i) * 16 + 4 * lg;
+        f32x4 va = {0.0f, 0.0f, 0.0f, 0.0f}, vb = va;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (bg && f + e < g.np) va[e] = to_f32(bg[f + e]);
-        if (bu && f + e < g.np) vb[e] = to_f32(bu[f + e]);
-      }
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        f32x4& a = acc[i][j];
-        f32x4& b = acc[NH + i][j];
-        a += va;
-        b += vb;
-        if (g.train) {
-          const int64_t mb = q0 / 16 + wq * NQ + j, fb = p0 / 16 + wp * NH + i;
-          if (mb * 16 < g.nq && fb < g.save_fb) save_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
+        for (int e = 0; e < 4; ++e) {
+          if (bg && f + e < g.np) va[e] = to_f32(bg[f + e]);
+          if (bu && f + e < g.np) vb[e] = to_f32(bu[f + e]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = activate(g.act, a[e]) * b[e];
+        for (int j = 0; j < NQ; ++j) {
+          f32x4& a = acc[i][j];
+          f32x4& b = acc[NH + i][j];
+          a += va;
+          b += vb;
+          if (g.train) {
+            const int64_t mb = q0 / 16 + wq * NQ + j, fb = p0 / 16 + wp * NH + i;
+            if (mb * 16 < g.nq && fb < g.save_fb) save_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v, dv;
+            activate<decltype(act)::value>(a[e], v, dv);
+            a[e] = v * b[e];
+          }
+          __builtin_amdgcn_sched_barrier(0);  // or values of many blocks are alive at once, and spill
+        }
       }
-    }
+    };
+    if (g.act == kSilu)
+      finish(std::integral_constant<int, kSilu>());
+    else if (g.act == kGelu)
+      finish(std::integral_constant<int, kGelu>());
+    else
+      finish(std::integral_constant<int, kSigmoid>());
     T* y = (T*)g.y;
     store_half<C, T>(lds, wq, wp, li, lg, (int)rows_0, [&](int i, int j) { return acc[i][j]; },
                      [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + p0 : (T*)nullptr; });
@@ -517,64 +558,117 @@ struct AdjointArgs {
   float* part;  // [workgroups along rows][2][F], or null
 };
 
+// Accumulators hold four columns a lane; memory wants whole lines. A wave's block of 16 rows x 64 columns goes through LDS of its
+// own: `kind` of 16 bytes a lane in memory's order, four columns a lane in the accumulators'.
+template <typename T>
+struct Turn {
+  static constexpr int kRow = 64 * (int)sizeof(T) + 16;  // bytes of a row in LDS
+  static constexpr int kPer = 16 / (int)sizeof(T), kPieces = 64 / kPer, kEach = 16 * kPieces / 64;
+  alignas(16) char at[16 * kRow];
+  TSF_DEV static int row(int lane, int e) { return (lane + 64 * e) / kPieces; }
+  TSF_DEV static int col(int lane, int e) { return (lane + 64 * e) % kPieces * kPer; }
+  TSF_DEV void put_piece(int lane, int e, u32x4 v) { *(u32x4*)(at + row(lane, e) * kRow + col(lane, e) * sizeof(T)) = v; }
+  TSF_DEV u32x4 get_piece(int lane, int e) const { return *(const u32x4*)(at + row(lane, e) * kRow + col(lane, e) * sizeof(T)); }
+  TSF_DEV void put_four(int li, int c, f32x4 v) { put4<T>(at + li * kRow + c * sizeof(T), v); }
+  TSF_DEV f32x4 get_four(int li, int c) const {
+    T v[4];
+    if constexpr (sizeof(T) == 2) {
+      const u32x2 w = *(const u32x2*)(at + li * kRow + c * 2);
+      return f32x4{low(w[0]), high(w[0]), low(w[1]), high(w[1])};
+    } else {
+      return __builtin_bit_cast(f32x4, *(const u32x4*)(at + li * kRow + c * 4));
+    }
+  }
+  // between a wave's writes and its other lanes' reads
+  TSF_DEV static void turned() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+};
+
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
+  union Lds {
+    Turn<T> dy;
+    Turn<bf16> d[2];
+  };
+  __shared__ Lds lds[4];
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
+  Lds& turn = lds[wave];
   const int64_t f0 = (int64_t)blockIdx.x * 64, first = (int64_t)blockIdx.y * g.blocks;
   const int64_t all = (g.rows + 15) / 16, last = first + g.blocks < all ? first + g.blocks : all;
   const int64_t plane = g.rows * 2 * g.F8;
+  constexpr int kDy = Turn<T>::kEach, kPer = Turn<T>::kPer;
+  const int blocks = (int)(g.save_fb - f0 / 16 < 4 ? g.save_fb - f0 / 16 : 4);
   f32x4 sa[4], sb[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) sa[i] = sb[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int64_t mb = first + wave; mb < last; mb += 4) {
-    const int64_t m = mb * 16 + li;
+    const int64_t m0 = mb * 16;
+    f32x4 a[4], b[4];
+    u32x4 in[kDy];
+#pragma unroll
+    for (int e = 0; e < kDy; ++e) {
+      const int64_t m = m0 + Turn<T>::row(lane, e), f = f0 + Turn<T>::col(lane, e);
+      const T* p = (const T*)g.dy + m * g.ld_dy + f;
+      T v[kPer];
+      if (m < g.rows && f + kPer <= g.F) {
+        __builtin_memcpy(v, p, 16);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = m < g.rows && f + k < g.F ? p[k] : from_f32<T>(0.0f);
+      }
+      __builtin_memcpy(&in[e], v, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < blocks) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + i, lane, a[i], b[i]);
+#pragma unroll
+    for (int e = 0; e < kDy; ++e) turn.dy.put_piece(lane, e, in[e]);
+    Turn<T>::turned();
+    f32x4 dy[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dy[i] = turn.dy.get_four(li, 16 * i + 4 * lg);
+    Turn<T>::turned();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t fb = f0 / 16 + i, f = f0 + 16 * i + 4 * lg;
-      if (fb >= g.save_fb) continue;
-      f32x4 a, b, da, db;
-      load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
-      float dy[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (m < g.rows) {
-        const T* p = (const T*)g.dy + m * g.ld_dy + f;
-        if (f + 4 <= g.F) {
-          T v[4];
-          __builtin_memcpy(v, p, sizeof(v));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dy[e] = to_f32(v[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (f + e < g.F) dy[e] = to_f32(p[e]);
-        }
-      }
+      if (i >= blocks) a[i] = b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v, dv;
-        activate<ACT>(a[e], v, dv);
-        const bool in = m < g.rows && f + e < g.F;
-        da[e] = in ? dy[e] * b[e] * dv : 0.0f;
-        db[e] = in ? dy[e] * v : 0.0f;
+        activate<ACT>(a[i][e], v, dv);
+        // columns and rows that do not exist have dy = 0
+        a[i][e] = dy[i][e] * b[i][e] * dv;
+        b[i][e] = dy[i][e] * v;
       }
-      sa[i] += da;
-      sb[i] += db;
-      if (m < g.rows && f < g.F8) {
-        bf16* to = g.d + m * 2 * g.F8 + f;
-        if constexpr (kPlanes == 1) {
-          *(u32x2*)to = u32x2{pack2(da[0], da[1]), pack2(da[2], da[3])};
-          *(u32x2*)(to + g.F8) = u32x2{pack2(db[0], db[1]), pack2(db[2], db[3])};
-        } else {
-          float pa[4][3], pb[4][3];
+      sa[i] += a[i];
+      sb[i] += b[i];
+    }
+    // a and b are da and db from here on; each plane of theirs in turn
 #pragma unroll
-          for (int e = 0; e < 4; ++e) split3(da[e], pa[e]), split3(db[e], pb[e]);
+    for (int n = 0; n < kPlanes; ++n) {
 #pragma unroll
-          for (int n = 0; n < 3; ++n) {
-            *(u32x2*)(to + n * plane) = u32x2{pack2(pa[0][n], pa[1][n]), pack2(pa[2][n], pa[3][n])};
-            *(u32x2*)(to + n * plane + g.F8) = u32x2{pack2(pb[0][n], pb[1][n]), pack2(pb[2][n], pb[3][n])};
-          }
+      for (int i = 0; i < 4; ++i) {
+        turn.d[0].put_four(li, 16 * i + 4 * lg, a[i]);
+        turn.d[1].put_four(li, 16 * i + 4 * lg, b[i]);
+        if (n + 1 < kPlanes) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[i][e] = split_rest(a[i][e]), b[i][e] = split_rest(b[i][e]);
         }
       }
+      Turn<T>::turned();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t m = m0 + Turn<bf16>::row(lane, e), f = f0 + Turn<bf16>::col(lane, e);
+        if (m < g.rows && f < g.F8) {
+          bf16* to = g.d + n * plane + m * 2 * g.F8 + f;
+          *(u32x4*)to = turn.d[0].get_piece(lane, e);
+          *(u32x4*)(to + g.F8) = turn.d[1].get_piece(lane, e);
+        }
+      }
+      Turn<T>::turned();
     }
   }
   if (!g.part) return;
@@ -595,18 +689,23 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   }
 }
 
-// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in order
+// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in a fixed order: 64 columns a
+// workgroup, every fourth part a wave.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int64_t parts, int64_t stride, int64_t n, T* out0, T* out1) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= 2 * n) return;
-  const int64_t h = i >= n, c = i - h * n;
-  T* out = h ? out1 : out0;
-  if (!out) return;
-  const float* p = part + h * stride + c;
+__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int parts, int64_t stride, int64_t n, T* out0, T* out1) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane, h = i >= n, c = i - h * n;
   float s = 0.0f;
-  for (int64_t k = 0; k < parts; ++k) s += p[k * 2 * stride];
-  out[c] = from_f32<T>(s);
+  if (i < 2 * n) {
+    const float* p = part + h * stride + c;
+#pragma unroll 8
+    for (int k = wave; k < parts; k += 4) s += p[(int64_t)k * 2 * stride];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  T* out = h ? out1 : out0;
+  if (wave == 0 && i < 2 * n && out) out[c] = from_f32<T>((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
 }
 
 // --------------------------------------------------------------------------------- a few rows
@@ -706,7 +805,11 @@ int64_t up256(int64_t a) { return up(a, 256) * 256; }
 
 constexpr int64_t kFewRows = 32;
 
+#ifndef L4
 using Large = Tile<256, 256, 4, 2>;
+#else
+using Large = Tile<256, 256, 2, 2>;
+#endif
 using Medium = Tile<128, 128, 2, 2>;
 using Small = Tile<64, 64, 2, 2>;
 
@@ -914,7 +1017,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
   a.dy = dy, a.ld_dy = ld_dy, a.rows = s.rows, a.F = s.F, a.F8 = s.F8, a.save_fb = up(s.F, 16), a.blocks = b.blocks;
   a.save_hi = pre, a.save_lo = pre_lo(const_cast<char*>(pre), s.rows, s.F), a.d = d, a.part = want_bias ? bias : nullptr;
   launch_adjoint<T>(a, act, dim3((unsigned)up(s.F, 64), (unsigned)b.wgs), st);
-  if (want_bias) sum_kernel<T><<<(unsigned)up(2 * s.F, kThreads), kThreads, 0, st>>>(bias, b.wgs, s.F, s.F, (T*)dbg, (T*)dbu);
+  if (want_bias) sum_kernel<T><<<(unsigned)up(2 * s.F, 64), kThreads, 0, st>>>(bias, (int)b.wgs, s.F, s.F, (T*)dbg, (T*)dbu);
 
   const int64_t plane = s.rows * 2 * s.F8;
   if (dx) {
@@ -943,7 +1046,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
     g.part = b.pw.splits > 1 ? part : nullptr;
     product<T, kWeight>(g, b.pw, st);
     if (g.part)
-      sum_kernel<T><<<(unsigned)up(2 * s.F * s.D, kThreads), kThreads, 0, st>>>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, (T*)dwg, (T*)dwu);
+      sum_kernel<T><<<(unsigned)up(2 * s.F * s.D, 64), kThreads, 0, st>>>(part, (int)b.pw.splits, s.F8 * s.D, s.F * s.D, (T*)dwg, (T*)dwu);
   }
   return tsf_launch_status();
 }
