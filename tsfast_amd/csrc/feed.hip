@@ -17,8 +17,8 @@ using namespace tsf;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kK = 32;               // of a stage: the contraction of one matrix instruction
-constexpr int kStages = 4;           // stages in LDS: one is read, three are on their way
+constexpr int kK = 64;               // of a stage: a row's part is a whole 128-byte line
+constexpr int kSlots = 2;            // stages in LDS
 constexpr int kMaxSegs = 12;         // products whose sum is formed: 2 sources x 6 pairs of planes
 constexpr int64_t kMaxLd = 1 << 22;  // elements between the rows of an operand: 256 rows stay below 2^31 bytes
 
@@ -155,25 +155,25 @@ struct Tile {
   static constexpr int NQ = BQ / WQ / 16, NH = HP / WP / 16;  // 16-row blocks a wave has of q, and of each half of p
   static constexpr int kQBytes = BQ * kK * 2, kHBytes = HP * kK * 2, kStage = kQBytes + 2 * kHBytes;
   static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave a stage
-  static constexpr int kRow = HP * 4 + 16;               // bytes of a row of outputs in LDS, at most
-  static constexpr int kLds = kStages * kStage > BQ * kRow ? kStages * kStage : BQ * kRow;
+  static constexpr int kLds = kSlots * kStage, kOwn = kLds / kWaves;  // a wave's own part, once the products are done
+  static_assert(16 * (NH * 16 * 4 + 16) <= kOwn, "");
   static_assert(kStage % (1024 * kWaves) == 0 && kQBytes % 1024 == 0 && kHBytes % 1024 == 0, "");
 };
 
-// One 1 KB piece of a panel of ROWS rows (of q or p) x 32 k, by one wave straight into LDS. As it lies: 16 rows of 64 bytes, the four
-// 16-byte chunks of a row turned so that 8 and 16 consecutive rows' same chunk fall on different banks. Turned: rows of k.
+// One 1 KB piece of a panel of ROWS rows (of q or p) x 64 k, by one wave straight into LDS. As it lies: 8 rows of 128 bytes, the eight
+// 16-byte chunks of a row turned so that 16 rows' same chunk fall on different banks. Turned: rows of k.
 template <int ROWS, bool TURNED>
 struct Panel {
   static constexpr int kChunks = ROWS / 8;  // of a row of k
   static constexpr uint32_t kNone = 0x80000000u;
-  TSF_DEV static uint32_t swz(uint32_t r) { return (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 3) & 1); }
+  TSF_DEV static uint32_t swz(uint32_t r) { return (r >> 1) & 7; }
   TSF_DEV static uint32_t turn(uint32_t kr) { return (((kr & 3) << 1) | (((kr >> 3) & 1) << 3)) & (kChunks - 1); }
 
   uint32_t off, need;  // the lane's byte offset in a stage, and which of the stage's k it starts at
   // `unit`: which 1 KB; rows: of the panel that exist
   TSF_DEV void set(uint32_t unit, uint32_t lane, int64_t ld, uint32_t rows) {
     if constexpr (!TURNED) {
-      const uint32_t r = 16 * unit + (lane >> 2), c = (lane & 3) ^ swz(r & 15);
+      const uint32_t r = 8 * unit + (lane >> 3), c = (lane & 7) ^ swz(r & 15);
       off = (uint32_t)(r * ld * 2) + c * 16;
       need = r < rows ? c * 8 : ~0u;
     } else {
@@ -200,31 +200,32 @@ struct Panel {
   }
 };
 
-// The wave's operand blocks of a panel: 16 rows, 8 of the 32 k a lane.
+// The wave's operand blocks of a panel: 16 rows, 8 of the 32 k of a half stage a lane.
 template <int ROWS, bool TURNED>
 struct Reader {
   using P = Panel<ROWS, TURNED>;
-  uint32_t lane_off;
-  uint32_t t, b;  // turned: what the chunk is turned by, and the rest of the lane's offset
+  uint32_t at[2];   // as it lies: the lane's offset in 16 rows, for each half
+  uint32_t t, b, m;  // turned: what the chunk is turned by, and the rest of the lane's offset
   TSF_DEV void set(uint32_t li, uint32_t lg) {
     if constexpr (!TURNED) {
-      lane_off = li * 64 + ((lg ^ P::swz(li)) << 4);
+      at[0] = li * 128 + ((lg ^ P::swz(li)) << 4);
+      at[1] = li * 128 + (((4 + lg) ^ P::swz(li)) << 4);
     } else {
       const uint32_t r = 8 * lg + (li >> 2);
       t = P::turn(r);
       b = r * (ROWS * 2) + 8 * (li & 1);
-      lane_off = (li >> 1) & 1;
+      m = (li >> 1) & 1;
     }
   }
-  TSF_DEV bf16x8 get(const char* panel, uint32_t block) const {
+  TSF_DEV bf16x8 get(const char* panel, uint32_t block, int half) const {
     bf16x8 v;
     if constexpr (!TURNED) {
-      const u32x4 w = *(const u32x4*)(panel + block * 1024 + lane_off);
+      const u32x4 w = *(const u32x4*)(panel + block * 2048 + at[half]);
       __builtin_memcpy(&v, &w, 16);
     } else {
       // the transposing read: lane li of a group of 16 points at 4 columns of row li / 4 and receives its own column of the 4
-      // rows. Rows 4 further on are turned alike.
-      const char* p = panel + b + (((2 * block + lane_off) ^ t) << 4);
+      // rows. Rows 4 and 32 further on are turned alike.
+      const char* p = panel + half * 32 * ROWS * 2 + b + (((2 * block + m) ^ t) << 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const auto w = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
@@ -253,64 +254,59 @@ TSF_DEV void put4(char* p, f32x4 v) {
   }
 }
 
-// A half tile of outputs, from accumulators to LDS and from there to memory in whole rows. `row(q)`: the address of row q of the tile, or
-// null; n: columns that exist.
+// Between a wave's writes of LDS and its other lanes' reads
+TSF_DEV void wave_turned() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A wave's part of a half tile of outputs, from accumulators through LDS of the wave's own to memory in whole rows. `row(q)`: the address of
+// row q of the wave's rows, or null; n: columns that exist.
 template <typename C, typename T, typename V, typename R>
-TSF_DEV void store_half(char* lds, uint32_t wq, uint32_t wp, uint32_t li, uint32_t lg, int n, V value, R row) {
-  constexpr int kRow = C::HP * (int)sizeof(T) + 16;
-  static_assert(C::BQ * kRow <= C::kLds, "");
-  __syncthreads();
+TSF_DEV void store_rows(char* own, uint32_t lane, int n, V value, R row) {
+  constexpr int kCols = C::NH * 16, kRow = kCols * (int)sizeof(T) + 16;
+  constexpr int kPer = 16 / (int)sizeof(T), kPieces = kCols / kPer;
+  const uint32_t li = lane & 15, lg = lane >> 4;
 #pragma unroll
-  for (int j = 0; j < C::NQ; ++j)
+  for (int j = 0; j < C::NQ; ++j) {
 #pragma unroll
-    for (int i = 0; i < C::NH; ++i)
-      put4<T>(lds + ((wq * C::NQ + j) * 16 + li) * kRow + ((wp * C::NH + i) * 16 + 4 * lg) * sizeof(T), value(i, j));
-  __syncthreads();
-  constexpr int kPer = 16 / (int)sizeof(T), kRowPieces = C::HP / kPer;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < C::BQ * kRowPieces; e += C::TH) {
-    const int q = e / kRowPieces, c = (e % kRowPieces) * kPer;
-    T* to = row(q);
-    if (!to || c >= n) continue;
-    const char* from = lds + q * kRow + c * sizeof(T);
-    if (c + kPer <= n && ((uintptr_t)(to + c) & 15) == 0) {
-      *(u32x4*)(to + c) = *(const u32x4*)from;
-    } else {
+    for (int i = 0; i < C::NH; ++i) put4<T>(own + li * kRow + (i * 16 + 4 * lg) * sizeof(T), value(i, j));
+    wave_turned();
 #pragma unroll
-      for (int k = 0; k < kPer; ++k)
-        if (c + k < n) to[c + k] = ((const T*)from)[k];
+    for (int e = 0; e < (16 * kPieces + 63) / 64; ++e) {
+      const uint32_t at = lane + 64 * e, q = at / kPieces, c = at % kPieces * kPer;
+      if (16 * kPieces % 64 != 0 && q >= 16) break;
+      T* to = row(16 * j + (int)q);
+      if (!to || (int)c >= n) continue;
+      const char* from = own + q * kRow + c * sizeof(T);
+      if ((int)c + kPer <= n && ((uintptr_t)(to + c) & 15) == 0) {
+        __builtin_nontemporal_store(*(const u32x4*)from, (u32x4*)(to + c));
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if ((int)c + k < n) to[c + k] = ((const T*)from)[k];
+      }
     }
+    wave_turned();
   }
 }
 
 // What a training step's forward leaves for its backward: a and b in blocks of 16 rows x 16 columns as accumulators have them (four columns
-// a lane). fp32 as it is, 32 bytes a lane; for bf16 24 bits of each, in 16 bytes (the upper 16 bits of a's and b's) and 8 (the next 8):
-// rounded to bf16 they would cost the gradients as much again as the rounding of da and db.
-TSF_DEV uint32_t round24(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return (u & 0x7fffffffu) < 0x7f800000u ? u + 0x7fu + ((u >> 8) & 1) : u;  // to nearest even; infinities and NaN as they are
-}
+// a lane). fp32 as it is, 32 bytes a lane; for bf16 the upper 24 bits of each, in 16 bytes (the upper 16 bits of a's and b's) and 8 (the
+// next 8). Rounded to bf16 they would cost the gradients as much again as the rounding of da and db does; what is cut off here is below
+// 2^-15 of a value.
 template <typename T>
-TSF_DEV void save_pre(char* hi, char* lo, int64_t block, uint32_t lane, f32x4 a, f32x4 b) {
+TSF_DEV void save_pre(char* hi, char* lo, uint32_t lane, f32x4 a, f32x4 b) {
   if constexpr (sizeof(T) == 4) {
-    char* p = hi + (block * 64 + lane) * 32;
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, a), (u32x4*)p);
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, b), (u32x4*)(p + 16));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, a), (u32x4*)(hi + lane * 32));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, b), (u32x4*)(hi + lane * 32 + 16));
   } else {
-    uint32_t r[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = round24(a[e]), r[4 + e] = round24(b[e]);
-    u32x4 h;
-    u32x2 l;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x07060302);  // the upper halves
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t x = __builtin_amdgcn_perm(r[4 * k + 1], r[4 * k], 0x0c0c0501), y = __builtin_amdgcn_perm(r[4 * k + 3], r[4 * k + 2], 0x0c0c0501);
-      l[k] = x | y << 16;
-    }
-    __builtin_nontemporal_store(h, (u32x4*)(hi + (block * 64 + lane) * 16));
-    __builtin_nontemporal_store(l, (u32x2*)(lo + (block * 64 + lane) * 8));
+    const u32x4 x = __builtin_bit_cast(u32x4, a), y = __builtin_bit_cast(u32x4, b);
+    auto upper = [](uint32_t v1, uint32_t v0) { return __builtin_amdgcn_perm(v1, v0, 0x07060302); };
+    auto next = [](const u32x4& v) { return __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0501), __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0501), 0x05040100); };
+    __builtin_nontemporal_store(u32x4{upper(x[1], x[0]), upper(x[3], x[2]), upper(y[1], y[0]), upper(y[3], y[2])}, (u32x4*)(hi + lane * 16));
+    __builtin_nontemporal_store(u32x2{next(x), next(y)}, (u32x2*)(lo + lane * 8));
   }
 }
 template <typename T>
@@ -379,7 +375,6 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
   const int kq = (int)g.kq, kp = (int)g.kp, per_seg = (kq + kK - 1) / kK;
   const int begin = (int)(split * g.split_stages);
   const int count = (int)(g.stages - begin < g.split_stages ? g.stages - begin : g.split_stages);
-  const int rounds = (count + 1) / 2;  // two stages a round: one past the end adds zeros
   int to_load = count, seg = begin / per_seg, k0 = (begin % per_seg) * kK;
   const bf16 *qb, *pb[kHalves];
   auto enter = [&]() __attribute__((always_inline)) {
@@ -427,14 +422,14 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
   struct Blocks {
     bf16x8 q[NQ], p[2 * NH];
   };
-  // part j of a stage's blocks, of NQ: one of q and as many of p
-  constexpr int kPart = 2 * NH / NQ;
-  static_assert(kPart * NQ == 2 * NH && C::kLoads == NQ, "");
-  auto read_part = [&](Blocks& f, int buf, int j) __attribute__((always_inline)) {
-    const char* from = lds + buf * C::kStage;
+  // part j, of NQ, of the blocks of a half stage: one of q and as many of p
+  constexpr int kPart = 2 * NH / NQ, kEachLoads = C::kLoads / NQ;
+  static_assert(kPart * NQ == 2 * NH && kEachLoads * NQ == C::kLoads, "");
+  auto read_part = [&](Blocks& f, int slot, int half, int j) __attribute__((always_inline)) {
+    const char* from = lds + slot * C::kStage;
 #pragma unroll
-    for (int i = j * kPart; i < (j + 1) * kPart; ++i) f.p[i] = rp.get(from + C::kQBytes + (i / NH) * C::kHBytes, wp * NH + i % NH);
-    f.q[j] = rq.get(from, wq * NQ + j);
+    for (int i = j * kPart; i < (j + 1) * kPart; ++i) f.p[i] = rp.get(from + C::kQBytes + (i / NH) * C::kHBytes, wp * NH + i % NH, half);
+    f.q[j] = rq.get(from, wq * NQ + j, half);
   };
   f32x4 acc[2 * NH][NQ];
 #pragma unroll
@@ -442,15 +437,21 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
 #pragma unroll
     for (int j = 0; j < NQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // Stage t's blocks are in registers when its turn comes. Its products run while stage t + 1's blocks are read from LDS and
-  // stage t + 4 is loaded into the place that stage t has left; t + 2 and t + 3 are on their way. A wave issues in order, so loads and
-  // reads stand evenly between the products: in front of them, they would wait for the other waves' (2.1 -> 1.4 ms, see below).
-  auto stage = [&](const Blocks& now, Blocks& next, int load_to, int read_from) __attribute__((always_inline)) {
-    stage_barrier<2 * C::kLoads>();
+  auto load_stage = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < C::kLoads; ++i) load_piece(slot, i);
+  };
+  // A half stage: its products, from blocks in registers, while the next half's blocks are read from LDS and, in every second one, the
+  // stage after the next is loaded into the slot that this stage has left. A wave issues in order, so reads and loads stand evenly
+  // between the products: in front of them they would wait for the other waves' first.
+  auto half_stage = [&](const Blocks& now, Blocks& next, int read_slot, int half, auto loads, int load_slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-      load_piece(load_to, j);
-      read_part(next, read_from, j);
+      if (loads) {
+#pragma unroll
+        for (int i = 0; i < kEachLoads; ++i) load_piece(load_slot, j * kEachLoads + i);
+      }
+      read_part(next, read_slot, half, j);
 #pragma unroll
       for (int i = 0; i < 2 * NH; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(now.p[i], now.q[j], acc[i][j], 0, 0, 0);
       constexpr int kReads = (TQ ? 2 : 1) + kPart * (TP ? 2 : 1), kEach = 2 * NH / kReads > 0 ? 2 * NH / kReads : 1;
@@ -462,28 +463,30 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
       __builtin_amdgcn_sched_group_barrier(0x008, 2 * NH, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    advance();
   };
   Blocks f0, f1;
+  load_stage(0);
+  advance();
+  load_stage(1);
+  stage_barrier<C::kLoads>();
 #pragma unroll
-  for (int t = 0; t < kStages; ++t) {
-#pragma unroll
-    for (int j = 0; j < C::kLoads; ++j) load_piece(t, j);
+  for (int j = 0; j < NQ; ++j) read_part(f0, 0, 0, j);
+  for (int t = 0; t < count; ++t) {
+    const int slot = t & 1;
+    half_stage(f0, f1, slot, 1, std::false_type(), 0);
     advance();
-  }
-  stage_barrier<3 * C::kLoads>();
-#pragma unroll
-  for (int j = 0; j < NQ; ++j) read_part(f0, 0, j);
-  int buf = 0;
-  for (int r = 0; r < rounds; ++r) {
-    stage(f0, f1, buf, buf + 1);
-    stage(f1, f0, buf + 1, (buf + 2) & 3);
-    buf = (buf + 2) & 3;
+    stage_barrier<0>();  // this stage's slot has been read, the next one's is loaded
+    half_stage(f1, f0, slot ^ 1, 0, std::true_type(), slot);
   }
   stage_barrier<0>();
 
+  char* own = lds + wave * C::kOwn;
+  auto left = [&](uint32_t columns) { return (int)columns - (int)(wp * NH * 16); };  // of the wave's columns of a half that exist
   if constexpr (FORM == kForward) {
     const T *bg = (const T*)g.bg, *bu = (const T*)g.bu;
+    // the wave's first block of 16 rows and of 16 columns, and where a training step keeps it
+    const int64_t rb = q0 / 16 + wq * NQ, cb = p0 / 16 + wp * NH, all_rb = (g.nq + 15) / 16, block0 = rb * g.save_fb + cb;
+    char *hi = g.save_hi + block0 * (sizeof(T) == 2 ? 1024 : 2048), *lo = g.save_lo + block0 * 512;
     auto finish = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NH; ++i) {
@@ -500,9 +503,9 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
           f32x4& b = acc[NH + i][j];
           a += va;
           b += vb;
-          if (g.train) {
-            const int64_t mb = q0 / 16 + wq * NQ + j, fb = p0 / 16 + wp * NH + i;
-            if (mb * 16 < g.nq && fb < g.save_fb) save_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + fb, lane, a, b);
+          if (g.train && rb + j < all_rb && cb + i < g.save_fb) {
+            const int64_t block = j * g.save_fb + i;
+            save_pre<T>(hi + block * (sizeof(T) == 2 ? 1024 : 2048), lo + block * 512, lane, a, b);
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -520,27 +523,26 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
       finish(std::integral_constant<int, kGelu>());
     else
       finish(std::integral_constant<int, kSigmoid>());
-    T* y = (T*)g.y;
-    store_half<C, T>(lds, wq, wp, li, lg, (int)rows_0, [&](int i, int j) { return acc[i][j]; },
-                     [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + p0 : (T*)nullptr; });
+    const int64_t c0 = p0 + wp * NH * 16;
+    T* y = (T*)g.y + (q0 + wq * NQ * 16) * g.np + c0;
+    store_rows<C, T>(own, lane, left(rows_0), [&](int i, int j) { return acc[i][j]; },
+                     [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * g.np : (T*)nullptr; });
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t c0 = h ? p1 : p0;
-      const int n = (int)(h ? rows_1 : rows_0);
+      const int64_t c0 = (h ? p1 : p0) + wp * NH * 16, r0 = q0 + wq * NQ * 16;
+      const int n = left(h ? rows_1 : rows_0);
       auto value = [&](int i, int j) { return acc[h * NH + i][j]; };
-      if (FORM == kInput) {
-        T* y = (T*)g.y;
-        store_half<C, T>(lds, wq, wp, li, lg, n, value, [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + c0 : (T*)nullptr; });
-      } else if (g.part) {
-        float* y = g.part + (int64_t)split * g.nq * g.np;
-        store_half<C, float>(lds, wq, wp, li, lg, n, value,
-                             [&](int q) { return (uint32_t)q < rows_q ? y + (q0 + q) * g.np + c0 : (float*)nullptr; });
+      if (FORM == kInput || g.part) {
+        using O = std::conditional_t<FORM == kInput, T, float>;
+        O* y = FORM == kInput ? (O*)g.y : (O*)(g.part + (int64_t)split * g.nq * g.np);
+        y += r0 * g.np + c0;
+        store_rows<C, O>(own, lane, n, value, [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * g.np : (O*)nullptr; });
       } else {
-        store_half<C, T>(lds, wq, wp, li, lg, n, value, [&](int q) {
-          const int64_t r = q0 + q, in = r < g.half_rows ? r : r - g.half_rows;
+        store_rows<C, T>(own, lane, n, value, [&](int q) {
+          const int64_t r = r0 + q, in = r < g.half_rows ? r : r - g.half_rows;
           T* y = (T*)(r < g.half_rows ? g.y : g.y1);
-          return (uint32_t)q < rows_q && in < g.valid_rows ? y + in * g.np + c0 : (T*)nullptr;
+          return (uint32_t)q + wq * NQ * 16 < rows_q && in < g.valid_rows ? y + in * g.np + c0 : (T*)nullptr;
         });
       }
     }
@@ -578,12 +580,6 @@ struct Turn {
     } else {
       return __builtin_bit_cast(f32x4, *(const u32x4*)(at + li * kRow + c * 4));
     }
-  }
-  // between a wave's writes and its other lanes' reads
-  TSF_DEV static void turned() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 };
 
@@ -627,11 +623,11 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
       if (i < blocks) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + i, lane, a[i], b[i]);
 #pragma unroll
     for (int e = 0; e < kDy; ++e) turn.dy.put_piece(lane, e, in[e]);
-    Turn<T>::turned();
+    wave_turned();
     f32x4 dy[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) dy[i] = turn.dy.get_four(li, 16 * i + 4 * lg);
-    Turn<T>::turned();
+    wave_turned();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i >= blocks) a[i] = b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -658,7 +654,7 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
           for (int e = 0; e < 4; ++e) a[i][e] = split_rest(a[i][e]), b[i][e] = split_rest(b[i][e]);
         }
       }
-      Turn<T>::turned();
+      wave_turned();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t m = m0 + Turn<bf16>::row(lane, e), f = f0 + Turn<bf16>::col(lane, e);
@@ -668,7 +664,7 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
           *(u32x4*)(to + g.F8) = turn.d[1].get_piece(lane, e);
         }
       }
-      Turn<T>::turned();
+      wave_turned();
     }
   }
   if (!g.part) return;
