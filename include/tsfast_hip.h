@@ -451,8 +451,8 @@ int tsfast_hip_feed_bwd(int64_t rows, int64_t D, int64_t F, int dtype, int activ
  *   NULL) of weight_dtype and bias_dtype. 2 <= K <= 8.
  * mamba_packed: the scan of tsfast_hip_mamba_fwd over each sequence, from h0 [S, D, N] (NULL: zeros) to h_last, float32. N <= 64.
  * mamba_step:   conv, x_proj [R + 2 N, D], dt_proj [D, R] with dt_bias [D] (or NULL), softplus, scan step, D skip and gate of one token x, z
- *   [B, D]; conv_state [B, D, K - 1] of io_dtype and ssm_state [B, D, N] float32 are overwritten. param_dtypes (host memory): the types of
- *   conv_weight, conv_bias, x_proj, dt_proj, dt_bias. 2 <= K <= 8, N <= 64, R + 2 N <= 2048.
+ *   [B, D]; conv_state [B, D, K - 1] of io_dtype and ssm_state [B, D, N] float32 are overwritten. param_dtype: the type of
+ *   conv_weight, conv_bias (or NULL), x_proj and dt_proj. 2 <= K <= 8, N <= 64, R + 2 N <= 1024.
  */
 int tsfast_hip_conv_packed(int64_t T, int64_t S, int64_t D, int64_t K, int io_dtype, int starts_int64, int weight_dtype,
                            int bias_dtype, const void* x, int64_t x_stride, const void* starts, const void* tails,
@@ -464,8 +464,8 @@ int tsfast_hip_mamba_packed(int64_t T, int64_t S, int64_t D, int64_t N, int io_d
                             const float* Dp, const void* starts, const float* h0, void* out, float* h_last, void* workspace,
                             int64_t workspace_bytes, void* stream);
 int64_t tsfast_hip_mamba_step_workspace_bytes(int64_t B, int64_t D, int64_t N, int64_t R, int64_t K);
-int tsfast_hip_mamba_step(int64_t B, int64_t D, int64_t N, int64_t R, int64_t K, int io_dtype, const int* param_dtypes,
-                          const void* x, int64_t x_stride, const void* z, int64_t z_stride, void* conv_state,
+int tsfast_hip_mamba_step(int64_t B, int64_t D, int64_t N, int64_t R, int64_t K, int io_dtype, int param_dtype,
+                          int dt_bias_dtype, const void* x, int64_t x_stride, const void* z, int64_t z_stride, void* conv_state,
                           float* ssm_state, const void* conv_weight, const void* conv_bias, const void* x_proj,
                           const void* dt_proj, const void* dt_bias, const float* A, const float* Dp, void* out,
                           void* workspace, int64_t workspace_bytes, void* stream);

@@ -163,11 +163,8 @@ def test_abi_refuses_before_any_launch():
         T, S, D, N, io, 0, draw, 8, A, p, 4, p, 4, p, 8, p, sz, p, p, None, p, last, ws, n, None)
     assert scan(N=0) == scan(io=3) == scan(sz=-1) == scan(A=None) == scan(draw=None) == scan(last=None) == -1
     assert scan(N=65) == -3 and scan(D=0) == 0 and scan(T=65536, D=256, N=16) == -2 == scan(T=65536, D=256, N=16, ws=p, n=100)
-    import ctypes
-
-    types = (ctypes.c_int * 5)()
-    step = lambda B=2, D=8, N=4, R=2, K=4, io=0, t=types, x=p, h=p, ws=p, n=0: lib.tsfast_hip_mamba_step(  # noqa: E731
-        B, D, N, R, K, io, t, x, 8, p, 8, p, h, p, None, p, p, None, p, p, p, ws, n, None)
-    assert step(B=-1) == step(R=0) == step(K=1) == step(io=2) == step(t=None) == step(x=None) == step(h=None) == -1
-    assert step(K=9) == step(N=65) == step(R=2041) == -3 and step(B=0) == 0 and step() == step(ws=None, n=1 << 20) == -2
+    step = lambda B=2, D=8, N=4, R=2, K=4, io=0, pt=0, bt=0, x=p, h=p, ws=p, n=0: lib.tsfast_hip_mamba_step(  # noqa: E731
+        B, D, N, R, K, io, pt, bt, x, 8, p, 8, p, h, p, None, p, p, None, p, p, p, ws, n, None)
+    assert step(B=-1) == step(R=0) == step(K=1) == step(io=2) == step(pt=2) == step(bt=-1) == step(x=None) == step(h=None) == -1
+    assert step(K=9) == step(N=65) == step(R=1017) == -3 and step(B=0) == 0 and step() == step(ws=None, n=1 << 20) == -2
     assert lib.tsfast_hip_mamba_step_workspace_bytes(2, 8, 4, 2, 4) >= 2 * 10 * 4

@@ -111,7 +111,7 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
         _int,
     ),
     "tsfast_hip_mamba_step_workspace_bytes": ([_i64] * 5, _i64),
-    "tsfast_hip_mamba_step": ([_i64] * 5 + [_int, _ptr] + [_ptr, _i64] * 2 + [_ptr] * 11 + [_i64, _ptr], _int),
+    "tsfast_hip_mamba_step": ([_i64] * 5 + [_int] * 3 + [_ptr, _i64] * 2 + [_ptr] * 11 + [_i64, _ptr], _int),
     "tsfast_hip_mat_adjoint_workspace_bytes": ([_i64] * 4, _i64),
     "tsfast_hip_mat_adjoint_bounds": ([_i64] * 4 + [_ptr] * 4 + [_i64, _ptr], _int),
 }

@@ -685,23 +685,41 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   }
 }
 
-// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in a fixed order: 64 columns a
-// workgroup, every fourth part a wave.
-template <typename T>
+// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in a fixed order: VL columns a lane,
+// every fourth part a wave. VL > 1: n and stride are multiples of it.
+template <typename T, int VL>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int parts, int64_t stride, int64_t n, T* out0, T* out1) {
-  __shared__ float sums[4][64];
+  __shared__ float sums[4][64][VL];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = (int64_t)blockIdx.x * 64 + lane, h = i >= n, c = i - h * n;
-  float s = 0.0f;
+  const int64_t i = ((int64_t)blockIdx.x * 64 + lane) * VL, h = i >= n, c = i - h * n;
+  float s[VL];
+#pragma unroll
+  for (int e = 0; e < VL; ++e) s[e] = 0.0f;
   if (i < 2 * n) {
     const float* p = part + h * stride + c;
-#pragma unroll 8
-    for (int k = wave; k < parts; k += 4) s += p[(int64_t)k * 2 * stride];
+#pragma unroll 4
+    for (int k = wave; k < parts; k += 4) {
+      float v[VL];
+      __builtin_memcpy(v, __builtin_assume_aligned(p + (int64_t)k * 2 * stride, 4 * VL), sizeof(v));
+#pragma unroll
+      for (int e = 0; e < VL; ++e) s[e] += v[e];
+    }
   }
-  sums[wave][lane] = s;
+#pragma unroll
+  for (int e = 0; e < VL; ++e) sums[wave][lane][e] = s[e];
   __syncthreads();
   T* out = h ? out1 : out0;
-  if (wave == 0 && i < 2 * n && out) out[c] = from_f32<T>((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
+  if (wave == 0 && i < 2 * n && out) {
+#pragma unroll
+    for (int e = 0; e < VL; ++e) out[c + e] = from_f32<T>((sums[0][lane][e] + sums[1][lane][e]) + (sums[2][lane][e] + sums[3][lane][e]));
+  }
+}
+template <typename T>
+void sum_parts(const float* part, int64_t parts, int64_t stride, int64_t n, void* out0, void* out1, hipStream_t st) {
+  if (n % 4 == 0 && stride % 4 == 0)
+    sum_kernel<T, 4><<<(unsigned)((2 * n + 255) / 256), kThreads, 0, st>>>(part, (int)parts, stride, n, (T*)out0, (T*)out1);
+  else
+    sum_kernel<T, 1><<<(unsigned)((2 * n + 63) / 64), kThreads, 0, st>>>(part, (int)parts, stride, n, (T*)out0, (T*)out1);
 }
 
 // --------------------------------------------------------------------------------- a few rows
@@ -725,15 +743,21 @@ TSF_DEV f32x4 mma(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
   for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[e], b.hi[e], c, 0, 0, 0);
   return c;
 }
-// 8 values of a row, the first n of them, zeros after; `in`: the row exists
-template <typename T>
-TSF_DEV Frag<T> load8(const T* p, int64_t n, bool in) {
+// 8 values of a row, the first n of them, zeros after. WHOLE: 8 or none; then loads are unconditional, from k = 0 where there are none: a load
+// under a condition is waited for before the next one starts.
+template <bool WHOLE, typename T>
+TSF_DEV Frag<T> load8(const T* row, int64_t k, int64_t n) {
   T v[8];
-  if (in && n >= 8) {
-    __builtin_memcpy(v, p, sizeof(v));
+  if constexpr (WHOLE) {
+    __builtin_memcpy(v, row + (n > 0 ? k : 0), sizeof(v));
+    uint32_t w[sizeof(v) / 4];
+    __builtin_memcpy(w, v, sizeof(v));
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(v) / 4); ++e) w[e] = n > 0 ? w[e] : 0;
+    __builtin_memcpy(v, w, sizeof(v));
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = in && e < n ? p[e] : from_f32<T>(0.0f);
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? row[k + e] : from_f32<T>(0.0f);
   }
   Frag<T> f;
   __builtin_memcpy(&f, v, sizeof(v));
@@ -747,25 +771,29 @@ struct FewArgs {
   int act;
 };
 
-template <typename T, int NT>
+template <typename T, int NT, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs g) {
   __shared__ f32x4 sums[4][2 * NT][64];
   const uint32_t tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4, wave = tid >> 6;
   const int64_t f0 = (int64_t)blockIdx.x * 16;
-  const bool fin = f0 + li < g.F;
-  const T *wg = (const T*)g.wg + (f0 + li) * g.ldg, *wu = (const T*)g.wu + (f0 + li) * g.ldu;
-  const T* x = (const T*)g.x + li * g.ldx;
+  // rows and columns that do not exist repeat the last one: their sums are not used
+  const int64_t f = f0 + li < g.F ? f0 + li : g.F - 1;
+  const T *wg = (const T*)g.wg + f * g.ldg, *wu = (const T*)g.wu + f * g.ldu;
+  const T* x[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) x[t] = (const T*)g.x + (16 * t + li < g.rows ? 16 * t + li : g.rows - 1) * g.ldx;
   f32x4 acc[2][NT];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[h][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int64_t k = 32 * wave + 8 * lg; k - 8 * lg < g.D; k += 128) {
-    const Frag<T> a = load8(wg + k, g.D - k, fin), b = load8(wu + k, g.D - k, fin);
+  for (int64_t k0 = 32 * wave; k0 < g.D; k0 += 128) {
+    const int64_t k = k0 + 8 * lg, n = g.D - k;
+    const Frag<T> a = load8<WHOLE>(wg, k, n), b = load8<WHOLE>(wu, k, n);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const Frag<T> v = load8(x + 16 * t * g.ldx + k, g.D - k, 16 * t + li < g.rows);
+      const Frag<T> v = load8<WHOLE>(x[t], k, n);
       acc[0][t] = mma(a, v, acc[0][t]);
       acc[1][t] = mma(b, v, acc[1][t]);
     }
@@ -777,9 +805,9 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs g) {
   __syncthreads();
   // a thread has column tid % 16 of row tid / 16 of each tile of rows: element (column 4 l + e, row li) of lane 16 l + li
   const uint32_t c = tid & 15, r = tid >> 4;
-  const int64_t f = f0 + c;
-  if (f >= g.F) return;
-  const float ba = g.bg ? to_f32(((const T*)g.bg)[f]) : 0.0f, bb = g.bu ? to_f32(((const T*)g.bu)[f]) : 0.0f;
+  const int64_t column = f0 + c;
+  if (column >= g.F) return;
+  const float ba = g.bg ? to_f32(((const T*)g.bg)[column]) : 0.0f, bb = g.bu ? to_f32(((const T*)g.bu)[column]) : 0.0f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t row = 16 * t + r;
@@ -790,7 +818,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs g) {
       const uint32_t at = (c >> 2) * 16 + r, e = c & 3;
       v[h] = (sums[0][h * NT + t][at][e] + sums[1][h * NT + t][at][e]) + (sums[2][h * NT + t][at][e] + sums[3][h * NT + t][at][e]);
     }
-    ((T*)g.y)[row * g.F + f] = from_f32<T>(activate(g.act, v[0] + ba) * (v[1] + bb));
+    ((T*)g.y)[row * g.F + column] = from_f32<T>(activate(g.act, v[0] + ba) * (v[1] + bb));
   }
 }
 
@@ -942,10 +970,9 @@ int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void*
   if (s.rows <= kFewRows && !pre) {
     FewArgs a = {c.x, c.wg, c.wu, bg, bu, y, s.rows, s.D, s.F, c.ldx, c.ldg, c.ldu, act};
     const unsigned grid = (unsigned)up(s.F, 16);
-    if (s.rows <= 16)
-      few_kernel<T, 1><<<grid, kThreads, 0, st>>>(a);
-    else
-      few_kernel<T, 2><<<grid, kThreads, 0, st>>>(a);
+    auto* const kernel = s.rows <= 16 ? (s.D % 8 == 0 ? few_kernel<T, 1, true> : few_kernel<T, 1, false>)
+                                      : (s.D % 8 == 0 ? few_kernel<T, 2, true> : few_kernel<T, 2, false>);
+    kernel<<<grid, kThreads, 0, st>>>(a);
     return tsf_launch_status();
   }
   Operands o = operands_of(s, c);
@@ -1013,7 +1040,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
   a.dy = dy, a.ld_dy = ld_dy, a.rows = s.rows, a.F = s.F, a.F8 = s.F8, a.save_fb = up(s.F, 16), a.blocks = b.blocks;
   a.save_hi = pre, a.save_lo = pre_lo(const_cast<char*>(pre), s.rows, s.F), a.d = d, a.part = want_bias ? bias : nullptr;
   launch_adjoint<T>(a, act, dim3((unsigned)up(s.F, 64), (unsigned)b.wgs), st);
-  if (want_bias) sum_kernel<T><<<(unsigned)up(2 * s.F, 64), kThreads, 0, st>>>(bias, (int)b.wgs, s.F, s.F, (T*)dbg, (T*)dbu);
+  if (want_bias) sum_parts<T>(bias, b.wgs, s.F, s.F, dbg, dbu, st);
 
   const int64_t plane = s.rows * 2 * s.F8;
   if (dx) {
@@ -1041,8 +1068,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
     g.segs = s.pairs, g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
     g.part = b.pw.splits > 1 ? part : nullptr;
     product<T, kWeight>(g, b.pw, st);
-    if (g.part)
-      sum_kernel<T><<<(unsigned)up(2 * s.F * s.D, 64), kThreads, 0, st>>>(part, (int)b.pw.splits, s.F8 * s.D, s.F * s.D, (T*)dwg, (T*)dwu);
+    if (g.part) sum_parts<T>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, dwg, dwu, st);
   }
   return tsf_launch_status();
 }

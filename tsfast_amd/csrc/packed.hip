@@ -21,28 +21,61 @@ constexpr int kMaxK = 8;
 struct Starts {
   const void* p;
   int wide;  // int64, else int32
-  int64_t S, T;
+  int S, T;
   // where sequence s begins (s = S: where the last one ends), within the tokens there are
-  TSF_DEV int64_t at(int64_t s) const {
+  TSF_DEV int at(int64_t s) const {
     const int64_t v = wide ? ((const int64_t*)p)[s] : (int64_t)((const int32_t*)p)[s];
-    return v < 0 ? 0 : v > T ? T : v;
+    return v < 0 ? 0 : v > T ? T : (int)v;
   }
-  // the sequence of token t: the last one that begins at or before it; -1: none yet, S: behind the last one
-  TSF_DEV int64_t of(int64_t t) const {
-    int64_t lo = 0, hi = S + 1;  // the first start behind t is in [lo, hi]
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (at(mid) <= t)
-        lo = mid + 1;
-      else
-        hi = mid;
+};
+
+// A token's sequence: the last one that begins at or before it (so it is not empty); -1: none yet, S: behind the last one. Where it begins
+// and ends: before and behind the sequences, where no token has one.
+struct Cursor {
+  int s, begin, end;
+  // for a token of each lane; all lanes of a wave call. Up to 64 starts come with one load of the wave (a search is a chain of loads)
+  TSF_DEV void find(const Starts& st, int t, int lane) {
+    if (st.S < 64) {
+      const int mine = st.at(lane < st.S ? lane : st.S);
+      int count = 0;
+      for (int l = 0; l <= st.S; ++l) count += __builtin_amdgcn_readlane(mine, l) <= t;
+      s = count - 1;
+      begin = s < 0 ? 0 : __shfl(mine, s < 0 ? 0 : s, kWave);
+      end = __shfl(mine, s < st.S ? s + 1 : st.S, kWave);
+    } else {
+      int lo = 0, hi = st.S + 1;  // the first start behind t is in [lo, hi]
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (st.at(mid) <= t)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      s = lo - 1;
+      begin = s < 0 ? 0 : st.at(s);
+      end = st.at(s < st.S ? s + 1 : st.S);
     }
-    return lo - 1;
+    if (s >= st.S) end = st.T;
+  }
+  // the same token in all lanes: scalar registers
+  TSF_DEV void find_uniform(const Starts& st, int t, int lane) {
+    find(st, t, lane);
+    s = __builtin_amdgcn_readfirstlane(s), begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+  }
+  TSF_DEV bool has(const Starts& st) const { return s >= 0 && s < st.S; }
+  // to the next sequence that is not over at t, or behind the last one; the present one is over
+  TSF_DEV void next(const Starts& st, int t) {
+    do {
+      ++s;
+      begin = end;
+      end = s < st.S ? st.at(s + 1) : st.T;
+    } while (s < st.S && end <= t);
   }
 };
 
 // ------------------------------------------------------------------------------------ convolution
-// A thread has 16 bytes of channels (8 bf16, 4 fp32) and kRun tokens, with the last K - 1 inputs in registers.
+// A thread has 16 bytes of channels (8 bf16, 4 fp32) and kRun tokens. Where no sequence begins or ends within or right before them, all of its
+// rows are loaded at once; elsewhere it goes token by token.
 constexpr int kRun = 16;
 struct ConvArgs {
   const void *x, *tails, *weight, *bias;
@@ -83,87 +116,116 @@ template <typename T, int K>
 __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
   constexpr int VL = 16 / (int)sizeof(T);
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t run = i / g.groups, c0 = (i % g.groups) * VL, T_all = g.starts.T, S = g.starts.S;
-  const int n = (int)(g.D - c0 < VL ? g.D - c0 : VL);
+  const int64_t run = i / g.groups, c0 = (i % g.groups) * VL;
+  const int n = (int)(g.D - c0 < VL ? g.D - c0 : VL), S = g.starts.S, T_all = g.starts.T;
   const T *x = (const T*)g.x + c0, *tails = (const T*)g.tails;
   T *out = (T*)g.out + c0, *tails_out = (T*)g.tails_out;
+  const int t0 = run < g.runs ? (int)run * kRun : 0, t1 = t0 + kRun < T_all ? t0 + kRun : T_all;
+  Cursor at;
+  at.find(g.starts, t0, threadIdx.x & 63);
   if (run >= g.runs) {  // an empty sequence leaves what it was given
     const int64_t s = run - g.runs;
     if (s >= S || g.starts.at(s + 1) > g.starts.at(s)) return;
-    const int64_t at = (s * g.D + c0) * (K - 1);
-    for (int e = 0; e < n * (K - 1); ++e) tails_out[at + e] = tails ? tails[at + e] : from_f32<T>(0.0f);
+    const int64_t to = (s * g.D + c0) * (K - 1);
+    for (int e = 0; e < n * (K - 1); ++e) tails_out[to + e] = tails ? tails[to + e] : from_f32<T>(0.0f);
     return;
   }
-  float w[K][VL], b[VL], past[K - 1][VL];  // past[k]: the input K - 1 - k tokens ago
+  float w[K][VL], b[VL];
 #pragma unroll
   for (int e = 0; e < VL; ++e) {
-    b[e] = g.bias && e < n ? param(g.bias, c0 + e, g.b_bf16) : 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][e] = e < n ? param(g.weight, (c0 + e) * K + k, g.w_bf16) : 0.0f;
+    const int64_t c = c0 + (e < n ? e : n - 1);
+    b[e] = g.bias ? param(g.bias, c, g.b_bf16) : 0.0f;
   }
-  const int64_t t0 = run * kRun, t1 = t0 + kRun < T_all ? t0 + kRun : T_all;
-  int64_t s = g.starts.of(t0);
-  int64_t begin = s < 0 ? 0 : g.starts.at(s), end = s < S ? g.starts.at(s + 1) : T_all;
-  if (s < 0) end = g.starts.at(0);
-  // tail value k of sequence s
+  if (g.w_bf16) {
+#pragma unroll
+    for (int e = 0; e < VL; ++e)
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[k][e] = to_f32(((const bf16*)g.weight)[(c0 + (e < n ? e : n - 1)) * K + k]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VL; ++e)
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[k][e] = ((const float*)g.weight)[(c0 + (e < n ? e : n - 1)) * K + k];
+  }
+  if (at.has(g.starts) && at.begin <= t0 - (K - 1) && at.end > t1 && t1 - t0 == kRun && n == VL) {
+    T rows[kRun + K - 1][VL];
+#pragma unroll
+    for (int k = 0; k < kRun + K - 1; ++k) __builtin_memcpy(rows[k], x + (int64_t)(t0 - (K - 1) + k) * g.sx, sizeof(rows[k]));
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      float y[VL];
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+        float a = b[e];
+#pragma unroll
+        for (int j = 0; j < K; ++j) a = fmaf(w[j][e], to_f32(rows[k + j][e]), a);
+        y[e] = a * sigmoid_fast(a);
+      }
+      store_row<T, VL>(out + (int64_t)(t0 + k) * g.D, y, VL);
+    }
+    return;
+  }
+  float past[K - 1][VL] = {};  // past[k]: the input K - 1 - k tokens ago
+  // tail value k of the present sequence
   auto carried = [&](int k, int e) __attribute__((always_inline)) {
-    return tails && e < n ? to_f32(tails[(s * g.D + c0 + e) * (K - 1) + k]) : 0.0f;
+    return tails && e < n ? to_f32(tails[((int64_t)at.s * g.D + c0 + e) * (K - 1) + k]) : 0.0f;
   };
-  if (s >= 0 && s < S) {
+  if (at.has(g.starts)) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-      const int64_t t = t0 - (K - 1) + k;
-      if (t >= begin) {
-        load_row<T, VL>(past[k], x + t * g.sx, n);
+      const int t = t0 - (K - 1) + k;
+      if (t >= at.begin) {
+        load_row<T, VL>(past[k], x + (int64_t)t * g.sx, n);
       } else {
-        const int64_t from = t - begin + (K - 1);  // in [0, K - 1): t >= t0 - (K - 1) >= begin - (K - 1)
+        const int from = t - at.begin + (K - 1);  // in [0, K - 1): t0 >= begin
 #pragma unroll
-        for (int e = 0; e < VL; ++e) past[k][e] = carried((int)from, e);
+        for (int e = 0; e < VL; ++e) past[k][e] = carried(from, e);
       }
     }
   }
-  for (int64_t t = t0; t < t1; ++t) {
-    if (t >= end) {  // the next sequence that is not empty begins here, or none
-      do {
-        ++s;
-        begin = end;
-        end = s < S ? g.starts.at(s + 1) : T_all;
-      } while (s < S && end <= t);
-      if (s < S) {
+  T rows[kRun][VL];  // all at once: a row that does not exist repeats the last one
+  if (n == VL) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k)
+    for (int i = 0; i < kRun; ++i) __builtin_memcpy(rows[i], x + (int64_t)(t0 + i < T_all ? t0 + i : T_all - 1) * g.sx, sizeof(rows[i]));
+  } else {
 #pragma unroll
-          for (int e = 0; e < VL; ++e) past[k][e] = carried(k, e);
+    for (int i = 0; i < kRun; ++i)
+#pragma unroll
+      for (int e = 0; e < VL; ++e) rows[i][e] = x[(int64_t)(t0 + i < T_all ? t0 + i : T_all - 1) * g.sx + (e < n ? e : n - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    const int t = t0 + i;
+    if (t < t1) {
+      if (t >= at.end) {
+        at.next(g.starts, t);
+        if (at.has(g.starts)) {
+#pragma unroll
+          for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int e = 0; e < VL; ++e) past[k][e] = carried(k, e);
+        }
       }
-    }
-    float y[VL];
-    if (s < 0 || s >= S) {
+      const bool has = at.has(g.starts);
+      float y[VL];
 #pragma unroll
-      for (int e = 0; e < VL; ++e) y[e] = 0.0f;
-      store_row<T, VL>(out + t * g.D, y, n);
-      continue;
-    }
-    float now[VL];
-    load_row<T, VL>(now, x + t * g.sx, n);
+      for (int e = 0; e < VL; ++e) {
+        float a = b[e];
 #pragma unroll
-    for (int e = 0; e < VL; ++e) {
-      float a = b[e];
+        for (int k = 0; k < K - 1; ++k) a = fmaf(w[k][e], past[k][e], a);
+        a = fmaf(w[K - 1][e], to_f32(rows[i][e]), a);
+        y[e] = has ? a * sigmoid_fast(a) : 0.0f;
 #pragma unroll
-      for (int k = 0; k < K - 1; ++k) a = fmaf(w[k][e], past[k][e], a);
-      a = fmaf(w[K - 1][e], now[e], a);
-      y[e] = a * sigmoid_fast(a);
-    }
-    store_row<T, VL>(out + t * g.D, y, n);
+        for (int k = 0; k < K - 1; ++k) past[k][e] = k + 1 < K - 1 ? past[k + 1 < K - 1 ? k + 1 : k][e] : to_f32(rows[i][e]);
+      }
+      store_row<T, VL>(out + (int64_t)t * g.D, y, n);
+      if (has && t == at.end - 1) {
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k)
+        for (int e = 0; e < VL; ++e)
 #pragma unroll
-      for (int e = 0; e < VL; ++e) past[k][e] = k + 1 < K - 1 ? past[k + 1 < K - 1 ? k + 1 : k][e] : now[e];
-    if (t == end - 1) {
-#pragma unroll
-      for (int e = 0; e < VL; ++e)
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k)
-          if (e < n) tails_out[(s * g.D + c0 + e) * (K - 1) + k] = from_f32<T>(past[k][e]);
+          for (int k = 0; k < K - 1; ++k)
+            if (e < n) tails_out[((int64_t)at.s * g.D + c0 + e) * (K - 1) + k] = from_f32<T>(past[k][e]);
+      }
     }
   }
 }
@@ -194,11 +256,12 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
   __shared__ float2 s_bc[kTok][4 * NPT];     // B, C
   __shared__ float s_y[MAP ? 1 : kTok][4][kCh];  // each wave's sum over its states
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t tile = blockIdx.x % g.tiles, seg = blockIdx.x / g.tiles, d = tile * kCh + lane, S = g.starts.S, T_all = g.starts.T;
+  const int64_t tile = blockIdx.x % g.tiles, seg = blockIdx.x / g.tiles, d = tile * kCh + lane;
+  const int S = g.starts.S, T_all = g.starts.T;
   const int N = g.N, n0 = wave * NPT;
   const bool act = d < g.D;
-  int64_t t0 = seg * g.seg_len;
-  const int64_t t1 = t0 + g.seg_len < T_all ? t0 + g.seg_len : T_all;
+  int t0 = (int)(seg * g.seg_len);
+  const int t1 = t0 + g.seg_len < T_all ? (int)(t0 + g.seg_len) : T_all;
 
   float A2[NPT], h[NPT];
 #pragma unroll
@@ -213,30 +276,27 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
       if (act && n0 + j < N) g.h_last[(s * g.D + d) * N + n0 + j] = h[j];
   };
 
-  int64_t s, end;  // the sequence of the present token, and its end
+  Cursor at;
   bool whole = false;
   if (MAP) {
     // the sequence that goes on in the next segment, if one does
-    s = g.starts.of(t1 - 1);
-    if (s < 0 || s >= S || t1 >= T_all || g.starts.at(s + 1) <= t1) return;
-    const int64_t begin = g.starts.at(s);
-    whole = begin < t0;  // the segment lies within the sequence
+    at.find_uniform(g.starts, t1 - 1, lane);
+    if (!at.has(g.starts) || t1 >= T_all || at.end <= t1) return;
+    whole = at.begin < t0;  // the segment lies within the sequence
     if (!whole) {
-      t0 = begin;
-      begin_state(s);
+      t0 = at.begin;
+      begin_state(at.s);
     }
-    end = g.starts.at(s + 1);
   } else {
     // sequences without a token leave what they were given
     for (int64_t e = seg; e < S; e += g.segs)
       if (g.starts.at(e + 1) <= g.starts.at(e)) begin_state(e), end_state(e);
-    s = g.starts.of(t0);
-    end = s < 0 ? g.starts.at(0) : s < S ? g.starts.at(s + 1) : T_all;
+    at.find_uniform(g.starts, t0, lane);
 #pragma unroll
     for (int j = 0; j < NPT; ++j) h[j] = 0.0f;
-    if (s >= 0 && s < S) {
-      if (g.starts.at(s) == t0) {
-        begin_state(s);
+    if (at.has(g.starts)) {
+      if (at.begin == t0) {
+        begin_state(at.s);
       } else {
         const float* from = g.maps + g.segs * g.D + (seg - 1) * N * g.D;
 #pragma unroll
@@ -248,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
   constexpr int kOwn = kTok / 4;  // tokens of its channel that a thread owns in a chunk: wave + 4 k
   constexpr int kBc = (kTok * 4 * NPT + kThreads - 1) / kThreads;
   T r_dr[kOwn], r_u[kOwn], r_z[kOwn], r_b[kBc], r_c[kBc];
-  auto load = [&](int64_t tc) __attribute__((always_inline)) {
+  auto load = [&](int tc) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
       const int64_t t = tc + wave + 4 * k;
@@ -267,11 +327,11 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
     }
   };
   const float dp = !MAP && act ? g.Dp[d] : 0.0f;
-  const int64_t first = g.starts.at(0), last = g.starts.at(S);  // tokens that have a sequence
+  const int first = g.starts.at(0), last = g.starts.at(S);  // tokens that have a sequence
   float sum = 0.0f;
   load(t0);
-  for (int64_t tc = t0; tc < t1; tc += kTok) {
-    const int len = (int)(t1 - tc < kTok ? t1 - tc : kTok);
+  for (int tc = t0; tc < t1; tc += kTok) {
+    const int len = t1 - tc < kTok ? t1 - tc : kTok;
     float o_u[kOwn], o_z[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
@@ -303,26 +363,23 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
       if (!MAP) s_y[i][wave][lane] = y;
     };
     // no sequence ends within the chunk, but for its last token
-    if (MAP || (s >= 0 && end - tc >= len)) {
+    if (MAP || (at.s >= 0 && at.end - tc >= len)) {
       if (len == kTok) {
 #pragma unroll
         for (int i = 0; i < kTok; ++i) step(i);
       } else {
         for (int i = 0; i < len; ++i) step(i);
       }
-      if (!MAP && s < S && end == tc + len) end_state(s);
+      if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
     } else {
       for (int i = 0; i < len; ++i) {
-        const int64_t t = tc + i;
-        if (t >= end) {  // the next sequence that is not empty begins here, or none
-          do {
-            ++s;
-            end = s < S ? g.starts.at(s + 1) : T_all;
-          } while (s < S && end <= t);
-          if (s < S) begin_state(s);
+        const int t = tc + i;
+        if (t >= at.end) {
+          at.next(g.starts, t);
+          if (at.s < S) begin_state(at.s);
         }
         step(i);
-        if (s >= 0 && s < S && t == end - 1) end_state(s);
+        if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
       }
     }
     __syncthreads();
@@ -353,32 +410,48 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
   }
 }
 
-// The states that enter the segments, in order: the state that segment k - 1 leaves replaces its map's. A lane has one state of one
-// channel. Segments that no sequence leaves have no map; what stands in its place is not used.
-__global__ void __launch_bounds__(64) join_kernel(ScanArgs g) {
-  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (i >= g.D * g.N) return;
-  const int64_t d = i % g.D, n = i / g.D;
+// The states that enter the segments: the state that segment k - 1 leaves replaces its map's. A workgroup has 64 states of a channel each,
+// a lane each; its waves take the segments in chunks of kAhead, whose maps are all loaded at once: compose the chunk's from a zero state,
+// take what enters it from the waves before, and go through it again. Segments that no sequence leaves have no map; what stands in
+// its place is not used. (One lane a state and the segments one after another: 31 us for 256 of them, for the loads' latency.)
+constexpr int kMaxSegs = 256, kAhead = 32, kJoinWaves = kMaxSegs / kAhead;
+__global__ void __launch_bounds__(64 * kJoinWaves) join_kernel(ScanArgs g) {
+  __shared__ float s_sum[kJoinWaves][64], s_end[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  const bool in = i < g.D * g.N;
+  const int64_t d = in ? i % g.D : 0, n = in ? i / g.D : 0;
   const float a = g.A[d * g.N + n] * kLog2e;
   float* state = g.maps + g.segs * g.D + n * g.D + d;
-  float x = 0.0f;
-  constexpr int kAhead = 8;
-  for (int64_t k = 0; k + 1 < g.segs; k += kAhead) {
-    float S[kAhead], e[kAhead];
+  float S[kAhead], e[kAhead];
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      const int64_t kk = k + q < g.segs ? k + q : g.segs - 1;
-      S[q] = g.maps[kk * g.D + d];
-      e[q] = state[kk * g.N * g.D];
-    }
+  for (int q = 0; q < kAhead; ++q) {
+    const int64_t k = wave * kAhead + q;
+    const bool has = k + 1 < g.segs;
+    S[q] = has ? g.maps[k * g.D + d] : 0.0f;
+    e[q] = has ? state[k * g.N * g.D] : 0.0f;
+  }
+  // x decayed over a sum of delta; in two parts: the factor may lie outside fp32 where its product with the state does not
+  auto decayed = [&](float s, float x) __attribute__((always_inline)) {
+    const float p = a * s, p0 = fminf(fmaxf(p, -126.0f), 127.0f), p1 = fminf(fmaxf(p - p0, -126.0f), 127.0f);
+    return fast_exp2(p0) * (x * fast_exp2(p1));
+  };
+  float x = 0.0f, sum = 0.0f;
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      if (k + q + 1 >= g.segs) break;
-      // in two parts: a segment's factor may lie outside fp32 where its product with the state does not
-      const float p = a * S[q], p0 = fminf(fmaxf(p, -126.0f), 127.0f), p1 = fminf(fmaxf(p - p0, -126.0f), 127.0f);
-      x = S[q] < 0.0f ? e[q] : fmaf(fast_exp2(p0), x * fast_exp2(p1), e[q]);
-      state[(k + q) * g.N * g.D] = x;
-    }
+  for (int q = 0; q < kAhead; ++q) {
+    x = S[q] < 0.0f ? e[q] : decayed(S[q], x) + e[q];
+    sum = S[q] < 0.0f || sum < 0.0f ? -1.0f : sum + S[q];
+  }
+  s_sum[wave][lane] = sum;
+  s_end[wave][lane] = x;
+  __syncthreads();
+  x = 0.0f;
+  for (int w = 0; w < wave; ++w) x = s_sum[w][lane] < 0.0f ? s_end[w][lane] : decayed(s_sum[w][lane], x) + s_end[w][lane];
+#pragma unroll
+  for (int q = 0; q < kAhead; ++q) {
+    const int64_t k = wave * kAhead + q;
+    x = S[q] < 0.0f ? e[q] : decayed(S[q], x) + e[q];
+    if (in && k + 1 < g.segs) state[k * g.N * g.D] = x;
   }
 }
 
@@ -387,20 +460,21 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int64_t kMaxGrid = (1 << 24) - 1;
 constexpr int kMaxN = 64;
+constexpr int64_t kMaxTokens = 1 << 30;
 
 int per_wave(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // Tokens of a segment: about four workgroups a CU, of 256 tokens or more
 int64_t segment_length(int64_t T, int64_t tiles) {
   int64_t segs = up(4 * (int64_t)device_cus(), tiles);
-  if (segs > 256) segs = 256;
+  if (segs > kMaxSegs) segs = kMaxSegs;
   int64_t len = up(up(T, segs), kTok) * kTok;
   return len < 256 ? 256 : len;
 }
 
 int packed_status(int64_t T, int64_t S, int64_t D, int io) {
   if (T < 0 || S < 0 || D < 0 || (io != TSF_DTYPE_F32 && io != TSF_DTYPE_BF16)) return TSF_ERR_ARG;
-  if (T > (int64_t)1 << 40 || S > (int64_t)1 << 31 || D > (int64_t)1 << 24) return TSF_ERR_UNSUPPORTED;
+  if (T > kMaxTokens || S > kMaxTokens || D > (int64_t)1 << 24) return TSF_ERR_UNSUPPORTED;
   return TSF_OK;
 }
 
@@ -446,7 +520,7 @@ int tsfast_hip_conv_packed(int64_t T, int64_t S, int64_t D, int64_t K, int io_dt
   if (D == 0 || (T == 0 && S == 0)) return TSF_OK;
   if (!starts || !weight || (T > 0 && (!x || !out || x_stride < 0)) || (S > 0 && !tails_out)) return TSF_ERR_ARG;
   ConvArgs a = {x, tails, weight, bias, out, tails_out, D, x_stride, up(D, io_dtype == TSF_DTYPE_BF16 ? 8 : 4), up(T, kRun),
-                Starts{starts, starts_int64, S, T}, weight_dtype == TSF_DTYPE_BF16, bias_dtype == TSF_DTYPE_BF16};
+                Starts{starts, starts_int64, (int)S, (int)T}, weight_dtype == TSF_DTYPE_BF16, bias_dtype == TSF_DTYPE_BF16};
   const unsigned grid = (unsigned)conv_grid(T, S, D, io_dtype);
   if (io_dtype == TSF_DTYPE_BF16)
     launch_conv<bf16>(a, K, grid, (hipStream_t)stream);
@@ -475,7 +549,7 @@ int tsfast_hip_mamba_packed(int64_t T, int64_t S, int64_t D, int64_t N, int io_d
   if (T > 0 && (!draw || !Bt || !Ct || !u || !z || !out)) return TSF_ERR_ARG;
   if (draw_stride < 0 || b_stride < 0 || c_stride < 0 || u_stride < 0 || z_stride < 0) return TSF_ERR_ARG;
   ScanArgs a = {draw, Bt, Ct, u, z, A, Dp, h0, out, h_last, draw_stride, b_stride, c_stride, u_stride, z_stride, D, up(D, kCh), 0, 1, (int)N,
-                Starts{starts, starts_int64, S, T}, (float*)workspace};
+                Starts{starts, starts_int64, (int)S, (int)T}, (float*)workspace};
   a.seg_len = segment_length(T, a.tiles);
   a.segs = T > 0 ? up(T, a.seg_len) : 1;
   if (a.segs * a.tiles > kMaxGrid) return TSF_ERR_UNSUPPORTED;
@@ -487,7 +561,7 @@ int tsfast_hip_mamba_packed(int64_t T, int64_t S, int64_t D, int64_t N, int io_d
       launch_scan<bf16, true>(a, grid, st);
     else
       launch_scan<float, true>(a, grid, st);
-    join_kernel<<<(unsigned)up(D * N, 64), 64, 0, st>>>(a);
+    join_kernel<<<(unsigned)up(D * N, 64), (unsigned)(64 * up(a.segs - 1, kAhead)), 0, st>>>(a);
   }
   const unsigned grid = (unsigned)(a.segs * a.tiles);
   if (io_dtype == TSF_DTYPE_BF16)

@@ -24,16 +24,18 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}  # feed.hip Act
 _MAX_WIDTH = 1 << 20  # D and F (feed.hip feed_status)
 _MAX_LD = 1 << 22  # elements between rows (feed.hip kMaxLd)
 _MAX_TILES = 1 << 24
+_FEW_ROWS = 32
 
 
 def supports(x, weight_gate, weight_up, bias_gate, bias_up) -> str | None:
     """Reason the fused block cannot handle these tensors, or None if it can."""
-    if x.device.type != "cuda":
+    dtype, dev = x.dtype, x.get_device()
+    if dev < 0:
         return f"x on {x.device.type}, hip backend is GPU-only"
-    if x.dtype not in _IO_DTYPES:
-        return f"x dtype {x.dtype} not float32/bfloat16"
+    if dtype not in _IO_DTYPES:
+        return f"x dtype {dtype} not float32/bfloat16"
     for t in (weight_gate, weight_up, bias_gate, bias_up):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+        if t is not None and (t.dtype != dtype or t.get_device() != dev):
             return f"a parameter is {t.dtype} on {t.device}, x {x.dtype} on {x.device}"
     F, D = weight_gate.shape
     if D > _MAX_WIDTH or F > _MAX_WIDTH:
@@ -86,7 +88,8 @@ def _forward(x, weight_gate, weight_up, bias_gate, bias_up, activation: int, tra
         y = torch.empty((*x.shape[:-1], F), device=x.device, dtype=x.dtype)
         kept = torch.empty(kept_bytes(rows, F, x.dtype), device=x.device, dtype=torch.uint8) if train else None
         where = (xr.data_ptr(), sx, wg.data_ptr(), sg, wu.data_ptr(), su)
-        nbytes = lib.tsfast_hip_feed_fwd_workspace_bytes(rows, D, F, io, *where, train)
+        # a few rows are read as they lie (feed.hip kFewRows; tests pin it against the library's size query)
+        nbytes = lib.tsfast_hip_feed_fwd_workspace_bytes(rows, D, F, io, *where, train) if train or rows > _FEW_ROWS else 0
         ws = _lib.workspace(nbytes, x.device) if nbytes > 0 else None
         _lib.check(
             lib.tsfast_hip_feed_fwd(
@@ -205,8 +208,13 @@ _feed_train_op.register_autograd(_backward, setup_context=_setup)
 
 def run(x, weight_gate, weight_up, bias_gate, bias_up, activation: str):
     """The fused block; see :func:`tsfast_amd.gated.gated_feed_forward`."""
-    tensors = [t for t in (x, weight_gate, weight_up, bias_gate, bias_up) if t is not None]
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (
+        x.requires_grad
+        or weight_gate.requires_grad
+        or weight_up.requires_grad
+        or (bias_gate is not None and bias_gate.requires_grad)
+        or (bias_up is not None and bias_up.requires_grad)
+    ):
         return _feed_train_op(x, weight_gate, weight_up, bias_gate, bias_up, act)[0]
     return _feed_op(x, weight_gate, weight_up, bias_gate, bias_up, act)

@@ -13,8 +13,6 @@ from __future__ import annotations
 
 __all__ = ["supports_conv", "conv", "supports_ssm", "ssm", "supports_step", "step"]
 
-import ctypes
-
 import torch
 
 from .. import _lib
@@ -22,24 +20,28 @@ from ..ops import custom_op
 
 _IO_DTYPES = {torch.float32: _lib.TSF_DTYPE_F32, torch.bfloat16: _lib.TSF_DTYPE_BF16}
 _MAX_GRID = (1 << 24) - 1
-_MAX_D, _MAX_T, _MAX_S = 1 << 24, 1 << 40, 1 << 31
-_MAX_N, _MAX_P = 64, 2048  # states; columns of x_proj (step.hip kMaxP)
+_MAX_D, _MAX_T, _MAX_S = 1 << 24, 1 << 30, 1 << 30
+_MAX_N, _MAX_P = 64, 1024  # states; columns of x_proj (step.hip kMaxP)
 
 
 def _tensor_reason(x, alike, params, wide, starts=None) -> str | None:
-    """``alike``: of x's type; ``params``: float32 or bfloat16; ``wide``: float32."""
-    dev = x.device
-    if dev.type != "cuda":
-        return f"x on {dev.type}, hip backend is GPU-only"
-    if x.dtype not in _IO_DTYPES:
-        return f"sequence dtype {x.dtype} not float32/bfloat16"
-    for group, dtypes in ((alike, (x.dtype,)), (params, tuple(_IO_DTYPES)), (wide, (torch.float32,))):
-        for t in group:
-            if t is not None and (t.dtype not in dtypes or t.device != dev):
-                return f"a tensor is {t.dtype} on {t.device}, needs one of {dtypes} on {dev}"
-    if starts is not None and starts.device != dev:
-        return f"starts on {starts.device}, x on {dev}"
-    return None
+    """``alike``: of x's type; ``params``: float32 or bfloat16; ``wide``: float32 (each a tuple, None where an optional tensor is absent)."""
+    dtype, dev = x.dtype, x.get_device()
+    if dev < 0:
+        return f"x on {x.device}, hip backend is GPU-only"
+    if dtype not in _IO_DTYPES:
+        return f"sequence dtype {dtype} not float32/bfloat16"
+    bad = starts if starts is not None and starts.get_device() != dev else None
+    for t in alike:
+        if t is not None and (t.dtype != dtype or t.get_device() != dev):
+            bad = t
+    for t in params:
+        if t is not None and (t.dtype not in _IO_DTYPES or t.get_device() != dev):
+            bad = t
+    for t in wide:
+        if t is not None and (t.dtype != torch.float32 or t.get_device() != dev):
+            bad = t
+    return None if bad is None else f"a tensor is {bad.dtype} on {bad.device}, x {dtype} on {x.device}"
 
 
 def _packed_reason(T: int, S: int, D: int) -> str | None:
@@ -85,7 +87,7 @@ def supports_step(x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, d
     (B, D), N, P, K = x.shape, A.shape[-1], x_proj.shape[0], conv_weight.shape[-1]
     if not 2 <= K <= 8 or N > _MAX_N or P > _MAX_P:
         return f"kernel width {K}, N={N} states or {P} columns of x_proj: at most 2..8, {_MAX_N} and {_MAX_P}"
-    if D > _MAX_D or B > _MAX_S or -(-B // 4) * -(-D // 64) > _MAX_GRID:
+    if D > _MAX_D or B > 1 << 31 or -(-B // 8) * -(-D // 64) > _MAX_GRID:
         return f"B={B}, D={D} needs more workgroups than one launch has"
     return None
 
@@ -98,7 +100,7 @@ def _screen(x, alike, params, wide, starts=None):
 
 def _rows(t):
     """``t [rows, width]`` with a dense last dimension."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(1) == 1 else t.contiguous()
 
 
 def _dense(t):
@@ -180,9 +182,6 @@ def ssm(draw, A, B_t, C_t, u, z, Dp, starts, h0):
     return _ssm_op(draw, A, B_t, C_t, u, z, Dp, starts, h0)
 
 
-_Types = ctypes.c_int * 5
-
-
 @custom_op("tsfast_hip::mamba_step", mutates_args=("conv_state", "ssm_state"))
 def _step_op(
     x: torch.Tensor,
@@ -202,18 +201,24 @@ def _step_op(
     _screen(x, (z, conv_state), params, (ssm_state, A, Dp))
     if not (conv_state.is_contiguous() and ssm_state.is_contiguous()):
         raise TypeError("the states must be contiguous")
-    x, z, A, Dp = _rows(x), _rows(z), A.contiguous(), Dp.contiguous()
-    params = tuple(map(_dense, params))
+    x, z = _rows(x), _rows(z)
+    A, Dp = (t if t.is_contiguous() else t.contiguous() for t in (A, Dp))
+    one = conv_weight.dtype
+    if x_proj.dtype != one or dt_proj.dtype != one or (conv_bias is not None and conv_bias.dtype != one):  # the kernels take these four in one type
+        params = (*(None if t is None else t.float() for t in params[:4]), dt_bias)
+    conv_weight, conv_bias, x_proj, dt_proj, dt_bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in params)
     (B, D), N, R, K = x.shape, A.shape[-1], dt_proj.shape[-1], conv_weight.shape[-1]
     with _lib.device_of(x):
         out = torch.empty(B, D, device=x.device, dtype=x.dtype)
         nbytes = lib.tsfast_hip_mamba_step_workspace_bytes(B, D, N, R, K)
         ws = _lib.workspace(nbytes, x.device)
-        types = _Types(*(_lib.TSF_DTYPE_F32 if t is None else _IO_DTYPES[t.dtype] for t in params))
         _lib.check(
             lib.tsfast_hip_mamba_step(
-                B, D, N, R, K, _IO_DTYPES[x.dtype], types, x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0),
-                *map(_lib.ptr, (conv_state, ssm_state, *params, A, Dp, out, ws)), nbytes, _lib.stream_of(x),
+                B, D, N, R, K, _IO_DTYPES[x.dtype], _IO_DTYPES[conv_weight.dtype], 0 if dt_bias is None else _IO_DTYPES[dt_bias.dtype],
+                x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0), conv_state.data_ptr(), ssm_state.data_ptr(), conv_weight.data_ptr(),
+                None if conv_bias is None else conv_bias.data_ptr(), x_proj.data_ptr(), dt_proj.data_ptr(),
+                None if dt_bias is None else dt_bias.data_ptr(), A.data_ptr(), Dp.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes,
+                _lib.stream_of(x),
             ),
             "tsfast_hip_mamba_step",
         )

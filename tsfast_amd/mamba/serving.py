@@ -48,7 +48,12 @@ _AUTO_ORDER = {"cuda": ("hip",)}
 
 
 def _no_gradient(what: str, instead: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    wanted = False
+    for t in tensors:
+        wanted = wanted or (t is not None and t.requires_grad)
+    if wanted:
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or use {instead}")
 
 
@@ -61,7 +66,7 @@ def _check_starts(starts):
 def _check(t, name: str, shape: tuple, dtype=None, optional: bool = False):
     if t is None and optional:
         return
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
@@ -171,13 +176,18 @@ def mamba_step(x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_p
     if dt_proj.dim() != 2 or dt_proj.shape[0] != D or dt_proj.shape[1] < 1:
         raise ValueError(f"dt_proj must be [{D}, R], got {tuple(dt_proj.shape)}")
     R, wide = dt_proj.shape[1], torch.float64 if x.dtype == torch.float64 else torch.float32
-    for t, name, shape, dtype in ((z, "z", (B, D), x.dtype), (conv_state, "conv_state", (B, D, K - 1), x.dtype), (A, "A", (D, N), wide),
-                                  (ssm_state, "ssm_state", (B, D, N), wide), (x_proj, "x_proj", (R + 2 * N, D), None), (Dp, "Dp", (D,), wide)):
-        _check(t, name, shape, dtype)
-    _check(dt_bias, "dt_bias", (D,), optional=True)
+    rows, channels, state = (B, D), (D,), (B, D, N)
+    if (
+        z.shape != rows or conv_state.shape != (B, D, K - 1) or ssm_state.shape != state or x_proj.shape != (R + 2 * N, D) or Dp.shape != channels
+        or A.shape[0] != D or z.dtype != x.dtype or conv_state.dtype != x.dtype or ssm_state.dtype != wide or A.dtype != wide or Dp.dtype != wide
+    ):  # all of it at once; by name what it is
+        for t, name, shape, dtype in ((z, "z", rows, x.dtype), (conv_state, "conv_state", (B, D, K - 1), x.dtype), (A, "A", (D, N), wide),
+                                      (ssm_state, "ssm_state", state, wide), (x_proj, "x_proj", (R + 2 * N, D), None), (Dp, "Dp", channels, wide)):
+            _check(t, name, shape, dtype)
+    _check(dt_bias, "dt_bias", channels, optional=True)
     args = (x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A, Dp)
     for t in (conv_weight, conv_bias, x_proj, dt_proj, dt_bias):
-        if t is not None and t.dtype not in (x.dtype, wide):
+        if t is not None and t.dtype != x.dtype and t.dtype != wide:
             raise ValueError(f"parameters must be {x.dtype} or {wide}, got {t.dtype}")
     mod = resolve("mamba.step", _STEP_BACKENDS, _AUTO_ORDER.get(x.device.type, ()), args)
     if mod is not None:
