@@ -96,6 +96,11 @@ def test_abi_refuses_before_any_launch():
         rows, D, F, io, act, x, sx, p, 8, p, 8, None, None, p, None, None, 0, None)
     assert fwd(rows=-1) == fwd(D=0) == fwd(io=2) == fwd(act=3) == fwd(x=None) == fwd(sx=7) == fwd(sx=(1 << 22) + 1) == -1
     assert fwd(D=(1 << 20) + 1) == -3 and fwd(rows=0) == 0
+    back = lib.tsfast_hip_feed_bwd_workspace_bytes
+    assert back(0, 8, 8, 0, None, 8, None, 8, None, 8) == 0 < back(1, 8, 8, 0, p, 8, p, 8, p, 8)
+    for rows, D, F in ((1, 1, 1), (1, 1 << 20, 1), (1, 1, 1 << 20), (33, 1 << 16, 1 << 16), (1 << 24, 1, 1), (1000, 768, 2048), (100_000, 64, 256)):
+        for io in (0, 1):
+            assert back(rows, D, F, io, p, D, p, D, p, D) > 0
     assert lib.tsfast_hip_feed_fwd(100, 8, 8, 0, 0, p, 8, p, 8, p, 8, None, None, p, None, None, 0, None) == -2
     bwd = lambda kept=p, gw=p, ws=p, n=0: lib.tsfast_hip_feed_bwd(  # noqa: E731
         4, 8, 8, 1, 0, p, 8, p, 8, p, 8, p, 8, kept, p, gw, p, None, None, ws, n, None)

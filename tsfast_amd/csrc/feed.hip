@@ -533,11 +533,12 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
       const int64_t c0 = (h ? p1 : p0) + wp * NH * 16, r0 = q0 + wq * NQ * 16;
       const int n = left(h ? rows_1 : rows_0);
       auto value = [&](int i, int j) { return acc[h * NH + i][j]; };
-      if (FORM == kInput || g.part) {
-        using O = std::conditional_t<FORM == kInput, T, float>;
-        O* y = FORM == kInput ? (O*)g.y : (O*)(g.part + (int64_t)split * g.nq * g.np);
-        y += r0 * g.np + c0;
-        store_rows<C, O>(own, lane, n, value, [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * g.np : (O*)nullptr; });
+      if (g.part) {
+        float* y = g.part + ((int64_t)split * g.nq + r0) * g.np + c0;
+        store_rows<C, float>(own, lane, n, value, [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * g.np : (float*)nullptr; });
+      } else if constexpr (FORM == kInput) {
+        T* y = (T*)g.y + r0 * g.np + c0;
+        store_rows<C, T>(own, lane, n, value, [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * g.np : (T*)nullptr; });
       } else {
         store_rows<C, T>(own, lane, n, value, [&](int q) {
           const int64_t r = r0 + q, in = r < g.half_rows ? r : r - g.half_rows;
@@ -685,22 +686,22 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   }
 }
 
-// out0 and out1 [n each] = sums over `parts` of part [part][2][stride] (the first n of each half), in a fixed order: VL columns a lane,
-// every fourth part a wave. VL > 1: n and stride are multiples of it.
+// out0 and out1 (or none) [n each] = sums over `parts` of part [part][halves][stride] (the first n of each half), in a fixed order: VL columns
+// a lane, every fourth part a wave. VL > 1: n and stride are multiples of it.
 template <typename T, int VL>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int parts, int64_t stride, int64_t n, T* out0, T* out1) {
+__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int parts, int64_t stride, int64_t n, int halves, T* out0, T* out1) {
   __shared__ float sums[4][64][VL];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i = ((int64_t)blockIdx.x * 64 + lane) * VL, h = i >= n, c = i - h * n;
   float s[VL];
 #pragma unroll
   for (int e = 0; e < VL; ++e) s[e] = 0.0f;
-  if (i < 2 * n) {
+  if (i < halves * n) {
     const float* p = part + h * stride + c;
 #pragma unroll 4
     for (int k = wave; k < parts; k += 4) {
       float v[VL];
-      __builtin_memcpy(v, __builtin_assume_aligned(p + (int64_t)k * 2 * stride, 4 * VL), sizeof(v));
+      __builtin_memcpy(v, __builtin_assume_aligned(p + (int64_t)k * halves * stride, 4 * VL), sizeof(v));
 #pragma unroll
       for (int e = 0; e < VL; ++e) s[e] += v[e];
     }
@@ -709,17 +710,16 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int pa
   for (int e = 0; e < VL; ++e) sums[wave][lane][e] = s[e];
   __syncthreads();
   T* out = h ? out1 : out0;
-  if (wave == 0 && i < 2 * n && out) {
+  if (wave == 0 && i < halves * n && out) {
 #pragma unroll
     for (int e = 0; e < VL; ++e) out[c + e] = from_f32<T>((sums[0][lane][e] + sums[1][lane][e]) + (sums[2][lane][e] + sums[3][lane][e]));
   }
 }
 template <typename T>
-void sum_parts(const float* part, int64_t parts, int64_t stride, int64_t n, void* out0, void* out1, hipStream_t st) {
-  if (n % 4 == 0 && stride % 4 == 0)
-    sum_kernel<T, 4><<<(unsigned)((2 * n + 255) / 256), kThreads, 0, st>>>(part, (int)parts, stride, n, (T*)out0, (T*)out1);
-  else
-    sum_kernel<T, 1><<<(unsigned)((2 * n + 63) / 64), kThreads, 0, st>>>(part, (int)parts, stride, n, (T*)out0, (T*)out1);
+void sum_parts(const float* part, int64_t parts, int64_t stride, int64_t n, int halves, void* out0, void* out1, hipStream_t st) {
+  const int vl = n % 4 == 0 && stride % 4 == 0 ? 4 : 1;
+  auto* const kernel = vl == 4 ? sum_kernel<T, 4> : sum_kernel<T, 1>;
+  kernel<<<(unsigned)((halves * n + 64 * vl - 1) / (64 * vl)), kThreads, 0, st>>>(part, (int)parts, stride, n, halves, (T*)out0, (T*)out1);
 }
 
 // --------------------------------------------------------------------------------- a few rows
@@ -829,15 +829,15 @@ int64_t up256(int64_t a) { return up(a, 256) * 256; }
 
 constexpr int64_t kFewRows = 32;
 
-#ifndef L4
 using Large = Tile<256, 256, 4, 2>;
-#else
-using Large = Tile<256, 256, 2, 2>;
-#endif
 using Medium = Tile<128, 128, 2, 2>;
 using Small = Tile<64, 64, 2, 2>;
 
-// How a product of nq x np outputs (np of each half where `dual`) and `stages` of k is cut.
+// How a product of nq x np outputs (np of each half where `dual`) and `stages` of k is cut: the tile, and the parts of k that side by side
+// workgroups take, whichever comes out least. A stage of one workgroup takes `alone` us while its CU has no other, and `shared` us of
+// the CU beside others; `ends` is what stands around the stages. Measured, us of the kernel with the large, the medium, the small tile: 256 x
+// 1536 -> 2 x 4096 bf16 36, 20, 16; 1024 rows 39, 29, 43; 2048 rows 44, 55, 82; 16384 rows with gradients 1200, 1392, 2480. Partial sums
+// are written and read at 4 TB/s. dx of 1000 rows, 768 -> 2 x 2048, whole 33 us, in parts 15 and their sum 2.
 struct Plan {
   int tile;  // 0: Large, 1: Medium, 2: Small
   int64_t tiles_q, tiles_p, splits, split_stages;
@@ -846,17 +846,20 @@ Plan plan_for(int64_t nq, int64_t np, int64_t stages, bool dual, bool may_split)
   const int64_t cus = device_cus();
   const struct {
     int bq, bp, per_cu;
-    double cost;  // of a stage of one workgroup, when the CU is full of them
-  } tiles[3] = {{256, 256, 1, 1.0}, {128, 128, 2, 0.35}, {64, 64, 4, 0.16}};
+    double alone, shared, ends;
+  } tiles[3] = {{256, 256, 1, 1.68, 1.68, 8.0}, {128, 128, 2, 0.8, 0.55, 4.0}, {64, 64, 4, 0.38, 0.21, 3.0}};
   Plan best = {};
   double least = 0;
   for (int t = 0; t < 3; ++t) {
-    const int64_t tq = up(nq, tiles[t].bq), tp = up(np, dual ? tiles[t].bp / 2 : tiles[t].bp);
+    const auto& c = tiles[t];
+    const int64_t tq = up(nq, c.bq), tp = up(np, dual ? c.bp / 2 : c.bp);
     for (int64_t s = 1; s <= (may_split ? 64 : 1); s *= 2) {
-      if (s > 1 && stages / s < 8) break;
-      const double rounds = (double)up(tq * tp * s, cus * tiles[t].per_cu);
-      double time = rounds * ((double)up(stages, s) + 12) * tiles[t].cost * tiles[t].per_cu;
-      if (s > 1) time += (double)(nq * np * s) / (double)(cus * 4096) + 8;
+      if (s > 1 && stages / s < 4) break;
+      const int64_t wgs = tq * tp * s, round = cus * c.per_cu, full = wgs / round, last = up(wgs % round, cus);
+      auto stage = [&](int64_t beside) { return c.alone > beside * c.shared ? c.alone : beside * c.shared; };
+      const double each = (double)up(stages, s);
+      double time = full * (each * stage(c.per_cu) + c.ends) + (last ? each * stage(last) + c.ends : 0.0);
+      if (s > 1) time += (double)(nq * np * (2 * s + 1) * 4) / 4e6 + 4.0;
       if (!best.splits || time < least) {
         least = time;
         best = Plan{t, tq, tp, s, up(stages, s)};
@@ -1000,7 +1003,7 @@ struct BwdSpace {
 };
 BwdSpace bwd_space(const Shape& s) {
   BwdSpace b;
-  b.px = plan_for(s.rows, s.D, s.stages_x, false, false);
+  b.px = plan_for(s.rows, s.D, s.stages_x, false, true);
   b.pw = plan_for(2 * s.F8, s.D, s.stages_w, false, true);
   const int64_t all = up(s.rows, 16), cols = up(s.F, 64);
   // rows of a workgroup: four blocks a wave or more, and about 2048 workgroups
@@ -1009,7 +1012,9 @@ BwdSpace bwd_space(const Shape& s) {
   b.wgs = up(all, b.blocks);
   b.d = up256((s.dtype == TSF_DTYPE_BF16 ? 1 : 3) * s.rows * 2 * s.F8 * 2);
   b.bias = up256(b.wgs * 2 * s.F * 4);
-  b.part = b.pw.splits > 1 ? up256(b.pw.splits * 2 * s.F8 * s.D * 4) : 0;
+  // both products' parts, one after the other
+  const int64_t px = b.px.splits > 1 ? b.px.splits * s.rows : 0, pw = b.pw.splits > 1 ? b.pw.splits * 2 * s.F8 : 0;
+  b.part = up256((px > pw ? px : pw) * s.D * 4);
   return b;
 }
 
@@ -1040,7 +1045,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
   a.dy = dy, a.ld_dy = ld_dy, a.rows = s.rows, a.F = s.F, a.F8 = s.F8, a.save_fb = up(s.F, 16), a.blocks = b.blocks;
   a.save_hi = pre, a.save_lo = pre_lo(const_cast<char*>(pre), s.rows, s.F), a.d = d, a.part = want_bias ? bias : nullptr;
   launch_adjoint<T>(a, act, dim3((unsigned)up(s.F, 64), (unsigned)b.wgs), st);
-  if (want_bias) sum_parts<T>(bias, b.wgs, s.F, s.F, dbg, dbu, st);
+  if (want_bias) sum_parts<T>(bias, b.wgs, s.F, s.F, 2, dbg, dbu, st);
 
   const int64_t plane = s.rows * 2 * s.F8;
   if (dx) {
@@ -1054,8 +1059,9 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
         g.p0[n] = g.p1[n] = w.p + pr[1] * w.plane;
       }
     g.ldq = 2 * s.F8, g.ldp = o.wg.ld, g.kq = s.F8, g.kp = s.F, g.nq = s.rows, g.np = s.D;
-    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx;
+    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx, g.part = b.px.splits > 1 ? part : nullptr;
     product<T, kInput>(g, b.px, st);
+    if (g.part) sum_parts<T>(part, b.px.splits, s.rows * s.D, s.rows * s.D, 1, dx, nullptr, st);
   }
   if (dwg || dwu) {
     ProductArgs g = {};
@@ -1068,7 +1074,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
     g.segs = s.pairs, g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
     g.part = b.pw.splits > 1 ? part : nullptr;
     product<T, kWeight>(g, b.pw, st);
-    if (g.part) sum_parts<T>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, dwg, dwu, st);
+    if (g.part) sum_parts<T>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, 2, dwg, dwu, st);
   }
   return tsf_launch_status();
 }
@@ -1102,6 +1108,7 @@ int64_t tsfast_hip_feed_fwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, 
 int64_t tsfast_hip_feed_bwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride, const void* w_gate,
                                             int64_t w_gate_stride, const void* w_up, int64_t w_up_stride) {
   if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;
+  if (rows == 0) return 0;
   const Shape s = shape_of(rows, D, F, dtype);
   const BwdSpace b = bwd_space(s);
   return operands_of(s, Call{x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride}).bytes + b.d + b.bias + b.part;
