@@ -30,7 +30,8 @@ struct Starts {
 };
 
 // A token's sequence: the last one that begins at or before it (so it is not empty); -1: none yet, S: behind the last one. Where it begins
-// and ends: before and behind the sequences, where no token has one.
+// and ends: before and behind the sequences, where no token has one. begin <= t even where starts decreases: what is addressed by
+// t - begin, or by the segment before t's, exists.
 struct Cursor {
   int s, begin, end;
   // for a token of each lane; all lanes of a wave call. Up to 64 starts come with one load of the wave (a search is a chain of loads)
@@ -40,7 +41,8 @@ struct Cursor {
       int count = 0;
       for (int l = 0; l <= st.S; ++l) count += __builtin_amdgcn_readlane(mine, l) <= t;
       s = count - 1;
-      begin = s < 0 ? 0 : __shfl(mine, s < 0 ? 0 : s, kWave);
+      const int from = __shfl(mine, s < 0 ? 0 : s, kWave);
+      begin = s < 0 ? 0 : from < t ? from : t;
       end = __shfl(mine, s < st.S ? s + 1 : st.S, kWave);
     } else {
       int lo = 0, hi = st.S + 1;  // the first start behind t is in [lo, hi]
