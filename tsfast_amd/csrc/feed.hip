@@ -606,22 +606,27 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
     const int64_t m0 = mb * 16;
     f32x4 a[4], b[4];
     u32x4 in[kDy];
+    // a load under a lane's condition is waited for before the next one starts: whole blocks have none
+    const bool whole = m0 + 16 <= g.rows && f0 + 64 <= g.F;
+    const T* dy0 = (const T*)g.dy + m0 * g.ld_dy + f0;
+    if (whole) {
 #pragma unroll
-    for (int e = 0; e < kDy; ++e) {
-      const int64_t m = m0 + Turn<T>::row(lane, e), f = f0 + Turn<T>::col(lane, e);
-      const T* p = (const T*)g.dy + m * g.ld_dy + f;
-      T v[kPer];
-      if (m < g.rows && f + kPer <= g.F) {
-        __builtin_memcpy(v, p, 16);
-      } else {
+      for (int e = 0; e < kDy; ++e) __builtin_memcpy(&in[e], dy0 + Turn<T>::row(lane, e) * g.ld_dy + Turn<T>::col(lane, e), 16);
+    } else {
+      const int rows = (int)(g.rows - m0 < 16 ? g.rows - m0 : 16), cols = (int)(g.F - f0 < 64 ? g.F - f0 : 64);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) v[k] = m < g.rows && f + k < g.F ? p[k] : from_f32<T>(0.0f);
+      for (int e = 0; e < kDy; ++e) {
+        const int r = Turn<T>::row(lane, e), c = Turn<T>::col(lane, e);
+        T v[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = dy0[(r < rows ? r : rows - 1) * g.ld_dy + (c + k < cols ? c + k : cols - 1)];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = r < rows && c + k < cols ? v[k] : from_f32<T>(0.0f);
+        __builtin_memcpy(&in[e], v, 16);
       }
-      __builtin_memcpy(&in[e], v, 16);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < blocks) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + i, lane, a[i], b[i]);
+    for (int i = 0; i < 4; ++i) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + (i < blocks ? i : 0), lane, a[i], b[i]);
 #pragma unroll
     for (int e = 0; e < kDy; ++e) turn.dy.put_piece(lane, e, in[e]);
     wave_turned();
@@ -659,7 +664,7 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t m = m0 + Turn<bf16>::row(lane, e), f = f0 + Turn<bf16>::col(lane, e);
-        if (m < g.rows && f < g.F8) {
+        if (whole || (m < g.rows && f < g.F8)) {
           bf16* to = g.d + n * plane + m * 2 * g.F8 + f;
           *(u32x4*)to = turn.d[0].get_piece(lane, e);
           *(u32x4*)(to + g.F8) = turn.d[1].get_piece(lane, e);
@@ -686,22 +691,37 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   }
 }
 
-// out0 and out1 (or none) [n each] = sums over `parts` of part [part][halves][stride] (the first n of each half), in a fixed order: VL columns
-// a lane, every fourth part a wave. VL > 1: n and stride are multiples of it.
+// What a backward leaves in parts, summed in a fixed order, up to three results in one launch (blockIdx.y): out0 and out1 (or none) [n each] =
+// sums over `parts` of part [part][halves][stride] (the first n of each half). VL columns a lane, every fourth part a wave. VL > 1: n and
+// stride are multiples of it.
+struct SumJob {
+  const float* part;
+  int64_t stride, n;
+  void *out0, *out1;
+  int parts, halves;
+};
+struct SumArgs {
+  SumJob job[3];
+  int jobs;
+  void add(const float* part, int64_t parts, int64_t stride, int64_t n, int halves, void* out0, void* out1) {
+    job[jobs++] = SumJob{part, stride, n, out0, out1, (int)parts, halves};
+  }
+};
 template <typename T, int VL>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int parts, int64_t stride, int64_t n, int halves, T* out0, T* out1) {
+__global__ void __launch_bounds__(kThreads) sum_kernel(SumArgs a) {
   __shared__ float sums[4][64][VL];
+  const SumJob& j = a.job[blockIdx.y];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = ((int64_t)blockIdx.x * 64 + lane) * VL, h = i >= n, c = i - h * n;
+  const int64_t i = ((int64_t)blockIdx.x * 64 + lane) * VL, h = i >= j.n, c = i - h * j.n;
   float s[VL];
 #pragma unroll
   for (int e = 0; e < VL; ++e) s[e] = 0.0f;
-  if (i < halves * n) {
-    const float* p = part + h * stride + c;
+  if (i < j.halves * j.n) {
+    const float* p = j.part + h * j.stride + c;
 #pragma unroll 4
-    for (int k = wave; k < parts; k += 4) {
+    for (int k = wave; k < j.parts; k += 4) {
       float v[VL];
-      __builtin_memcpy(v, __builtin_assume_aligned(p + (int64_t)k * halves * stride, 4 * VL), sizeof(v));
+      __builtin_memcpy(v, __builtin_assume_aligned(p + (int64_t)k * j.halves * j.stride, 4 * VL), sizeof(v));
 #pragma unroll
       for (int e = 0; e < VL; ++e) s[e] += v[e];
     }
@@ -709,17 +729,24 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const float* part, int pa
 #pragma unroll
   for (int e = 0; e < VL; ++e) sums[wave][lane][e] = s[e];
   __syncthreads();
-  T* out = h ? out1 : out0;
-  if (wave == 0 && i < halves * n && out) {
+  T* out = (T*)(h ? j.out1 : j.out0);
+  if (wave == 0 && i < j.halves * j.n && out) {
 #pragma unroll
     for (int e = 0; e < VL; ++e) out[c + e] = from_f32<T>((sums[0][lane][e] + sums[1][lane][e]) + (sums[2][lane][e] + sums[3][lane][e]));
   }
 }
 template <typename T>
-void sum_parts(const float* part, int64_t parts, int64_t stride, int64_t n, int halves, void* out0, void* out1, hipStream_t st) {
-  const int vl = n % 4 == 0 && stride % 4 == 0 ? 4 : 1;
+void sum_parts(const SumArgs& a, hipStream_t st) {
+  int vl = 4;
+  int64_t most = 0;
+  for (int k = 0; k < a.jobs; ++k) {
+    const SumJob& j = a.job[k];
+    if (j.n % 4 || j.stride % 4) vl = 1;
+    if (j.halves * j.n > most) most = j.halves * j.n;
+  }
+  if (most == 0) return;
   auto* const kernel = vl == 4 ? sum_kernel<T, 4> : sum_kernel<T, 1>;
-  kernel<<<(unsigned)((halves * n + 64 * vl - 1) / (64 * vl)), kThreads, 0, st>>>(part, (int)parts, stride, n, halves, (T*)out0, (T*)out1);
+  kernel<<<dim3((unsigned)((most + 64 * vl - 1) / (64 * vl)), (unsigned)a.jobs), kThreads, 0, st>>>(a);
 }
 
 // --------------------------------------------------------------------------------- a few rows
@@ -835,19 +862,21 @@ using Small = Tile<64, 64, 2, 2>;
 
 // How a product of nq x np outputs (np of each half where `dual`) and `stages` of k is cut: the tile, and the parts of k that side by side
 // workgroups take, whichever comes out least. A stage of one workgroup takes `alone` us while its CU has no other, and `shared` us of
-// the CU beside others; `ends` is what stands around the stages. Measured, us of the kernel with the large, the medium, the small tile: 256 x
+// the CU beside others; `ends` is what stands around the stages; the last workgroups' stores, `out_bytes` of each output, have nothing to go on beside.
+// Measured, us of the kernel with the large, the medium, the small tile: 256 x
 // 1536 -> 2 x 4096 bf16 36, 20, 16; 1024 rows 39, 29, 43; 2048 rows 44, 55, 82; 16384 rows with gradients 1200, 1392, 2480. Partial sums
 // are written and read at 4 TB/s. dx of 1000 rows, 768 -> 2 x 2048, whole 33 us, in parts 15 and their sum 2.
 struct Plan {
   int tile;  // 0: Large, 1: Medium, 2: Small
   int64_t tiles_q, tiles_p, splits, split_stages;
 };
-Plan plan_for(int64_t nq, int64_t np, int64_t stages, bool dual, bool may_split) {
+Plan plan_for(int64_t nq, int64_t np, int64_t stages, int out_bytes, bool dual, bool may_split) {
   const int64_t cus = device_cus();
   const struct {
     int bq, bp, per_cu;
     double alone, shared, ends;
   } tiles[3] = {{256, 256, 1, 1.68, 1.68, 8.0}, {128, 128, 2, 0.8, 0.55, 4.0}, {64, 64, 4, 0.38, 0.21, 3.0}};
+  constexpr double kStore = 18500.0;  // bytes a us of a CU where all store
   Plan best = {};
   double least = 0;
   for (int t = 0; t < 3; ++t) {
@@ -859,6 +888,7 @@ Plan plan_for(int64_t nq, int64_t np, int64_t stages, bool dual, bool may_split)
       auto stage = [&](int64_t beside) { return c.alone > beside * c.shared ? c.alone : beside * c.shared; };
       const double each = (double)up(stages, s);
       double time = full * (each * stage(c.per_cu) + c.ends) + (last ? each * stage(last) + c.ends : 0.0);
+      if (s == 1) time += (double)(c.bq * c.bp / (dual ? 2 : 1) * out_bytes) / kStore;
       if (s > 1) time += (double)(nq * np * (2 * s + 1) * 4) / 4e6 + 4.0;
       if (!best.splits || time < least) {
         least = time;
@@ -991,7 +1021,7 @@ int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void*
   g.ldq = o.x.ld, g.ldp = o.wg.ld, g.kq = g.kp = up8(s.D), g.nq = s.rows, g.np = s.F;
   g.segs = s.pairs, g.stages = s.stages_f, g.act = act, g.train = pre != nullptr, g.bg = bg, g.bu = bu, g.y = y;
   if (pre) g.save_hi = pre, g.save_lo = pre_lo(pre, s.rows, s.F), g.save_fb = up(s.F, 16);
-  product<T, kForward>(g, plan_for(s.rows, s.F, s.stages_f, true, false), st);
+  product<T, kForward>(g, plan_for(s.rows, s.F, s.stages_f, (int)sizeof(T) + (pre ? (sizeof(T) == 2 ? 6 : 8) : 0), true, false), st);
   return tsf_launch_status();
 }
 
@@ -999,22 +1029,23 @@ int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void*
 struct BwdSpace {
   Plan px, pw;
   int64_t wgs, blocks;  // of the adjoint's rows
-  int64_t d, bias, part;
+  int64_t d, bias, part_x, part;  // part: of both products, dx's first
 };
 BwdSpace bwd_space(const Shape& s) {
   BwdSpace b;
-  b.px = plan_for(s.rows, s.D, s.stages_x, false, true);
-  b.pw = plan_for(2 * s.F8, s.D, s.stages_w, false, true);
+  const int size = s.dtype == TSF_DTYPE_BF16 ? 2 : 4;
+  b.px = plan_for(s.rows, s.D, s.stages_x, size, false, true);
+  b.pw = plan_for(2 * s.F8, s.D, s.stages_w, size, false, true);
   const int64_t all = up(s.rows, 16), cols = up(s.F, 64);
-  // rows of a workgroup: four blocks a wave or more, and about 2048 workgroups
-  b.blocks = up(all * cols, 2048);
-  if (b.blocks < 16) b.blocks = 16;
+  // rows of a workgroup: a block a wave or more (1000 x 2048 bf16 with four at least 23 us, with one 11), and three workgroups a CU, as
+  // registers allow: more leave more sums of columns for the next kernel (32768 x 256 fp32: 2048 of them 41 + 14 us, 768 38 + 7)
+  b.blocks = up(all * cols, 3 * (int64_t)device_cus());
+  if (b.blocks < 4) b.blocks = 4;
   b.wgs = up(all, b.blocks);
   b.d = up256((s.dtype == TSF_DTYPE_BF16 ? 1 : 3) * s.rows * 2 * s.F8 * 2);
   b.bias = up256(b.wgs * 2 * s.F * 4);
-  // both products' parts, one after the other
-  const int64_t px = b.px.splits > 1 ? b.px.splits * s.rows : 0, pw = b.pw.splits > 1 ? b.pw.splits * 2 * s.F8 : 0;
-  b.part = up256((px > pw ? px : pw) * s.D * 4);
+  b.part_x = b.px.splits > 1 ? up256(b.px.splits * s.rows * s.D * 4) : 0;
+  b.part = b.part_x + (b.pw.splits > 1 ? up256(b.pw.splits * 2 * s.F8 * s.D * 4) : 0);
   return b;
 }
 
@@ -1038,14 +1069,16 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
   char* at = ws + o.bytes;
   bf16* d = (bf16*)at;
   float* bias = (float*)(at + b.d);
-  float* part = (float*)(at + b.d + b.bias);
+  float* part_x = (float*)(at + b.d + b.bias);
+  float* part_w = (float*)(at + b.d + b.bias + b.part_x);
+  SumArgs sums = {};
   const bool want_bias = dbg || dbu;
 
   AdjointArgs a = {};
   a.dy = dy, a.ld_dy = ld_dy, a.rows = s.rows, a.F = s.F, a.F8 = s.F8, a.save_fb = up(s.F, 16), a.blocks = b.blocks;
   a.save_hi = pre, a.save_lo = pre_lo(const_cast<char*>(pre), s.rows, s.F), a.d = d, a.part = want_bias ? bias : nullptr;
   launch_adjoint<T>(a, act, dim3((unsigned)up(s.F, 64), (unsigned)b.wgs), st);
-  if (want_bias) sum_parts<T>(bias, b.wgs, s.F, s.F, 2, dbg, dbu, st);
+  if (want_bias) sums.add(bias, b.wgs, s.F, s.F, 2, dbg, dbu);
 
   const int64_t plane = s.rows * 2 * s.F8;
   if (dx) {
@@ -1059,9 +1092,9 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
         g.p0[n] = g.p1[n] = w.p + pr[1] * w.plane;
       }
     g.ldq = 2 * s.F8, g.ldp = o.wg.ld, g.kq = s.F8, g.kp = s.F, g.nq = s.rows, g.np = s.D;
-    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx, g.part = b.px.splits > 1 ? part : nullptr;
+    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx, g.part = b.px.splits > 1 ? part_x : nullptr;
     product<T, kInput>(g, b.px, st);
-    if (g.part) sum_parts<T>(part, b.px.splits, s.rows * s.D, s.rows * s.D, 1, dx, nullptr, st);
+    if (g.part) sums.add(g.part, b.px.splits, s.rows * s.D, s.rows * s.D, 1, dx, nullptr);
   }
   if (dwg || dwu) {
     ProductArgs g = {};
@@ -1072,10 +1105,11 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
     }
     g.ldq = 2 * s.F8, g.ldp = o.x.ld, g.kq = g.kp = s.rows, g.nq = 2 * s.F8, g.np = s.D;
     g.segs = s.pairs, g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
-    g.part = b.pw.splits > 1 ? part : nullptr;
+    g.part = b.pw.splits > 1 ? part_w : nullptr;
     product<T, kWeight>(g, b.pw, st);
-    if (g.part) sum_parts<T>(part, b.pw.splits, s.F8 * s.D, s.F * s.D, 2, dwg, dwu, st);
+    if (g.part) sums.add(g.part, b.pw.splits, s.F8 * s.D, s.F * s.D, 2, dwg, dwu);
   }
+  sum_parts<T>(sums, st);
   return tsf_launch_status();
 }
 

@@ -67,6 +67,10 @@ def _screen(x, *others):
             raise TypeError(f"{t.dtype} on {t.device}, expected {dtype} on {x.device}")
 
 
+def _empty(t):
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _dense(t):
     return None if t is None else t.contiguous()
 
@@ -161,10 +165,9 @@ def _feed_bwd_op(
         raise TypeError(f"kept: {kept.numel()} of {kept.dtype} on {kept.device}, expected the forward's on {x.device}")
     (xr, sx), (wg, sg), (wu, su), (gr, sgy) = _rows(x, D), _rows(weight_gate, D), _rows(weight_up, D), _rows(gy, F)
     with _lib.device_of(x):
-        empty = lambda want, *shape: torch.empty(shape if want else (0,), device=x.device, dtype=x.dtype)  # noqa: E731
-        gx = empty(want_x, *x.shape)
-        gwg, gwu = empty(want_weights, F, D), empty(want_weights, F, D)
-        gbg, gbu = empty(has_bias_gate, F), empty(has_bias_up, F)
+        gx = _empty(x) if want_x else x.new_empty(0)
+        gwg, gwu = (_empty(w) if want_weights else x.new_empty(0) for w in (weight_gate, weight_up))
+        gbg, gbu = (x.new_empty(F if want else 0) for want in (has_bias_gate, has_bias_up))
         where = (xr.data_ptr(), sx, wg.data_ptr(), sg, wu.data_ptr(), su)
         nbytes = lib.tsfast_hip_feed_bwd_workspace_bytes(rows, D, F, io, *where)
         ws = _lib.workspace(nbytes, x.device)
