@@ -326,3 +326,11 @@ def test_supports_reasons(gpu):
     big = torch.randn(6, 65, device="cuda")  # more states than the kernels hold: the torch path
     y, _ = mamba.mamba_ssm_packed(s["draw"], -torch.rand(4, 65, device="cuda"), big, big, s["u"], s["z"], m["Dp"], at)
     assert torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("T", [127, 128, 129, 159, 160, 161, 193])
+def test_around_the_first_cuts(gpu, T, dtype):
+    """Rows that are just short enough for one segment, and the first ones that are not."""
+    for starts in ([0, T], [0, 31, 32, 64, 97, T - 1], [33, 95, 95, 128 if T > 128 else 120, T]):
+        check_packed(make(T, 70, 16, 4, 2, 1, dtype, dev="cuda", seed=15), starts, True, dtype)

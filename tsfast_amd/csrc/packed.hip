@@ -309,39 +309,41 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
 
   constexpr int kOwn = kTok / 4;  // tokens of its channel that a thread owns in a chunk: wave + 4 k
   constexpr int kBc = (kTok * 4 * NPT + kThreads - 1) / kThreads;
-  T r_dr[kOwn], r_u[kOwn], r_z[kOwn], r_b[kBc], r_c[kBc];
-  auto load = [&](int tc) __attribute__((always_inline)) {
+  struct Chunk {
+    T dr[kOwn], u[kOwn], z[kOwn], b[kBc], c[kBc];
+  };
+  // two chunks ahead. Tokens, channels and states that do not exist repeat the last one, so that no load stands under a condition
+  const int64_t dc = act ? d : g.D - 1;
+  auto load = [&](Chunk& r, int tc) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
-      const int64_t t = tc + wave + 4 * k;
-      const bool in = act && t < t1;
-      r_dr[k] = in ? ((const T*)g.draw)[t * g.sdraw + d] : from_f32<T>(0.0f);
-      r_u[k] = in ? ((const T*)g.u)[t * g.su + d] : from_f32<T>(0.0f);
-      if (!MAP) r_z[k] = in ? ((const T*)g.z)[t * g.sz + d] : from_f32<T>(0.0f);
+      const int i = tc + wave + 4 * k;
+      const int64_t t = i < t1 ? i : t1 - 1;
+      r.dr[k] = ((const T*)g.draw)[t * g.sdraw + dc];
+      r.u[k] = ((const T*)g.u)[t * g.su + dc];
+      if (!MAP) r.z[k] = ((const T*)g.z)[t * g.sz + dc];
     }
 #pragma unroll
     for (int k = 0; k < kBc; ++k) {
-      const int i = tid + k * kThreads, n = i % (4 * NPT);
-      const int64_t t = tc + i / (4 * NPT);
-      const bool in = n < N && t < t1;
-      r_b[k] = in ? ((const T*)g.Bt)[t * g.sb + n] : from_f32<T>(0.0f);
-      if (!MAP) r_c[k] = in ? ((const T*)g.Ct)[t * g.sc + n] : from_f32<T>(0.0f);
+      const int i = tid + k * kThreads, n = i % (4 * NPT), m = tc + i / (4 * NPT);
+      const int64_t t = m < t1 ? m : t1 - 1;
+      const int nc = n < N ? n : N - 1;
+      r.b[k] = ((const T*)g.Bt)[t * g.sb + nc];
+      if (!MAP) r.c[k] = ((const T*)g.Ct)[t * g.sc + nc];
     }
   };
   const float dp = !MAP && act ? g.Dp[d] : 0.0f;
   const int first = g.starts.at(0), last = g.starts.at(S);  // tokens that have a sequence
   float sum = 0.0f;
-  load(t0);
-  for (int tc = t0; tc < t1; tc += kTok) {
+  auto chunk = [&](Chunk& r, int tc) __attribute__((always_inline)) {
     const int len = t1 - tc < kTok ? t1 - tc : kTok;
     float o_u[kOwn], o_z[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
       const int i = wave + 4 * k;
-      o_u[k] = to_f32(r_u[k]);
-      if (!MAP) o_z[k] = to_f32(r_z[k]);
-      // tokens past the end: delta = 0 and no input, a step that changes nothing
-      const float delta = i < len ? softplus_fast(to_f32(r_dr[k])) : 0.0f;
+      o_u[k] = to_f32(r.u[k]);
+      if (!MAP) o_z[k] = to_f32(r.z[k]);
+      const float delta = i < len ? softplus_fast(to_f32(r.dr[k])) : 0.0f;  // nothing is done with tokens past the end
       if (MAP) sum += delta;
       s_sc[i][lane] = make_float2(delta, delta * o_u[k]);
     }
@@ -349,9 +351,9 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
     for (int k = 0; k < kBc; ++k) {
       const int i = tid + k * kThreads;
       if (kTok * 4 * NPT % kThreads == 0 || i < kTok * 4 * NPT)
-        s_bc[i / (4 * NPT)][i % (4 * NPT)] = make_float2(to_f32(r_b[k]), MAP ? 0.0f : to_f32(r_c[k]));
+        s_bc[i / (4 * NPT)][i % (4 * NPT)] = i % (4 * NPT) < N ? make_float2(to_f32(r.b[k]), MAP ? 0.0f : to_f32(r.c[k])) : make_float2(0.0f, 0.0f);
     }
-    if (tc + kTok < t1) load(tc + kTok);
+    load(r, tc + 2 * kTok);
     __syncthreads();
     auto step = [&](int i) __attribute__((always_inline)) {
       const float2 sc = s_sc[i][lane];
@@ -397,6 +399,15 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
           ((T*)g.out)[t * g.D + d] = from_f32<T>(has ? o : 0.0f);
         }
       }
+    }
+  };
+  if (t0 < t1) {
+    Chunk even, odd;
+    load(even, t0);
+    load(odd, t0 + kTok);
+    for (int tc = t0; tc < t1; tc += 2 * kTok) {
+      chunk(even, tc);
+      if (tc + kTok < t1) chunk(odd, tc + kTok);
     }
   }
   if (MAP) {
@@ -466,12 +477,16 @@ constexpr int64_t kMaxTokens = 1 << 30;
 
 int per_wave(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
-// Tokens of a segment: about four workgroups a CU, of 256 tokens or more
+// Tokens of a segment. A row that fills the chip is cut for six workgroups a CU (what LDS holds; 16384 x 1536 x 16 with four 229 us, with
+// six 214), not below 64 tokens. A row that does not is latency, 0.15 us a token: segments of 32 (4096 x 256 x 16 with 256 tokens 84 us, 128
+// 51, 64 34, 32 30), whole where the two passes more cost as much (77 tokens: 15 us whole).
 int64_t segment_length(int64_t T, int64_t tiles) {
-  int64_t segs = up(4 * (int64_t)device_cus(), tiles);
+  if (T <= 128) return T > 0 ? T : 1;
+  const int64_t cus = device_cus(), least = up(T, 32) * tiles <= 2 * cus ? 32 : 64;
+  int64_t segs = up(6 * cus, tiles);
   if (segs > kMaxSegs) segs = kMaxSegs;
-  int64_t len = up(up(T, segs), kTok) * kTok;
-  return len < 256 ? 256 : len;
+  const int64_t len = up(up(T, segs), kTok) * kTok;
+  return len < least ? least : len;
 }
 
 int packed_status(int64_t T, int64_t S, int64_t D, int io) {
