@@ -90,8 +90,9 @@ def test_abi_refuses_before_any_launch():
     assert size(100, 64, 32, 1, p + 2, 64, p, 64, p, 64, 0) >= 100 * 64 * 2  # x is packed
     assert size(100, 64, 32, 1, p, 64, p, 64, p, 72, 0) >= 2 * 32 * 64 * 2  # the weights' rows are not equally far apart
     assert size(100, 63, 32, 0, p, 63, p, 63, p, 63, 0) >= 3 * 2 * 64 * (100 + 2 * 32)
-    few = feed_hip._FEW_ROWS  # few rows are read as they lie
-    assert size(few, 63, 32, 0, p, 63, p, 63, p, 63, 0) == 0 < min(size(few, 63, 32, 0, p, 63, p, 63, p, 63, 1), size(few + 1, 63, 32, 0, p, 63, p, 63, p, 63, 0))
+    for few, io in zip(feed_hip._FEW_ROWS.values(), (0, 1)):  # few rows are read as they lie
+        where = (p, 63, p, 63, p, 63)
+        assert size(few, 63, 32, io, *where, 0) == 0 < min(size(few, 63, 32, io, *where, 1), size(few + 1, 63, 32, io, *where, 0))
     fwd = lambda rows=4, D=8, F=8, io=1, act=0, x=p, sx=8: lib.tsfast_hip_feed_fwd(  # noqa: E731
         rows, D, F, io, act, x, sx, p, 8, p, 8, None, None, p, None, None, 0, None)
     assert fwd(rows=-1) == fwd(D=0) == fwd(io=2) == fwd(act=3) == fwd(x=None) == fwd(sx=7) == fwd(sx=(1 << 22) + 1) == -1

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from oracle import feed_oracle
-from tsfast_amd import _lib, gated
+from tsfast_amd import gated
 from tsfast_amd.gated import feed_hip
 
 pytestmark = pytest.mark.gpu
@@ -66,7 +66,7 @@ def _check(x, wg, wu, bg, bu, gy, act, dtype):
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
 @pytest.mark.parametrize(
     "rows,D,F,bias",
-    [(1, 1, 1, True), (1, 8, 16, False), (5, 33, 47, True), (16, 64, 64, False), (17, 40, 130, True), (33, 195, 517, True), (64, 64, 32, False), (257, 96, 264, True)],
+    [(1, 1, 1, True), (1, 8, 16, False), (5, 33, 47, True), (16, 64, 64, False), (17, 40, 130, True), (33, 195, 517, True), (49, 131, 70, True), (64, 64, 32, False), (257, 96, 264, True)],
 )
 def test_small_sizes(gpu, rows, D, F, bias, act, dtype):
     _check(*_inputs((rows,), D, F, dtype, bias), act, dtype)
@@ -249,11 +249,6 @@ def test_supports_reasons(gpu):
     assert "GPU-only" in ok(x.cpu(), w) and "float64" in ok(x.double(), w.double()) and "parameter" in ok(x, w, w.cpu())
     y = gated.gated_feed_forward(x.double(), w.double(), w.double())  # the torch path
     assert y.dtype == torch.float64 and torch.allclose(y, feed_oracle.feed(x, w, w, None, None, "silu"))
-    lib = _lib.load()
-    p = torch.zeros(64, device="cuda")
-    for rows in (feed_hip._FEW_ROWS, feed_hip._FEW_ROWS + 1):
-        need = lib.tsfast_hip_feed_fwd_workspace_bytes(rows, 16, 16, 0, p.data_ptr(), 16, p.data_ptr(), 16, p.data_ptr(), 16, 0)
-        assert (need > 0) == (rows > feed_hip._FEW_ROWS)
 
 
 def test_beyond_32_bit_offsets(gpu):
@@ -267,3 +262,10 @@ def test_beyond_32_bit_offsets(gpu):
     mag, reaches = feed_oracle.reach(x[-n:], wg, wu, None, None, "silu", gy[-n:])
     _near(y[-n:], want, mag, mag, BF, 1, "y")
     _near(gx[-n:], wgrads[0], sums[0], reaches[0], BF, 2, "dx")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,D,F,bias", [(33, 2048, 61, True), (100, 2000, 517, True), (200, 1031, 64, False), (130, 4096, 1000, True), (65, 1536, 9, True)])
+def test_parts_of_a_long_contraction(gpu, rows, D, F, bias, dtype):
+    """Few tiles and a long k: every product is taken in parts, joined behind them."""
+    _check(*_inputs((rows,), D, F, dtype, bias, seed=10), "gelu", dtype)

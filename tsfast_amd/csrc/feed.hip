@@ -142,7 +142,8 @@ struct ProductArgs {
   int segs, act, train;
   const void *bg, *bu;      // forward
   void *y, *y1;             // y, dx; dWg and dWu
-  float* part;              // dW: sums of each split [split][nq][np], or null
+  float* part;              // sums of each split [split][nq][np] (forward: [split][nq][2][part_ld]), or null
+  int64_t part_ld;
   char *save_hi, *save_lo;  // forward of a training step: a and b, see save_pre
   int64_t save_fb;          // blocks of 16 columns
   int64_t half_rows, valid_rows;  // dW: rows of q a half has, and those of them that exist
@@ -482,7 +483,14 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
 
   char* own = lds + wave * C::kOwn;
   auto left = [&](uint32_t columns) { return (int)columns - (int)(wp * NH * 16); };  // of the wave's columns of a half that exist
-  if constexpr (FORM == kForward) {
+  if (FORM == kForward && C::BQ < 256 && g.part) {  // join_kernel goes on
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* y = g.part + (((int64_t)split * g.nq + q0 + wq * NQ * 16) * 2 + h) * g.part_ld + p0 + wp * NH * 16;
+      store_rows<C, float>(own, lane, left(rows_0), [&](int i, int j) { return acc[h * NH + i][j]; },
+                           [&](int q) { return (uint32_t)q + wq * NQ * 16 < rows_q ? y + q * 2 * g.part_ld : (float*)nullptr; });
+    }
+  } else if constexpr (FORM == kForward) {
     const T *bg = (const T*)g.bg, *bu = (const T*)g.bu;
     // the wave's first block of 16 rows and of 16 columns, and where a training step keeps it
     const int64_t rb = q0 / 16 + wq * NQ, cb = p0 / 16 + wp * NH, all_rb = (g.nq + 15) / 16, block0 = rb * g.save_fb + cb;
@@ -691,6 +699,50 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   }
 }
 
+// A forward in parts of k: their sums, and what product_kernel does with them otherwise. A wave has a block of 16 rows x 16 columns, four columns a
+// lane as accumulators have them.
+struct JoinArgs {
+  const float* part;  // [splits][rows][2][F8]
+  const void *bg, *bu;
+  void* y;
+  char *save_hi, *save_lo;  // or null
+  int64_t rows, F, F8, save_fb;
+  int splits, act;
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(JoinArgs g) {
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int64_t block = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rb = block / g.save_fb, cb = block % g.save_fb;
+  if (rb * 16 >= g.rows) return;
+  const int64_t m = rb * 16 + li, f = cb * 16 + 4 * lg;
+  const bool in = m < g.rows && f < g.F;
+  const float* p = g.part + (in ? m * 2 * g.F8 + f : 0);
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+#pragma unroll 4
+  for (int k = 0; k < g.splits; ++k) {
+    a += *(const f32x4*)(p + (int64_t)k * g.rows * 2 * g.F8);
+    b += *(const f32x4*)(p + (int64_t)k * g.rows * 2 * g.F8 + g.F8);
+  }
+  T y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool has = in && f + e < g.F;
+    a[e] = has ? a[e] + (g.bg ? to_f32(((const T*)g.bg)[f + e]) : 0.0f) : 0.0f;
+    b[e] = has ? b[e] + (g.bu ? to_f32(((const T*)g.bu)[f + e]) : 0.0f) : 0.0f;
+    y[e] = from_f32<T>(activate(g.act, a[e]) * b[e]);
+  }
+  if (g.save_hi) save_pre<T>(g.save_hi + block * (sizeof(T) == 2 ? 1024 : 2048), g.save_lo + block * 512, lane, a, b);
+  if (!in) return;
+  T* to = (T*)g.y + m * g.F + f;
+  if (f + 4 <= g.F) {
+    __builtin_memcpy(to, y, sizeof(y));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (f + e < g.F) to[e] = y[e];
+  }
+}
+
 // What a backward leaves in parts, summed in a fixed order, up to three results in one launch (blockIdx.y): out0 and out1 (or none) [n each] =
 // sums over `parts` of part [part][halves][stride] (the first n of each half). VL columns a lane, every fourth part a wave. VL > 1: n and
 // stride are multiples of it.
@@ -854,7 +906,8 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up8(int64_t a) { return up(a, 8) * 8; }
 int64_t up256(int64_t a) { return up(a, 256) * 256; }
 
-constexpr int64_t kFewRows = 32;
+// Rows that few_kernel takes. 33 rows of 2048 -> 2 x 5461 fp32 81 us by product_kernel (45 of them for the planes of the weights), 56 this way
+int64_t few_rows(int dtype) { return dtype == TSF_DTYPE_BF16 ? 32 : 64; }
 
 using Large = Tile<256, 256, 4, 2>;
 using Medium = Tile<128, 128, 2, 2>;
@@ -883,13 +936,13 @@ Plan plan_for(int64_t nq, int64_t np, int64_t stages, int out_bytes, bool dual, 
     const auto& c = tiles[t];
     const int64_t tq = up(nq, c.bq), tp = up(np, dual ? c.bp / 2 : c.bp);
     for (int64_t s = 1; s <= (may_split ? 64 : 1); s *= 2) {
-      if (s > 1 && stages / s < 4) break;
+      if (s > 1 && (stages / s < 4 || (dual && t == 0))) break;  // the large tile has no registers to spare for it
       const int64_t wgs = tq * tp * s, round = cus * c.per_cu, full = wgs / round, last = up(wgs % round, cus);
       auto stage = [&](int64_t beside) { return c.alone > beside * c.shared ? c.alone : beside * c.shared; };
       const double each = (double)up(stages, s);
       double time = full * (each * stage(c.per_cu) + c.ends) + (last ? each * stage(last) + c.ends : 0.0);
       if (s == 1) time += (double)(c.bq * c.bp / (dual ? 2 : 1) * out_bytes) / kStore;
-      if (s > 1) time += (double)(nq * np * (2 * s + 1) * 4) / 4e6 + 4.0;
+      if (s > 1) time += (double)(nq * np * (dual ? 2 : 1) * (2 * s + 1) * 4) / 4e6 + 4.0;
       if (!best.splits || time < least) {
         least = time;
         best = Plan{t, tq, tp, s, up(stages, s)};
@@ -998,18 +1051,34 @@ void pack_operands(const Shape& s, const Call& c, Operands& o, char* ws, hipStre
   if (jobs) pack_kernel<T><<<dim3((unsigned)up(most, kThreads), (unsigned)jobs), kThreads, 0, st>>>(a);
 }
 
+Plan forward_plan(const Shape& s, bool train) {
+  const bool half = s.dtype == TSF_DTYPE_BF16;
+  return plan_for(s.rows, s.F, s.stages_f, (half ? 2 : 4) + (train ? half ? 6 : 8 : 0), true, true);
+}
+int64_t forward_part(const Shape& s, const Plan& p) { return p.splits > 1 ? up256(p.splits * s.rows * 2 * s.F8 * 4) : 0; }
+
+template <typename T, int NT>
+void launch_few(const FewArgs& a, hipStream_t st) {
+  auto* const kernel = a.D % 8 == 0 ? few_kernel<T, NT, true> : few_kernel<T, NT, false>;
+  kernel<<<(unsigned)up(a.F, 16), kThreads, 0, st>>>(a);
+}
+
 template <typename T>
 int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void* bu, void* y, char* pre, char* ws, int64_t ws_bytes, hipStream_t st) {
-  if (s.rows <= kFewRows && !pre) {
-    FewArgs a = {c.x, c.wg, c.wu, bg, bu, y, s.rows, s.D, s.F, c.ldx, c.ldg, c.ldu, act};
-    const unsigned grid = (unsigned)up(s.F, 16);
-    auto* const kernel = s.rows <= 16 ? (s.D % 8 == 0 ? few_kernel<T, 1, true> : few_kernel<T, 1, false>)
-                                      : (s.D % 8 == 0 ? few_kernel<T, 2, true> : few_kernel<T, 2, false>);
-    kernel<<<grid, kThreads, 0, st>>>(a);
+  if (s.rows <= few_rows(s.dtype) && !pre) {
+    const FewArgs a = {c.x, c.wg, c.wu, bg, bu, y, s.rows, s.D, s.F, c.ldx, c.ldg, c.ldu, act};
+    if (s.rows <= 16)
+      launch_few<T, 1>(a, st);
+    else if (s.rows <= 32)
+      launch_few<T, 2>(a, st);
+    else if constexpr (sizeof(T) == 4)
+      launch_few<T, 4>(a, st);
     return tsf_launch_status();
   }
   Operands o = operands_of(s, c);
-  if (o.bytes && (!ws || ws_bytes < o.bytes)) return TSF_ERR_WORKSPACE;
+  const Plan plan = forward_plan(s, pre != nullptr);
+  const int64_t bytes = o.bytes + forward_part(s, plan);
+  if (bytes && (!ws || ws_bytes < bytes)) return TSF_ERR_WORKSPACE;
   pack_operands<T>(s, c, o, ws, st);
   ProductArgs g = {};
   for (int i = 0; i < s.pairs; ++i) {
@@ -1021,7 +1090,13 @@ int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void*
   g.ldq = o.x.ld, g.ldp = o.wg.ld, g.kq = g.kp = up8(s.D), g.nq = s.rows, g.np = s.F;
   g.segs = s.pairs, g.stages = s.stages_f, g.act = act, g.train = pre != nullptr, g.bg = bg, g.bu = bu, g.y = y;
   if (pre) g.save_hi = pre, g.save_lo = pre_lo(pre, s.rows, s.F), g.save_fb = up(s.F, 16);
-  product<T, kForward>(g, plan_for(s.rows, s.F, s.stages_f, (int)sizeof(T) + (pre ? (sizeof(T) == 2 ? 6 : 8) : 0), true, false), st);
+  if (plan.splits > 1) g.part = (float*)(ws + o.bytes), g.part_ld = s.F8;
+  product<T, kForward>(g, plan, st);
+  if (g.part) {
+    const int64_t fb = up(s.F, 16);
+    const JoinArgs j = {g.part, bg, bu, y, g.save_hi, g.save_lo, s.rows, s.F, s.F8, fb, (int)plan.splits, act};
+    join_kernel<T><<<(unsigned)up(up(s.rows, 16) * fb, 4), kThreads, 0, st>>>(j);
+  }
   return tsf_launch_status();
 }
 
@@ -1135,8 +1210,10 @@ int64_t tsfast_hip_feed_kept_bytes(int64_t rows, int64_t D, int64_t F, int dtype
 int64_t tsfast_hip_feed_fwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride, const void* w_gate,
                                             int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, int train) {
   if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;
-  if (rows <= kFewRows && !train) return 0;
-  return operands_of(shape_of(rows, D, F, dtype), Call{x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride}).bytes;
+  if (rows <= few_rows(dtype) && !train) return 0;
+  if (rows == 0) return 0;
+  const Shape s = shape_of(rows, D, F, dtype);
+  return operands_of(s, Call{x, w_gate, w_up, x_stride, w_gate_stride, w_up_stride}).bytes + forward_part(s, forward_plan(s, train));
 }
 
 int64_t tsfast_hip_feed_bwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride, const void* w_gate,

@@ -24,7 +24,7 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}  # feed.hip Act
 _MAX_WIDTH = 1 << 20  # D and F (feed.hip feed_status)
 _MAX_LD = 1 << 22  # elements between rows (feed.hip kMaxLd)
 _MAX_TILES = 1 << 24
-_FEW_ROWS = 32
+_FEW_ROWS = {torch.float32: 64, torch.bfloat16: 32}  # read as they lie, without a workspace (feed.hip few_rows; tests pin it)
 
 
 def supports(x, weight_gate, weight_up, bias_gate, bias_up) -> str | None:
@@ -92,8 +92,7 @@ def _forward(x, weight_gate, weight_up, bias_gate, bias_up, activation: int, tra
         y = torch.empty((*x.shape[:-1], F), device=x.device, dtype=x.dtype)
         kept = torch.empty(kept_bytes(rows, F, x.dtype), device=x.device, dtype=torch.uint8) if train else None
         where = (xr.data_ptr(), sx, wg.data_ptr(), sg, wu.data_ptr(), su)
-        # a few rows are read as they lie (feed.hip kFewRows; tests pin it against the library's size query)
-        nbytes = lib.tsfast_hip_feed_fwd_workspace_bytes(rows, D, F, io, *where, train) if train or rows > _FEW_ROWS else 0
+        nbytes = lib.tsfast_hip_feed_fwd_workspace_bytes(rows, D, F, io, *where, train) if train or rows > _FEW_ROWS[x.dtype] else 0
         ws = _lib.workspace(nbytes, x.device) if nbytes > 0 else None
         _lib.check(
             lib.tsfast_hip_feed_fwd(
