@@ -76,9 +76,8 @@ struct Cursor {
 };
 
 // ------------------------------------------------------------------------------------ convolution
-// A thread has 16 bytes of channels (8 bf16, 4 fp32) and kRun tokens. Where no sequence begins or ends within or right before them, all of its
+// A thread has 16 bytes of channels (8 bf16, 4 fp32) and RUN tokens. Where no sequence begins or ends within or right before them, all of its
 // rows are loaded at once; elsewhere it goes token by token.
-constexpr int kRun = 16;
 struct ConvArgs {
   const void *x, *tails, *weight, *bias;
   void *out, *tails_out;
@@ -114,7 +113,7 @@ TSF_DEV void store_row(T* p, const float* v, int n) {
   }
 }
 
-template <typename T, int K>
+template <typename T, int K, int RUN>
 __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
   constexpr int VL = 16 / (int)sizeof(T);
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
   const int n = (int)(g.D - c0 < VL ? g.D - c0 : VL), S = g.starts.S, T_all = g.starts.T;
   const T *x = (const T*)g.x + c0, *tails = (const T*)g.tails;
   T *out = (T*)g.out + c0, *tails_out = (T*)g.tails_out;
-  const int t0 = run < g.runs ? (int)run * kRun : 0, t1 = t0 + kRun < T_all ? t0 + kRun : T_all;
+  const int t0 = run < g.runs ? (int)run * RUN : 0, t1 = t0 + RUN < T_all ? t0 + RUN : T_all;
   Cursor at;
   at.find(g.starts, t0, threadIdx.x & 63);
   if (run >= g.runs) {  // an empty sequence leaves what it was given
@@ -149,12 +148,12 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
 #pragma unroll
       for (int k = 0; k < K; ++k) w[k][e] = ((const float*)g.weight)[(c0 + (e < n ? e : n - 1)) * K + k];
   }
-  if (at.has(g.starts) && at.begin <= t0 - (K - 1) && at.end > t1 && t1 - t0 == kRun && n == VL) {
-    T rows[kRun + K - 1][VL];
+  if (at.has(g.starts) && at.begin <= t0 - (K - 1) && at.end > t1 && t1 - t0 == RUN && n == VL) {
+    T rows[RUN + K - 1][VL];
 #pragma unroll
-    for (int k = 0; k < kRun + K - 1; ++k) __builtin_memcpy(rows[k], x + (int64_t)(t0 - (K - 1) + k) * g.sx, sizeof(rows[k]));
+    for (int k = 0; k < RUN + K - 1; ++k) __builtin_memcpy(rows[k], x + (int64_t)(t0 - (K - 1) + k) * g.sx, sizeof(rows[k]));
 #pragma unroll
-    for (int k = 0; k < kRun; ++k) {
+    for (int k = 0; k < RUN; ++k) {
       float y[VL];
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
@@ -185,18 +184,18 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
       }
     }
   }
-  T rows[kRun][VL];  // all at once: a row that does not exist repeats the last one
+  T rows[RUN][VL];  // all at once: a row that does not exist repeats the last one
   if (n == VL) {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) __builtin_memcpy(rows[i], x + (int64_t)(t0 + i < T_all ? t0 + i : T_all - 1) * g.sx, sizeof(rows[i]));
+    for (int i = 0; i < RUN; ++i) __builtin_memcpy(rows[i], x + (int64_t)(t0 + i < T_all ? t0 + i : T_all - 1) * g.sx, sizeof(rows[i]));
   } else {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
+    for (int i = 0; i < RUN; ++i)
 #pragma unroll
       for (int e = 0; e < VL; ++e) rows[i][e] = x[(int64_t)(t0 + i < T_all ? t0 + i : T_all - 1) * g.sx + (e < n ? e : n - 1)];
   }
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) {
+  for (int i = 0; i < RUN; ++i) {
     const int t = t0 + i;
     if (t < t1) {
       if (t >= at.end) {
@@ -495,16 +494,18 @@ int packed_status(int64_t T, int64_t S, int64_t D, int io) {
   return TSF_OK;
 }
 
-template <typename T>
-void launch_conv(const ConvArgs& a, int64_t K, unsigned grid, hipStream_t st) {
+template <typename T, int RUN>
+void launch_conv(ConvArgs a, int64_t K, hipStream_t st) {
+  a.runs = up(a.starts.T, RUN);
+  const unsigned grid = (unsigned)up((a.runs + a.starts.S) * a.groups, kThreads);
   switch (K) {
-    case 2: conv_kernel<T, 2><<<grid, kThreads, 0, st>>>(a); break;
-    case 3: conv_kernel<T, 3><<<grid, kThreads, 0, st>>>(a); break;
-    case 4: conv_kernel<T, 4><<<grid, kThreads, 0, st>>>(a); break;
-    case 5: conv_kernel<T, 5><<<grid, kThreads, 0, st>>>(a); break;
-    case 6: conv_kernel<T, 6><<<grid, kThreads, 0, st>>>(a); break;
-    case 7: conv_kernel<T, 7><<<grid, kThreads, 0, st>>>(a); break;
-    default: conv_kernel<T, 8><<<grid, kThreads, 0, st>>>(a); break;
+    case 2: conv_kernel<T, 2, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    case 3: conv_kernel<T, 3, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    case 4: conv_kernel<T, 4, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    case 5: conv_kernel<T, 5, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    case 6: conv_kernel<T, 6, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    case 7: conv_kernel<T, 7, RUN><<<grid, kThreads, 0, st>>>(a); break;
+    default: conv_kernel<T, 8, RUN><<<grid, kThreads, 0, st>>>(a); break;
   }
 }
 
@@ -519,9 +520,18 @@ void launch_scan(const ScanArgs& a, unsigned grid, hipStream_t st) {
   }
 }
 
-int64_t conv_grid(int64_t T, int64_t S, int64_t D, int io) {
-  return up((up(T, kRun) + S) * up(D, io == TSF_DTYPE_BF16 ? 8 : 4), kThreads);
+// Tokens of a thread: four, which are done soonest (77 x 128 fp32 5 us, with sixteen 10; 65536 x 128 bf16 21 and 26), or sixteen, which read the
+// taps and the rows before a run least often, where these are most, with 8 channels of bf16, and sixteen leave ten waves a CU or more (16384 x
+// 1536 bf16 30 us, with four 37; fp32 48 and 44).
+template <typename T>
+void launch_conv(const ConvArgs& a, int64_t K, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (up(a.starts.T, 16) * a.groups >= 640 * (int64_t)device_cus()) return launch_conv<T, 16>(a, K, st);
+  }
+  launch_conv<T, 4>(a, K, st);
 }
+
+int64_t conv_grid(int64_t T, int64_t S, int64_t D, int io) { return up((up(T, 4) + S) * up(D, io == TSF_DTYPE_BF16 ? 8 : 4), kThreads); }
 
 }  // namespace
 
@@ -536,13 +546,12 @@ int tsfast_hip_conv_packed(int64_t T, int64_t S, int64_t D, int64_t K, int io_dt
   if (K > kMaxK || conv_grid(T, S, D, io_dtype) > kMaxGrid) return TSF_ERR_UNSUPPORTED;
   if (D == 0 || (T == 0 && S == 0)) return TSF_OK;
   if (!starts || !weight || (T > 0 && (!x || !out || x_stride < 0)) || (S > 0 && !tails_out)) return TSF_ERR_ARG;
-  ConvArgs a = {x, tails, weight, bias, out, tails_out, D, x_stride, up(D, io_dtype == TSF_DTYPE_BF16 ? 8 : 4), up(T, kRun),
+  ConvArgs a = {x, tails, weight, bias, out, tails_out, D, x_stride, up(D, io_dtype == TSF_DTYPE_BF16 ? 8 : 4), 0,
                 Starts{starts, starts_int64, (int)S, (int)T}, weight_dtype == TSF_DTYPE_BF16, bias_dtype == TSF_DTYPE_BF16};
-  const unsigned grid = (unsigned)conv_grid(T, S, D, io_dtype);
   if (io_dtype == TSF_DTYPE_BF16)
-    launch_conv<bf16>(a, K, grid, (hipStream_t)stream);
+    launch_conv<bf16>(a, K, (hipStream_t)stream);
   else
-    launch_conv<float>(a, K, grid, (hipStream_t)stream);
+    launch_conv<float>(a, K, (hipStream_t)stream);
   return tsf_launch_status();
 }
 

@@ -59,7 +59,7 @@ def supports_conv(x, starts, weight, bias, tails) -> str | None:
     if not 2 <= K <= 8:
         return f"kernel width {K} outside the supported range [2, 8]"
     T, D = x.shape
-    if -(-(-(-T // 16) + starts.shape[0] - 1) * -(-D // (8 if x.dtype == torch.bfloat16 else 4)) // 256) > _MAX_GRID:
+    if -(-(-(-T // 4) + starts.shape[0] - 1) * -(-D // (8 if x.dtype == torch.bfloat16 else 4)) // 256) > _MAX_GRID:
         return f"T={T}, S={starts.shape[0] - 1}, D={D} needs more workgroups than one launch has"
     return None
 
