@@ -334,3 +334,42 @@ def test_around_the_first_cuts(gpu, T, dtype):
     """Rows that are just short enough for one segment, and the first ones that are not."""
     for starts in ([0, T], [0, 31, 32, 64, 97, T - 1], [33, 95, 95, 128 if T > 128 else 120, T]):
         check_packed(make(T, 70, 16, 4, 2, 1, dtype, dev="cuda", seed=15), starts, True, dtype)
+
+
+def test_compile_traces_a_layer_in_service(gpu):
+    m, at = make(300, 24, 8, 4, 3, 5, F32, dev="cuda", seed=16), torch.tensor([0, 130, 290], device="cuda")
+    tails, h0 = m["state"](2)
+
+    def f(conv_state, ssm_state):
+        u, left, y, last = packed(m, at, tails, h0)
+        out = mamba.mamba_step(**dict(_step_args(m), conv_state=conv_state, ssm_state=ssm_state))
+        return u * 1.0, left, y + 0.0, last, out, conv_state + 0.0, ssm_state + 0.0
+
+    t = m["token"]
+    with torch.no_grad():
+        a, b = (fn(t["conv_state"].clone(), t["ssm_state"].clone()) for fn in (f, torch.compile(f, fullgraph=True)))
+    assert same(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_step_beyond_32_bit_offsets(gpu, dtype):
+    """More than 2^31 states: the last rows as they are alone (they lie in other workgroups' rows there: to float32 rounding)."""
+    B, D, N = 8200, 4096, 64
+    m = make(1, D, N, 4, 8, 6, dtype, dev="cuda", seed=17)
+    t = m["token"]
+    big = {k: v[:1].expand(B, *v.shape[1:]).contiguous() for k, v in t.items()}
+    for k, v in t.items():
+        big[k][-6:] = v
+    args = _step_args(m)
+    y = mamba.mamba_step(**{**args, **big})
+    _near_step(args, dtype, "step")
+    want = mamba.mamba_step(**{**args, **{k: v.clone() for k, v in _fresh(m).items()}})
+    near(y[-6:], want.double(), tag("rows", dtype), 2)
+    near(big["ssm_state"][-6:], t["ssm_state"].double(), "h")
+    assert torch.equal(big["conv_state"][-6:], t["conv_state"])
+
+
+def _fresh(m):
+    """The tokens of test_step_beyond_32_bit_offsets before its step."""
+    t = make(1, *m["A"].shape, 4, 8, 6, m["token"]["x"].dtype, dev="cuda", seed=17)["token"]
+    return t
