@@ -924,29 +924,31 @@ using Large = Tile<256, 256, 4, 2>;
 using Medium = Tile<128, 128, 2, 2>;
 using Small = Tile<64, 64, 2, 2>;
 
-// How a product of nq x np outputs (np of each half where `dual`) and `stages` of k is cut: the tile, and the parts of k that side by side
+// How a product of nq x np outputs (forward: np of each half) and `stages` of k is cut: the tile, and the parts of k that side by side
 // workgroups take, whichever comes out least. A stage of one workgroup takes `alone` us while its CU has no other, and `shared` us of
 // the CU beside others; `ends` is what stands around the stages; the last workgroups' stores, `out_bytes` of each output, have nothing to go on beside.
-// Measured, us of the kernel with the large, the medium, the small tile: 256 x
-// 1536 -> 2 x 4096 bf16 36, 20, 16; 1024 rows 39, 29, 43; 2048 rows 44, 55, 82; 16384 rows with gradients 1200, 1392, 2480. Partial sums
-// are written and read at 4 TB/s. dx of 1000 rows, 768 -> 2 x 2048, whole 33 us, in parts 15 and their sum 2.
+// Measured, us of the kernel with the large, the medium, the small tile: 256 x 1536 -> 2 x 4096 bf16 36, 20, 16; 1024 rows 39, 29, 43; 2048
+// rows 44, 55, 82; 16384 rows with gradients 1200, 1392, 2480. With both operands turned the small tile's stage alone takes longer (dWg
+// and dWu of 8192 rows, 256 -> 2 x 1024 bf16, by this rule in medium tiles 19 us, in small ones 23). Partial sums are written and read at
+// 4 TB/s. dx of 1000 rows, 768 -> 2 x 2048, whole 33 us, in parts 15 and their sum 2.
 struct Plan {
   int tile;  // 0: Large, 1: Medium, 2: Small
   int64_t tiles_q, tiles_p, splits, split_stages;
 };
-Plan plan_for(int64_t nq, int64_t np, int64_t stages, int out_bytes, bool dual, bool may_split) {
+Plan plan_for(Form form, int64_t nq, int64_t np, int64_t stages, int out_bytes) {
+  const bool dual = form == kForward;
   const int64_t cus = device_cus();
   const struct {
     int bq, bp, per_cu;
     double alone, shared, ends;
-  } tiles[3] = {{256, 256, 1, 1.68, 1.68, 8.0}, {128, 128, 2, 0.8, 0.55, 4.0}, {64, 64, 4, 0.38, 0.21, 3.0}};
+  } tiles[3] = {{256, 256, 1, 1.68, 1.68, 8.0}, {128, 128, 2, 0.8, 0.55, 4.0}, {64, 64, 4, form == kWeight ? 0.65 : 0.38, 0.21, 3.0}};
   constexpr double kStore = 18500.0;  // bytes a us of a CU where all store
   Plan best = {};
   double least = 0;
   for (int t = 0; t < 3; ++t) {
     const auto& c = tiles[t];
     const int64_t tq = up(nq, c.bq), tp = up(np, dual ? c.bp / 2 : c.bp);
-    for (int64_t s = 1; s <= (may_split ? 64 : 1); s *= 2) {
+    for (int64_t s = 1; s <= 64; s *= 2) {
       if (s > 1 && (stages / s < 4 || (dual && t == 0))) break;  // the large tile has no registers to spare for it
       const int64_t wgs = tq * tp * s, round = cus * c.per_cu, full = wgs / round, last = up(wgs % round, cus);
       auto stage = [&](int64_t beside) { return c.alone > beside * c.shared ? c.alone : beside * c.shared; };
@@ -1064,7 +1066,7 @@ void pack_operands(const Shape& s, const Call& c, Operands& o, char* ws, hipStre
 
 Plan forward_plan(const Shape& s, bool train) {
   const bool half = s.dtype == TSF_DTYPE_BF16;
-  return plan_for(s.rows, s.F, s.stages_f, (half ? 2 : 4) + (train ? half ? 6 : 8 : 0), true, true);
+  return plan_for(kForward, s.rows, s.F, s.stages_f, (half ? 2 : 4) + (train ? half ? 6 : 8 : 0));
 }
 int64_t forward_part(const Shape& s, const Plan& p) { return p.splits > 1 ? up256(p.splits * s.rows * 2 * s.F8 * 4) : 0; }
 
@@ -1120,8 +1122,8 @@ struct BwdSpace {
 BwdSpace bwd_space(const Shape& s) {
   BwdSpace b;
   const int size = s.dtype == TSF_DTYPE_BF16 ? 2 : 4;
-  b.px = plan_for(s.rows, s.D, s.stages_x, size, false, true);
-  b.pw = plan_for(2 * s.F8, s.D, s.stages_w, size, false, true);
+  b.px = plan_for(kInput, s.rows, s.D, s.stages_x, size);
+  b.pw = plan_for(kWeight, 2 * s.F8, s.D, s.stages_w, size);
   const int64_t all = up(s.rows, 16), cols = up(s.F, 64);
   // rows of a workgroup: a block a wave or more (1000 x 2048 bf16 with four at least 23 us, with one 11), and three workgroups a CU, as
   // registers allow: more leave more sums of columns for the next kernel (32768 x 256 fp32: 2048 of them 41 + 14 us, 768 38 + 7)
