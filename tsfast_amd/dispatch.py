@@ -26,6 +26,8 @@ from types import ModuleType
 
 import torch
 
+from .ops import has_tangent
+
 #: Recognised preferences (tsfast's list plus "hip"); "reference" disables fused kernels.
 BACKENDS = ("auto", "hip", "triton", "c", "metal", "reference")
 
@@ -74,15 +76,23 @@ def resolve(
     ``"reference"`` -> None; ``"auto"`` -> try ``auto_order``; an explicit family -> only that
     family; a family missing from ``registry`` -> reference path silently; an import failure
     or a ``supports()`` reason -> warn once per ``"{op}.{family}"`` and try the next candidate.
-    (Semantics of ``tsfast/models/_core/dispatch.py:80-135``.)
+    Arguments with a forward-mode tangent -> reference path, with the same warning: the kernels
+    have no such derivative. (Semantics of ``tsfast/models/_core/dispatch.py:80-135``.)
     """
     requested = get_backend() if requested is None else requested
     if requested == "reference":
         return None
     names = auto_order if requested == "auto" else (requested,)
+    dual = has_tangent(args)
     for name in names:
         target = registry.get(name)
         if target is None:
+            continue
+        if dual:
+            warn_fallback(
+                f"{op}.{name}.forward_mode",
+                f"backend {name!r} unusable for {op}: no forward-mode derivative; using the reference implementation",
+            )
             continue
         if isinstance(target, str):
             try:

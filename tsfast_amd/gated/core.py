@@ -230,7 +230,8 @@ def gated_feed_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, 
         activation: ``"silu"``, ``"gelu"`` (by erf) or ``"sigmoid"`` (a gated linear unit).
 
     Returns:
-        ``[..., F]`` in x's type, differentiable in all tensors. The projection back to the stream's width is the caller's.
+        ``[..., F]`` in x's type, differentiable in all tensors (forward mode takes the torch path). The projection back to the
+        stream's width is the caller's.
 
     All values must be finite for float32: the fused kernel forms float32 products from parts of the factors, and an
     infinite factor makes NaN of the rows or columns that it reaches.

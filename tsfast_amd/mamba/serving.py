@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from ..dispatch import resolve
+from ..ops import has_tangent
 from . import core, packed_hip
 
 
@@ -48,6 +49,8 @@ _AUTO_ORDER = {"cuda": ("hip",)}
 
 
 def _no_gradient(what: str, instead: str, *tensors):
+    if has_tangent(tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it without tangents, or use {instead}")
     if not torch.is_grad_enabled():
         return
     wanted = False

@@ -5,7 +5,8 @@ kernels would see (dense GPU tensors, or None; no trace, transform, mode, forwar
 profiler) runs the op's function directly, under an ``autograd.Function`` with the op's own rules
 when a gradient is wanted. Every other call goes through the registered op, also under
 ``torch.set_default_device``, which is a mode, and where a program has registered a kernel, cast or
-autograd rule of its own on the op (from Python). The dispatcher's Python layers bound small passes: a
+autograd rule of its own on the op (from Python). No op has a forward-mode rule, and the registered op
+would drop a tangent without a word: a call with one (``has_tangent``) raises. The dispatcher's Python layers bound small passes: a
 truncated-BPTT chunk (8 x 4096 x 128, forward and backward) took 263 us through them and takes 192
 us without, a Mamba window (64 x 512 x 128) 239 and 201 us, a forward call without gradients 49 and
 44 us.
@@ -13,11 +14,12 @@ us without, a Mamba window (64 x 512 x 128) 239 and 201 us, a forward call witho
 
 from __future__ import annotations
 
-__all__ = ["custom_op"]
+__all__ = ["custom_op", "has_tangent"]
 
 import inspect
 
 import torch
+from torch._functorch.pyfunctorch import temporarily_clear_interpreter_stack
 from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
@@ -32,6 +34,7 @@ _registered = torch.library._impls  # what Python code has registered on any op,
 # dispatch keys of a plain dense GPU tensor (made in and outside inference mode); any other key
 # (conjugate or negative views, subclasses, functional, sparse, nested, batched ..) needs the dispatcher
 _plain_keys: set[int] = set()
+_functorch = torch._C._functorch
 _NUMBER_TYPES = (int, float, bool)
 _NUMBERS = (*_NUMBER_TYPES, "int", "float", "bool")  # as annotations, evaluated or not
 
@@ -64,6 +67,31 @@ def _unobserved() -> bool:
         and forward_ad._current_level < 0
         and not _profiler()
     )
+
+
+def _is_dual(t) -> bool:
+    layers = []
+    while _functorch.is_functorch_wrapped_tensor(t):
+        if _functorch.is_gradtrackingtensor(t):
+            layers.append(_functorch.maybe_get_level(t))
+        t = _functorch.get_unwrapped(t)
+    if _transform() is None:
+        return forward_ad.unpack_dual(t).tangent is not None
+    # what a jvp has wrapped counts as dual, whether or not it depends on the jvp's primals
+    if any(i.level() in layers for i in _functorch.get_interpreter_stack() if i.key() == _functorch.TransformType.Jvp):
+        return True
+    with temporarily_clear_interpreter_stack():
+        return forward_ad.unpack_dual(t).tangent is not None
+
+
+def has_tangent(values) -> bool:
+    """Whether one of them (or of a tuple among them) is a tensor with a tangent of forward-mode differentiation, also inside
+    transforms. Inside a trace every call under a forward-mode level counts."""
+    if forward_ad._current_level < 0:
+        return False
+    if torch.compiler.is_compiling():
+        return True
+    return any(has_tangent(t) if isinstance(t, (tuple, list)) else isinstance(t, torch.Tensor) and _is_dual(t) for t in values)
 
 
 class _Op:
@@ -114,6 +142,8 @@ class _Op:
 
     def __call__(self, *args, **kwargs):
         if kwargs or torch.compiler.is_compiling() or not _unobserved() or self._overridden():
+            if has_tangent((*args, *kwargs.values())) and not self._overridden():
+                raise RuntimeError(f"{self._op} has no forward-mode derivative")
             return self._op(*args, **kwargs)
         wants_grad = False
         for i, t in enumerate(args):
