@@ -1,0 +1,54 @@
+"""A Mamba layer in service on the GPU: values that are not finite go where the definition takes them, and no further."""
+
+import pytest
+import torch
+
+from tests.test_serving import BF, F32, make
+from tsfast_amd import mamba
+
+pytestmark = pytest.mark.gpu
+
+NAN = float("nan")
+
+
+def scan(m, at, h0=None, **other):
+    s = {**m["seq"], **other}
+    return mamba.mamba_ssm_packed(s["draw"], m["A"], s["B_t"], s["C_t"], s["u"], s["z"], m["Dp"], at, h0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("N", [3, 16, 40])
+@pytest.mark.parametrize("starts,t", [([0, 60], 0), ([0, 60], 59), ([3, 30, 900, 1100], 35), ([3, 30, 900, 1100], 899), ([0, 2000], 700)])
+def test_a_nan_step_size_stays_in_its_sequence_and_channel(gpu, starts, t, N, dtype):
+    """softplus of NaN is NaN, so from that token on the channel's outputs and last state are, in short rows and in rows cut into segments; all
+    others keep their bits."""
+    m = make(starts[-1] + 7, 70, N, 4, 2, 1, dtype, dev="cuda", seed=1)
+    at, d = torch.tensor(starts, device="cuda"), 65
+    h0 = m["state"](len(starts) - 1)[1]
+    want, want_last = scan(m, at, h0)
+    draw = m["seq"]["draw"].clone()
+    draw[t, d] = NAN
+    y, last = scan(m, at, h0, draw=draw)
+    s = next(i for i, e in enumerate(starts[1:]) if t < e)
+    assert y[t : starts[s + 1], d].isnan().all() and last[s, d].isnan().all()
+    y[t : starts[s + 1], d] = want[t : starts[s + 1], d]
+    last[s, d] = want_last[s, d]
+    assert torch.equal(y, want) and torch.equal(last, want_last)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_a_nan_step_bias_shows_in_its_channel(gpu, dtype):
+    m = make(1, 70, 16, 4, 5, 9, dtype, dev="cuda", seed=2)
+    weights = dict(conv_weight=m["conv"]["weight"], conv_bias=m["conv"]["bias"], **m["proj"], A=m["A"], Dp=m["Dp"])
+
+    def step(**other):
+        token = {k: t.clone() for k, t in m["token"].items()}
+        return mamba.mamba_step(**token, **{**weights, **other}), token["ssm_state"]
+
+    want, want_h = step()
+    bias = weights["dt_bias"].clone()
+    bias[33] = NAN
+    y, h = step(dt_bias=bias)
+    assert y[:, 33].isnan().all() and h[:, 33].isnan().all()
+    y[:, 33], h[:, 33] = want[:, 33], want_h[:, 33]
+    assert torch.equal(y, want) and torch.equal(h, want_h)

@@ -196,7 +196,7 @@ TSF_DEV SoftplusParts softplus_parts(float x) {
   const float lg = __builtin_amdgcn_logf(u) * kLn2;
   const float lp = dm == 0.0f ? e : lg * (e * __builtin_amdgcn_rcpf(dm));
   SoftplusParts r;
-  r.value = x > 20.0f ? x : lp;
+  r.value = x <= 20.0f ? lp : x;  // a NaN stays one (fminf makes 20 of it)
   r.e = e;
   r.u = u;
   return r;
