@@ -654,12 +654,18 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
     wave_turned();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (i >= blocks) a[i] = b[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (!whole) {  // what stands in the place of rows and columns that do not exist may be NaN, which dy = 0 leaves
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = m0 + li < g.rows && f0 + 16 * i + 4 * lg + e < g.F;
+          a[i][e] = in ? a[i][e] : 0.0f;
+          b[i][e] = in ? b[i][e] : 0.0f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v, dv;
         activate<ACT>(a[i][e], v, dv);
-        // columns and rows that do not exist have dy = 0
         a[i][e] = dy[i][e] * b[i][e] * dv;
         b[i][e] = dy[i][e] * v;
       }
