@@ -45,3 +45,20 @@ def test_rows_that_do_not_exist_are_in_no_sum(gpu, rows, dtype):
     for n in ("served", "y", "dwu", "dbg", "dbu"):
         _alike(got[n], want[n], n)
     assert want["dbg"][0] == 0 and want["dbg"][39] == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_a_large_gradient_at_a_closed_gate(gpu, act, dtype):
+    """dy b is beyond float32 where the gate's derivative is zero: no NaN, and float32's part of the magnitudes in the biases' gradients. An act(a)
+    or act'(a) below 2^-126, float32's least, may be zero there (silu(-150) is -1e-63): off by up to |dy| 2^-126 in db, and |b| times it in da."""
+    x, wg, wu, bg, bu, gy = _inputs((70,), 16, 24, dtype, True, seed=6)
+    wg.zero_(), wu.zero_(), gy.zero_()
+    bg[2], bu[2], gy[3, 2] = 30.0 if act == "sigmoid" else -150.0, 64.0, 2.0**127
+    got = _all(x, wg, wu, bg, bu, gy, act)
+    _, wants, _ = feed_oracle.feed(x, wg, wu, bg, bu, act, gy)
+    reaches = feed_oracle.reach(x, wg, wu, bg, bu, act, gy)[1]
+    for n, i in (("dbg", 3), ("dbu", 4)):
+        assert torch.isfinite(got[n]).all(), n
+        assert ((got[n].double() - wants[i]).abs() <= 1e-5 * reaches[i] + 2.0**-8 * wants[i].abs() + 2.0**127 * 2.0**-126 * 64).all(), n
+    assert torch.isfinite(got["dx"]).all()
