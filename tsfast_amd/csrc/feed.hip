@@ -73,7 +73,7 @@ TSF_DEV float activate(int act, float a) {
 }
 
 // ------------------------------------------------------------------------------------- operands
-// A matrix operand as planes of bf16 whose sum it is: one for bf16 values, three for fp32 ones (8 bits of the mantissa each). Rows
+// A matrix operand as planes of bf16 whose sum it is: one for bf16 values, three for fp32 ones (8 bits of the mantissa each, split3). Rows
 // are 16-byte aligned and their length is a multiple of 8, zeros where the matrix ends before.
 struct PackJob {
   const void* src;
@@ -85,15 +85,20 @@ struct PackArgs {
   PackJob job[3];
 };
 
-// What is left of a value beside its first part, the nearest bf16; nothing of an infinity or of a value that rounds to one.
-TSF_DEV float split_rest(float x) {
-  const float h = (float)(__bf16)x;
-  return fabsf(h) <= 3.4028235e38f ? x - h : 0.0f;
+// The parts of a float: its nearest bf16 (bf16's largest where that would be infinite), that of what is left, and of what is left then. An
+// infinity or NaN is parts (+-1, 0, itself): times a finite factor's parts, and times such a one's, the six products (kPairs) have it exactly
+// once or with its own sign, where (itself, 0, 0) would meet the zeros among the factor's parts.
+TSF_DEV float lead(float x) {
+  constexpr float kMost = 3.3895314e38f;  // bf16's largest
+  const float h = fminf(fmaxf((float)(__bf16)x, -kMost), kMost);
+  return __builtin_isfinite(x) ? h : copysignf(1.0f, x);
 }
 TSF_DEV void split3(float x, float* part) {
-  part[0] = x;
-  part[1] = split_rest(x);
-  part[2] = split_rest(part[1]);
+  const bool finite = __builtin_isfinite(x);
+  part[0] = lead(x);
+  const float rest = x - part[0];
+  part[1] = finite ? rest : 0.0f;
+  part[2] = finite ? rest - (float)(__bf16)rest : x;
 }
 
 template <typename T>
@@ -672,16 +677,26 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
       sa[i] += a[i];
       sb[i] += b[i];
     }
-    // a and b are da and db from here on; each plane of theirs in turn
+    // a and b are what is left of da and db from here on; each part of theirs in turn (split3's)
+    auto part = [](const f32x4& v, int n) __attribute__((always_inline)) {
+      f32x4 p = v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = kPlanes == 1 || n == 2 ? v[e] : n == 0 ? lead(v[e]) : __builtin_isfinite(v[e]) ? v[e] : 0.0f;
+      return p;
+    };
 #pragma unroll
     for (int n = 0; n < kPlanes; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        turn.d[0].put_four(li, 16 * i + 4 * lg, a[i]);
-        turn.d[1].put_four(li, 16 * i + 4 * lg, b[i]);
+        const f32x4 pa = part(a[i], n), pb = part(b[i], n);
+        turn.d[0].put_four(li, 16 * i + 4 * lg, pa);
+        turn.d[1].put_four(li, 16 * i + 4 * lg, pb);
         if (n + 1 < kPlanes) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[i][e] = split_rest(a[i][e]), b[i][e] = split_rest(b[i][e]);
+          for (int e = 0; e < 4; ++e) {
+            a[i][e] = __builtin_isfinite(a[i][e]) ? a[i][e] - (float)(__bf16)pa[e] : a[i][e];
+            b[i][e] = __builtin_isfinite(b[i][e]) ? b[i][e] - (float)(__bf16)pb[e] : b[i][e];
+          }
         }
       }
       wave_turned();

@@ -232,9 +232,6 @@ def gated_feed_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, 
     Returns:
         ``[..., F]`` in x's type, differentiable in all tensors (forward mode takes the torch path). The projection back to the
         stream's width is the caller's.
-
-    All values must be finite for float32: the fused kernel forms float32 products from parts of the factors, and an
-    infinite factor makes NaN of the rows or columns that it reaches.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}, expected one of {tuple(_ACTIVATIONS)}")

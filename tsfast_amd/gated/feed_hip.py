@@ -7,7 +7,7 @@ float32, 24 with bfloat16).
 
 All tensors are float32 or bfloat16 alike, rows at any stride and alignment (a last dimension that is not dense
 is copied). Products are formed on the bfloat16 matrix cores and summed in float32; float32 operands go in as three
-bfloat16 parts each, six products, which keeps float32's accuracy for finite values.
+bfloat16 parts each, six products, which keeps float32's accuracy and takes infinities and NaN where float32 products would.
 """
 
 from __future__ import annotations
