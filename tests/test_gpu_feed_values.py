@@ -121,3 +121,19 @@ def test_a_large_gradient_at_a_closed_gate(gpu, act, dtype):
         assert torch.isfinite(got[n]).all(), n
         assert ((got[n].double() - wants[i]).abs() <= 1e-5 * reaches[i] + 2.0**-8 * wants[i].abs() + 2.0**127 * 2.0**-126 * 64).all(), n
     assert torch.isfinite(got["dx"]).all()
+
+
+@pytest.mark.parametrize("rows", [50, 4000])
+def test_gelus_tail(gpu, rows):
+    """gelu keeps its accuracy where it is small. With D = F = 1, unit weights and b = 1 a is x exactly and y is act(a): its factors are off by 7e-8
+    (the fit), 2^-22 (rcp and exp, one unit each, and the argument of t), 12 x 2^-24 at most (P's nine steps and three products): under 1.1e-6
+    of the value. act' adds a phi'(a), which is off by as much of itself."""
+    a = torch.linspace(-12.5, 6, rows, device="cuda")[:, None]
+    one, none = torch.ones(1, 1, device="cuda"), torch.zeros(1, 1, device="cuda")
+    t = (a, one, none, torch.zeros(1, device="cuda"), torch.ones(1, device="cuda"), torch.ones(rows, 1, device="cuda"))
+    got, want = _all(*t, "gelu"), _want(*t, "gelu")
+    for n in ("served", "y"):
+        assert ((got[n].double() - want[n]).abs() <= 1.1e-6 * want[n].abs()).all(), n
+    w = a.double()
+    sizes = 0.5 * torch.special.erfc(-w / 2**0.5) + w.abs() * torch.exp(-w * w / 2) / (2 * torch.pi) ** 0.5
+    assert ((got["dx"].double() - want["dx"]).abs() <= 1.1e-6 * sizes).all()

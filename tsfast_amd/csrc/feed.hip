@@ -43,13 +43,18 @@ TSF_DEV float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 // ------------------------------------------------------------------------------------ activations
 // The upper tail of the normal distribution, erfc(s) / 2 with s = |a| / sqrt 2, as exp(-s^2) t P(t), t = 1 / (1 + s / 2): P is fitted to the
-// least relative error over s <= 12 (4e-8; beyond, the exp is zero in fp32), so gelu keeps its relative accuracy where it is small.
+// least relative error over s <= 12 (7e-8; beyond, the exp is zero in fp32). The exp's argument reaches 122, where its rounding alone would
+// be 5e-6 of the exp: what a^2 and its product with log2(e) / 2 are rounded by is carried along, so gelu keeps to 1e-6 of itself where it is small.
 template <int ACT>
 TSF_DEV void activate(float a, float& f, float& df) {
   if constexpr (ACT == kGelu) {
-    const float s = fabsf(a) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.5f, s, 1.0f));
-    const float e = fast_exp2(-s * s * kLog2e);
+    const float m = fminf(fabsf(a), 16.0f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35355339059327376f, m, 1.0f));
+    constexpr double kHalf = 0.72134752044448170;  // log2(e) / 2
+    constexpr float kHigh = (float)kHalf, kLow = (float)(kHalf - kHigh);
+    const float sq = m * m, x = sq * kHigh;
+    const float rest = fmaf(fmaf(m, m, -sq), kHigh, fmaf(sq, kLow, fmaf(sq, kHigh, -x)));
+    const float e0 = fast_exp2(-x), e = fmaf(e0, -kLn2 * rest, e0);
     const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.029682316f, 0.14300884f), -0.24509346f), 0.14074159f), -0.014488542f), 0.101840235f), 0.12142658f), 0.14120482f), 0.14104223f);
     const float tail = t * poly * e;
     const float phi = a < 0.0f ? tail : 1.0f - tail;
