@@ -3,12 +3,13 @@
 import pytest
 import torch
 
+from oracle import serving_oracle as O
 from tests.test_serving import BF, F32, make
 from tsfast_amd import mamba
 
 pytestmark = pytest.mark.gpu
 
-NAN = float("nan")
+INF, NAN = float("inf"), float("nan")
 
 
 def scan(m, at, h0=None, **other):
@@ -52,3 +53,51 @@ def test_a_nan_step_bias_shows_in_its_channel(gpu, dtype):
     assert y[:, 33].isnan().all() and h[:, 33].isnan().all()
     y[:, 33], h[:, 33] = want[:, 33], want_h[:, 33]
     assert torch.equal(y, want) and torch.equal(h, want_h)
+
+
+def _alike(got, want):
+    """Infinities with their signs and NaN at the same places."""
+    got, want = got.double().cpu(), want.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    at = want.isinf()
+    assert torch.equal(got.isinf(), at) and torch.equal(got[at], want[at])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("N", [1, 2, 3, 5, 16, 17])
+@pytest.mark.parametrize("starts,t", [([0, 20], 7), ([2, 30, 900, 1100], 40)])
+def test_an_infinite_step_size_makes_states_infinite(gpu, starts, t, N, dtype):
+    """The states that a wave has beyond N take no part: with an infinite delta 0 times it, NaN, would be among the sums."""
+    m = make(starts[-1] + 7, 70, N, 4, 2, 1, dtype, dev="cuda", seed=3)
+    at = torch.tensor(starts, device="cuda")
+    m["seq"]["draw"][t, 3] = INF
+    s = m["seq"]
+    got, want = scan(m, at), O.ssm_packed(s["draw"], m["A"], s["B_t"], s["C_t"], s["u"], s["z"], m["Dp"], at)
+    assert want[1].isinf().any()
+    for g, w in zip(got, want):
+        _alike(g, w)
+
+
+def _step_both(m):
+    weights = dict(conv_weight=m["conv"]["weight"], conv_bias=m["conv"]["bias"], **m["proj"], A=m["A"], Dp=m["Dp"])
+    y, tail, h = O.step(**m["token"], **weights)
+    got = mamba.mamba_step(**m["token"], **weights)
+    return (got, m["token"]["ssm_state"]), (y, h)
+
+
+@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("value", [INF, NAN])
+@pytest.mark.parametrize("B,D,N,R", [(1, 5, 1, 1), (20, 70, 1, 1), (9, 130, 4, 1), (5, 300, 16, 3)])
+def test_a_step_from_values_that_are_not_finite(gpu, B, D, N, R, value, dtype):
+    """Infinities with their signs and NaN where float64 has them, in the row with such an input; other rows keep their bits."""
+    m, plain = (make(1, D, N, 4, R, B, dtype, dev="cuda", seed=3) for _ in range(2))
+    b, d = B // 2, D - 1
+    for t in (m, plain):  # u of this channel is +inf, not silu(-inf), which is NaN
+        t["conv"]["weight"][d, 0].abs_()
+    m["token"]["x"][b, d] = value
+    (want_y, want_h), _ = _step_both(plain)
+    got, want = _step_both(m)
+    for g, w, other in zip(got, want, (want_y, want_h)):
+        _alike(g[b], w[b])
+        rest = torch.arange(B, device="cuda") != b
+        assert torch.equal(g[rest], other[rest])

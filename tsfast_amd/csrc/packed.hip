@@ -7,6 +7,8 @@
 // Sequence s has the tokens starts[s] .. starts[s + 1) of T; a sequence may be empty. The states that a sequence leaves (its
 // last K - 1 inputs; h after its last token) go out for the steps token by token behind it. Tokens without a sequence give zeros.
 // starts is read on the device: the host knows T and S only. Whatever starts holds, no access leaves the tensors and every loop ends.
+#include <type_traits>
+
 #include "common.h"
 #include "tsfast_hip.h"
 
@@ -357,24 +359,28 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
     }
     load(r, tc + 2 * kTok);
     __syncthreads();
-    auto step = [&](int i) __attribute__((always_inline)) {
+    // all: the wave's states all exist. Those that do not stay out: zeros, but for an infinite delta, with which their products are NaN
+    auto step = [&](int i, auto all) __attribute__((always_inline)) {
       const float2 sc = s_sc[i][lane];
       float y = 0.0f;
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
-        const float2 bc = s_bc[i][n0 + j];
-        h[j] = fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x);
-        y = fmaf(h[j], bc.y, y);
+        if (all || n0 + j < N) {
+          const float2 bc = s_bc[i][n0 + j];
+          h[j] = fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x);
+          y = fmaf(h[j], bc.y, y);
+        }
       }
       if (!MAP) s_y[i][wave][lane] = y;
     };
+    const bool all = n0 + NPT <= N;
     // no sequence ends within the chunk, but for its last token
     if (MAP || (at.s >= 0 && at.end - tc >= len)) {
-      if (len == kTok) {
+      if (len == kTok && all) {
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) step(i);
+        for (int i = 0; i < kTok; ++i) step(i, std::true_type());
       } else {
-        for (int i = 0; i < len; ++i) step(i);
+        for (int i = 0; i < len; ++i) step(i, std::false_type());
       }
       if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
     } else {
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
           at.next(g.starts, t);
           if (at.s < S) begin_state(at.s);
         }
-        step(i);
+        step(i, std::false_type());
         if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
       }
     }

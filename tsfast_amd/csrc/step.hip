@@ -8,6 +8,8 @@
 // advance_kernel adds the slices' sums, forms delta and moves the scan's state, in place. Everything in between is float32. Products
 // with float32 parameters are float32 matrix instructions; with bfloat16 ones the float32 factor goes in as three bfloat16 parts, exact to
 // 2^-24, on the bfloat16 matrix cores (48 cycles for 32 channels instead of 256).
+#include <type_traits>
+
 #include "common.h"
 #include "tsfast_hip.h"
 
@@ -377,25 +379,32 @@ __global__ void __launch_bounds__(kThreads, NV == 1 ? 3 : 2) advance_kernel(Step
       const float4 c = s_c[r][tid >> 2];
       float y = 0.0f;
       float* p = g.h + ((b0 + r) * g.D + dh) * N + 4 * q;
+      auto advance = [&](auto all) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        // of states that do not exist B and C are zero, and so stays h
-        const f32x4 Bt = *(const f32x4*)&s_bc[0][r][16 * j + 4 * q], Ct = *(const f32x4*)&s_bc[1][r][16 * j + 4 * q];
+        for (int j = 0; j < NV; ++j) {
+          const f32x4 Bt = *(const f32x4*)&s_bc[0][r][16 * j + 4 * q], Ct = *(const f32x4*)&s_bc[1][r][16 * j + 4 * q];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          hr[j][e] = fmaf(fast_exp2(c.x * A2[j][e]), hr[j][e], c.y * Bt[e]);
-          y = fmaf(hr[j][e], Ct[e], y);
-        }
-        if (act) {
-          if (full) {
-            __builtin_memcpy(p + 16 * j, &hr[j], 16);
-          } else {
+          for (int e = 0; e < 4; ++e) {
+            // states that do not exist stay out: zeros, but for an infinite delta, with which their products are NaN
+            const float to = fmaf(fast_exp2(c.x * A2[j][e]), hr[j][e], c.y * Bt[e]);
+            hr[j][e] = all || 16 * j + 4 * q + e < N ? to : 0.0f;
+            y = fmaf(hr[j][e], Ct[e], y);
+          }
+          if (act) {
+            if (all) {
+              __builtin_memcpy(p + 16 * j, &hr[j], 16);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (16 * j + 4 * q + e < N) p[16 * j + e] = hr[j][e];
+              for (int e = 0; e < 4; ++e)
+                if (16 * j + 4 * q + e < N) p[16 * j + e] = hr[j][e];
+            }
           }
         }
-      }
+      };
+      if (full)
+        advance(std::true_type());
+      else
+        advance(std::false_type());
       if (kAhead < kRowsA && r + kAhead < kRowsA) load_state(hr, r + kAhead);
       y += __shfl_xor(y, 1, kWave);
       y += __shfl_xor(y, 2, kWave);
