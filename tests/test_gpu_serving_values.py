@@ -85,7 +85,7 @@ def _step_both(m):
     return (got, m["token"]["ssm_state"]), (y, h)
 
 
-@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("value", [INF, NAN])
 @pytest.mark.parametrize("B,D,N,R", [(1, 5, 1, 1), (20, 70, 1, 1), (9, 130, 4, 1), (5, 300, 16, 3)])
 def test_a_step_from_values_that_are_not_finite(gpu, B, D, N, R, value, dtype):
@@ -101,3 +101,21 @@ def test_a_step_from_values_that_are_not_finite(gpu, B, D, N, R, value, dtype):
         _alike(g[b], w[b])
         rest = torch.arange(B, device="cuda") != b
         assert torch.equal(g[rest], other[rest])
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_a_step_from_u_above_bfloat16s_largest(gpu, sign):
+    """u = 3.4e38 between float32's and bfloat16's largest: what x_proj makes of it, and with it the other channels, to the package's 1e-5 of the
+    largest value."""
+    m = make(1, 70, 16, 2, 3, 9, BF, dev="cuda", seed=4)
+    m["proj"]["x_proj"].mul_(2.0**-60)
+    m["proj"]["x_proj"][:, 5] = (m["proj"]["x_proj"][:, 5] * 2.0**60).sign() * 2.0**-126 * torch.linspace(0.5, 1.0, 35, device="cuda").to(BF)
+    m["conv"]["weight"][5, 0] = torch.tensor([1.0, 1.9921875])
+    m["conv"]["bias"][5] = 0.0
+    m["token"]["x"][:, 5], m["token"]["conv_state"][:, 5, 0] = 2.0**127, 1e36
+    m["proj"]["x_proj"][:, 5] *= sign
+    (y, h), (want_y, want_h) = _step_both(m)
+    keep = torch.arange(70, device="cuda") != 5
+    assert want_h[:, keep].abs().max() > 1
+    assert (h[:, keep].double() - want_h.to("cuda")[:, keep]).abs().max() <= 1e-5 * want_h[:, keep.to(want_h.device)].abs().max()
+    assert torch.isfinite(y[:, keep]).all()

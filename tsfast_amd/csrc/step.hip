@@ -89,12 +89,15 @@ struct Side<bf16, ROWS> {
   TSF_DEV Side(char* lds, int cols) : at(lds), stride(cols + 8) {}
   TSF_DEV void put(int row, int col, float v) const {
     bf16* p = (bf16*)at + row * stride + col;
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-      const bf16 part = from_f32<bf16>(v);
-      p[n * ROWS * stride] = part;
-      v -= to_f32(part);
-    }
+    // at most bf16's largest at first: a float above it is the sum of its parts too, an infinity (bf16's largest, itself, itself)
+    constexpr float kMost = 3.3895314e38f;
+    const bf16 first = from_f32<bf16>(fminf(fmaxf(v, -kMost), kMost));
+    const float rest = v - to_f32(first);
+    const bf16 second = from_f32<bf16>(rest);
+    const float last = rest - to_f32(second);
+    p[0] = first;
+    p[ROWS * stride] = second;
+    p[2 * ROWS * stride] = from_f32<bf16>(last == last ? last : rest);
   }
   template <int N>
   TSF_DEV void multiply(const Eight<bf16>* w, int row, int col, f32x4* acc) const {
