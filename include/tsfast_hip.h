@@ -420,8 +420,11 @@ int tsfast_hip_residual_norm_bwd(int64_t rows, int64_t width, int dtype, int res
  * the workspace first (which is why its size depends on the addresses and strides). activation: 0 silu, 1 gelu (erf), 2 sigmoid.
  * `kept` (feed_kept_bytes; contents are the library's) takes a training forward's projections for the backward of the same
  * inputs; NULL: inference. grad_x may be NULL (not wanted), grad_w_gate and grad_w_up both, grad_b_gate and grad_b_up each.
- * Sums are float32 in a fixed order. D, F up to 2^20. No counterpart in the reference.
+ * Sums are float32 in a fixed order. D, F up to 2^20; every product is one launch of less than 2^32 threads. No counterpart in the reference.
+ * feed_plan: how the products of a call are cut, plan[3][4] = for y, dx, dWg and dWu: edge of the tile (0: the kernel of few rows), parts of
+ * k, workgroups, threads of each.
  */
+int tsfast_hip_feed_plan(int64_t rows, int64_t D, int64_t F, int dtype, int train, int64_t* plan);
 int64_t tsfast_hip_feed_kept_bytes(int64_t rows, int64_t D, int64_t F, int dtype);
 int64_t tsfast_hip_feed_fwd_workspace_bytes(int64_t rows, int64_t D, int64_t F, int dtype, const void* x, int64_t x_stride,
                                             const void* w_gate, int64_t w_gate_stride, const void* w_up,

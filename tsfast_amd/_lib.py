@@ -99,6 +99,7 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
         [_i64] * 2 + [_int, _int, _f32] + [_ptr, _i64] * 2 + [_ptr] * 3 + [_ptr, _i64] * 2 + [_ptr] * 6 + [_i64, _ptr],
         _int,
     ),
+    "tsfast_hip_feed_plan": ([_i64] * 3 + [_int, _int, _ptr], _int),
     "tsfast_hip_feed_kept_bytes": ([_i64] * 3 + [_int], _i64),
     "tsfast_hip_feed_fwd_workspace_bytes": ([_i64] * 3 + [_int] + [_ptr, _i64] * 3 + [_int], _i64),
     "tsfast_hip_feed_bwd_workspace_bytes": ([_i64] * 3 + [_int] + [_ptr, _i64] * 3, _i64),

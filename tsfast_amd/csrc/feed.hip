@@ -109,35 +109,35 @@ TSF_DEV void split3(float x, float* part) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pack_kernel(PackArgs a) {
   const PackJob& j = a.job[blockIdx.y];
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= j.items) return;
   const int per = j.cols8 / 8;
-  const int64_t row = i / per;
-  const int c = (int)(i % per) * 8;
-  const T* src = (const T*)j.src + row * j.ld + c;
-  T v[8];
-  if (c + 8 <= j.cols) {
-    __builtin_memcpy(v, src, sizeof(v));
-  } else {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < j.items; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t row = i / per;
+    const int c = (int)(i % per) * 8;
+    const T* src = (const T*)j.src + row * j.ld + c;
+    T v[8];
+    if (c + 8 <= j.cols) {
+      __builtin_memcpy(v, src, sizeof(v));
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < j.cols ? src[e] : from_f32<T>(0.0f);
-  }
-  bf16* dst = j.dst + row * j.cols8 + c;
-  if constexpr (sizeof(T) == 2) {
-    __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, 16);
-  } else {
-    const int64_t plane = j.rows * j.cols8;
-    u32x4 w[3];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float p0[3], p1[3];
-      split3(v[2 * k], p0);
-      split3(v[2 * k + 1], p1);
-#pragma unroll
-      for (int n = 0; n < 3; ++n) w[n][k] = pack2(p0[n], p1[n]);
+      for (int e = 0; e < 8; ++e) v[e] = c + e < j.cols ? src[e] : from_f32<T>(0.0f);
     }
+    bf16* dst = j.dst + row * j.cols8 + c;
+    if constexpr (sizeof(T) == 2) {
+      __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, 16);
+    } else {
+      const int64_t plane = j.rows * j.cols8;
+      u32x4 w[3];
 #pragma unroll
-    for (int n = 0; n < 3; ++n) *(u32x4*)(dst + n * plane) = w[n];
+      for (int k = 0; k < 4; ++k) {
+        float p0[3], p1[3];
+        split3(v[2 * k], p0);
+        split3(v[2 * k + 1], p1);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) w[n][k] = pack2(p0[n], p1[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < 3; ++n) *(u32x4*)(dst + n * plane) = w[n];
+    }
   }
 }
 
@@ -943,6 +943,10 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up8(int64_t a) { return up(a, 8) * 8; }
 int64_t up256(int64_t a) { return up(a, 256) * 256; }
 
+constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;  // of a launch
+// workgroups for n items, one a thread, or as many as a launch has: the kernel strides
+int64_t strided(int64_t n) { return up(n, kThreads) < kMaxThreads / kThreads ? up(n, kThreads) : kMaxThreads / kThreads; }
+
 // Rows that few_kernel takes. 33 rows of 2048 -> 2 x 5461 fp32 81 us by product_kernel (45 of them for the planes of the weights), 56 this way
 int64_t few_rows(int dtype) { return dtype == TSF_DTYPE_BF16 ? 32 : 64; }
 
@@ -965,9 +969,11 @@ Plan plan_for(Form form, int64_t nq, int64_t np, int64_t stages, int out_bytes) 
   const bool dual = form == kForward;
   const int64_t cus = device_cus();
   const struct {
-    int bq, bp, per_cu;
+    int bq, bp, threads, per_cu;
     double alone, shared, ends;
-  } tiles[3] = {{256, 256, 1, 1.68, 1.68, 8.0}, {128, 128, 2, 0.8, 0.55, 4.0}, {64, 64, 4, form == kWeight ? 0.65 : 0.38, 0.21, 3.0}};
+  } tiles[3] = {{Large::BQ, Large::BP, Large::TH, 1, 1.68, 1.68, 8.0},
+                {Medium::BQ, Medium::BP, Medium::TH, 2, 0.8, 0.55, 4.0},
+                {Small::BQ, Small::BP, Small::TH, 4, form == kWeight ? 0.65 : 0.38, 0.21, 3.0}};
   constexpr double kStore = 18500.0;  // bytes a us of a CU where all store
   Plan best = {};
   double least = 0;
@@ -976,6 +982,7 @@ Plan plan_for(Form form, int64_t nq, int64_t np, int64_t stages, int out_bytes) 
     const int64_t tq = up(nq, c.bq), tp = up(np, dual ? c.bp / 2 : c.bp);
     for (int64_t s = 1; s <= 64; s *= 2) {
       if (s > 1 && (stages / s < 4 || (dual && t == 0))) break;  // the large tile has no registers to spare for it
+      if (tq * tp * s * c.threads > kMaxThreads) break;
       const int64_t wgs = tq * tp * s, round = cus * c.per_cu, full = wgs / round, last = up(wgs % round, cus);
       auto stage = [&](int64_t beside) { return c.alone > beside * c.shared ? c.alone : beside * c.shared; };
       const double each = (double)up(stages, s);
@@ -1029,8 +1036,10 @@ int feed_status(int64_t rows, int64_t D, int64_t F, int dtype, int act) {
   if (rows < 0 || D < 1 || F < 1 || act < 0 || act > 2) return TSF_ERR_ARG;
   if (dtype != TSF_DTYPE_F32 && dtype != TSF_DTYPE_BF16) return TSF_ERR_ARG;
   if (D > kMaxLd / 4 || F > kMaxLd / 4 || rows > ((int64_t)1 << 31) - 64) return TSF_ERR_UNSUPPORTED;
-  // tiles of a launch, with the smallest tile and the most splits
-  if (up(rows, 64) * up(F, 32) > (1 << 24) || up(rows, 64) * up(D, 64) > (1 << 24)) return TSF_ERR_UNSUPPORTED;
+  // every product in one launch: y and dx in the smallest tile, dWg and dWu in the largest (plan_for takes no cut that would be more)
+  if (up(rows, Small::BQ) * up(F, Small::HP) > kMaxThreads / Small::TH || up(rows, Small::BQ) * up(D, Small::BP) > kMaxThreads / Small::TH)
+    return TSF_ERR_UNSUPPORTED;
+  if (up(2 * up8(F), Large::BQ) * up(D, Large::BP) > kMaxThreads / Large::TH) return TSF_ERR_UNSUPPORTED;
   return TSF_OK;
 }
 bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > kMaxLd; }
@@ -1087,7 +1096,7 @@ void pack_operands(const Shape& s, const Call& c, Operands& o, char* ws, hipStre
   add(o.x, c.x, s.rows, c.ldx);
   add(o.wg, c.wg, s.F, c.ldg);
   add(o.wu, c.wu, s.F, c.ldu);
-  if (jobs) pack_kernel<T><<<dim3((unsigned)up(most, kThreads), (unsigned)jobs), kThreads, 0, st>>>(a);
+  if (jobs) pack_kernel<T><<<dim3((unsigned)strided(most), (unsigned)jobs), kThreads, 0, st>>>(a);
 }
 
 Plan forward_plan(const Shape& s, bool train) {
@@ -1229,17 +1238,29 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) zero_kernel(T* p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i < n) p[i] = from_f32<T>(0.0f);
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = from_f32<T>(0.0f);
 }
 template <typename T>
 void zero(void* p, int64_t n, hipStream_t st) {
-  if (p && n > 0) zero_kernel<T><<<(unsigned)up(n, kThreads), kThreads, 0, st>>>((T*)p, n);
+  if (p && n > 0) zero_kernel<T><<<(unsigned)strided(n), kThreads, 0, st>>>((T*)p, n);
 }
 
 }  // namespace
 
 extern "C" {
+
+int tsfast_hip_feed_plan(int64_t rows, int64_t D, int64_t F, int dtype, int train, int64_t* plan) {
+  const int rc = feed_status(rows, D, F, dtype, 0);
+  if (rc != TSF_OK) return rc;
+  if (rows == 0 || !plan) return TSF_ERR_ARG;
+  const Shape s = shape_of(rows, D, F, dtype);
+  const BwdSpace b = bwd_space(s);
+  const int edge[3] = {Large::BQ, Medium::BQ, Small::BQ}, threads[3] = {Large::TH, Medium::TH, Small::TH};
+  int64_t* to = plan;
+  for (const Plan& p : {forward_plan(s, train), b.px, b.pw}) *to++ = edge[p.tile], *to++ = p.splits, *to++ = p.tiles_q * p.tiles_p * p.splits, *to++ = threads[p.tile];
+  if (rows <= few_rows(dtype) && !train) plan[0] = 0, plan[1] = 1, plan[2] = up(F, 16), plan[3] = kThreads;
+  return TSF_OK;
+}
 
 int64_t tsfast_hip_feed_kept_bytes(int64_t rows, int64_t D, int64_t F, int dtype) {
   if (feed_status(rows, D, F, dtype, 0) != TSF_OK) return -1;

@@ -23,7 +23,7 @@ _IO_DTYPES = {torch.float32: _lib.TSF_DTYPE_F32, torch.bfloat16: _lib.TSF_DTYPE_
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}  # feed.hip Act
 _MAX_WIDTH = 1 << 20  # D and F (feed.hip feed_status)
 _MAX_LD = 1 << 22  # elements between rows (feed.hip kMaxLd)
-_MAX_TILES = 1 << 24
+_MAX_TILES = (1 << 24) - 1  # workgroups of 256 threads in a launch
 _FEW_ROWS = {torch.float32: 64, torch.bfloat16: 32}  # read as they lie, without a workspace (feed.hip few_rows; tests pin it)
 
 
@@ -41,7 +41,8 @@ def supports(x, weight_gate, weight_up, bias_gate, bias_up) -> str | None:
     if D > _MAX_WIDTH or F > _MAX_WIDTH:
         return f"widths D={D}, F={F} above {_MAX_WIDTH}"
     rows = x.numel() // D
-    if rows > (1 << 31) - 64 or -(-rows // 64) * max(-(-F // 32), -(-D // 64)) > _MAX_TILES:
+    tiles = max(-(-rows // 64) * max(-(-F // 32), -(-D // 64)), 2 * -(-(-(-F // 8) * 16) // 256) * -(-D // 256))  # feed.hip feed_status
+    if rows > (1 << 31) - 64 or tiles > _MAX_TILES:
         return f"{rows} rows of D={D}, F={F} need more workgroups than one launch has"
     return None
 
