@@ -165,8 +165,8 @@ def mamba_step(x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_p
     Args:
         x, z: ``[B, D]`` of one type (the halves of in_proj's output, any distance between rows).
         conv_state: the last K - 1 inputs ``[B, D, K - 1]`` of x's type, and ssm_state: ``[B, D, N]`` float32; overwritten.
-        conv_weight: ``[D, 1, K]``; conv_bias: ``[D]`` or None; x_proj: ``[R + 2 N, D]``; dt_proj: ``[D, R]``; dt_bias: ``[D]`` or None; float32 or
-            x's type. A: ``[D, N]``, Dp: ``[D]``, float32.
+        conv_weight: ``[D, 1, K]``; conv_bias: ``[D]`` or None; x_proj: ``[R + 2 N, D]``; dt_proj: ``[D, R]``; dt_bias: ``[D]`` or None; float32
+            or bfloat16 each, or x's type. A: ``[D, N]``, Dp: ``[D]``, float32.
 
     Returns:
         ``out [B, D]`` in x's type. For prediction: the step has no gradient, and asking for one is an error.
@@ -190,8 +190,8 @@ def mamba_step(x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_p
     _check(dt_bias, "dt_bias", channels, optional=True)
     args = (x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A, Dp)
     for t in (conv_weight, conv_bias, x_proj, dt_proj, dt_bias):
-        if t is not None and t.dtype != x.dtype and t.dtype != wide:
-            raise ValueError(f"parameters must be {x.dtype} or {wide}, got {t.dtype}")
+        if t is not None and t.dtype not in (x.dtype, torch.float32, torch.bfloat16):
+            raise ValueError(f"parameters must be float32, bfloat16 or {x.dtype}, got {t.dtype}")
     mod = resolve("mamba.step", _STEP_BACKENDS, _AUTO_ORDER.get(x.device.type, ()), args)
     if mod is not None:
         return mod.run(*args)
