@@ -149,7 +149,7 @@ struct ProductArgs {
   int64_t ldq, ldp, kq, kp;  // kq, kp: rows of k that each operand has in a segment, as many stages
   int64_t nq, np;           // extent of C (forward: np of each half)
   int64_t tiles_q, tiles_p, stages, split_stages;
-  int segs, act, train;
+  int act, train;
   const void *bg, *bu;      // forward
   void *y, *y1;             // y, dx; dWg and dWu
   float* part;              // sums of each split [split][nq][np] (forward: [split][nq][2][part_ld]), or null
@@ -201,9 +201,9 @@ struct Panel {
     const uint64_t a = (uint64_t)at;
     const auto uniform = [](uint32_t v) __attribute__((always_inline)) { return (int)__builtin_amdgcn_readfirstlane(v); };
     const i32x4 rsrc = {uniform((uint32_t)a), uniform((uint32_t)(a >> 32) & 0xffff), uniform(bytes), kBufWord3};
-    // Written out, for the compiler makes every later read of LDS wait for the builtin's loads to arrive (vmcnt(0)), which would
-    // leave one stage on its way instead of three. Only the waits of stage_barrier cover these loads.
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(to)), "v"(v), "s"(rsrc), "s"(uniform(so)) : "memory");
+    // Written out, for the compiler makes every later read of LDS wait for the builtin's loads to arrive (vmcnt(0)): no stage would be on its
+    // way while the one before is read and multiplied. Only the waits of stage_barrier cover these loads.
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(to)), "v"(v), "s"(rsrc), "s"(uniform(so)) : "memory", "m0");
   }
   // the bytes from `at` that the lanes which read may reach
   TSF_DEV static uint32_t reach(uint32_t rows, uint32_t k, int64_t ld) {
@@ -381,11 +381,8 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
   static_assert(kQw * C::kWaves == kQ && kPw * C::kWaves == 2 * kH, "");
   Panel<C::BQ, TQ> lq[kQw];
   Panel<C::HP, TP> lp[kPw];
-  // a piece of p lies in one of its halves: which one goes by the piece, or by the wave
-  constexpr bool kByPiece = kH % C::kWaves == 0;
-  static_assert(kByPiece || kPw == 1, "");
-  constexpr int kHalves = kByPiece ? 2 : 1;
-  auto half_of = [&](int i) __attribute__((always_inline)) { return kByPiece ? i / (kPw / kHalves) : (int)(wave >= kH); };
+  static_assert(kH % C::kWaves == 0, "the wave's pieces of p: as many of each half, the first's first");
+  auto half_of = [](int i) __attribute__((always_inline)) { return i / (kPw / 2); };
 #pragma unroll
   for (int i = 0; i < kQw; ++i) lq[i].set(wave + i * C::kWaves, lane, g.ldq, rows_q);
 #pragma unroll
@@ -394,15 +391,11 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
   const int begin = (int)(split * g.split_stages);
   const int count = (int)(g.stages - begin < g.split_stages ? g.stages - begin : g.split_stages);
   int to_load = count, seg = begin / per_seg, k0 = (begin % per_seg) * kK;
-  const bf16 *qb, *pb[kHalves];
+  const bf16 *qb, *pb[2];
   auto enter = [&]() __attribute__((always_inline)) {
     qb = g.q[seg] + (TQ ? q0 + k0 * g.ldq : q0 * g.ldq);
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const bool second = kByPiece ? h != 0 : wave >= kH;
-      const int64_t at = second ? p1 : p0;
-      pb[h] = (second ? g.p1 : g.p0)[seg] + (TP ? at + k0 * g.ldp : at * g.ldp);
-    }
+    pb[0] = g.p0[seg] + (TP ? p0 + k0 * g.ldp : p0 * g.ldp);
+    pb[1] = g.p1[seg] + (TP ? p1 + k0 * g.ldp : p1 * g.ldp);
   };
   enter();
   const uint32_t reach_q = Panel<C::BQ, TQ>::reach(rows_q, kq, g.ldq);
@@ -416,7 +409,7 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
       lq[i].load(qb, reach_q, TQ ? 0 : k0 * 2, left > 0 ? left : 0, to);
     } else {
       const int n = i - kQw;
-      lp[n].load(pb[kByPiece ? half_of(n) : 0], half_of(n) ? reach_1 : reach_0, TP ? 0 : k0 * 2, left > 0 ? left : 0, to);
+      lp[n].load(pb[half_of(n)], half_of(n) ? reach_1 : reach_0, TP ? 0 : k0 * 2, left > 0 ? left : 0, to);
     }
   };
   auto advance = [&]() __attribute__((always_inline)) {
@@ -427,9 +420,7 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
       enter();
     } else {
       if (TQ) qb += kK * g.ldq;
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h)
-        if (TP) pb[h] += kK * g.ldp;
+      if (TP) pb[0] += kK * g.ldp, pb[1] += kK * g.ldp;
     }
   };
 
@@ -1136,7 +1127,7 @@ int feed_fwd(const Shape& s, const Call& c, int act, const void* bg, const void*
     g.p1[i] = o.wu.p + pr[1] * o.wu.plane;
   }
   g.ldq = o.x.ld, g.ldp = o.wg.ld, g.kq = g.kp = up8(s.D), g.nq = s.rows, g.np = s.F;
-  g.segs = s.pairs, g.stages = s.stages_f, g.act = act, g.train = pre != nullptr, g.bg = bg, g.bu = bu, g.y = y;
+  g.stages = s.stages_f, g.act = act, g.train = pre != nullptr, g.bg = bg, g.bu = bu, g.y = y;
   if (pre) g.save_hi = pre, g.save_lo = pre_lo(pre, s.rows, s.F), g.save_fb = up(s.F, 16);
   if (plan.splits > 1) g.part = (float*)(ws + o.bytes), g.part_ld = s.F8;
   product<T, kForward>(g, plan, st);
@@ -1215,7 +1206,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
         g.p0[n] = g.p1[n] = w.p + pr[1] * w.plane;
       }
     g.ldq = 2 * s.F8, g.ldp = o.wg.ld, g.kq = s.F8, g.kp = s.F, g.nq = s.rows, g.np = s.D;
-    g.segs = 2 * s.pairs, g.stages = s.stages_x, g.y = dx, g.part = b.px.splits > 1 ? part_x : nullptr;
+    g.stages = s.stages_x, g.y = dx, g.part = b.px.splits > 1 ? part_x : nullptr;
     product<T, kInput>(g, b.px, st);
     if (g.part) sums.add(g.part, b.px.splits, s.rows * s.D, s.rows * s.D, 1, dx, nullptr);
   }
@@ -1227,7 +1218,7 @@ int feed_bwd(const Shape& s, const Call& c, int act, const void* dy, int64_t ld_
       g.p0[i] = g.p1[i] = o.x.p + pr[1] * o.x.plane;
     }
     g.ldq = 2 * s.F8, g.ldp = o.x.ld, g.kq = g.kp = s.rows, g.nq = 2 * s.F8, g.np = s.D;
-    g.segs = s.pairs, g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
+    g.stages = s.stages_w, g.y = dwg, g.y1 = dwu, g.half_rows = s.F8, g.valid_rows = s.F;
     g.part = b.pw.splits > 1 ? part_w : nullptr;
     product<T, kWeight>(g, b.pw, st);
     if (g.part) sums.add(g.part, b.pw.splits, s.F8 * s.D, s.F * s.D, 2, dwg, dwu);
