@@ -43,9 +43,10 @@ TSF_DEV float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 // ------------------------------------------------------------------------------------ activations
 // The upper tail of the normal distribution, erfc(s) / 2 with s = |a| / sqrt 2, as exp(-s^2) t P(t), t = 1 / (1 + s / 2): P is fitted to the
-// least relative error over s <= 12 (7e-8; beyond, the exp is zero in fp32). The exp's argument reaches 122, where its rounding alone would
-// be 5e-6 of the exp: what a^2 and its product with log2(e) / 2 are rounded by is carried along, so gelu keeps to 1e-6 of itself where it is small.
-template <int ACT>
+// least relative error over s <= 12 (7e-8; beyond, the exp is zero in fp32). The exp's argument reaches 122, where its rounding is 2e-5 of the
+// exp: nothing beside bf16's 2^-8, but for float32 (T) what a^2 and its product with log2(e) / 2 are rounded by is carried along, so gelu keeps to
+// 1e-6 of itself where it is small.
+template <int ACT, typename T>
 TSF_DEV void activate(float a, float& f, float& df) {
   if constexpr (ACT == kGelu) {
     const float m = fminf(fabsf(a), 16.0f);
@@ -53,8 +54,11 @@ TSF_DEV void activate(float a, float& f, float& df) {
     constexpr double kHalf = 0.72134752044448170;  // log2(e) / 2
     constexpr float kHigh = (float)kHalf, kLow = (float)(kHalf - kHigh);
     const float sq = m * m, x = sq * kHigh;
-    const float rest = fmaf(fmaf(m, m, -sq), kHigh, fmaf(sq, kLow, fmaf(sq, kHigh, -x)));
-    const float e0 = fast_exp2(-x), e = fmaf(e0, -kLn2 * rest, e0);
+    float e = fast_exp2(-x);
+    if constexpr (sizeof(T) == 4) {
+      const float rest = fmaf(fmaf(m, m, -sq), kHigh, fmaf(sq, kLow, fmaf(sq, kHigh, -x)));
+      e = fmaf(e, -kLn2 * rest, e);
+    }
     const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.029682316f, 0.14300884f), -0.24509346f), 0.14074159f), -0.014488542f), 0.101840235f), 0.12142658f), 0.14120482f), 0.14104223f);
     const float tail = t * poly * e;
     const float phi = a < 0.0f ? tail : 1.0f - tail;
@@ -66,14 +70,15 @@ TSF_DEV void activate(float a, float& f, float& df) {
     df = ACT == kSilu ? fmaf(a * sig, 1.0f - sig, sig) : sig * (1.0f - sig);
   }
 }
+template <typename T>
 TSF_DEV float activate(int act, float a) {
   float f, df;
   if (act == kSilu)
-    activate<kSilu>(a, f, df);
+    activate<kSilu, T>(a, f, df);
   else if (act == kGelu)
-    activate<kGelu>(a, f, df);
+    activate<kGelu, T>(a, f, df);
   else
-    activate<kSigmoid>(a, f, df);
+    activate<kSigmoid, T>(a, f, df);
   return f;
 }
 
@@ -526,7 +531,7 @@ __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v, dv;
-            activate<decltype(act)::value>(a[e], v, dv);
+            activate<decltype(act)::value, T>(a[e], v, dv);
             a[e] = v * b[e];
           }
           __builtin_amdgcn_sched_barrier(0);  // or values of many blocks are alive at once, and spill
@@ -628,6 +633,8 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
     // a load under a lane's condition is waited for before the next one starts: whole blocks have none
     const bool whole = m0 + 16 <= g.rows && f0 + 64 <= g.F;
     const T* dy0 = (const T*)g.dy + m0 * g.ld_dy + f0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + (i < blocks ? i : 0), lane, a[i], b[i]);
     if (whole) {
 #pragma unroll
       for (int e = 0; e < kDy; ++e) __builtin_memcpy(&in[e], dy0 + Turn<T>::row(lane, e) * g.ld_dy + Turn<T>::col(lane, e), 16);
@@ -643,9 +650,16 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
         for (int k = 0; k < kPer; ++k) v[k] = r < rows && c + k < cols ? v[k] : from_f32<T>(0.0f);
         __builtin_memcpy(&in[e], v, 16);
       }
-    }
+      // what stands in the place of rows and columns that do not exist may be NaN, which dy = 0 leaves
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_pre<T>(g.save_hi, g.save_lo, mb * g.save_fb + f0 / 16 + (i < blocks ? i : 0), lane, a[i], b[i]);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool exists = li < rows && 16 * i + 4 * lg + e < cols;
+          a[i][e] = exists ? a[i][e] : 0.0f;
+          b[i][e] = exists ? b[i][e] : 0.0f;
+        }
+    }
 #pragma unroll
     for (int e = 0; e < kDy; ++e) turn.dy.put_piece(lane, e, in[e]);
     wave_turned();
@@ -655,18 +669,10 @@ __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
     wave_turned();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (!whole) {  // what stands in the place of rows and columns that do not exist may be NaN, which dy = 0 leaves
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = m0 + li < g.rows && f0 + 16 * i + 4 * lg + e < g.F;
-          a[i][e] = in ? a[i][e] : 0.0f;
-          b[i][e] = in ? b[i][e] : 0.0f;
-        }
-      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float v, dv;
-        activate<ACT>(a[i][e], v, dv);
+        activate<ACT, T>(a[i][e], v, dv);
         a[i][e] = dy[i][e] * dv * b[i][e];  // |dv| < 1.2: no infinity in between that a closed gate (dv = 0) makes NaN
         b[i][e] = dy[i][e] * v;
       }
@@ -756,7 +762,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(JoinArgs g) {
     const bool has = in && f + e < g.F;
     a[e] = has ? a[e] + (g.bg ? to_f32(((const T*)g.bg)[f + e]) : 0.0f) : 0.0f;
     b[e] = has ? b[e] + (g.bu ? to_f32(((const T*)g.bu)[f + e]) : 0.0f) : 0.0f;
-    y[e] = from_f32<T>(activate(g.act, a[e]) * b[e]);
+    y[e] = from_f32<T>(activate<T>(g.act, a[e]) * b[e]);
   }
   if (g.save_hi) save_pre<T>(g.save_hi + block * (sizeof(T) == 2 ? 1024 : 2048), g.save_lo + block * 512, lane, a, b);
   if (!in) return;
@@ -925,7 +931,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(FewArgs g) {
       const uint32_t at = (c >> 2) * 16 + r, e = c & 3;
       v[h] = (sums[0][h * NT + t][at][e] + sums[1][h * NT + t][at][e]) + (sums[2][h * NT + t][at][e] + sums[3][h * NT + t][at][e]);
     }
-    ((T*)g.y)[row * g.F + column] = from_f32<T>(activate(g.act, v[0] + ba) * (v[1] + bb));
+    ((T*)g.y)[row * g.F + column] = from_f32<T>(activate<T>(g.act, v[0] + ba) * (v[1] + bb));
   }
 }
 

@@ -373,27 +373,32 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
       }
       if (!MAP) s_y[i][wave][lane] = y;
     };
-    const bool all = n0 + NPT <= N;
-    // no sequence ends within the chunk, but for its last token
-    if (MAP || (at.s >= 0 && at.end - tc >= len)) {
-      if (len == kTok && all) {
+    auto walk = [&](auto all) __attribute__((always_inline)) {
+      // no sequence ends within the chunk, but for its last token
+      if (MAP || (at.s >= 0 && at.end - tc >= len)) {
+        if (all && len == kTok) {
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) step(i, std::true_type());
-      } else {
-        for (int i = 0; i < len; ++i) step(i, std::false_type());
-      }
-      if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
-    } else {
-      for (int i = 0; i < len; ++i) {
-        const int t = tc + i;
-        if (t >= at.end) {
-          at.next(g.starts, t);
-          if (at.s < S) begin_state(at.s);
+          for (int i = 0; i < kTok; ++i) step(i, all);
+        } else {
+          for (int i = 0; i < len; ++i) step(i, all);
         }
-        step(i, std::false_type());
-        if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
+        if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
+      } else {
+        for (int i = 0; i < len; ++i) {
+          const int t = tc + i;
+          if (t >= at.end) {
+            at.next(g.starts, t);
+            if (at.s < S) begin_state(at.s);
+          }
+          step(i, all);
+          if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
+        }
       }
-    }
+    };
+    if (n0 + NPT <= N)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
     __syncthreads();
     if (!MAP) {
 #pragma unroll

@@ -25,6 +25,7 @@ from contextlib import contextmanager
 from types import ModuleType
 
 import torch
+from torch.autograd import forward_ad
 
 from .ops import has_tangent
 
@@ -83,7 +84,7 @@ def resolve(
     if requested == "reference":
         return None
     names = auto_order if requested == "auto" else (requested,)
-    dual = has_tangent(args)
+    dual = forward_ad._current_level >= 0 and has_tangent(args)
     for name in names:
         target = registry.get(name)
         if target is None:

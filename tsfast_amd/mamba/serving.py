@@ -21,6 +21,7 @@ __all__ = ["mamba_conv_packed", "mamba_ssm_packed", "mamba_step"]
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from ..dispatch import resolve
 from ..ops import has_tangent
@@ -49,7 +50,7 @@ _AUTO_ORDER = {"cuda": ("hip",)}
 
 
 def _no_gradient(what: str, instead: str, *tensors):
-    if has_tangent(tensors):
+    if forward_ad._current_level >= 0 and has_tangent(tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative: call it without tangents, or use {instead}")
     if not torch.is_grad_enabled():
         return
