@@ -7,8 +7,6 @@
 // Sequence s has the tokens starts[s] .. starts[s + 1) of T; a sequence may be empty. The states that a sequence leaves (its
 // last K - 1 inputs; h after its last token) go out for the steps token by token behind it. Tokens without a sequence give zeros.
 // starts is read on the device: the host knows T and S only. Whatever starts holds, no access leaves the tensors and every loop ends.
-#include <type_traits>
-
 #include "common.h"
 #include "tsfast_hip.h"
 
@@ -254,13 +252,17 @@ struct ScanArgs {
   float* maps;  // of segments: sums of delta [segs][D], then states [segs][N][D]
 };
 
-// The walk of one segment. MAP: only the state it hands to the next one, from the last sequence's first token in it (or its own
+// Waves a SIMD that the registers are to allow where a wave has states that do not exist: what they allow by themselves where it has none.
+constexpr int scan_waves(int npt) { return npt >= 16 ? 3 : npt >= 8 ? 4 : npt >= 2 ? 5 : 4; }
+
+// The walk of one segment. ALL: N = 4 NPT, every state exists. MAP: only the state it hands to the next one, from the last sequence's first token in it (or its own
 // first token with no state), with the sum of delta that decays what enters; -1: nothing that enters reaches the next segment.
-template <typename T, int NPT, bool MAP>
-__global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
+template <typename T, int NPT, bool MAP, bool ALL>
+__global__ void __launch_bounds__(kThreads, ALL ? 1 : scan_waves(NPT)) scan_kernel(ScanArgs g) {
   __shared__ float2 s_sc[kTok][kCh];         // delta, delta u
   __shared__ float2 s_bc[kTok][4 * NPT];     // B, C
   __shared__ float s_y[MAP ? 1 : kTok][4][kCh];  // each wave's sum over its states
+  __shared__ int s_odd[2];                       // whether a chunk has an infinite or NaN delta u; chunks in turn
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t tile = blockIdx.x % g.tiles, seg = blockIdx.x / g.tiles, d = tile * kCh + lane;
   const int S = g.starts.S, T_all = g.starts.T;
@@ -339,8 +341,9 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
   const float dp = !MAP && act ? g.Dp[d] : 0.0f;
   const int first = g.starts.at(0), last = g.starts.at(S);  // tokens that have a sequence
   float sum = 0.0f;
-  auto chunk = [&](Chunk& r, int tc) __attribute__((always_inline)) {
+  auto chunk = [&](Chunk& r, int tc, int turn) __attribute__((always_inline)) {
     const int len = t1 - tc < kTok ? t1 - tc : kTok;
+    bool odd = false;
     float o_u[kOwn], o_z[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
@@ -350,7 +353,9 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
       const float delta = i < len ? softplus_fast(to_f32(r.dr[k])) : 0.0f;  // nothing is done with tokens past the end
       if (MAP) sum += delta;
       s_sc[i][lane] = make_float2(delta, delta * o_u[k]);
+      odd = odd || !__builtin_isfinite(delta * o_u[k]);
     }
+    if (!ALL && odd) s_odd[turn] = 1;
 #pragma unroll
     for (int k = 0; k < kBc; ++k) {
       const int i = tid + k * kThreads;
@@ -359,46 +364,54 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
     }
     load(r, tc + 2 * kTok);
     __syncthreads();
-    // all: the wave's states all exist. Those that do not stay out: zeros, but for an infinite delta, with which their products are NaN
-    auto step = [&](int i, auto all) __attribute__((always_inline)) {
+    auto step = [&](int i) __attribute__((always_inline)) {
       const float2 sc = s_sc[i][lane];
       float y = 0.0f;
 #pragma unroll
       for (int j = 0; j < NPT; ++j) {
-        if (all || n0 + j < N) {
-          const float2 bc = s_bc[i][n0 + j];
-          h[j] = fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x);
-          y = fmaf(h[j], bc.y, y);
-        }
+        const float2 bc = s_bc[i][n0 + j];
+        h[j] = fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x);
+        y = fmaf(h[j], bc.y, y);
       }
       if (!MAP) s_y[i][wave][lane] = y;
     };
-    auto walk = [&](auto all) __attribute__((always_inline)) {
-      // no sequence ends within the chunk, but for its last token
-      if (MAP || (at.s >= 0 && at.end - tc >= len)) {
-        if (all && len == kTok) {
+    // Beside an infinite or NaN delta u the zeros of states that do not exist would be NaN among the sums: without them. 16384 x 1536 with 17
+    // states 304 us, with 40 575; with masks in every chunk 40 would take 800, and without any, as wrong as that is, 302 and 549.
+    auto step_without = [&](int i) __attribute__((always_inline)) {
+      const float2 sc = s_sc[i][lane];
+      float y = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kTok; ++i) step(i, all);
-        } else {
-          for (int i = 0; i < len; ++i) step(i, all);
-        }
-        if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
-      } else {
-        for (int i = 0; i < len; ++i) {
-          const int t = tc + i;
-          if (t >= at.end) {
-            at.next(g.starts, t);
-            if (at.s < S) begin_state(at.s);
-          }
-          step(i, all);
-          if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
-        }
+      for (int j = 0; j < NPT; ++j) {
+        const float2 bc = s_bc[i][n0 + j];
+        h[j] = n0 + j < N ? fmaf(fast_exp2(sc.x * A2[j]), h[j], sc.y * bc.x) : 0.0f;
+        y = n0 + j < N ? fmaf(h[j], bc.y, y) : y;
       }
+      s_y[MAP ? 0 : i][wave][lane] = y;
     };
-    if (n0 + NPT <= N)
-      walk(std::true_type());
-    else
-      walk(std::false_type());
+    const bool without = !ALL && n0 + NPT > N && __builtin_amdgcn_readfirstlane(s_odd[turn]) != 0;
+    if (!ALL && tid == 0) s_odd[turn ^ 1] = 0;  // read before the last barrier, set after the next one
+    if (!without && (MAP || (at.s >= 0 && at.end - tc >= len))) {  // no sequence ends within the chunk, but for its last token
+      if (len == kTok) {
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) step(i);
+      } else {
+        for (int i = 0; i < len; ++i) step(i);
+      }
+      if (!MAP && at.s < S && at.end == tc + len) end_state(at.s);
+    } else {
+      for (int i = 0; i < len; ++i) {
+        const int t = tc + i;
+        if (t >= at.end) {
+          at.next(g.starts, t);
+          if (at.s < S) begin_state(at.s);
+        }
+        if (without)
+          step_without(i);
+        else
+          step(i);
+        if (at.has(g.starts) && t == at.end - 1) end_state(at.s);
+      }
+    }
     __syncthreads();
     if (!MAP) {
 #pragma unroll
@@ -418,9 +431,13 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ScanArgs g) {
     Chunk even, odd;
     load(even, t0);
     load(odd, t0 + kTok);
+    if (!ALL) {
+      if (tid < 2) s_odd[tid] = 0;
+      __syncthreads();
+    }
     for (int tc = t0; tc < t1; tc += 2 * kTok) {
-      chunk(even, tc);
-      if (tc + kTok < t1) chunk(odd, tc + kTok);
+      chunk(even, tc, 0);
+      if (tc + kTok < t1) chunk(odd, tc + kTok, 1);
     }
   }
   if (MAP) {
@@ -523,14 +540,21 @@ void launch_conv(ConvArgs a, int64_t K, hipStream_t st) {
   }
 }
 
+template <typename T, int NPT, bool MAP>
+void launch_scan(const ScanArgs& a, unsigned grid, hipStream_t st) {
+  if (MAP || a.N == 4 * NPT)  // maps: states that do not exist go nowhere
+    scan_kernel<T, NPT, MAP, true><<<grid, kThreads, 0, st>>>(a);
+  else
+    scan_kernel<T, NPT, false, false><<<grid, kThreads, 0, st>>>(a);
+}
 template <typename T, bool MAP>
 void launch_scan(const ScanArgs& a, unsigned grid, hipStream_t st) {
   switch (per_wave(a.N)) {
-    case 1: scan_kernel<T, 1, MAP><<<grid, kThreads, 0, st>>>(a); break;
-    case 2: scan_kernel<T, 2, MAP><<<grid, kThreads, 0, st>>>(a); break;
-    case 4: scan_kernel<T, 4, MAP><<<grid, kThreads, 0, st>>>(a); break;
-    case 8: scan_kernel<T, 8, MAP><<<grid, kThreads, 0, st>>>(a); break;
-    default: scan_kernel<T, 16, MAP><<<grid, kThreads, 0, st>>>(a); break;
+    case 1: launch_scan<T, 1, MAP>(a, grid, st); break;
+    case 2: launch_scan<T, 2, MAP>(a, grid, st); break;
+    case 4: launch_scan<T, 4, MAP>(a, grid, st); break;
+    case 8: launch_scan<T, 8, MAP>(a, grid, st); break;
+    default: launch_scan<T, 16, MAP>(a, grid, st); break;
   }
 }
 
