@@ -206,7 +206,7 @@ TSF_DEV float softplus_fast(float x) { return softplus_parts(x).value; }
 // above 20 passed through, on the transcendental unit (v_exp, v_log)
 TSF_DEV float softplus_ref(float x) {
   const float e = __builtin_amdgcn_exp2f(fminf(x, 20.0f) * kLog2e);
-  return x > 20.0f ? x : __builtin_amdgcn_logf(1.0f + e) * kLn2;
+  return x <= 20.0f ? __builtin_amdgcn_logf(1.0f + e) * kLn2 : x;  // a NaN stays one
 }
 TSF_DEV float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
 

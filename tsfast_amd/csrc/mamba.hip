@@ -759,7 +759,7 @@ __global__ void __launch_bounds__((BCfg<NS, DT_>::TH), (BCfg<NS, DT_>::OCC)) mam
         // passed through; d softplus / d draw = e^x / (1 + e^x)
         const float e = fast_exp2(fminf(xd, 20.0f) * kLog2e);
         const float up = 1.0f + e;
-        const float delta = live ? (xd > 20.0f ? xd : __builtin_amdgcn_logf(up) * kLn2) : 0.0f;
+        const float delta = live ? (xd <= 20.0f ? __builtin_amdgcn_logf(up) * kLn2 : xd) : 0.0f;
         const float sg = sigmoid_fast(zz);
         const float gyv = live ? go * zz * sg : 0.0f;
         o_u[k] = uu;
