@@ -420,7 +420,8 @@ int tsfast_hip_residual_norm_bwd(int64_t rows, int64_t width, int dtype, int res
  * the workspace first (which is why its size depends on the addresses and strides). activation: 0 silu, 1 gelu (erf), 2 sigmoid.
  * `kept` (feed_kept_bytes; contents are the library's) takes a training forward's projections for the backward of the same
  * inputs; NULL: inference. grad_x may be NULL (not wanted), grad_w_gate and grad_w_up both, grad_b_gate and grad_b_up each.
- * Sums are float32 in a fixed order. D, F up to 2^20; every product is one launch of less than 2^32 threads. No counterpart in the reference.
+ * Sums are float32 in a fixed order, cut by rows, D, F and whether kept is wanted; infinities and NaN go where float32 products take them.
+ * bfloat16: grad_y's products with the activation and with b are rounded to bfloat16 before theirs with the weights and x. D, F up to 2^20; every product is one launch of less than 2^32 threads. No counterpart in the reference.
  * feed_plan: how the products of a call are cut, plan[3][4] = for y, dx, dWg and dWu: edge of the tile (0: the kernel of few rows), parts of
  * k, workgroups, threads of each.
  */

@@ -351,8 +351,9 @@ TSF_DEV void load_pre(const char* hi, const char* lo, int64_t block, uint32_t la
 // way, and a wave holds the operands of half a stage in registers while it reads the other half's, so the matrix instructions wait for neither.
 // Stages of 64 k, not 32, make every load a whole 128-byte line (the three large products 5.4 -> 4.4 ms). What bounds it: the matrix cores at
 // the clock that power leaves them (1.6 to 1.8 GHz here), and between a tile's last product and its last store nothing else runs on a CU.
-// Measured, 65536 x 1536 -> 2 x 4096 bf16: y with what a backward needs 1.69 ms (980 TFLOP/s), dx 1.29 ms (1280), dWg and dWu 1.35 ms (1220); a
-// library product of the same sizes, without the activation and what is kept, 1.40, 1.11 and 1.21 ms.
+// Measured, 65536 x 1536 -> 2 x 4096 bf16: y with what a backward needs 1.69 ms (980 TFLOP/s), dx 1.30 ms (1270), dWg and dWu 1.35 ms (1220); a
+// library product of the same sizes, without the activation and what is kept, 1.40, 1.11 and 1.21 ms. fp32, 16384 x 1536 -> 2 x 4096: packing and y
+// 1.78 ms (231 TFLOP/s), a library product of those sizes alone 2.81 ms.
 template <typename T, typename C, int FORM>
 __global__ void __launch_bounds__(C::TH, C::kPerSimd) product_kernel(ProductArgs g) {
   constexpr bool TQ = FORM == kWeight, TP = FORM != kForward;  // turned operands
@@ -606,8 +607,8 @@ struct Turn {
 };
 
 // da = dy b act'(a), db = dy act(a) as planes of bf16 for the two products behind it, rounded once each, and their sums over rows for the
-// biases, of the values before that rounding. Bound by memory: 65536 x 4096 bf16 reads 2.1 GB and writes 1.1 GB in 0.66 ms (4.9 TB/s),
-// 32768 x 256 fp32 38 us (5.3 TB/s, in part from the cache).
+// biases, of the values before that rounding. Bound by memory: 65536 x 4096 bf16 reads 2.1 GB and writes 1.1 GB in 0.67 ms (4.8 TB/s),
+// 32768 x 256 fp32 40 us (5.0 TB/s, in part from the cache).
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kThreads) adjoint_kernel(AdjointArgs g) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3;

@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs g) {
 // A workgroup has 64 channels and a run of tokens (a segment). Each of its four waves has a quarter of the states of all 64, a
 // channel a lane, in registers; what depends on a token and a channel (softplus, gates) is done once, by the thread that owns the pair,
 // and goes through LDS, a chunk of kTok tokens at a time. Vector instructions bound it: a token's state is about six
-// issue slots (its exp two) and a share of some thirty of a token and channel, 95 us for 16384 x 1536 x 16 at 2.4 GHz, where the walk takes 121;
-// segments' maps have to form the same exps before (70, takes 84), and the join is 11. Memory would allow 45 us. A short row is the latency of its tokens, 0.15 us each.
+// issue slots (its exp two) and a share of some thirty of a token and channel, 95 us for 16384 x 1536 x 16 at 2.4 GHz, where the walk takes 123;
+// segments' maps have to form the same exps before (70, takes 85), and the join is 11. Memory would allow 45 us. A short row is the latency of its tokens, 0.15 us each.
 constexpr int kTok = 16;
 constexpr int kCh = 64;
 struct ScanArgs {

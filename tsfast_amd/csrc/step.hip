@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kThreads) project_kernel(StepArgs g) {
 }
 
 // A workgroup: 64 channels of up to 8 rows. States: 4 lanes a channel, 4 states of each 16 a lane. delta: 16 channels a wave.
-// Three waves a SIMD, for three workgroups a CU: 256 sequences of 1536 channels 16.8 us, with two (180 registers) 20.7, with four (which
-// spill) 25.
+// Three waves a SIMD, for three workgroups a CU: 256 sequences of 1536 channels 15.7 us, with two (180 registers) 4 more, with four (which
+// spill) 8.
 template <typename T, typename P, int NV>
 __global__ void __launch_bounds__(kThreads, NV == 1 ? 3 : 2) advance_kernel(StepArgs g) {
   extern __shared__ __attribute__((aligned(16))) char s_dt[];  // [rows][R], zeros up to a multiple of 32

@@ -232,6 +232,12 @@ def gated_feed_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, 
     Returns:
         ``[..., F]`` in x's type, differentiable in all tensors (forward mode takes the torch path). The projection back to the
         stream's width is the caller's.
+
+    Sums are float32 and y is rounded once. In a bfloat16 backward the gradients of both projections are rounded to bfloat16 before their products
+    with the weights and x (the weights' gradients are 2.3e-3 of their norm off instead of one rounding's 1.7e-3), and of the projections the forward
+    keeps 24 bits; the biases' gradients are sums of unrounded values. The same call gives the same bits. How its sums are cut, and with it
+    a row's last bits, depends on the number of rows, D, F and on whether a gradient is wanted: a row alone and among others agree to float32
+    rounding before y's own.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}, expected one of {tuple(_ACTIVATIONS)}")

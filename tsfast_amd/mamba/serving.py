@@ -170,7 +170,8 @@ def mamba_step(x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_p
             or bfloat16 each, or x's type. A: ``[D, N]``, Dp: ``[D]``, float32.
 
     Returns:
-        ``out [B, D]`` in x's type. For prediction: the step has no gradient, and asking for one is an error.
+        ``out [B, D]`` in x's type. For prediction: the step has no gradient, and asking for one is an error. The channels whose products with
+        x_proj are summed together depend on B and D: a sequence alone and in a batch agree to float32 rounding.
     """
     _no_gradient("mamba_step", "mamba_conv and mamba_ssm", x, z, conv_state, ssm_state, conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A, Dp)
     if x.dim() != 2 or A.dim() != 2 or A.shape[1] < 1:
