@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kThreads, ALL ? 1 : scan_waves(NPT)) scan_kern
       }
       if (!MAP) s_y[i][wave][lane] = y;
     };
-    // Beside an infinite or NaN delta u the zeros of states that do not exist would be NaN among the sums: without them. 16384 x 1536 with 17
-    // states 304 us, with 40 575; with masks in every chunk 40 would take 800, and without any, as wrong as that is, 302 and 549.
+    // Beside an infinite or NaN delta u the zeros of states that do not exist would be NaN among the sums: there, without them. 16384 x 1536 with 17
+    // states 304 us, with 40 575 (without this path 302 and 549; with masks in every chunk instead 40 states took 800).
     auto step_without = [&](int i) __attribute__((always_inline)) {
       const float2 sc = s_sc[i][lane];
       float y = 0.0f;
